@@ -17,9 +17,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libccfuser_b200.so")
-TORCH_SOURCES = [os.path.join(CSRC, f) for f in ("torch_norm.cpp", "norm.h")]
+TORCH_SOURCES = [os.path.join(CSRC, f) for f in ("torch_norm.cpp", "torch_tokens.cpp", "torch_ops.h", "norm.h", "embedding.h", "logprobs.h",
+                                                 "dropout.h")]
 SOURCES = ["gemm.cu", "gemm2.cu", "gemm_swap.cu", "gemm_wgrad.cu", "moe_kernels.cu", "route.cu", "combine.cu", "router.cu", "runtime.cu",
-           "no_alloc.cu", "norm.cu"]
+           "no_alloc.cu", "norm.cu", "embedding.cu", "logprobs.cu", "dropout.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 
@@ -99,7 +100,7 @@ def build_torch_module() -> str:
     tmp = path + ".tmp"
     subprocess.check_call(["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
                            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-                           *("-I" + i for i in inc), TORCH_SOURCES[0], "-o", tmp, "-L", LIB_DIR, "-lccfuser_b200", "-Wl,-rpath,$ORIGIN",
+                           *("-I" + i for i in inc), *(f for f in TORCH_SOURCES if f.endswith(".cpp")), "-o", tmp, "-L", LIB_DIR, "-lccfuser_b200", "-Wl,-rpath,$ORIGIN",
                            "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
                            "-ltorch_python"])
     os.replace(tmp, path)

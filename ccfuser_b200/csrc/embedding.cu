@@ -1,0 +1,518 @@
+// Sums of embedding lookups and their dense gradients: y_t = scale * W[id_t] + P[pos_t] + T[type_t], the input of the example models
+// (stock GPT-2 / BERT / Transformer-XL: mix_moe/mix_moe/examples/models/moe_gpt.py, moe_bert.py,
+// transformer-xl/mem_transformer_mix_moe.py).
+//
+// Both directions are bound by bytes. Forward: the used rows in, y out. Backward: dW[v] = scale * sum of dy_t over the tokens with id v, in
+// fp32, rounded once; dy is read once and every row of the gradient written once. The tokens are sorted by (id, place) first, so that a
+// row's sum runs over its tokens in their order: no atomics on values, the same bits every time.
+#include "elements.cuh"
+#include "embedding.h"
+
+namespace ccf {
+
+constexpr int kSortChunk = 2048;     // keys that one block sorts in shared memory
+constexpr int kEmbWarps = 8;
+constexpr int kJoinWarps = 16;
+constexpr uint32_t kNoRow = 0xffffffffu;   // id of a token without a gradient: skipped row, index out of range
+
+// What the 32 lanes of a warp hold of a row: 32 * kE consecutive elements from a column on. kVec: 16 bytes per lane; otherwise (rows off
+// 16-byte boundaries) one element per lane and access.
+template <int kType, bool kVec>
+struct Slice {
+  static constexpr int kE = kElemsPer16<kType>;
+  static constexpr int kCols = 32 * kE;
+  uint4 q;
+  float s[kVec ? 1 : kE];
+
+  static __device__ __forceinline__ int col(int i) { return kVec ? lane_id() * kE + i : lane_id() + 32 * i; }
+  __device__ __forceinline__ void load(const void* p, size_t at, int left, bool on) {
+    if constexpr (kVec) {
+      q = make_uint4(0, 0, 0, 0);
+      if (on && lane_id() * kE < left)
+        q = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p) + at * kElemBytes<kType>) + lane_id());
+    } else {
+#pragma unroll
+      for (int i = 0; i < kE; ++i) s[i] = on && col(i) < left ? load_elem<kType>(p, static_cast<long long>(at) + col(i)) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[kE]) const {
+    if constexpr (kVec) {
+      unpack16<kType>(q, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kE; ++i) f[i] = s[i];
+    }
+  }
+  static __device__ __forceinline__ void store(void* p, size_t at, int left, const float (&f)[kE]) {
+    if constexpr (kVec) {
+      if (lane_id() * kE < left)
+        reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p) + at * kElemBytes<kType>)[lane_id()] = pack16<kType>(f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kE; ++i)
+        if (col(i) < left) store_elem<kType>(p, static_cast<long long>(at) + col(i), f[i]);
+    }
+  }
+  static __device__ __forceinline__ void store_f32(float* p, int left, const float (&f)[kE]) {
+#pragma unroll
+    for (int i = 0; i < kE; ++i)
+      if (col(i) < left) p[col(i)] = f[i];
+  }
+  static __device__ __forceinline__ void add_f32(const float* p, int left, bool on, float (&f)[kE]) {
+#pragma unroll
+    for (int i = 0; i < kE; ++i) f[i] += on && col(i) < left ? p[col(i)] : 0.f;
+  }
+};
+
+// ---- forward -----------------------------------------------------------------------------------------------------------
+constexpr int kFwdSlices = 2;   // slices of a row per warp
+
+template <int kType, bool kVec>
+__global__ void __launch_bounds__(32 * kEmbWarps) embedding_fwd_kernel(const __grid_constant__ CcfEmbed e, void* __restrict__ y, int* status) {
+  using S = Slice<kType, kVec>;
+  const int first = blockIdx.y * kFwdSlices * S::kCols;
+  const uint32_t tokens = static_cast<uint32_t>(e.tokens), seq = static_cast<uint32_t>(e.seq);
+  for (uint32_t t = blockIdx.x * kEmbWarps + (threadIdx.x >> 5); t < tokens; t += gridDim.x * kEmbWarps) {
+    float sum[kFwdSlices][S::kE];
+    S part[CCF_EMBED_TABLES][kFwdSlices];
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < CCF_EMBED_TABLES; ++k) {
+      if (k >= e.tables) break;
+      const CcfEmbedTable& w = e.table[k];
+      const long long id = w.ids != nullptr ? load_index(w.ids, t, w.wide) : static_cast<long long>(t % seq);
+      const bool on = id >= 0 && id < w.rows;
+      bad = bad || !on;
+#pragma unroll
+      for (int j = 0; j < kFwdSlices; ++j) {
+        const int c = first + j * S::kCols;
+        part[k][j].load(w.weight, static_cast<size_t>(on ? id : 0) * w.ld + c, e.d - c, on);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < CCF_EMBED_TABLES; ++k) {
+      if (k >= e.tables) break;
+#pragma unroll
+      for (int j = 0; j < kFwdSlices; ++j) {
+        float f[S::kE];
+        part[k][j].get(f);
+#pragma unroll
+        for (int i = 0; i < S::kE; ++i) sum[j][i] = k == 0 ? f[i] * e.table[0].scale : fmaf(f[i], e.table[k].scale, sum[j][i]);
+      }
+    }
+    if (bad) {
+      if (lane_id() == 0 && blockIdx.y == 0) report_status(status, CCF_ERR_INDEX, static_cast<int>(t) & 0x7fffff);
+#pragma unroll
+      for (int j = 0; j < kFwdSlices; ++j)
+#pragma unroll
+        for (int i = 0; i < S::kE; ++i) sum[j][i] = __int_as_float(0x7fc00000);
+    }
+#pragma unroll
+    for (int j = 0; j < kFwdSlices; ++j) {
+      const int c = first + j * S::kCols;
+      S::store(y, static_cast<size_t>(t) * e.d + c, e.d - c, sum[j]);
+    }
+  }
+}
+
+// ---- backward ----------------------------------------------------------------------------------------------------------
+// Scratch of one table. `keys`: (id << 32 | token), sorted. `present`: a bit per row that some token has. A run of equal ids is cut where
+// a piece of the sorted tokens ends: a piece leaves the sum of a run that came from the piece before in `head`, of one that began in it and goes on in
+// `tail`; `list` holds the pieces that left a tail.
+struct GradTable {
+  const void* ids;
+  void* grad;
+  uint64_t* sorted_chunks;
+  uint64_t* keys;
+  uint32_t* present;
+  float* head;
+  float* tail;
+  int* list;
+  int* count;
+  long long rows;
+  long long skip;
+  float scale;
+  int wide;
+};
+struct GradArgs {
+  GradTable table[CCF_EMBED_TABLES];
+  const void* dy;
+  int* status;
+  uint32_t tokens, seq, batch;
+  uint32_t piece, pieces, chunks, slices;
+  int tables, d;
+};
+
+__device__ __forceinline__ uint32_t id_of(uint64_t key) { return static_cast<uint32_t>(key >> 32); }
+
+// The i-th token in the order of the ids. Positions need no sort: place s of every sequence, in the order of the sequences.
+__device__ __forceinline__ uint64_t key_at(const GradArgs& g, const GradTable& t, uint32_t i) {
+  if (t.ids != nullptr) return t.keys[i];   // not through the read-only path: an earlier launch of this call wrote it
+  const uint32_t s = i / g.batch;
+  return static_cast<uint64_t>(s) << 32 | ((i - s * g.batch) * g.seq + s);
+}
+
+// Each block sorts one chunk of keys (bitonic, in shared memory). One chunk: that is the whole order, and the rows that occur are marked here.
+__global__ void __launch_bounds__(kSortChunk / 2) embedding_sort_kernel(const __grid_constant__ GradArgs g) {
+  __shared__ uint64_t key[kSortChunk];
+  const GradTable& t = g.table[blockIdx.y];
+  let_next_in();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *t.count = 0;
+  if (t.ids == nullptr) return;
+  const uint32_t words = static_cast<uint32_t>((t.rows + 31) / 32);
+  for (uint32_t w = blockIdx.x * blockDim.x + threadIdx.x; w < words; w += gridDim.x * blockDim.x) t.present[w] = 0;
+  const uint32_t base = blockIdx.x * kSortChunk, n = min(g.tokens - base, static_cast<uint32_t>(kSortChunk));
+  uint32_t len = 64;
+  while (len < n) len *= 2;
+  for (uint32_t i = threadIdx.x; i < len; i += blockDim.x) {
+    uint64_t k = ~0ull;
+    if (i < n) {
+      const long long id = load_index(t.ids, base + i, t.wide);
+      const bool in = id >= 0 && id < t.rows;
+      if (!in) report_status(g.status, CCF_ERR_INDEX, static_cast<int>(base + i) & 0x7fffff);
+      k = static_cast<uint64_t>(in && id != t.skip ? static_cast<uint32_t>(id) : kNoRow) << 32 | (base + i);
+    }
+    key[i] = k;
+  }
+  for (uint32_t size = 2; size <= len; size *= 2) {
+    for (uint32_t j = size / 2; j > 0; j /= 2) {
+      __syncthreads();
+      if (threadIdx.x < len / 2) {
+        const uint32_t i = 2 * threadIdx.x - (threadIdx.x & (j - 1));
+        const uint64_t a = key[i], b = key[i + j];
+        if ((a > b) == ((i & size) == 0)) {
+          key[i] = b;
+          key[i + j] = a;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+    t.sorted_chunks[base + i] = key[i];
+    if (g.chunks == 1) {
+      const uint32_t id = id_of(key[i]);
+      if (id != kNoRow && (i == 0 || id_of(key[i - 1]) != id)) atomicOr(t.present + id / 32, 1u << (id % 32));
+    }
+  }
+}
+
+// A key's place among all: its place in its own chunk and, for every other chunk, the keys there that are smaller. Keys differ.
+__global__ void __launch_bounds__(256) embedding_merge_kernel(const __grid_constant__ GradArgs g) {
+  after_previous();
+  const GradTable& t = g.table[blockIdx.y];
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (t.ids == nullptr || i >= g.tokens) return;
+  const uint64_t* src = t.sorted_chunks;
+  const uint64_t k = src[i];
+  const uint32_t own = i / kSortChunk;
+  uint32_t place = i % kSortChunk;
+  for (uint32_t c = 0; c < g.chunks; ++c) {
+    if (c == own) continue;
+    const uint64_t* p = src + c * kSortChunk;
+    uint32_t lo = 0, hi = min(g.tokens - c * kSortChunk, static_cast<uint32_t>(kSortChunk));
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (p[mid] < k) lo = mid + 1;
+      else hi = mid;
+    }
+    place += lo;
+  }
+  t.keys[place] = k;
+  const uint32_t id = id_of(k);
+  if (id != kNoRow && (i % kSortChunk == 0 || id_of(src[i - 1]) != id)) atomicOr(t.present + id / 32, 1u << (id % 32));
+}
+
+// The first blocks of a table sum: a warp takes one piece of the sorted tokens and one slice of the columns. The others write the zeros of
+// the rows that no token has, 32 rows each.
+template <int kType, bool kVec>
+__global__ void __launch_bounds__(32 * kEmbWarps) embedding_sum_kernel(const __grid_constant__ GradArgs g) {
+  using S = Slice<kType, kVec>;
+  constexpr int kUnroll = kVec ? 8 : 2;
+  after_previous();
+  const GradTable& t = g.table[blockIdx.y];
+  const uint32_t warp = threadIdx.x >> 5, units = g.pieces * g.slices, sum_blocks = (units + kEmbWarps - 1) / kEmbWarps;
+  if (blockIdx.x >= sum_blocks) {
+    const uint32_t w = blockIdx.x - sum_blocks;
+    if (w >= (t.rows + 31) / 32) return;
+    uint32_t present = 0;
+    if (t.ids != nullptr) present = t.present[w];
+    else if (w < (g.seq + 31) / 32) present = g.seq - w * 32 >= 32 ? 0xffffffffu : (1u << (g.seq - w * 32)) - 1u;
+    const float zero[S::kE] = {};
+    for (uint32_t r = warp; r < 32; r += kEmbWarps) {
+      const long long row = static_cast<long long>(w) * 32 + r;
+      if ((present >> r & 1) || row >= t.rows) continue;
+      for (int c = 0; c < g.d; c += S::kCols) S::store(t.grad, static_cast<size_t>(row) * g.d + c, g.d - c, zero);
+    }
+    return;
+  }
+  const uint32_t unit = blockIdx.x * kEmbWarps + warp;
+  if (unit >= units) return;
+  const uint32_t piece = unit / g.slices, c = (unit - piece * g.slices) * S::kCols;
+  const int left = g.d - static_cast<int>(c);
+  const uint32_t begin = piece * g.piece, n = min(g.piece, g.tokens - begin);
+  const uint64_t mine = lane_id() < n ? key_at(g, t, begin + lane_id()) : ~0ull;
+  const uint32_t before = begin > 0 ? id_of(key_at(g, t, begin - 1)) : kNoRow;
+  const uint32_t after = begin + n < g.tokens ? id_of(key_at(g, t, begin + n)) : kNoRow;
+  float acc[S::kE] = {};
+  uint32_t run = __shfl_sync(0xffffffffu, id_of(mine), 0);
+  bool from_before = begin > 0 && run == before;
+  auto finish = [&](bool goes_on) {
+    if (run != kNoRow) {
+      if (from_before) {
+        S::store_f32(t.head + static_cast<size_t>(piece) * g.d + c, left, acc);
+      } else if (goes_on) {
+        S::store_f32(t.tail + static_cast<size_t>(piece) * g.d + c, left, acc);
+        if (c == 0 && lane_id() == 0) t.list[atomicAdd(t.count, 1)] = static_cast<int>(piece);
+      } else {
+#pragma unroll
+        for (int i = 0; i < S::kE; ++i) acc[i] *= t.scale;
+        S::store(t.grad, static_cast<size_t>(run) * g.d + c, left, acc);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < S::kE; ++i) acc[i] = 0.f;
+    from_before = false;
+  };
+  for (uint32_t j0 = 0; j0 < n; j0 += kUnroll) {
+    S part[kUnroll];
+    uint32_t id[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const uint64_t k = __shfl_sync(0xffffffffu, mine, (j0 + u) & 31);
+      id[u] = j0 + u < n ? id_of(k) : kNoRow;
+      part[u].load(g.dy, static_cast<size_t>(static_cast<uint32_t>(k)) * g.d + c, left, id[u] != kNoRow);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (j0 + u >= n) break;
+      if (id[u] != run) {
+        finish(false);
+        run = id[u];
+      }
+      float f[S::kE];
+      part[u].get(f);
+#pragma unroll
+      for (int i = 0; i < S::kE; ++i) acc[i] += f[i];
+    }
+  }
+  finish(after == run);
+}
+
+// Runs that cross pieces: tail of the piece where the run began, then the heads of those behind it. kJoinWarps warps take every
+// kJoinWarps-th piece each, and their sums are added in the warps' order.
+template <int kType, bool kVec>
+__global__ void __launch_bounds__(32 * kJoinWarps) embedding_join_kernel(const __grid_constant__ GradArgs g) {
+  using S = Slice<kType, kVec>;
+  constexpr int kUnroll = 4;
+  __shared__ float red[kJoinWarps][S::kCols];
+  after_previous();
+  const GradTable& t = g.table[blockIdx.y];
+  const uint32_t warp = threadIdx.x >> 5, items = static_cast<uint32_t>(*t.count) * g.slices;
+  for (uint32_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const uint32_t piece = static_cast<uint32_t>(t.list[it / g.slices]), c = it % g.slices * S::kCols;
+    const int left = g.d - static_cast<int>(c);
+    const uint32_t run = id_of(key_at(g, t, (piece + 1) * g.piece - 1));
+    float acc[S::kE] = {};
+    bool on = true;
+    for (uint32_t q = piece + 1 + warp; on && q < g.pieces; q += kUnroll * kJoinWarps) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const uint32_t p = q + u * kJoinWarps;
+        on = on && p < g.pieces && id_of(key_at(g, t, p * g.piece)) == run;
+        S::add_f32(t.head + static_cast<size_t>(on ? p : piece) * g.d + c, left, on, acc);
+      }
+    }
+    S::store_f32(red[warp], S::kCols, acc);
+    __syncthreads();
+    for (int j = threadIdx.x; j < S::kCols && j < left; j += 32 * kJoinWarps) {
+      float s = t.tail[static_cast<size_t>(piece) * g.d + c + j];
+#pragma unroll
+      for (int k = 0; k < kJoinWarps; ++k) s += red[k][j];
+      store_elem<kType>(t.grad, static_cast<long long>(static_cast<size_t>(run) * g.d + c + j), s * t.scale);
+    }
+    __syncthreads();
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------
+static uint32_t piece_of(long long tokens, int d) {
+  // long enough that few runs are cut, short enough that the pieces fill the card: 148 SMs with 32 warps
+  const long long slices = (d + 127) / 128;
+  for (uint32_t p = 8; p < 32; p *= 2)
+    if ((tokens + p - 1) / p * slices <= 148 * 32) return p;
+  return 32;
+}
+
+static size_t up16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
+
+// Lays the scratch out; returns its size.
+static size_t lay_out(GradTable* t, void* base, long long tokens, long long rows, int d, bool sorted) {
+  const size_t n = static_cast<size_t>(tokens), piece = piece_of(tokens, d), pieces = (n + piece - 1) / piece;
+  uint8_t* p = static_cast<uint8_t*>(base);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* r = p + at;
+    at += up16(bytes);
+    return r;
+  };
+  GradTable x{};
+  x.count = reinterpret_cast<int*>(take(4));
+  x.list = reinterpret_cast<int*>(take(4 * pieces));
+  x.head = reinterpret_cast<float*>(take(4 * pieces * d));
+  x.tail = reinterpret_cast<float*>(take(4 * pieces * d));
+  if (sorted) {
+    x.present = reinterpret_cast<uint32_t*>(take((static_cast<size_t>(rows) + 31) / 32 * 4));
+    x.sorted_chunks = reinterpret_cast<uint64_t*>(take(8 * n));
+    x.keys = n > kSortChunk ? reinterpret_cast<uint64_t*>(take(8 * n)) : x.sorted_chunks;
+  }
+  if (t != nullptr) {
+    t->count = x.count;
+    t->list = x.list;
+    t->head = x.head;
+    t->tail = x.tail;
+    t->present = x.present;
+    t->sorted_chunks = x.sorted_chunks;
+    t->keys = x.keys;
+  }
+  return at;
+}
+
+static bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static bool valid(const CcfEmbed* e) {
+  if (e == nullptr || e->tables < 1 || e->tables > CCF_EMBED_TABLES || e->type < 0 || e->type > 2 || e->d < 1 || e->tokens < 1 ||
+      e->tokens > 0x7fffffffll || e->seq < 1 || e->tokens % e->seq != 0)
+    return false;
+  for (int k = 0; k < e->tables; ++k) {
+    const CcfEmbedTable& t = e->table[k];
+    if (t.rows < 1 || t.rows > 0x7fffffffll || (t.ids == nullptr && t.rows < e->seq)) return false;
+  }
+  return true;
+}
+
+template <typename... KArgs>
+static cudaError_t launch_behind(void (*kern)(KArgs...), dim3 grid, int threads, cudaStream_t st, KArgs... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr = early_attribute();
+  cfg.attrs = &attr;
+  cfg.numAttrs = early_launches(0, st);
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+template <int kType, bool kVec>
+static int launch_fwd(const CcfEmbed& e, void* y, int* status, cudaStream_t st) {
+  const unsigned slices = (e.d + Slice<kType, kVec>::kCols - 1) / Slice<kType, kVec>::kCols, gy = (slices + kFwdSlices - 1) / kFwdSlices;
+  const long long need = (e.tokens + kEmbWarps - 1) / kEmbWarps, most = 1 + 16ll * sm_count() / gy;
+  embedding_fwd_kernel<kType, kVec><<<dim3(static_cast<unsigned>(need < most ? need : most), gy), 32 * kEmbWarps, 0, st>>>(e, y, status);
+  return launch_result();
+}
+
+template <int kType, bool kVec>
+static int launch_bwd(GradArgs& g, cudaStream_t st) {
+  using S = Slice<kType, kVec>;
+  g.slices = (g.d + S::kCols - 1) / S::kCols;
+  unsigned most = 0;
+  bool sorted = false;
+  for (int k = 0; k < g.tables; ++k) {
+    const unsigned blocks = (g.pieces * g.slices + kEmbWarps - 1) / kEmbWarps + static_cast<unsigned>((g.table[k].rows + 31) / 32);
+    most = blocks > most ? blocks : most;
+    sorted = sorted || g.table[k].ids != nullptr;
+  }
+  int launches = 2;
+  embedding_sort_kernel<<<dim3(sorted ? g.chunks : 1, g.tables), kSortChunk / 2, 0, st>>>(g);
+  cudaError_t err = cudaGetLastError();
+  if (err == cudaSuccess && sorted && g.chunks > 1) {
+    err = launch_behind(embedding_merge_kernel, dim3((g.tokens + 255) / 256, g.tables), 256, st, g);
+    ++launches;
+  }
+  if (err == cudaSuccess) err = launch_behind(embedding_sum_kernel<kType, kVec>, dim3(most, g.tables), 32 * kEmbWarps, st, g);
+  if (err == cudaSuccess && g.pieces > 1) {
+    const unsigned blocks = g.pieces * g.slices, wave = 2 * sm_count();
+    err = launch_behind(embedding_join_kernel<kType, kVec>, dim3(blocks < wave ? blocks : wave, g.tables), 32 * kJoinWarps, st, g);
+    ++launches;
+  }
+  return err == cudaSuccess ? launches : -static_cast<int>(err);
+}
+
+}  // namespace ccf
+
+extern "C" {
+
+int ccf_sizeof_embed() { return static_cast<int>(sizeof(CcfEmbed)); }
+
+// y [tokens, d] = the sum over the tables of scale * weight[id]. An index out of range is recorded in `status` (code 5, the token) and gives a row
+// of NaN. At most 2^31 - 1 tokens and rows; tokens is a multiple of seq.
+int ccf_embedding_fwd(const CcfEmbed* e, void* y, int* status, void* stream) {
+  using namespace ccf;
+  if (!valid(e) || y == nullptr) return -2;
+  const int size = e->type == kFp32 ? 4 : 2;
+  bool vec = e->d * size % 16 == 0 && on16(y);
+  for (int k = 0; k < e->tables; ++k) {
+    if (e->table[k].weight == nullptr || e->table[k].ld < e->d) return -2;
+    vec = vec && on16(e->table[k].weight) && e->table[k].ld * size % 16 == 0;
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (e->type * 2 + vec) {
+    case 0: return launch_fwd<kBf16, false>(*e, y, status, st);
+    case 1: return launch_fwd<kBf16, true>(*e, y, status, st);
+    case 2: return launch_fwd<kFp16, false>(*e, y, status, st);
+    case 3: return launch_fwd<kFp16, true>(*e, y, status, st);
+    case 4: return launch_fwd<kFp32, false>(*e, y, status, st);
+    default: return launch_fwd<kFp32, true>(*e, y, status, st);
+  }
+}
+
+// Bytes of scratch that a table needs in ccf_embedding_bwd; sorted: it has ids. 0: a size out of range.
+long long ccf_embedding_scratch(long long tokens, long long rows, int d, int sorted) {
+  if (tokens < 1 || tokens > 0x7fffffffll || rows < 1 || rows > 0x7fffffffll || d < 1) return 0;
+  return static_cast<long long>(ccf::lay_out(nullptr, nullptr, tokens, rows, d, sorted != 0));
+}
+
+// grad [rows, d] of every table from dy [tokens, d]: all rows are written, those that no token has with zeros. `scratch` of each table on a
+// 16-byte boundary. A token whose index is out of range adds nothing and is recorded in `status`. Returns the number of its launches, or a negative
+// code.
+int ccf_embedding_bwd(const CcfEmbed* e, const void* dy, int* status, void* stream) {
+  using namespace ccf;
+  if (!valid(e) || dy == nullptr) return -2;
+  const int size = e->type == kFp32 ? 4 : 2;
+  GradArgs g{};
+  bool vec = e->d * size % 16 == 0 && on16(dy);
+  g.dy = dy;
+  g.status = status;
+  g.tokens = static_cast<uint32_t>(e->tokens);
+  g.seq = static_cast<uint32_t>(e->seq);
+  g.batch = g.tokens / g.seq;
+  g.piece = piece_of(e->tokens, e->d);
+  g.pieces = (g.tokens + g.piece - 1) / g.piece;
+  g.chunks = (g.tokens + kSortChunk - 1) / kSortChunk;
+  g.tables = e->tables;
+  g.d = e->d;
+  for (int k = 0; k < e->tables; ++k) {
+    const CcfEmbedTable& t = e->table[k];
+    if (t.grad == nullptr || t.scratch == nullptr || !on16(t.scratch)) return -2;
+    vec = vec && on16(t.grad);
+    GradTable& o = g.table[k];
+    lay_out(&o, t.scratch, e->tokens, t.rows, e->d, t.ids != nullptr);
+    o.ids = t.ids;
+    o.grad = t.grad;
+    o.rows = t.rows;
+    o.skip = t.skip;
+    o.scale = t.scale;
+    o.wide = t.wide;
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (e->type * 2 + vec) {
+    case 0: return launch_bwd<kBf16, false>(g, st);
+    case 1: return launch_bwd<kBf16, true>(g, st);
+    case 2: return launch_bwd<kFp16, false>(g, st);
+    case 3: return launch_bwd<kFp16, true>(g, st);
+    case 4: return launch_bwd<kFp32, false>(g, st);
+    default: return launch_bwd<kFp32, true>(g, st);
+  }
+}
+
+}  // extern "C"

@@ -25,7 +25,8 @@ enum CcfStatus {
   CCF_ERR_MBAR_TIMEOUT = 1,   // a pipeline barrier inside one CTA never completed
   CCF_ERR_FLAG_TIMEOUT = 2,   // a peer's arrival flag / counter never reached its target
   CCF_ERR_BOUNDS = 3,         // an index failed a debug bounds check; the access was skipped
-  CCF_ERR_OVERFLOW = 4        // more rows routed to a rank than its receive buffer holds
+  CCF_ERR_OVERFLOW = 4,       // more rows routed to a rank than its receive buffer holds
+  CCF_ERR_INDEX = 5           // a token or target id outside its table; detail: the token
 };
 
 // Rows pushed by the dispatch role. All peer_* pointers are addresses in *this* process' address space

@@ -1,0 +1,540 @@
+// Log probabilities of given tokens, with the entropy and the best alternatives of every row of logits, and their gradient: the loss of the
+// example models (mix_moe/mix_moe/examples/models/moe_gpt.py and transformer-xl/mem_transformer_mix_moe.py take torch's cross-entropy) and the scores
+// of a sampled or a given text.
+//
+// With z = x / T over the first `vocab` columns, M the largest x, u_j = (x_j - M) / (T ln 2), S = sum 2^u_j, Q = sum 2^u_j u_j:
+//   lp_j = (x_j - M) / T - ln S        H = ln S - ln 2 * Q / S        (both terms of H are >= 0: nothing cancels)
+//   dx_j = 1/T * ( g [j = t] + sum_k g_k [j = top_k] - p_j (g + sum_k g_k + g_H (lp_j + H)) ),   p_j = 2^u_j / S
+// One pass over the logits with running M, S and Q forward; one pass that reads them and writes the gradient backward. Both are bound by those
+// bytes; next to them stand one exponential and about five more instructions an element. Statistics in fp32.
+#include <cooperative_groups.h>
+
+#include "elements.cuh"
+#include "logprobs.h"
+
+namespace ccf {
+
+constexpr int kUnroll = 4;                 // 16-byte pieces that a thread has in flight
+constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
+constexpr float kFloorU = -1000.f;         // 2^kFloorU is 0, and 0 * kFloorU is 0 where 0 * -inf would be NaN
+constexpr uint32_t kNanOrder = 0xfffffffeu;
+
+__device__ __forceinline__ float exp2_fast(float u) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(u));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+
+// A whole number in the order of the floats; NaN above all, as in torch.topk; -0 is 0.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  if (v != v) return kNanOrder;
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t order) {
+  return order == kNanOrder ? __int_as_float(0x7fc00000) : __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+// Larger value first, then lower index; 0 is no element.
+__device__ __forceinline__ uint64_t top_key(float v, uint32_t index) { return static_cast<uint64_t>(order_of(v)) << 32 | (0xffffffffu - index); }
+
+template <int kType>
+constexpr uint32_t kNegInf2 = kType == kBf16 ? 0xff80ff80u : kType == kFp16 ? 0xfc00fc00u : 0xff800000u;
+
+// largest of the elements of kUnroll pieces; NaN if one is
+template <int kType>
+__device__ __forceinline__ float max_of(const uint4 (&q)[kUnroll]) {
+  if constexpr (kType == kFp32) {
+    float m = neg_inf();
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k)
+      m = max_nan(m, max_nan(max_nan(__uint_as_float(q[k].x), __uint_as_float(q[k].y)), max_nan(__uint_as_float(q[k].z), __uint_as_float(q[k].w))));
+    return m;
+  } else {
+    using H2 = typename std::conditional<kType == kFp16, __half2, __nv_bfloat162>::type;
+    auto as = [](uint32_t w) { return *reinterpret_cast<H2*>(&w); };
+    H2 m = as(kNegInf2<kType>);
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(as(q[k].x), as(q[k].y)), __hmax2_nan(as(q[k].z), as(q[k].w))));
+    const float2 f = unpack2(*reinterpret_cast<uint32_t*>(&m), kType == kFp16);
+    return max_nan(f.x, f.y);
+  }
+}
+
+// How the elements of a row lie: up to a 16-byte boundary single ones, then whole pieces, then single ones again.
+template <int kType>
+struct RowShape {
+  static constexpr int kE = kElemsPer16<kType>;
+  int head, pieces, tail;
+  __device__ __forceinline__ RowShape(const uint8_t* p, int n) {
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) / kElemBytes<kType>;
+    head = min((kE - off) % kE, n);
+    pieces = (n - head) / kE;
+    tail = n - head - pieces * kE;
+  }
+};
+
+// running statistics of one thread
+struct Running {
+  float m = neg_inf();
+  f32x2 s = 0, q = 0;
+  __device__ __forceinline__ void raise(float to, float c) {   // before elements up to `to`
+    if (to <= m) return;
+    const float next = max_nan(m, to), d = fmaxf((m - next) * c, kFloorU), f = exp2_fast(d);
+    q = mul2(fma2(s, bc2(d), q), bc2(f));
+    s = mul2(s, bc2(f));
+    m = next;
+  }
+  __device__ __forceinline__ void add2x(float a, float b, float c) {
+    float u0, u1;
+    upk2(mul2(add2(pk2(a, b), bc2(-m)), bc2(c)), u0, u1);
+    u0 = fmaxf(u0, kFloorU);
+    u1 = fmaxf(u1, kFloorU);
+    const f32x2 e = pk2(exp2_fast(u0), exp2_fast(u1));
+    s = add2(s, e);
+    q = fma2(e, pk2(u0, u1), q);
+  }
+};
+
+struct RowStats {
+  float m, s, q;
+};
+__device__ __forceinline__ void rescale(RowStats& a, float m, float c) {
+  const float d = fmaxf((a.m - m) * c, kFloorU), f = exp2_fast(d);
+  a.q = fmaf(a.s, d, a.q) * f;
+  a.s *= f;
+  a.m = m;
+}
+template <int kLanes>
+__device__ __forceinline__ void reduce_lanes(RowStats& a, float c) {
+  float m = a.m;
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  rescale(a, m, c);
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o /= 2) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.q += __shfl_xor_sync(0xffffffffu, a.q, o);
+  }
+}
+
+template <int kThreads>
+constexpr int kListLen = kThreads == 32 ? 256 : 1024;
+
+template <int kThreads>
+struct RowShared {
+  RowStats part[kThreads / 32];
+  RowStats all;
+  uint64_t top[CCF_LOGPROBS_MAX_TOP];
+  uint64_t best[kThreads / 32];
+  uint64_t list[kListLen<kThreads>];
+  int listed;
+};
+struct RowSharedPlain {   // without alternatives
+  RowStats part[16];
+  RowStats all;
+};
+
+template <int kThreads>
+__device__ __forceinline__ void row_sync() {
+  if constexpr (kThreads == 32) __syncwarp();
+  else __syncthreads();
+}
+template <int kThreads>
+__device__ __forceinline__ int row_count(bool on) {
+  if constexpr (kThreads == 32) return __popc(__ballot_sync(0xffffffffu, on));
+  else return __syncthreads_count(on);
+}
+
+// The k largest elements of this block's share of a row, in order, into sh.top. `m`: the largest of the thread's own elements. The k-th largest of the
+// threads' maxima bounds the k-th largest element from below, so only threads whose maximum reaches it look at their elements again (k of them,
+// but for ties), and only elements that reach it are candidates: a few more than k. The bound is found on 16 bits, by halving. Should the
+// candidates not fit the list (many equal elements), the elements are taken one after the other instead, each the largest below the one before.
+template <int kType, int kThreads>
+__device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_t* p, const RowShape<kType>& shape, int first, int last, float m, float edge,
+                                           int edge_index, int k) {
+  constexpr int kE = kElemsPer16<kType>;
+  const int tid = kThreads == 32 ? lane_id() : threadIdx.x, lane = lane_id();
+  const uint4* pieces = reinterpret_cast<const uint4*>(p + shape.head * kElemBytes<kType>);
+  const uint32_t mine = m == neg_inf() ? 0u : order_of(m) >> 16;
+  if (tid == 0) sh.listed = 0;
+  if (tid < CCF_LOGPROBS_MAX_TOP) sh.top[tid] = 0;
+  uint32_t bound = 0;
+#pragma unroll 1
+  for (int b = 15; b >= 0; --b)
+    if (row_count<kThreads>(mine >= (bound | 1u << b)) >= k) bound |= 1u << b;
+  bound = bound > 0 ? bound : 1u;
+  row_sync<kThreads>();
+  auto consider = [&](float v, int index) {
+    if (v == neg_inf() || order_of(v) >> 16 < bound) return;
+    const int at = atomicAdd(&sh.listed, 1);
+    if (at < kListLen<kThreads>) sh.list[at] = top_key(v, index);
+  };
+  uint32_t owners = __ballot_sync(0xffffffffu, mine >= bound);
+  while (owners != 0) {
+    const int owner = __ffs(owners) - 1;
+    owners &= owners - 1;
+    for (int v = first + tid - lane + owner + lane * kThreads; v < last; v += 32 * kThreads) {
+      float f[kE];
+      unpack16<kType>(__ldg(pieces + v), f);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) consider(f[i], shape.head + v * kE + i);
+    }
+  }
+  if (edge_index >= 0) consider(edge, edge_index);
+  row_sync<kThreads>();
+  const int n = sh.listed;
+  if (n <= kListLen<kThreads>) {
+    for (int i = tid; i < n; i += kThreads) {
+      const uint64_t key = sh.list[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += sh.list[j] > key;
+      if (rank < k) sh.top[rank] = key;
+    }
+    row_sync<kThreads>();
+    return;
+  }
+  uint64_t below = ~0ull;
+  for (int r = 0; r < k; ++r) {
+    uint64_t best = 0;
+    auto look = [&](float v, int index) {
+      const uint64_t key = v == neg_inf() ? 0 : top_key(v, index);
+      if (key < below && key > best) best = key;
+    };
+    for (int v = first + tid; v < last; v += kThreads) {
+      float f[kE];
+      unpack16<kType>(__ldg(pieces + v), f);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) look(f[i], shape.head + v * kE + i);
+    }
+    if (edge_index >= 0) look(edge, edge_index);
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) {
+      const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
+      best = other > best ? other : best;
+    }
+    if constexpr (kThreads > 32) {
+      if (lane == 0) sh.best[threadIdx.x >> 5] = best;
+      __syncthreads();
+#pragma unroll 1
+      for (int w = 0; w < kThreads / 32; ++w) best = sh.best[w] > best ? sh.best[w] : best;
+      __syncthreads();
+    }
+    if (tid == 0) sh.top[r] = best;
+    if (best == 0) break;
+    below = best;
+  }
+  row_sync<kThreads>();
+}
+
+// kThreads per row; a warp per row, eight rows a block, where rows are short. Rows of wide vocabularies may be shared by a cluster of `split` blocks,
+// each with its part of the columns, whose statistics and alternatives the first one joins: a few rows would leave most of the card idle.
+template <int kType, int kThreads, bool kTop>
+__global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_kernel(const __grid_constant__ CcfLogprobs a, int split) {
+  namespace cg = cooperative_groups;
+  constexpr int kE = kElemsPer16<kType>, kRows = kThreads == 32 ? 8 : 1;
+  using Shared = typename std::conditional<kTop, RowShared<kThreads>, RowSharedPlain>::type;
+  __shared__ Shared shared[kRows];
+  const int warp = threadIdx.x >> 5, lane = lane_id(), tid = kThreads == 32 ? lane : threadIdx.x;
+  const int rank = static_cast<int>(blockIdx.x % static_cast<unsigned>(split));
+  const long long row = kThreads == 32 ? blockIdx.x * 8ll + warp : static_cast<long long>(blockIdx.x / static_cast<unsigned>(split));
+  if (kThreads == 32 && row >= a.rows) return;
+  Shared& sh = shared[kThreads == 32 ? warp : 0];
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(a.x) + static_cast<size_t>(row) * a.ld * kElemBytes<kType>;
+  const RowShape<kType> shape(p, a.vocab);
+  const int first = static_cast<int>(static_cast<long long>(shape.pieces) * rank / split);
+  const int last = static_cast<int>(static_cast<long long>(shape.pieces) * (rank + 1) / split);
+  const uint4* pieces = reinterpret_cast<const uint4*>(p + shape.head * kElemBytes<kType>);
+  const float c = a.inv_t * kLog2e;
+  long long target = 0;
+  float logit = 0.f;
+  if (rank == 0 && tid == 0) {
+    target = load_index(a.targets, row, a.wide);
+    if (target >= 0 && target < a.vocab) logit = load_elem<kType>(p, target);
+  }
+  // single elements in front of and behind the whole pieces: one for each of the first threads
+  int edge_index = -1;
+  if (rank == 0 && tid < shape.head) edge_index = tid;
+  if (rank == split - 1 && tid >= shape.head && tid < shape.head + shape.tail) edge_index = tid + shape.pieces * kE;
+  const float edge = edge_index >= 0 ? load_elem<kType>(p, edge_index) : neg_inf();
+  Running run;
+  for (int v = first + tid; v < last; v += kUnroll * kThreads) {
+    uint4 q[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      q[u] = make_uint4(kNegInf2<kType>, kNegInf2<kType>, kNegInf2<kType>, kNegInf2<kType>);
+      if (v + u * kThreads < last) q[u] = load16_once(pieces + v + u * kThreads);
+    }
+    run.raise(max_of<kType>(q), c);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float f[kE];
+      unpack16<kType>(q[u], f);
+#pragma unroll
+      for (int i = 0; i < kE; i += 2) run.add2x(f[i], f[i + 1], c);
+    }
+  }
+  run.raise(edge, c);
+  run.add2x(edge, neg_inf(), c);
+  RowStats st{run.m, 0.f, 0.f};
+  {
+    float x, y;
+    upk2(run.s, x, y);
+    st.s = x + y;
+    upk2(run.q, x, y);
+    st.q = x + y;
+  }
+  reduce_lanes<32>(st, c);
+  if constexpr (kThreads > 32) {
+    constexpr int kWarps = kThreads / 32;
+    if (lane == 0) sh.part[warp] = st;
+    __syncthreads();
+    st = sh.part[lane % kWarps];
+    reduce_lanes<kWarps>(st, c);
+  }
+  if constexpr (kTop) select_top<kType, kThreads>(sh, p, shape, first, last, run.m, edge, edge_index, a.top_k);
+  if constexpr (kThreads > 32) {
+    if (split > 1) {
+      cg::cluster_group cluster = cg::this_cluster();
+      if (tid == 0) sh.all = st;
+      cluster.sync();
+      if (rank == 0) {
+        st = RowStats{neg_inf(), 0.f, 0.f};
+        if (lane < split) st = *cluster.map_shared_rank(&sh.all, lane);
+        reduce_lanes<32>(st, c);
+        if constexpr (kTop) {
+          const int n = split * a.top_k;
+          for (int i = tid; i < n; i += kThreads) sh.list[i] = cluster.map_shared_rank(sh.top, i / a.top_k)[i % a.top_k];
+          __syncthreads();
+          if (tid < CCF_LOGPROBS_MAX_TOP) sh.top[tid] = 0;
+          __syncthreads();
+          for (int i = tid; i < n; i += kThreads) {
+            const uint64_t key = sh.list[i];
+            int r = 0;
+            for (int j = 0; j < n; ++j) r += sh.list[j] > key;
+            if (key != 0 && r < a.top_k) sh.top[r] = key;
+          }
+          __syncthreads();
+        }
+      }
+      cluster.sync();   // nobody leaves while its shared memory is read
+      if (rank != 0) return;
+    }
+  }
+  const float log_s = logf(st.s);
+  const bool none = st.m == neg_inf(), bad = !(st.m < __int_as_float(0x7f800000));
+  const float nan = __int_as_float(0x7fc00000);
+  if (tid == 0) {
+    const float h = bad ? nan : none ? 0.f : fmaf(-kLn2, st.q / st.s, log_s);
+    float lp = bad ? nan : none ? neg_inf() : (logit - st.m) * a.inv_t - log_s;
+    if (target == a.ignore) {
+      lp = 0.f;
+    } else if (target < 0 || target >= a.vocab) {
+      report_status(a.status, CCF_ERR_INDEX, static_cast<int>(row) & 0x7fffff);
+      lp = nan;
+    }
+    a.logprobs[row] = lp;
+    a.entropy[row] = h;
+    if (a.stats != nullptr) {
+      a.stats[row * 3] = st.m;
+      a.stats[row * 3 + 1] = st.s;
+      a.stats[row * 3 + 2] = h;
+    }
+  }
+  if constexpr (kTop) {
+    if (tid < a.top_k) {
+      const uint64_t key = sh.top[tid];
+      const float v = value_of(static_cast<uint32_t>(key >> 32));
+      a.top_ids[row * a.top_k + tid] = key != 0 ? static_cast<long long>(0xffffffffu - static_cast<uint32_t>(key)) : -1ll;
+      a.top_logprobs[row * a.top_k + tid] = key == 0 ? neg_inf() : bad ? nan : (v - st.m) * a.inv_t - log_s;
+    }
+  }
+}
+
+// The coefficients of a row: dx_j = hot_j - 2^u_j (w0 + w1 u_j).
+struct RowGrad {
+  float m, w0, w1, g;
+  bool zero;
+};
+template <int kType>
+__device__ __forceinline__ RowGrad row_grad(const CcfLogprobs& a, long long row, long long target) {
+  RowGrad r;
+  const float s = a.stats[row * 3 + 1], h = a.stats[row * 3 + 2];
+  r.m = a.stats[row * 3];
+  r.g = a.d_logprobs != nullptr && target != a.ignore && target >= 0 && target < a.vocab ? a.d_logprobs[row] : 0.f;
+  const float gh = a.d_entropy != nullptr ? a.d_entropy[row] : 0.f;
+  float all = r.g;
+  bool any = r.g != 0.f || gh != 0.f;
+  if (a.d_top != nullptr) {
+    for (int k = 0; k < a.top_k; ++k) {
+      if (a.top_ids[row * a.top_k + k] < 0) continue;
+      const float gk = a.d_top[row * a.top_k + k];
+      all += gk;
+      any = any || gk != 0.f;
+    }
+  }
+  r.zero = !any || r.m == neg_inf();
+  const float scale = a.inv_t / s;
+  r.w0 = scale * fmaf(gh, h - logf(s), all);
+  r.w1 = scale * gh * kLn2;
+  if (!(r.m < __int_as_float(0x7f800000))) r.w0 = __int_as_float(0x7fc00000);
+  return r;
+}
+
+// kThreads per row and part of its columns (blockIdx.y of gridDim.y), a warp per row where rows are short.
+template <int kType, int kThreads>
+__global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_bwd_kernel(const __grid_constant__ CcfLogprobs a) {
+  constexpr int kE = kElemsPer16<kType>;
+  const int warp = threadIdx.x >> 5, tid = kThreads == 32 ? lane_id() : threadIdx.x;
+  const long long row = kThreads == 32 ? blockIdx.x * 8ll + warp : static_cast<long long>(blockIdx.x);
+  if (kThreads == 32 && row >= a.rows) return;
+  const int split = static_cast<int>(gridDim.y), rank = static_cast<int>(blockIdx.y);
+  const size_t at = static_cast<size_t>(row) * a.ld * kElemBytes<kType>;
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(a.x) + at;
+  uint8_t* o = reinterpret_cast<uint8_t*>(a.dx) + at;
+  const RowShape<kType> shape(p, a.width);
+  const int first = static_cast<int>(static_cast<long long>(shape.pieces) * rank / split);
+  const int last = static_cast<int>(static_cast<long long>(shape.pieces) * (rank + 1) / split);
+  const uint4* pieces = reinterpret_cast<const uint4*>(p + shape.head * kElemBytes<kType>);
+  uint4* out = reinterpret_cast<uint4*>(o + shape.head * kElemBytes<kType>);
+  const long long target = load_index(a.targets, row, a.wide);
+  const RowGrad r = row_grad<kType>(a, row, target);
+  const float c = a.inv_t * kLog2e;
+  int edge_index = -1;
+  if (rank == 0 && tid < shape.head) edge_index = tid;
+  if (rank == split - 1 && tid >= shape.head && tid < shape.head + shape.tail) edge_index = tid + shape.pieces * kE;
+  if (r.zero) {
+    for (int v = first + tid; v < last; v += kThreads) out[v] = make_uint4(0, 0, 0, 0);
+    if (edge_index >= 0) store_elem<kType>(o, edge_index, 0.f);
+    return;
+  }
+  auto grad = [&](float x) {
+    const float u = fmaxf((x - r.m) * c, kFloorU);
+    return -exp2_fast(u) * fmaf(r.w1, u, r.w0);
+  };
+  const int full = (a.vocab - shape.head) / kE;   // pieces that lie in the vocabulary as a whole (may be negative: none)
+  for (int v0 = first + tid; v0 < last; v0 += kUnroll * kThreads) {
+    uint4 q[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      const int v = v0 + k * kThreads;
+      q[k] = make_uint4(0, 0, 0, 0);
+      if (v < last && shape.head + v * kE < a.vocab) q[k] = load16_once(pieces + v);
+    }
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      const int v = v0 + k * kThreads;
+      if (v >= last) break;
+      float f[kE];
+      unpack16<kType>(q[k], f);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) f[i] = grad(f[i]);
+      if (v >= full) {
+#pragma unroll
+        for (int i = 0; i < kE; ++i)
+          if (shape.head + v * kE + i >= a.vocab) f[i] = 0.f;
+      }
+      out[v] = pack16<kType>(f);
+    }
+  }
+  if (edge_index >= 0) store_elem<kType>(o, edge_index, edge_index < a.vocab ? grad(load_elem<kType>(p, edge_index)) : 0.f);
+  // the target's and the alternatives' own terms, by rewriting those elements
+  row_sync<kThreads>();
+  const int begin = rank == 0 ? 0 : shape.head + first * kE, end = rank == split - 1 ? a.width : shape.head + last * kE;
+  const int tops = a.d_top != nullptr ? a.top_k : 0;
+  for (int i = tid; i <= tops; i += kThreads) {
+    const long long j = i == 0 ? target : a.top_ids[row * a.top_k + i - 1];
+    if (j < begin || j >= end || j >= a.vocab) continue;
+    float g = i == 0 ? r.g : a.d_top[row * a.top_k + i - 1];
+    bool twice = false;   // the target is an alternative as well: that one writes for both
+    if (i == 0)
+      for (int k = 0; k < tops; ++k) twice = twice || a.top_ids[row * a.top_k + k] == target;
+    else if (j == target)
+      g += r.g;
+    if (!twice) store_elem<kType>(o, j, fmaf(a.inv_t, g, grad(load_elem<kType>(p, j))));
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------
+static bool valid(const CcfLogprobs* a) {
+  return a != nullptr && a->x != nullptr && a->targets != nullptr && a->rows >= 1 && a->rows <= 0x0fffffffll && a->vocab >= 1 && a->vocab <= (1 << 30) &&
+         a->width >= a->vocab && a->width <= (1 << 30) && (a->ld >= a->width || a->rows == 1) && a->top_k >= 0 && a->top_k <= CCF_LOGPROBS_MAX_TOP &&
+         a->top_k <= a->vocab && a->type >= 0 && a->type <= 2 && (reinterpret_cast<uintptr_t>(a->x) & 15) == 0 && a->inv_t > 0.f;
+}
+
+template <int kType, int kThreads, bool kTop>
+static int launch_fwd(const CcfLogprobs& a, int split, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kThreads == 32 ? static_cast<unsigned>((a.rows + 7) / 8) : static_cast<unsigned>(a.rows * split));
+  cfg.blockDim = dim3(kThreads == 32 ? 256 : kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(split);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<kType, kThreads, kTop>, a, split);
+  return e == cudaSuccess ? 0 : -static_cast<int>(e);
+}
+
+template <int kType, bool kTop>
+static int choose_fwd(const CcfLogprobs& a, cudaStream_t st) {
+  if (a.vocab <= 1024) return launch_fwd<kType, 32, kTop>(a, 1, st);
+  if (a.vocab <= 8192) return launch_fwd<kType, 128, kTop>(a, 1, st);
+  int split = 1;
+  while (split < 8 && a.rows * split < 2 * sm_count()) split *= 2;
+  return launch_fwd<kType, 512, kTop>(a, split, st);
+}
+
+template <int kType>
+static int choose_bwd(const CcfLogprobs& a, cudaStream_t st) {
+  const unsigned rows = static_cast<unsigned>(a.rows);
+  if (a.width <= 1024) {
+    logprobs_bwd_kernel<kType, 32><<<(rows + 7) / 8, 256, 0, st>>>(a);
+  } else {
+    int split = 1;
+    const int pieces = a.width / kElemsPer16<kType>;
+    while (split < 64 && a.rows * split < 8 * sm_count() && pieces / split > 256 * kUnroll) split *= 2;
+    logprobs_bwd_kernel<kType, 256><<<dim3(rows, split), 256, 0, st>>>(a);
+  }
+  return launch_result();
+}
+
+}  // namespace ccf
+
+extern "C" {
+
+int ccf_sizeof_logprobs() { return static_cast<int>(sizeof(CcfLogprobs)); }
+
+// logprobs, entropy [rows] and, for top_k > 0, top_logprobs and top_ids [rows, top_k]. A row without a finite logit: log probability -inf, entropy 0.
+// A row with NaN or +inf: NaN. An ignored target: 0. A target outside the vocabulary: NaN, and recorded in `status` (code 5, the row).
+// Alternatives: by value, equal ones by index; where no logit above -inf is left: id -1, -inf. x on a 16-byte boundary; its rows may begin anywhere.
+int ccf_logprobs_fwd(const CcfLogprobs* a, void* stream) {
+  using namespace ccf;
+  if (!valid(a) || a->logprobs == nullptr || a->entropy == nullptr || (a->top_k > 0 && (a->top_ids == nullptr || a->top_logprobs == nullptr))) return -2;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const bool top = a->top_k > 0;
+  if (a->type == kBf16) return top ? choose_fwd<kBf16, true>(*a, st) : choose_fwd<kBf16, false>(*a, st);
+  if (a->type == kFp16) return top ? choose_fwd<kFp16, true>(*a, st) : choose_fwd<kFp16, false>(*a, st);
+  return top ? choose_fwd<kFp32, true>(*a, st) : choose_fwd<kFp32, false>(*a, st);
+}
+
+// dx [rows, width] in the layout of x from the gradients of the outputs that are given: zeros behind the vocabulary and in rows without a gradient.
+int ccf_logprobs_bwd(const CcfLogprobs* a, void* stream) {
+  using namespace ccf;
+  if (!valid(a) || a->dx == nullptr || (reinterpret_cast<uintptr_t>(a->dx) & 15) != 0 || a->stats == nullptr ||
+      (a->d_top != nullptr && (a->top_k == 0 || a->top_ids == nullptr)))
+    return -2;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (a->type == kBf16) return choose_bwd<kBf16>(*a, st);
+  if (a->type == kFp16) return choose_bwd<kFp16>(*a, st);
+  return choose_bwd<kFp32>(*a, st);
+}
+
+}  // extern "C"

@@ -8,25 +8,20 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
-#include <atomic>
 #include <optional>
 
 #include "norm.h"
+#include "torch_ops.h"
 
 namespace {
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-std::atomic<long long> g_launches{0};
+using ccf_torch::check;
+using ccf_torch::g_launches;
+using ccf_torch::packed;
 
-void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", rc); }
-
-// as the kernels read it: contiguous and on a 16-byte boundary (a view may begin anywhere)
-at::Tensor packed(const at::Tensor& t) {
-  const at::Tensor c = t.contiguous();
-  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
-}
 at::Tensor rows_of(const at::Tensor& t, int64_t rows, int64_t d) { return packed(t.reshape({rows, d})); }
 
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
@@ -81,5 +76,6 @@ PYBIND11_MODULE(_ccf_torch, m) {
       [](const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias, const at::Tensor& status, double eps,
          int64_t wait_ns) { return LayerNormFn::apply(x, weight, bias, status, eps, wait_ns); },
       py::call_guard<py::gil_scoped_release>());
+  ccf_torch::add_token_ops(m);
   m.def("launches", [] { return g_launches.load(); });
 }

@@ -1,0 +1,289 @@
+// The autograd functions around embedding.cu, logprobs.cu and dropout.cu. ops/embedding.py, ops/logprobs.py and ops/dropout.py check the
+// arguments, and hold the same functions in Python for where this module is missing or a graph is being traced.
+#include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <optional>
+
+#include "dropout.h"
+#include "embedding.h"
+#include "logprobs.h"
+#include "torch_ops.h"
+
+namespace {
+
+using ccf_torch::check;
+using ccf_torch::g_launches;
+using ccf_torch::packed;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<at::Tensor>;
+
+int type_code(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? 0 : t.scalar_type() == at::kHalf ? 1 : 2; }
+void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "ccfuser_b200: this operator's gradient cannot be differentiated again (create_graph=True)"); }
+
+// ---- embedding ---------------------------------------------------------------------------------------------------------
+// A table as the kernels read it: rows with any distance, their elements next to each other.
+at::Tensor table_of(const at::Tensor& w) { return w.stride(1) == 1 && w.stride(0) >= w.size(1) ? w : w.contiguous(); }
+
+void add_table(CcfEmbed& e, const at::Tensor& ids, int64_t rows, double scale, int64_t skip) {
+  CcfEmbedTable& t = e.table[e.tables++];
+  t.rows = rows;
+  t.scale = static_cast<float>(scale);
+  t.skip = skip;
+  if (ids.defined()) {
+    t.ids = ids.data_ptr();
+    t.wide = ids.scalar_type() == at::kLong;
+  }
+}
+
+// One gradient launch for up to three tables: grads[k] [rows, d] from dy [tokens, d].
+void run_grad(CcfEmbed& e, const at::Tensor& dy, const std::vector<at::Tensor>& grads, const at::Tensor& status) {
+  std::vector<at::Tensor> scratch;
+  bool sorted = false;
+  for (int k = 0; k < e.tables; ++k) {
+    sorted = sorted || e.table[k].ids != nullptr;
+    scratch.push_back(at::empty({ccf_embedding_scratch(e.tokens, e.table[k].rows, e.d, e.table[k].ids != nullptr)}, dy.options().dtype(at::kByte)));
+    e.table[k].scratch = scratch.back().data_ptr();
+    e.table[k].grad = grads[k].data_ptr();
+  }
+  const int launches = ccf_embedding_bwd(&e, dy.data_ptr(), status.data_ptr<int>(), stream());
+  TORCH_CHECK(launches > 0, "ccf_embedding_bwd failed with code ", launches);
+  g_launches += launches;
+}
+
+struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& ids, const at::Tensor& weight, const OptTensor& position,
+                            const OptTensor& position_ids, const OptTensor& type, const OptTensor& type_ids, double scale, int64_t skip,
+                            const at::Tensor& status) {
+    const c10::cuda::CUDAGuard guard(weight.device());
+    const at::Tensor tables[3] = {table_of(weight), position.has_value() ? table_of(*position) : at::Tensor(),
+                                  type.has_value() ? table_of(*type) : at::Tensor()};
+    const at::Tensor index[3] = {ids.contiguous(), position_ids.has_value() ? position_ids->contiguous() : at::Tensor(),
+                                 type_ids.has_value() ? type_ids->contiguous() : at::Tensor()};
+    CcfEmbed e{};
+    e.tokens = ids.numel();
+    e.seq = ids.dim() > 0 ? ids.size(-1) : 1;
+    e.d = static_cast<int>(weight.size(1));
+    e.type = type_code(weight);
+    for (int k = 0; k < 3; ++k) {
+      if (!tables[k].defined()) continue;
+      add_table(e, index[k], tables[k].size(0), k == 0 ? scale : 1.0, k == 0 ? skip : -1);
+      e.table[e.tables - 1].weight = tables[k].data_ptr();
+      e.table[e.tables - 1].ld = tables[k].size(0) > 1 ? tables[k].stride(0) : e.d;
+    }
+    auto shape = ids.sizes().vec();
+    shape.push_back(e.d);
+    const at::Tensor y = at::empty(shape, weight.options());
+    check(ccf_embedding_fwd(&e, y.data_ptr(), status.data_ptr<int>(), stream()), "ccf_embedding_fwd");
+    ++g_launches;
+    ctx->save_for_backward({index[0], index[1], index[2]});
+    ctx->saved_data["rows"] = std::vector<int64_t>{weight.size(0), position.has_value() ? position->size(0) : 0, type.has_value() ? type->size(0) : 0};
+    // autograd counts the tensors that are there: ids, weight, position, its ids, type
+    ctx->saved_data["edges"] = std::vector<int64_t>{1, 2, 2 + position.has_value() + position_ids.has_value()};
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["skip"] = skip;
+    ctx->saved_data["status"] = status;
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once();
+    variable_list out(9);
+    if (!grads[0].defined()) return out;
+    const auto index = ctx->get_saved_variables();
+    const auto rows = ctx->saved_data["rows"].toIntVector();
+    const c10::cuda::CUDAGuard guard(grads[0].device());
+    const at::Tensor dy = packed(grads[0]);
+    CcfEmbed e{};
+    e.tokens = index[0].numel();
+    e.seq = index[0].dim() > 0 ? index[0].size(-1) : 1;
+    e.d = static_cast<int>(dy.size(-1));
+    e.type = type_code(dy);
+    constexpr int kInput[3] = {1, 2, 4};
+    const auto edges = ctx->saved_data["edges"].toIntVector();
+    std::vector<at::Tensor> dw;
+    for (int k = 0; k < 3; ++k) {
+      if (rows[k] == 0 || !ctx->needs_input_grad(edges[k])) continue;
+      add_table(e, index[k], rows[k], k == 0 ? ctx->saved_data["scale"].toDouble() : 1.0, k == 0 ? ctx->saved_data["skip"].toInt() : -1);
+      dw.push_back(at::empty({rows[k], e.d}, dy.options()));
+      out[kInput[k]] = dw.back();
+    }
+    if (e.tables > 0) run_grad(e, dy, dw, ctx->saved_data["status"].toTensor());
+    return out;
+  }
+};
+
+at::Tensor embedding_grad(const at::Tensor& grad, const at::Tensor& ids, int64_t rows, double scale, int64_t skip, const at::Tensor& status) {
+  const c10::cuda::CUDAGuard guard(grad.device());
+  const at::Tensor dy = packed(grad), index = ids.contiguous();
+  CcfEmbed e{};
+  e.tokens = index.numel();
+  e.seq = 1;
+  e.d = static_cast<int>(dy.size(-1));
+  e.type = type_code(dy);
+  add_table(e, index, rows, scale, skip);
+  const at::Tensor dw = at::empty({rows, e.d}, dy.options());
+  run_grad(e, dy, {dw}, status);
+  return dw;
+}
+
+// ---- log probabilities -------------------------------------------------------------------------------------------------
+struct LogprobsFn : torch::autograd::Function<LogprobsFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& targets, int64_t top_k, double temperature,
+                               int64_t vocab, int64_t ignore, const at::Tensor& status) {
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const int64_t width = logits.size(-1), rows = targets.numel();
+    at::Tensor x = logits.reshape({rows, width});
+    if (x.stride(1) != 1 || (rows > 1 && x.stride(0) < width)) x = x.contiguous();
+    if (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) x = x.clone(at::MemoryFormat::Contiguous);
+    const at::Tensor t = targets.contiguous();
+    const auto f32 = logits.options().dtype(at::kFloat);
+    const auto shape = targets.sizes();
+    const at::Tensor lp = at::empty(shape, f32), entropy = at::empty(shape, f32);
+    at::Tensor top, top_ids, stats;
+    CcfLogprobs a{};
+    a.x = x.data_ptr();
+    a.targets = t.data_ptr();
+    a.wide = t.scalar_type() == at::kLong;
+    a.logprobs = lp.data_ptr<float>();
+    a.entropy = entropy.data_ptr<float>();
+    a.status = status.data_ptr<int>();
+    a.rows = rows;
+    a.ld = rows > 1 ? x.stride(0) : width;
+    a.ignore = ignore;
+    a.vocab = static_cast<int>(vocab);
+    a.width = static_cast<int>(width);
+    a.top_k = static_cast<int>(top_k);
+    a.type = type_code(x);
+    a.inv_t = static_cast<float>(1.0 / temperature);
+    if (top_k > 0) {
+      auto wide = shape.vec();
+      wide.push_back(top_k);
+      top = at::empty(wide, f32);
+      top_ids = at::empty(wide, f32.dtype(at::kLong));
+      a.top_logprobs = top.data_ptr<float>();
+      a.top_ids = reinterpret_cast<long long*>(top_ids.data_ptr<int64_t>());
+    }
+    const bool training = logits.requires_grad();
+    if (training) {
+      stats = at::empty({rows, 3}, f32);
+      a.stats = stats.data_ptr<float>();
+    }
+    check(ccf_logprobs_fwd(&a, stream()), "ccf_logprobs_fwd");
+    ++g_launches;
+    if (training) {
+      ctx->save_for_backward({x, t, stats, top_ids});
+      ctx->saved_data["args"] = std::vector<int64_t>{top_k, vocab, ignore, a.ld};
+      ctx->saved_data["inv_t"] = 1.0 / temperature;
+      ctx->saved_data["shape"] = logits.sizes();
+    }
+    ctx->set_materialize_grads(false);
+    if (top_k == 0) return {lp, entropy};
+    ctx->mark_non_differentiable({top_ids});
+    return {lp, entropy, top, top_ids};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once();
+    variable_list out(7);
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &t = saved[1], &stats = saved[2];
+    const auto args = ctx->saved_data["args"].toIntVector();
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int64_t rows = x.size(0), width = x.size(1), ld = args[3];
+    at::Tensor g[3];
+    for (int i = 0; i < 3 && i < static_cast<int>(grads.size()); ++i)
+      if (grads[i].defined()) g[i] = grads[i].contiguous();
+    if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return out;
+    const at::Tensor whole = at::empty({rows, ld}, x.options());   // rows lie as those of the logits do
+    CcfLogprobs a{};
+    a.x = x.data_ptr();
+    a.targets = t.data_ptr();
+    a.wide = t.scalar_type() == at::kLong;
+    a.stats = stats.data_ptr<float>();
+    a.top_ids = args[0] > 0 ? reinterpret_cast<long long*>(saved[3].data_ptr<int64_t>()) : nullptr;
+    a.d_logprobs = g[0].defined() ? g[0].data_ptr<float>() : nullptr;
+    a.d_entropy = g[1].defined() ? g[1].data_ptr<float>() : nullptr;
+    a.d_top = g[2].defined() ? g[2].data_ptr<float>() : nullptr;
+    a.dx = whole.data_ptr();
+    a.rows = rows;
+    a.ld = ld;
+    a.top_k = static_cast<int>(args[0]);
+    a.vocab = static_cast<int>(args[1]);
+    a.ignore = args[2];
+    a.width = static_cast<int>(width);
+    a.type = type_code(x);
+    a.inv_t = static_cast<float>(ctx->saved_data["inv_t"].toDouble());
+    check(ccf_logprobs_bwd(&a, stream()), "ccf_logprobs_bwd");
+    ++g_launches;
+    out[0] = whole.narrow(1, 0, width).view(ctx->saved_data["shape"].toIntVector());
+    return out;
+  }
+};
+
+// ---- dropout -----------------------------------------------------------------------------------------------------------
+at::Tensor run_dropout(const at::Tensor& x, const at::Tensor& residual, const long long* state, long long* copy, int64_t call, int64_t drop) {
+  const at::Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  check(ccf_dropout(x.data_ptr(), residual.defined() ? residual.data_ptr() : nullptr, y.data_ptr(), state, copy, static_cast<unsigned>(call),
+                    static_cast<unsigned>(drop), x.numel(), type_code(x), stream()),
+        "ccf_dropout");
+  ++g_launches;
+  return y;
+}
+
+struct DropoutFn : torch::autograd::Function<DropoutFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& residual, const at::Tensor& state, int64_t call, int64_t drop) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor used = at::empty({2}, state.options());   // the seed and step of this pass: the state may move on before the backward pass
+    const at::Tensor y = run_dropout(packed(x), residual.has_value() ? packed(*residual) : at::Tensor(),
+                                     reinterpret_cast<const long long*>(state.data_ptr<int64_t>()),
+                                     reinterpret_cast<long long*>(used.data_ptr<int64_t>()), call, drop);
+    ctx->save_for_backward({used});
+    ctx->saved_data["call"] = call;
+    ctx->saved_data["drop"] = drop;
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once();
+    variable_list out(5);
+    const c10::cuda::CUDAGuard guard(grads[0].device());
+    if (ctx->needs_input_grad(1)) out[1] = grads[0];
+    if (ctx->needs_input_grad(0)) {
+      const at::Tensor used = ctx->get_saved_variables()[0];
+      out[0] = run_dropout(packed(grads[0]), at::Tensor(), reinterpret_cast<const long long*>(used.data_ptr<int64_t>()), nullptr,
+                           ctx->saved_data["call"].toInt(), ctx->saved_data["drop"].toInt());
+    }
+    return out;
+  }
+};
+
+}  // namespace
+
+void ccf_torch::add_token_ops(py::module_& m) {
+  m.def(
+      "embedding",
+      [](const at::Tensor& ids, const at::Tensor& weight, const OptTensor& position, const OptTensor& position_ids, const OptTensor& type,
+         const OptTensor& type_ids, double scale, int64_t skip, const at::Tensor& status) {
+        return EmbeddingFn::apply(ids, weight, position, position_ids, type, type_ids, scale, skip, status);
+      },
+      py::call_guard<py::gil_scoped_release>());
+  m.def("embedding_grad", &embedding_grad, py::call_guard<py::gil_scoped_release>());
+  m.def(
+      "token_logprobs",
+      [](const at::Tensor& logits, const at::Tensor& targets, int64_t top_k, double temperature, int64_t vocab, int64_t ignore,
+         const at::Tensor& status) { return LogprobsFn::apply(logits, targets, top_k, temperature, vocab, ignore, status); },
+      py::call_guard<py::gil_scoped_release>());
+  m.def(
+      "dropout",
+      [](const at::Tensor& x, const OptTensor& residual, const at::Tensor& state, int64_t call, int64_t drop) {
+        return DropoutFn::apply(x, residual, state, call, drop);
+      },
+      py::call_guard<py::gil_scoped_release>());
+}

@@ -1,4 +1,4 @@
-"""Exceptions raised by the communication layer."""
+"""Exceptions raised for what a kernel recorded in the status word."""
 
 
 class MoECommError(RuntimeError):
@@ -21,3 +21,7 @@ class MoECommTimeout(MoECommError):
 
 class MoEOverflow(MoECommError):
     """More rows were routed to a rank than its receive buffer was sized for."""
+
+
+class TokenIndexError(MoECommError, IndexError):
+    """A token, position, type or target id lay outside its table; its row of the output is NaN."""

@@ -21,7 +21,8 @@ ACT_NONE, ACT_GELU, ACT_RELU = range(3)
 MAJ_K, MAJ_MN = 0, 1
 ACT_CODE = {"gelu": ACT_GELU, "relu": ACT_RELU, "none": ACT_NONE, "swiglu": ACT_NONE}
 
-ERR_NAMES = {1: "pipeline barrier timeout", 2: "peer flag timeout", 3: "bounds check", 4: "receive buffer overflow"}
+ERR_NAMES = {1: "pipeline barrier timeout", 2: "peer flag timeout", 3: "bounds check", 4: "receive buffer overflow",
+             5: "index out of range"}
 
 _vp = C.c_void_p
 
@@ -127,6 +128,26 @@ class LayerGrads(C.Structure):
                 ("router_w", _vp), ("x", _vp), ("slot_grad", _vp), ("router_dw", _vp), ("router_db", _vp)]
 
 
+class EmbedTable(C.Structure):
+    """Mirror of CcfEmbedTable (csrc/embedding.h)."""
+    _fields_ = [("weight", _vp), ("ids", _vp), ("grad", _vp), ("scratch", _vp), ("rows", C.c_longlong), ("ld", C.c_longlong),
+                ("skip", C.c_longlong), ("scale", C.c_float), ("wide", C.c_int)]
+
+
+class Embed(C.Structure):
+    """Mirror of CcfEmbed (csrc/embedding.h)."""
+    _fields_ = [("table", EmbedTable * 3), ("tokens", C.c_longlong), ("seq", C.c_longlong), ("tables", C.c_int), ("d", C.c_int),
+                ("type", C.c_int), ("pad0", C.c_int)]
+
+
+class Logprobs(C.Structure):
+    """Mirror of CcfLogprobs (csrc/logprobs.h)."""
+    _fields_ = [("x", _vp), ("targets", _vp), ("logprobs", _vp), ("entropy", _vp), ("top_logprobs", _vp), ("top_ids", _vp), ("stats", _vp),
+                ("d_logprobs", _vp), ("d_entropy", _vp), ("d_top", _vp), ("dx", _vp), ("status", _vp), ("rows", C.c_longlong),
+                ("ld", C.c_longlong), ("ignore", C.c_longlong), ("vocab", C.c_int), ("width", C.c_int), ("top_k", C.c_int),
+                ("type", C.c_int), ("wide", C.c_int), ("inv_t", C.c_float)]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -167,8 +188,8 @@ def _build_locked(needed, make):
 
 
 def torch_module():
-    """The autograd functions in C++ (csrc/torch_norm.cpp), or None where this torch has no module and none can be built: the
-    kernels do not need it (ops/norm.py has the function in Python). Tried once; says so once."""
+    """The autograd functions in C++ (csrc/torch_norm.cpp, csrc/torch_tokens.cpp), or None where this torch has no module and none can be
+    built: the kernels do not need it (ops/norm.py and its neighbours have the functions in Python). Tried once; says so once."""
     global _torch_module, _torch_module_tried
     if _torch_module is not None or _torch_module_tried:
         return _torch_module
@@ -189,8 +210,8 @@ def torch_module():
                 _torch_module = module
             except Exception as e:  # noqa: BLE001
                 import warnings
-                warnings.warn(f"ccfuser_b200: {_build.torch_path()} could not be built or loaded ({e}); LayerNorm's autograd "
-                              "function runs in Python, on the same kernels")
+                warnings.warn(f"ccfuser_b200: {_build.torch_path()} could not be built or loaded ({e}); the autograd functions "
+                              "of LayerNorm, embeddings, log probabilities and dropout run in Python, on the same kernels")
             _torch_module_tried = True
     return _torch_module
 
@@ -218,7 +239,7 @@ def load(build_if_missing: bool = True):
         for name, struct in (("gemm_args", GemmArgs), ("dispatch_args", DispatchArgs),
                              ("gemm_launch", GemmLaunch), ("plan_args", PlanArgs), ("layer", Layer),
                              ("layer_grads", LayerGrads), ("barrier_args", BarrierArgs),
-                             ("sgd_multi", SgdMulti)):
+                             ("sgd_multi", SgdMulti), ("embed", Embed), ("logprobs", Logprobs)):
             want = getattr(lib, "ccf_sizeof_" + name)()
             if want != C.sizeof(struct):
                 raise RuntimeError(f"ctypes mirror of {name} is {C.sizeof(struct)} bytes, library has {want}")
@@ -262,6 +283,12 @@ def _declare(lib):
         "ccf_layernorm_fwd": ([p, p, p, p, p, p, i, i, C.c_float, i, p], i),
         "ccf_layernorm_bwd_parts": ([i, i], i),
         "ccf_layernorm_bwd": ([p, p, p, p, p, p, p, p, p, i, i, i, p, ull, p], i),
+        "ccf_embedding_fwd": ([C.POINTER(Embed), p, p, p], i),
+        "ccf_embedding_scratch": ([ll, ll, i, i], ll),
+        "ccf_embedding_bwd": ([C.POINTER(Embed), p, p, p], i),
+        "ccf_logprobs_fwd": ([C.POINTER(Logprobs), p], i),
+        "ccf_logprobs_bwd": ([C.POINTER(Logprobs), p], i),
+        "ccf_dropout": ([p, p, p, p, p, C.c_uint, C.c_uint, ll, i, p], i),
         "ccf_symm_alloc": ([ull, C.POINTER(p)], i),
         "ccf_symm_free": ([p], i),
         "ccf_symm_handle_bytes": ([], i),
@@ -349,6 +376,9 @@ ARG_ERRORS = {-2: "argument out of range", -3: "n must be a multiple of 32", -4:
                    "m_per_group % 256 == 0",
               -14: "the rows to be dispatched must begin on a 16-byte boundary",
               -15: "the box of a tensor map is 32 or 64 columns wide"}
+
+
+DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # csrc/elements.cuh
 
 
 def check(rc: int, what: str):

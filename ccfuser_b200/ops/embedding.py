@@ -1,0 +1,206 @@
+"""Sums of embedding lookups on the library's kernels (csrc/embedding.cu): what the models put in front of their first block.
+
+``embedding`` adds up to three lookups in one pass, ``scale * weight[ids] + position_weight[position] + type_weight[type_ids]``, in fp32
+with one rounding: word and position table of GPT, word table times sqrt(d_model) of Transformer-XL, word, position and type table of BERT
+(mix_moe/mix_moe/examples/models/moe_gpt.py, transformer-xl/mem_transformer_mix_moe.py, models/moe_bert.py of the reference use torch's). The
+gradients are dense. A word's gradient is the sum over its tokens in their order, in fp32, after a sort of the tokens by id: no atomics,
+the same bits every time. The autograd function is C++ (csrc/torch_tokens.cpp); the Python one below stands in where that module is missing and
+while a graph is traced.
+
+An id outside its table does not fault the GPU: its row is NaN, it adds nothing to a gradient, and it is recorded in the device's status word, which
+``ops.gemm.Workspace.get(device).check()`` raises as ``TokenIndexError``. On the CPU, and for other types than bf16, fp16 and fp32, the same
+sums run on torch's operations, which raise ``IndexError``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from .. import native as N
+from . import gemm as G
+
+MAX_TOKENS = 2 ** 31 - 1
+_INDEX = (torch.int64, torch.int32)
+
+
+def _fill(e, ids, rows, scale, skip):
+    t = e.table[e.tables]
+    t.rows, t.scale, t.skip = rows, scale, skip
+    if ids is not None:
+        t.ids, t.wide = ids.data_ptr(), int(ids.dtype == torch.int64)
+    e.tables += 1
+    return t
+
+
+def _run_grad(e, dy, grads, status):
+    lib = N.load()
+    scratch = []
+    for k, g in enumerate(grads):
+        t = e.table[k]
+        scratch.append(torch.empty(lib.ccf_embedding_scratch(e.tokens, t.rows, e.d, int(bool(t.ids))), dtype=torch.uint8, device=dy.device))
+        t.scratch, t.grad = scratch[-1].data_ptr(), g.data_ptr()
+    n = lib.ccf_embedding_bwd(C.byref(e), dy.data_ptr(), status, N.stream_ptr())
+    N.check(min(n, 0), "ccf_embedding_bwd")
+    N.count(n)
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    """The C++ function in Python."""
+
+    @staticmethod
+    def forward(ctx, ids, weight, position, position_ids, types, type_ids, scale, skip):
+        index = [None if t is None else t.contiguous() for t in (ids, position_ids, type_ids)]
+        e = N.Embed(tokens=ids.numel(), seq=ids.shape[-1] if ids.dim() else 1, d=weight.shape[1], type=N.DTYPE_CODE[weight.dtype])
+        held = []
+        for k, w in enumerate((weight, position, types)):
+            if w is None:
+                continue
+            held.append(w if w.stride(1) == 1 and w.stride(0) >= w.shape[1] else w.contiguous())
+            t = _fill(e, index[k], w.shape[0], scale if k == 0 else 1.0, skip if k == 0 else -1)
+            t.weight, t.ld = held[-1].data_ptr(), held[-1].stride(0) if w.shape[0] > 1 else e.d
+        y = torch.empty(*ids.shape, e.d, dtype=weight.dtype, device=weight.device)
+        with torch.cuda.device(weight.device):
+            N.check(N.load().ccf_embedding_fwd(C.byref(e), y.data_ptr(), G.Workspace.status_of(y), N.stream_ptr()), "ccf_embedding_fwd")
+        N.count(1)
+        ctx.save_for_backward(*index)
+        ctx.rows = [0 if w is None else w.shape[0] for w in (weight, position, types)]
+        ctx.scale, ctx.skip = scale, skip
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        index, out, grads = ctx.saved_tensors, [None] * 8, []
+        dy = G.packed(dy)
+        e = N.Embed(tokens=index[0].numel(), seq=index[0].shape[-1] if index[0].dim() else 1, d=dy.shape[-1], type=N.DTYPE_CODE[dy.dtype])
+        for k, at in enumerate((1, 2, 4)):
+            if ctx.rows[k] and ctx.needs_input_grad[at]:
+                _fill(e, index[k], ctx.rows[k], ctx.scale if k == 0 else 1.0, ctx.skip if k == 0 else -1)
+                out[at] = torch.empty(ctx.rows[k], e.d, dtype=dy.dtype, device=dy.device)
+                grads.append(out[at])
+        if grads:
+            with torch.cuda.device(dy.device):
+                _run_grad(e, dy, grads, G.Workspace.status_of(dy))
+        return tuple(out)
+
+
+def _check_ids(name, ids, device):
+    if ids.dtype not in _INDEX:
+        raise TypeError(f"{name}: indices are int64 or int32, not {ids.dtype}")
+    if ids.device != device:
+        raise ValueError(f"{name} is on {ids.device}, the table on {device}")
+
+
+def _check_table(name, table, weight):
+    if table.dim() != 2 or table.shape[1] != weight.shape[1] or table.dtype != weight.dtype or table.device != weight.device:
+        raise ValueError(f"{name}: [rows, {weight.shape[1]}] of {weight.dtype} on {weight.device}, got {tuple(table.shape)} of "
+                         f"{table.dtype} on {table.device}")
+
+
+def _skip(padding_idx, rows):
+    if padding_idx is None:
+        return -1
+    if not -rows <= padding_idx < rows:
+        raise ValueError(f"padding_idx {padding_idx} lies outside the table's {rows} rows")
+    return padding_idx % rows
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *, position_weight: Optional[torch.Tensor] = None,
+              position_ids: Optional[torch.Tensor] = None, type_weight: Optional[torch.Tensor] = None,
+              type_ids: Optional[torch.Tensor] = None, padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``scale * weight[ids] + position_weight[position_ids] + type_weight[type_ids]``, ``[*ids.shape, d]``.
+
+    ``position_ids`` (broadcast to the shape of ``ids``) default to the index along the last dimension of ``ids``. The tables are ``[rows, d]`` of one
+    type. ``padding_idx``: that row of ``weight`` gets no gradient (it is looked up like any other). The result cannot be differentiated twice."""
+    if weight.dim() != 2:
+        raise ValueError(f"weight: [rows, d], got {tuple(weight.shape)}")
+    _check_ids("ids", ids, weight.device)
+    skip = _skip(padding_idx, weight.shape[0])
+    if position_weight is not None:
+        _check_table("position_weight", position_weight, weight)
+        if position_ids is not None:
+            _check_ids("position_ids", position_ids, weight.device)
+            if position_ids.shape != ids.shape:
+                position_ids = position_ids.expand(ids.shape)
+        elif (ids.shape[-1] if ids.dim() else 1) > position_weight.shape[0]:
+            raise ValueError(f"{ids.shape[-1]} positions, and {position_weight.shape[0]} rows in position_weight")
+    elif position_ids is not None:
+        raise ValueError("position_ids without position_weight")
+    if (type_weight is None) != (type_ids is None):
+        raise ValueError("type_weight and type_ids go together")
+    if type_weight is not None:
+        _check_table("type_weight", type_weight, weight)
+        _check_ids("type_ids", type_ids, weight.device)
+        if type_ids.shape != ids.shape:
+            type_ids = type_ids.expand(ids.shape)
+    if not (weight.is_cuda and weight.dtype in N.DTYPE_CODE and ids.numel() > 0 and weight.numel() > 0):
+        return _embedding_torch(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx)
+    if ids.numel() > MAX_TOKENS:
+        raise ValueError(f"{ids.numel()} tokens: at most 2^31 - 1 in one call")
+    module = N.torch_module()
+    if module is None or torch.jit.is_tracing():
+        return _EmbeddingFn.apply(ids, weight, position_weight, position_ids, type_weight, type_ids, float(scale), skip)
+    return module.embedding(ids, weight, position_weight, position_ids, type_weight, type_ids, scale, skip, G.Workspace.of(weight).status)
+
+
+def _embedding_torch(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx):
+    y = F.embedding(ids, weight, padding_idx)
+    if scale != 1.0:
+        y = y * scale
+    if position_weight is not None:
+        if position_ids is None:
+            position_ids = torch.arange(ids.shape[-1] if ids.dim() else 1, device=ids.device)
+            position_ids = position_ids if ids.dim() else position_ids[0]
+        y = y + F.embedding(position_ids, position_weight)
+    if type_weight is not None:
+        y = y + F.embedding(type_ids, type_weight)
+    return y
+
+
+def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
+    """The dense gradient ``[num_rows, d]`` of a table from the gradient ``[*ids.shape, d]`` of its lookups: what ``embedding`` does in its
+    backward pass, without a graph."""
+    _check_ids("ids", ids, grad.device)
+    if num_rows < 1 or grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
+        raise ValueError(f"grad: {list(ids.shape)} + [d] and at least one row, got {list(grad.shape)} and {num_rows} rows")
+    skip = _skip(padding_idx, num_rows)
+    if not (grad.is_cuda and grad.dtype in N.DTYPE_CODE and grad.numel() > 0):
+        grad = grad.detach()
+        out = torch.zeros(num_rows, grad.shape[-1], dtype=grad.dtype if grad.dtype == torch.float64 else torch.float32, device=grad.device)
+        out.index_add_(0, ids.reshape(-1).long(), grad.reshape(-1, grad.shape[-1]).to(out.dtype))
+        if skip >= 0:
+            out[skip] = 0.0
+        return out.mul_(scale).to(grad.dtype)
+    if ids.numel() > MAX_TOKENS or num_rows > MAX_TOKENS:
+        raise ValueError("at most 2^31 - 1 tokens and rows in one call")
+    module = N.torch_module()
+    with torch.no_grad():
+        if module is not None and not torch.jit.is_tracing():
+            return module.embedding_grad(grad, ids, num_rows, scale, skip, G.Workspace.of(grad).status)
+        dy, index = G.packed(grad), ids.contiguous()
+        e = N.Embed(tokens=index.numel(), seq=1, d=dy.shape[-1], type=N.DTYPE_CODE[dy.dtype])
+        _fill(e, index, num_rows, float(scale), skip)
+        out = torch.empty(num_rows, e.d, dtype=dy.dtype, device=dy.device)
+        with torch.cuda.device(dy.device):
+            _run_grad(e, dy, [out], G.Workspace.status_of(dy))
+        return out
+
+
+class Embedding(nn.Embedding):
+    """``nn.Embedding`` (same parameters, same state-dict keys) on ``embedding``, with a factor ``scale`` and the other tables as arguments of its call.
+    ``max_norm``, ``scale_grad_by_freq`` and ``sparse`` are refused."""
+
+    def __init__(self, *args, scale: float = 1.0, **kw):
+        super().__init__(*args, **kw)
+        if self.max_norm is not None or self.scale_grad_by_freq or self.sparse:
+            raise ValueError("max_norm, scale_grad_by_freq and sparse are not supported")
+        self.scale = scale
+
+    def forward(self, ids, position_weight=None, position_ids=None, type_weight=None, type_ids=None):
+        return embedding(ids, self.weight, self.scale, position_weight=position_weight, position_ids=position_ids, type_weight=type_weight,
+                         type_ids=type_ids, padding_idx=self.padding_idx)

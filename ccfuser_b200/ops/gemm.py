@@ -89,12 +89,14 @@ class Workspace:
                               f"(raise config.recv_factor or set a capacity_factor)")
         if v:
             code, detail = v & 0xff, v >> 8
-            from ..errors import MoECommError, MoECommTimeout, MoEOverflow
+            from ..errors import MoECommError, MoECommTimeout, MoEOverflow, TokenIndexError
             msg = f"{what}: {N.ERR_NAMES.get(code, 'error')}: {describe_status(code, detail)} (code {code}, detail {detail:#x})"
             if code in (1, 2):
                 raise MoECommTimeout(msg, where=what, tile=detail)
             if code == 4:
                 raise MoEOverflow(msg)
+            if code == 5:
+                raise TokenIndexError(msg)
             raise MoECommError(msg)
 
 
@@ -129,6 +131,8 @@ def describe_status(code: int, detail: int) -> str:
         return f"row {detail} carried an out-of-range source rank or slot (access skipped)"
     if code == 4:
         return f"receive buffer of rank {detail} too small for the rows routed to it"
+    if code == 5:
+        return f"an id of token {detail} lies outside its table (its row is NaN, and it adds nothing to a gradient)"
     return f"unknown code {code}, detail {detail:#x}"
 
 
