@@ -45,6 +45,28 @@ __device__ __forceinline__ uint64_t top_key(float v, uint32_t index) { return st
 
 template <int kType>
 constexpr uint32_t kNegInf2 = kType == kBf16 ? 0xff80ff80u : kType == kFp16 ? 0xfc00fc00u : 0xff800000u;
+// Elements are raised to this before the arithmetic, so that -inf needs no care there (0 * -inf): -1e30 in bf16 and fp32, the lowest fp16.
+template <int kType>
+constexpr uint32_t kFloorBits = kType == kBf16 ? 0xf14af14au : kType == kFp16 ? 0xfbfffbffu : 0xf149f2cau;
+template <int kType>
+constexpr float kFloor = kType == kFp16 ? -65504.f : -1e30f;
+
+template <int kType>
+struct Pair {
+  using T = typename std::conditional<kType == kFp16, __half2, __nv_bfloat162>::type;
+  static __device__ __forceinline__ T of(uint32_t w) { return *reinterpret_cast<T*>(&w); }
+  static __device__ __forceinline__ uint32_t bits(T v) { return *reinterpret_cast<uint32_t*>(&v); }
+};
+
+template <int kType>
+__device__ __forceinline__ uint32_t raise_word(uint32_t w) {
+  if constexpr (kType == kFp32) return __float_as_uint(fmaxf(__uint_as_float(w), __uint_as_float(kFloorBits<kType>)));
+  else return Pair<kType>::bits(__hmax2(Pair<kType>::of(w), Pair<kType>::of(kFloorBits<kType>)));
+}
+template <int kType>
+__device__ __forceinline__ uint4 raised(const uint4& q) {
+  return make_uint4(raise_word<kType>(q.x), raise_word<kType>(q.y), raise_word<kType>(q.z), raise_word<kType>(q.w));
+}
 
 // largest of the elements of kUnroll pieces; NaN if one is
 template <int kType>
@@ -56,12 +78,12 @@ __device__ __forceinline__ float max_of(const uint4 (&q)[kUnroll]) {
       m = max_nan(m, max_nan(max_nan(__uint_as_float(q[k].x), __uint_as_float(q[k].y)), max_nan(__uint_as_float(q[k].z), __uint_as_float(q[k].w))));
     return m;
   } else {
-    using H2 = typename std::conditional<kType == kFp16, __half2, __nv_bfloat162>::type;
-    auto as = [](uint32_t w) { return *reinterpret_cast<H2*>(&w); };
-    H2 m = as(kNegInf2<kType>);
+    using P = Pair<kType>;
+    typename P::T m = P::of(kNegInf2<kType>);
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(as(q[k].x), as(q[k].y)), __hmax2_nan(as(q[k].z), as(q[k].w))));
-    const float2 f = unpack2(*reinterpret_cast<uint32_t*>(&m), kType == kFp16);
+    for (int k = 0; k < kUnroll; ++k)
+      m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(P::of(q[k].x), P::of(q[k].y)), __hmax2_nan(P::of(q[k].z), P::of(q[k].w))));
+    const float2 f = unpack2(P::bits(m), kType == kFp16);
     return max_nan(f.x, f.y);
   }
 }
@@ -79,33 +101,20 @@ struct RowShape {
   }
 };
 
-// running statistics of one thread
-struct Running {
-  float m = neg_inf();
-  f32x2 s = 0, q = 0;
-  __device__ __forceinline__ void raise(float to, float c) {   // before elements up to `to`
-    if (to <= m) return;
-    const float next = max_nan(m, to), d = fmaxf((m - next) * c, kFloorU), f = exp2_fast(d);
-    q = mul2(fma2(s, bc2(d), q), bc2(f));
-    s = mul2(s, bc2(f));
-    m = next;
-  }
-  __device__ __forceinline__ void add2x(float a, float b, float c) {
-    float u0, u1;
-    upk2(mul2(add2(pk2(a, b), bc2(-m)), bc2(c)), u0, u1);
-    u0 = fmaxf(u0, kFloorU);
-    u1 = fmaxf(u1, kFloorU);
-    const f32x2 e = pk2(exp2_fast(u0), exp2_fast(u1));
-    s = add2(s, e);
-    q = fma2(e, pk2(u0, u1), q);
-  }
-};
+// u_j = x_j c - m c, with m c rounded once and the same for all of a row: one fused operation, whose rounding of m c cancels in every quotient. That
+// holds where m c is finite and raised elements vanish; elsewhere (rows of the type's lowest value, an extreme temperature) u_j = (x_j - m) c.
+template <int kType>
+__device__ __forceinline__ bool fused_ok(float mc, float c) {
+  const float low = kFloor<kType> * c;
+  return low - mc < -200.f && fabsf(mc) < 1e37f && low > -1e38f;
+}
 
 struct RowStats {
   float m, s, q;
 };
+// the same sums relative to a larger m
 __device__ __forceinline__ void rescale(RowStats& a, float m, float c) {
-  const float d = fmaxf((a.m - m) * c, kFloorU), f = exp2_fast(d);
+  const float d = a.m == m ? 0.f : fmaxf(a.m * c - m * c, kFloorU), f = exp2_fast(d);
   a.q = fmaf(a.s, d, a.q) * f;
   a.s *= f;
   a.m = m;
@@ -123,20 +132,65 @@ __device__ __forceinline__ void reduce_lanes(RowStats& a, float c) {
   }
 }
 
+// running statistics of one thread
+template <int kType>
+struct Running {
+  float m = neg_inf(), mc = neg_inf();
+  f32x2 s = 0, q = 0;
+  __device__ __forceinline__ void raise(float to, float c) {   // before elements up to `to`
+    if (to <= m) return;
+    m = max_nan(m, to);
+    const float next = m * c, d = fmaxf(mc - next, kFloorU), f = exp2_fast(d);   // m has changed: the two products differ, or both are infinite
+    q = mul2(fma2(s, bc2(d), q), bc2(f));
+    s = mul2(s, bc2(f));
+    mc = next;
+  }
+  __device__ __forceinline__ void add(f32x2 u) {
+    float u0, u1;
+    upk2(u, u0, u1);
+    const f32x2 e = pk2(exp2_fast(u0), exp2_fast(u1));
+    s = add2(s, e);
+    q = fma2(e, u, q);
+  }
+  __device__ __forceinline__ void piece(const uint4& v, float c, bool fused) {
+    constexpr int kE = kElemsPer16<kType>;
+    float f[kE];
+    if (fused) {
+      unpack16<kType>(raised<kType>(v), f);
+#pragma unroll
+      for (int i = 0; i < kE; i += 2) add(fma2(pk2(f[i], f[i + 1]), bc2(c), bc2(-mc)));
+    } else {
+      unpack16<kType>(v, f);
+#pragma unroll
+      for (int i = 0; i < kE; i += 2) add(pk2(fmaxf((f[i] - m) * c, kFloorU), fmaxf((f[i + 1] - m) * c, kFloorU)));
+    }
+  }
+  __device__ __forceinline__ RowStats done() const {
+    float a, b, x, y;
+    upk2(s, a, b);
+    upk2(q, x, y);
+    return {m, a + b, x + y};
+  }
+};
 template <int kThreads>
 constexpr int kListLen = kThreads == 32 ? 256 : 1024;
+template <int kThreads>
+constexpr int kGroups = kThreads == 32 ? 32 : 64;
 
 template <int kThreads>
 struct RowShared {
   RowStats part[kThreads / 32];
   RowStats all;
+  uint32_t group[kGroups<kThreads>];   // largest element of a group of threads
   uint64_t top[CCF_LOGPROBS_MAX_TOP];
   uint64_t best[kThreads / 32];
   uint64_t list[kListLen<kThreads>];
+  uint32_t bound;
   int listed;
 };
+template <int kThreads>
 struct RowSharedPlain {   // without alternatives
-  RowStats part[16];
+  RowStats part[kThreads / 32];
   RowStats all;
 };
 
@@ -145,37 +199,63 @@ __device__ __forceinline__ void row_sync() {
   if constexpr (kThreads == 32) __syncwarp();
   else __syncthreads();
 }
+
+// sh.list[0, n) by rank into sh.top, the k largest
 template <int kThreads>
-__device__ __forceinline__ int row_count(bool on) {
-  if constexpr (kThreads == 32) return __popc(__ballot_sync(0xffffffffu, on));
-  else return __syncthreads_count(on);
+__device__ __forceinline__ void rank_list(RowShared<kThreads>& sh, int n, int k, int tid) {
+  for (int i = tid; i < n; i += kThreads) {
+    const uint64_t key = sh.list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += sh.list[j] > key;
+    if (key != 0 && rank < k) sh.top[rank] = key;
+  }
 }
 
-// The k largest elements of this block's share of a row, in order, into sh.top. `m`: the largest of the thread's own elements. The k-th largest of the
-// threads' maxima bounds the k-th largest element from below, so only threads whose maximum reaches it look at their elements again (k of them,
-// but for ties), and only elements that reach it are candidates: a few more than k. The bound is found on 16 bits, by halving. Should the
-// candidates not fit the list (many equal elements), the elements are taken one after the other instead, each the largest below the one before.
+// Before the rows' first barrier: what select_top starts from.
+template <int kThreads>
+__device__ __forceinline__ uint32_t group_maxima(RowShared<kThreads>& sh, float m, int tid) {
+  const uint32_t mine = m == neg_inf() ? 0u : order_of(m);
+  uint32_t g = mine;
+#pragma unroll
+  for (int o = kThreads / kGroups<kThreads> / 2; o > 0; o /= 2) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+  if (tid % (kThreads / kGroups<kThreads>) == 0) sh.group[tid / (kThreads / kGroups<kThreads>)] = g;
+  if (tid == 0) {
+    sh.listed = 0;
+    sh.bound = 1;
+  }
+  if (tid < CCF_LOGPROBS_MAX_TOP) sh.top[tid] = 0;
+  return mine;
+}
+
+// The k largest elements of this block's share of a row, in order, into sh.top. The threads' maxima, in groups, are elements themselves: the k-th largest of
+// them bounds the k-th largest element from below. Only threads whose own maximum reaches the bound look at their elements again (about k of them), and
+// only elements that reach it are listed: a few more than k. Should they not fit the list (many equal elements), they are taken one after the
+// other instead, each the largest below the one before. `m`: the order of the thread's largest element, 0 for none.
 template <int kType, int kThreads>
-__device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_t* p, const RowShape<kType>& shape, int first, int last, float m, float edge,
-                                           int edge_index, int k) {
+__device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_t* p, const RowShape<kType>& shape, int first, int last, uint32_t m,
+                                           float edge, int edge_index, int k) {
   constexpr int kE = kElemsPer16<kType>;
   const int tid = kThreads == 32 ? lane_id() : threadIdx.x, lane = lane_id();
   const uint4* pieces = reinterpret_cast<const uint4*>(p + shape.head * kElemBytes<kType>);
-  const uint32_t mine = m == neg_inf() ? 0u : order_of(m) >> 16;
-  if (tid == 0) sh.listed = 0;
-  if (tid < CCF_LOGPROBS_MAX_TOP) sh.top[tid] = 0;
-  uint32_t bound = 0;
-#pragma unroll 1
-  for (int b = 15; b >= 0; --b)
-    if (row_count<kThreads>(mine >= (bound | 1u << b)) >= k) bound |= 1u << b;
-  bound = bound > 0 ? bound : 1u;
+  if (tid < kGroups<kThreads>) {
+    const uint32_t g = sh.group[tid];
+    int above = 0, from = 0;
+#pragma unroll 8
+    for (int i = 0; i < kGroups<kThreads>; ++i) {
+      const uint32_t o = sh.group[i];
+      above += o > g;
+      from += o >= g;
+    }
+    if (g != 0 && above < k && k <= from) sh.bound = g;   // the k-th largest of the groups; fewer elements than that: every finite one counts
+  }
   row_sync<kThreads>();
+  const uint32_t bound = sh.bound;
   auto consider = [&](float v, int index) {
-    if (v == neg_inf() || order_of(v) >> 16 < bound) return;
+    if (v == neg_inf() || order_of(v) < bound) return;
     const int at = atomicAdd(&sh.listed, 1);
     if (at < kListLen<kThreads>) sh.list[at] = top_key(v, index);
   };
-  uint32_t owners = __ballot_sync(0xffffffffu, mine >= bound);
+  uint32_t owners = __ballot_sync(0xffffffffu, m >= bound);
   while (owners != 0) {
     const int owner = __ffs(owners) - 1;
     owners &= owners - 1;
@@ -190,12 +270,7 @@ __device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_
   row_sync<kThreads>();
   const int n = sh.listed;
   if (n <= kListLen<kThreads>) {
-    for (int i = tid; i < n; i += kThreads) {
-      const uint64_t key = sh.list[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += sh.list[j] > key;
-      if (rank < k) sh.top[rank] = key;
-    }
+    rank_list<kThreads>(sh, n, k, tid);
     row_sync<kThreads>();
     return;
   }
@@ -235,20 +310,20 @@ __device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_
 // kThreads per row; a warp per row, eight rows a block, where rows are short. Rows of wide vocabularies may be shared by a cluster of `split` blocks,
 // each with its part of the columns, whose statistics and alternatives the first one joins: a few rows would leave most of the card idle.
 template <int kType, int kThreads, bool kTop>
-__global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_kernel(const __grid_constant__ CcfLogprobs a, int split) {
+__global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_kernel(const __grid_constant__ CcfLogprobs a, int log_split) {
   namespace cg = cooperative_groups;
   constexpr int kE = kElemsPer16<kType>, kRows = kThreads == 32 ? 8 : 1;
-  using Shared = typename std::conditional<kTop, RowShared<kThreads>, RowSharedPlain>::type;
+  using Shared = typename std::conditional<kTop, RowShared<kThreads>, RowSharedPlain<kThreads>>::type;
   __shared__ Shared shared[kRows];
   const int warp = threadIdx.x >> 5, lane = lane_id(), tid = kThreads == 32 ? lane : threadIdx.x;
-  const int rank = static_cast<int>(blockIdx.x % static_cast<unsigned>(split));
-  const long long row = kThreads == 32 ? blockIdx.x * 8ll + warp : static_cast<long long>(blockIdx.x / static_cast<unsigned>(split));
+  const int split = 1 << log_split, rank = static_cast<int>(blockIdx.x) & (split - 1);
+  const long long row = kThreads == 32 ? blockIdx.x * 8ll + warp : static_cast<long long>(blockIdx.x >> log_split);
   if (kThreads == 32 && row >= a.rows) return;
   Shared& sh = shared[kThreads == 32 ? warp : 0];
   const uint8_t* p = reinterpret_cast<const uint8_t*>(a.x) + static_cast<size_t>(row) * a.ld * kElemBytes<kType>;
   const RowShape<kType> shape(p, a.vocab);
-  const int first = static_cast<int>(static_cast<long long>(shape.pieces) * rank / split);
-  const int last = static_cast<int>(static_cast<long long>(shape.pieces) * (rank + 1) / split);
+  const int first = static_cast<int>(static_cast<unsigned>(shape.pieces) * rank >> log_split);   // at most 2^28 pieces and 8 blocks
+  const int last = static_cast<int>(static_cast<unsigned>(shape.pieces) * (rank + 1) >> log_split);
   const uint4* pieces = reinterpret_cast<const uint4*>(p + shape.head * kElemBytes<kType>);
   const float c = a.inv_t * kLog2e;
   long long target = 0;
@@ -262,7 +337,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
   if (rank == 0 && tid < shape.head) edge_index = tid;
   if (rank == split - 1 && tid >= shape.head && tid < shape.head + shape.tail) edge_index = tid + shape.pieces * kE;
   const float edge = edge_index >= 0 ? load_elem<kType>(p, edge_index) : neg_inf();
-  Running run;
+  Running<kType> run;
   for (int v = first + tid; v < last; v += kUnroll * kThreads) {
     uint4 q[kUnroll];
 #pragma unroll
@@ -271,24 +346,15 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
       if (v + u * kThreads < last) q[u] = load16_once(pieces + v + u * kThreads);
     }
     run.raise(max_of<kType>(q), c);
+    const bool fused = fused_ok<kType>(run.mc, c);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float f[kE];
-      unpack16<kType>(q[u], f);
-#pragma unroll
-      for (int i = 0; i < kE; i += 2) run.add2x(f[i], f[i + 1], c);
-    }
+    for (int u = 0; u < kUnroll; ++u) run.piece(q[u], c, fused);
   }
   run.raise(edge, c);
-  run.add2x(edge, neg_inf(), c);
-  RowStats st{run.m, 0.f, 0.f};
-  {
-    float x, y;
-    upk2(run.s, x, y);
-    st.s = x + y;
-    upk2(run.q, x, y);
-    st.q = x + y;
-  }
+  run.add(pk2(fmaxf(fused_ok<kType>(run.mc, c) ? fmaf(edge, c, -run.mc) : (edge - run.m) * c, kFloorU), kFloorU));
+  RowStats st = run.done();
+  uint32_t largest = 0;
+  if constexpr (kTop) largest = group_maxima<kThreads>(sh, run.m, tid);
   reduce_lanes<32>(st, c);
   if constexpr (kThreads > 32) {
     constexpr int kWarps = kThreads / 32;
@@ -296,8 +362,10 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
     __syncthreads();
     st = sh.part[lane % kWarps];
     reduce_lanes<kWarps>(st, c);
+  } else {
+    __syncwarp();
   }
-  if constexpr (kTop) select_top<kType, kThreads>(sh, p, shape, first, last, run.m, edge, edge_index, a.top_k);
+  if constexpr (kTop) select_top<kType, kThreads>(sh, p, shape, first, last, largest, edge, edge_index, a.top_k);
   if constexpr (kThreads > 32) {
     if (split > 1) {
       cg::cluster_group cluster = cg::this_cluster();
@@ -313,12 +381,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
           __syncthreads();
           if (tid < CCF_LOGPROBS_MAX_TOP) sh.top[tid] = 0;
           __syncthreads();
-          for (int i = tid; i < n; i += kThreads) {
-            const uint64_t key = sh.list[i];
-            int r = 0;
-            for (int j = 0; j < n; ++j) r += sh.list[j] > key;
-            if (key != 0 && r < a.top_k) sh.top[r] = key;
-          }
+          rank_list<kThreads>(sh, n, a.top_k, tid);
           __syncthreads();
         }
       }
@@ -326,12 +389,14 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
       if (rank != 0) return;
     }
   }
-  const float log_s = logf(st.s);
+  const float log_s = logf(st.s), mc = st.m * c;
+  // lp_j = (x_j - M) / T - log_sum: the sum stands relative to the rounded M c, so the rounding is taken out of it
+  const float log_sum = fused_ok<kType>(mc, c) ? fmaf(-kLn2, fmaf(st.m, c, -mc), log_s) : log_s;
   const bool none = st.m == neg_inf(), bad = !(st.m < __int_as_float(0x7f800000));
   const float nan = __int_as_float(0x7fc00000);
   if (tid == 0) {
     const float h = bad ? nan : none ? 0.f : fmaf(-kLn2, st.q / st.s, log_s);
-    float lp = bad ? nan : none ? neg_inf() : (logit - st.m) * a.inv_t - log_s;
+    float lp = bad ? nan : none ? neg_inf() : (logit - st.m) * a.inv_t - log_sum;
     if (target == a.ignore) {
       lp = 0.f;
     } else if (target < 0 || target >= a.vocab) {
@@ -351,7 +416,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
       const uint64_t key = sh.top[tid];
       const float v = value_of(static_cast<uint32_t>(key >> 32));
       a.top_ids[row * a.top_k + tid] = key != 0 ? static_cast<long long>(0xffffffffu - static_cast<uint32_t>(key)) : -1ll;
-      a.top_logprobs[row * a.top_k + tid] = key == 0 ? neg_inf() : bad ? nan : (v - st.m) * a.inv_t - log_s;
+      a.top_logprobs[row * a.top_k + tid] = key == 0 ? neg_inf() : bad ? nan : (v - st.m) * a.inv_t - log_sum;
     }
   }
 }
@@ -413,8 +478,10 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_bwd_
     if (edge_index >= 0) store_elem<kType>(o, edge_index, 0.f);
     return;
   }
+  const float mc = r.m * c;
+  const bool fused = fused_ok<kType>(mc, c);
   auto grad = [&](float x) {
-    const float u = fmaxf((x - r.m) * c, kFloorU);
+    const float u = fmaxf(fused ? fmaf(x, c, -mc) : (x - r.m) * c, kFloorU);
     return -exp2_fast(u) * fmaf(r.w1, u, r.w0);
   };
   const int full = (a.vocab - shape.head) / kE;   // pieces that lie in the vocabulary as a whole (may be negative: none)
@@ -431,9 +498,20 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_bwd_
       const int v = v0 + k * kThreads;
       if (v >= last) break;
       float f[kE];
-      unpack16<kType>(q[k], f);
+      if (fused) {
+        unpack16<kType>(raised<kType>(q[k]), f);
 #pragma unroll
-      for (int i = 0; i < kE; ++i) f[i] = grad(f[i]);
+        for (int i = 0; i < kE; i += 2) {
+          const f32x2 u = fma2(pk2(f[i], f[i + 1]), bc2(c), bc2(-mc));
+          float u0, u1;
+          upk2(u, u0, u1);
+          upk2(mul2(pk2(exp2_fast(u0), exp2_fast(u1)), fma2(bc2(-r.w1), u, bc2(-r.w0))), f[i], f[i + 1]);
+        }
+      } else {
+        unpack16<kType>(q[k], f);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) f[i] = grad(f[i]);
+      }
       if (v >= full) {
 #pragma unroll
         for (int i = 0; i < kE; ++i)
@@ -468,8 +546,9 @@ static bool valid(const CcfLogprobs* a) {
 }
 
 template <int kType, int kThreads, bool kTop>
-static int launch_fwd(const CcfLogprobs& a, int split, cudaStream_t st) {
+static int launch_fwd(const CcfLogprobs& a, int log_split, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
+  const int split = 1 << log_split;
   cfg.gridDim = dim3(kThreads == 32 ? static_cast<unsigned>((a.rows + 7) / 8) : static_cast<unsigned>(a.rows * split));
   cfg.blockDim = dim3(kThreads == 32 ? 256 : kThreads);
   cfg.stream = st;
@@ -479,17 +558,16 @@ static int launch_fwd(const CcfLogprobs& a, int split, cudaStream_t st) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = split > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<kType, kThreads, kTop>, a, split);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<kType, kThreads, kTop>, a, log_split);
   return e == cudaSuccess ? 0 : -static_cast<int>(e);
 }
 
 template <int kType, bool kTop>
 static int choose_fwd(const CcfLogprobs& a, cudaStream_t st) {
-  if (a.vocab <= 1024) return launch_fwd<kType, 32, kTop>(a, 1, st);
-  if (a.vocab <= 8192) return launch_fwd<kType, 128, kTop>(a, 1, st);
-  int split = 1;
-  while (split < 8 && a.rows * split < 2 * sm_count()) split *= 2;
-  return launch_fwd<kType, 512, kTop>(a, split, st);
+  if (a.vocab <= 1024) return launch_fwd<kType, 32, kTop>(a, 0, st);
+  int log_split = 0;
+  while (log_split < 3 && a.rows << log_split < 2 * sm_count() && a.vocab >> log_split > 8192) ++log_split;
+  return launch_fwd<kType, 256, kTop>(a, log_split, st);
 }
 
 template <int kType>
