@@ -132,11 +132,19 @@ __device__ __forceinline__ void reduce_lanes(RowStats& a, float c) {
   }
 }
 
-// running statistics of one thread
-template <int kType>
+// running statistics of one thread; with kTop also the place of the turn that holds its largest element, and the largest of the other turns
+template <int kType, bool kTop>
 struct Running {
-  float m = neg_inf(), mc = neg_inf();
+  float m = neg_inf(), mc = neg_inf(), second = neg_inf();
+  int at = 0;
   f32x2 s = 0, q = 0;
+  __device__ __forceinline__ void turn(float largest, int v, float c) {
+    if constexpr (kTop) {
+      second = max_nan(second, fminf(m, largest));   // NaN stands above all
+      if (largest > m || largest != largest) at = v;
+    }
+    raise(largest, c);
+  }
   __device__ __forceinline__ void raise(float to, float c) {   // before elements up to `to`
     if (to <= m) return;
     m = max_nan(m, to);
@@ -175,13 +183,10 @@ struct Running {
 template <int kThreads>
 constexpr int kListLen = kThreads == 32 ? 256 : 1024;
 template <int kThreads>
-constexpr int kGroups = kThreads == 32 ? 32 : 64;
-
-template <int kThreads>
 struct RowShared {
   RowStats part[kThreads / 32];
   RowStats all;
-  uint32_t group[kGroups<kThreads>];   // largest element of a group of threads
+  uint32_t group[kThreads < 128 ? kThreads : 128];   // largest element of a group of threads
   uint64_t top[CCF_LOGPROBS_MAX_TOP];
   uint64_t best[kThreads / 32];
   uint64_t list[kListLen<kThreads>];
@@ -211,14 +216,21 @@ __device__ __forceinline__ void rank_list(RowShared<kThreads>& sh, int n, int k,
   }
 }
 
-// Before the rows' first barrier: what select_top starts from.
+// Groups whose largest elements bound the k-th largest: more than k of them keep the bound tight.
 template <int kThreads>
-__device__ __forceinline__ uint32_t group_maxima(RowShared<kThreads>& sh, float m, int tid) {
+__device__ __forceinline__ int log_group(int k) {   // log2 of the threads in a group
+  constexpr int kLog = kThreads == 32 ? 5 : kThreads == 128 ? 7 : 8;
+  return max(0, min(5, kLog - 1 - (32 - __clz(k))));
+}
+
+// Before the row's first barrier: what select_top starts from.
+template <int kThreads>
+__device__ __forceinline__ uint32_t group_maxima(RowShared<kThreads>& sh, float m, int tid, int k) {
   const uint32_t mine = m == neg_inf() ? 0u : order_of(m);
+  const int log = log_group<kThreads>(k);
   uint32_t g = mine;
-#pragma unroll
-  for (int o = kThreads / kGroups<kThreads> / 2; o > 0; o /= 2) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-  if (tid % (kThreads / kGroups<kThreads>) == 0) sh.group[tid / (kThreads / kGroups<kThreads>)] = g;
+  for (int o = 1 << log >> 1; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+  if ((tid & ((1 << log) - 1)) == 0) sh.group[tid >> log] = g;
   if (tid == 0) {
     sh.listed = 0;
     sh.bound = 1;
@@ -227,46 +239,54 @@ __device__ __forceinline__ uint32_t group_maxima(RowShared<kThreads>& sh, float 
   return mine;
 }
 
-// The k largest elements of this block's share of a row, in order, into sh.top. The threads' maxima, in groups, are elements themselves: the k-th largest of
-// them bounds the k-th largest element from below. Only threads whose own maximum reaches the bound look at their elements again (about k of them), and
-// only elements that reach it are listed: a few more than k. Should they not fit the list (many equal elements), they are taken one after the
-// other instead, each the largest below the one before. `m`: the order of the thread's largest element, 0 for none.
+// The k largest elements of this block's share of a row, in order, into sh.top. The largest elements of groups of threads are elements themselves: the k-th
+// largest of those bounds the k-th largest element from below. Only threads whose own largest element reaches the bound look at elements again (a few more than
+// k), for most of them those of the one turn that held it, an element a lane; and only elements that reach the bound are listed. Should they
+// not fit the list (many equal elements), they are taken one after the other instead, each the largest below the one before.
 template <int kType, int kThreads>
-__device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_t* p, const RowShape<kType>& shape, int first, int last, uint32_t m,
-                                           float edge, int edge_index, int k) {
+__device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_t* p, const RowShape<kType>& shape, int first, int last,
+                                           const Running<kType, true>& run, uint32_t largest, float edge, int edge_index, int k) {
   constexpr int kE = kElemsPer16<kType>;
   const int tid = kThreads == 32 ? lane_id() : threadIdx.x, lane = lane_id();
   const uint4* pieces = reinterpret_cast<const uint4*>(p + shape.head * kElemBytes<kType>);
-  if (tid < kGroups<kThreads>) {
+  const int groups = kThreads >> log_group<kThreads>(k);
+  if (tid < groups) {
     const uint32_t g = sh.group[tid];
     int above = 0, from = 0;
-#pragma unroll 8
-    for (int i = 0; i < kGroups<kThreads>; ++i) {
+    for (int i = 0; i < groups; ++i) {
       const uint32_t o = sh.group[i];
       above += o > g;
       from += o >= g;
     }
-    if (g != 0 && above < k && k <= from) sh.bound = g;   // the k-th largest of the groups; fewer elements than that: every finite one counts
+    if (g != 0 && above < k && k <= from) sh.bound = g;   // the k-th largest; where there are fewer elements than that, every finite one counts
   }
   row_sync<kThreads>();
   const uint32_t bound = sh.bound;
-  auto consider = [&](float v, int index) {
-    if (v == neg_inf() || order_of(v) < bound) return;
+  auto list = [&](float v, int index) {
     const int at = atomicAdd(&sh.listed, 1);
     if (at < kListLen<kThreads>) sh.list[at] = top_key(v, index);
   };
-  uint32_t owners = __ballot_sync(0xffffffffu, m >= bound);
+  auto consider = [&](float v, int index) {
+    if (v != neg_inf() && order_of(v) >= bound) list(v, index);
+  };
+  if (edge_index >= 0) consider(edge, edge_index);
+  uint32_t owners = __ballot_sync(0xffffffffu, largest >= bound);
+  const uint32_t wide = __ballot_sync(0xffffffffu, run.second != neg_inf() && order_of(run.second) >= bound);
   while (owners != 0) {
     const int owner = __ffs(owners) - 1;
     owners &= owners - 1;
-    for (int v = first + tid - lane + owner + lane * kThreads; v < last; v += 32 * kThreads) {
-      float f[kE];
-      unpack16<kType>(__ldg(pieces + v), f);
+    if (wide >> owner & 1) {
+      for (int v = first + tid - lane + owner + lane * kThreads; v < last; v += 32 * kThreads) {
+        float f[kE];
+        unpack16<kType>(__ldg(pieces + v), f);
 #pragma unroll
-      for (int i = 0; i < kE; ++i) consider(f[i], shape.head + v * kE + i);
+        for (int i = 0; i < kE; ++i) consider(f[i], shape.head + v * kE + i);
+      }
+    } else {
+      const int v = __shfl_sync(0xffffffffu, run.at, owner) + lane / kE * kThreads, index = shape.head + v * kE + lane % kE;
+      if (lane < kUnroll * kE && v < last) consider(load_elem<kType>(p, index), index);
     }
   }
-  if (edge_index >= 0) consider(edge, edge_index);
   row_sync<kThreads>();
   const int n = sh.listed;
   if (n <= kListLen<kThreads>) {
@@ -337,24 +357,36 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
   if (rank == 0 && tid < shape.head) edge_index = tid;
   if (rank == split - 1 && tid >= shape.head && tid < shape.head + shape.tail) edge_index = tid + shape.pieces * kE;
   const float edge = edge_index >= 0 ? load_elem<kType>(p, edge_index) : neg_inf();
-  Running<kType> run;
-  for (int v = first + tid; v < last; v += kUnroll * kThreads) {
+  Running<kType, kTop> run;
+  int v = first + tid;
+  auto turn = [&](const uint4(&q)[kUnroll]) {
+    run.turn(max_of<kType>(q), v, c);
+    const bool fused = fused_ok<kType>(run.mc, c);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) run.piece(q[u], c, fused);
+  };
+  for (; v + (kUnroll - 1) * kThreads < last; v += kUnroll * kThreads) {
+    uint4 q[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) q[u] = load16_once(pieces + v + u * kThreads);
+    turn(q);
+  }
+  if (v < last) {
     uint4 q[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       q[u] = make_uint4(kNegInf2<kType>, kNegInf2<kType>, kNegInf2<kType>, kNegInf2<kType>);
       if (v + u * kThreads < last) q[u] = load16_once(pieces + v + u * kThreads);
     }
-    run.raise(max_of<kType>(q), c);
-    const bool fused = fused_ok<kType>(run.mc, c);
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) run.piece(q[u], c, fused);
+    turn(q);
   }
+  // of the whole pieces; a single element is taken as it is
+  const float own = run.m;
   run.raise(edge, c);
   run.add(pk2(fmaxf(fused_ok<kType>(run.mc, c) ? fmaf(edge, c, -run.mc) : (edge - run.m) * c, kFloorU), kFloorU));
   RowStats st = run.done();
   uint32_t largest = 0;
-  if constexpr (kTop) largest = group_maxima<kThreads>(sh, run.m, tid);
+  if constexpr (kTop) largest = group_maxima<kThreads>(sh, own, tid, a.top_k);
   reduce_lanes<32>(st, c);
   if constexpr (kThreads > 32) {
     constexpr int kWarps = kThreads / 32;
@@ -365,7 +397,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
   } else {
     __syncwarp();
   }
-  if constexpr (kTop) select_top<kType, kThreads>(sh, p, shape, first, last, largest, edge, edge_index, a.top_k);
+  if constexpr (kTop) select_top<kType, kThreads>(sh, p, shape, first, last, run, largest, edge, edge_index, a.top_k);
   if constexpr (kThreads > 32) {
     if (split > 1) {
       cg::cluster_group cluster = cg::this_cluster();
@@ -565,6 +597,7 @@ static int launch_fwd(const CcfLogprobs& a, int log_split, cudaStream_t st) {
 template <int kType, bool kTop>
 static int choose_fwd(const CcfLogprobs& a, cudaStream_t st) {
   if (a.vocab <= 1024) return launch_fwd<kType, 32, kTop>(a, 0, st);
+  if (a.rows >= 4 * sm_count()) return launch_fwd<kType, 128, kTop>(a, 0, st);
   int log_split = 0;
   while (log_split < 3 && a.rows << log_split < 2 * sm_count() && a.vocab >> log_split > 8192) ++log_split;
   return launch_fwd<kType, 256, kTop>(a, log_split, st);
