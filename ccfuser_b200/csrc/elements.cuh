@@ -25,6 +25,9 @@ __device__ __forceinline__ void unpack16(const uint4& q, float (&f)[kElemsPer16<
   for (int i = 0; i < 4; ++i) {
     if constexpr (kType == kFp32) {
       f[i] = __uint_as_float(w[i]);
+    } else if constexpr (kType == kBf16) {   // a bf16 is the upper half of a float
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     } else {
       const float2 t = unpack2(w[i], kType == kFp16);
       f[2 * i] = t.x;

@@ -10,9 +10,9 @@
 
 namespace ccf {
 
-constexpr int kSortChunk = 2048;     // keys that one block sorts in shared memory
+constexpr int kSortChunk = 1024;     // keys that one block sorts in shared memory
 constexpr int kEmbWarps = 8;
-constexpr int kJoinWarps = 16;
+constexpr int kJoinWarps = 8;
 constexpr uint32_t kNoRow = 0xffffffffu;   // id of a token without a gradient: skipped row, index out of range
 
 // What the 32 lanes of a warp hold of a row: 32 * kE consecutive elements from a column on. kVec: 16 bytes per lane; otherwise (rows off
@@ -54,69 +54,102 @@ struct Slice {
     }
   }
   static __device__ __forceinline__ void store_f32(float* p, int left, const float (&f)[kE]) {
+    if constexpr (kVec) {
+      if (lane_id() * kE >= left) return;
 #pragma unroll
-    for (int i = 0; i < kE; ++i)
-      if (col(i) < left) p[col(i)] = f[i];
+      for (int i = 0; i < kE; i += 4) reinterpret_cast<float4*>(p + col(i))[0] = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kE; ++i)
+        if (col(i) < left) p[col(i)] = f[i];
+    }
   }
   static __device__ __forceinline__ void add_f32(const float* p, int left, bool on, float (&f)[kE]) {
+    if constexpr (kVec) {
+      if (!on || lane_id() * kE >= left) return;
 #pragma unroll
-    for (int i = 0; i < kE; ++i) f[i] += on && col(i) < left ? p[col(i)] : 0.f;
+      for (int i = 0; i < kE; i += 4) {
+        const float4 v = reinterpret_cast<const float4*>(p + col(i))[0];
+        f[i] += v.x;
+        f[i + 1] += v.y;
+        f[i + 2] += v.z;
+        f[i + 3] += v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kE; ++i) f[i] += on && col(i) < left ? p[col(i)] : 0.f;
+    }
+  }
+  static __device__ __forceinline__ void store_zero(void* p, size_t at, int left) {   // past the L2 where it may: nobody reads it soon
+    if constexpr (kVec) {
+      if (lane_id() * kE < left) __stcs(reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p) + at * kElemBytes<kType>) + lane_id(), make_uint4(0, 0, 0, 0));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kE; ++i)
+        if (col(i) < left) store_elem<kType>(p, static_cast<long long>(at) + col(i), 0.f);
+    }
   }
 };
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
-constexpr int kFwdSlices = 2;   // slices of a row per warp
+// A warp takes one slice of the columns for up to 8 consecutive tokens: their ids in one load, then kFwdRows tokens' rows of every table in flight. With a
+// token at a time the chain from an id to its row was walked for every kilobyte. Few tokens: fewer for each warp, so that they spread over the card.
+constexpr int kFwdTokens = 8, kFwdRows = 4;
 
-template <int kType, bool kVec>
-__global__ void __launch_bounds__(32 * kEmbWarps) embedding_fwd_kernel(const __grid_constant__ CcfEmbed e, void* __restrict__ y, int* status) {
+template <int kType, bool kVec, int kTables>
+__global__ void __launch_bounds__(32 * kEmbWarps) embedding_fwd_kernel(const __grid_constant__ CcfEmbed e, void* __restrict__ y, int* status, uint32_t each,
+                                                                       uint32_t slices) {
   using S = Slice<kType, kVec>;
-  const int first = blockIdx.y * kFwdSlices * S::kCols;
-  const uint32_t tokens = static_cast<uint32_t>(e.tokens), seq = static_cast<uint32_t>(e.seq);
-  for (uint32_t t = blockIdx.x * kEmbWarps + (threadIdx.x >> 5); t < tokens; t += gridDim.x * kEmbWarps) {
-    float sum[kFwdSlices][S::kE];
-    S part[CCF_EMBED_TABLES][kFwdSlices];
-    bool bad = false;
+  const uint32_t unit = blockIdx.x * kEmbWarps + (threadIdx.x >> 5), part = unit / slices, c = (unit - part * slices) * S::kCols;
+  const uint32_t tokens = static_cast<uint32_t>(e.tokens), begin = part * each;
+  if (begin >= tokens) return;
+  const uint32_t n = min(each, tokens - begin);
+  const int left = e.d - static_cast<int>(c);
+  long long id[kTables];
+  bool in = true;
 #pragma unroll
-    for (int k = 0; k < CCF_EMBED_TABLES; ++k) {
-      if (k >= e.tables) break;
-      const CcfEmbedTable& w = e.table[k];
-      const long long id = w.ids != nullptr ? load_index(w.ids, t, w.wide) : static_cast<long long>(t % seq);
-      const bool on = id >= 0 && id < w.rows;
-      bad = bad || !on;
+  for (int k = 0; k < kTables; ++k) {
+    const CcfEmbedTable& w = e.table[k];
+    const uint32_t t = begin + min(static_cast<uint32_t>(lane_id()), n - 1);
+    id[k] = w.ids != nullptr ? load_index(w.ids, t, w.wide) : static_cast<long long>(t % static_cast<uint32_t>(e.seq));
+    const bool here = id[k] >= 0 && id[k] < w.rows;
+    in = in && here;
+    id[k] = here ? id[k] : 0;
+  }
+  const uint32_t good = __ballot_sync(0xffffffffu, in);
+  if (c == 0 && !in && lane_id() < n) report_status(status, CCF_ERR_INDEX, static_cast<int>(begin + lane_id()) & 0x7fffff);
+  for (uint32_t t0 = 0; t0 < n; t0 += kFwdRows) {
+    S row[kTables][kFwdRows];
 #pragma unroll
-      for (int j = 0; j < kFwdSlices; ++j) {
-        const int c = first + j * S::kCols;
-        part[k][j].load(w.weight, static_cast<size_t>(on ? id : 0) * w.ld + c, e.d - c, on);
+    for (int u = 0; u < kFwdRows; ++u) {
+#pragma unroll
+      for (int k = 0; k < kTables; ++k) {
+        const long long r = __shfl_sync(0xffffffffu, id[k], t0 + u);
+        row[k][u].load(e.table[k].weight, static_cast<size_t>(r) * e.table[k].ld + c, left, t0 + u < n);
       }
     }
 #pragma unroll
-    for (int k = 0; k < CCF_EMBED_TABLES; ++k) {
-      if (k >= e.tables) break;
+    for (int u = 0; u < kFwdRows; ++u) {
+      if (t0 + u >= n) break;
+      float sum[S::kE];
 #pragma unroll
-      for (int j = 0; j < kFwdSlices; ++j) {
+      for (int k = 0; k < kTables; ++k) {
         float f[S::kE];
-        part[k][j].get(f);
+        row[k][u].get(f);
 #pragma unroll
-        for (int i = 0; i < S::kE; ++i) sum[j][i] = k == 0 ? f[i] * e.table[0].scale : fmaf(f[i], e.table[k].scale, sum[j][i]);
+        for (int i = 0; i < S::kE; ++i) sum[i] = k == 0 ? f[i] * e.table[0].scale : fmaf(f[i], e.table[k].scale, sum[i]);
       }
-    }
-    if (bad) {
-      if (lane_id() == 0 && blockIdx.y == 0) report_status(status, CCF_ERR_INDEX, static_cast<int>(t) & 0x7fffff);
+      if (!(good >> (t0 + u) & 1)) {
 #pragma unroll
-      for (int j = 0; j < kFwdSlices; ++j)
-#pragma unroll
-        for (int i = 0; i < S::kE; ++i) sum[j][i] = __int_as_float(0x7fc00000);
-    }
-#pragma unroll
-    for (int j = 0; j < kFwdSlices; ++j) {
-      const int c = first + j * S::kCols;
-      S::store(y, static_cast<size_t>(t) * e.d + c, e.d - c, sum[j]);
+        for (int i = 0; i < S::kE; ++i) sum[i] = __int_as_float(0x7fc00000);
+      }
+      S::store(y, static_cast<size_t>(begin + t0 + u) * e.d + c, left, sum);
     }
   }
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------
-// Scratch of one table. `keys`: (id << 32 | token), sorted. `present`: a bit per row that some token has. A run of equal ids is cut where
+// Scratch of one table. `keys`: (id << 32 | token), sorted. `slot`: for a row that some token has, one of its tokens. A run of equal ids is cut where
 // a piece of the sorted tokens ends: a piece leaves the sum of a run that came from the piece before in `head`, of one that began in it and goes on in
 // `tail`; `list` holds the pieces that left a tail.
 struct GradTable {
@@ -124,7 +157,7 @@ struct GradTable {
   void* grad;
   uint64_t* sorted_chunks;
   uint64_t* keys;
-  uint32_t* present;
+  uint32_t* slot;
   float* head;
   float* tail;
   int* list;
@@ -152,102 +185,132 @@ __device__ __forceinline__ uint64_t key_at(const GradArgs& g, const GradTable& t
   return static_cast<uint64_t>(s) << 32 | ((i - s * g.batch) * g.seq + s);
 }
 
-// Each block sorts one chunk of keys (bitonic, in shared memory). One chunk: that is the whole order, and the rows that occur are marked here.
-__global__ void __launch_bounds__(kSortChunk / 2) embedding_sort_kernel(const __grid_constant__ GradArgs g) {
-  __shared__ uint64_t key[kSortChunk];
+// Each block sorts one chunk of keys, one for each thread: bitonic, with exchanges inside a warp by shuffles and the others through shared memory.
+// Every token also leaves its place in `slot` at its id, whichever of equal ids comes last: a row is used if the token named there has its id. So
+// `slot` needs no zeros beforehand, and what it says is the same whoever won. 17 us with 2048 keys in shared memory alone, ? now.
+__global__ void __launch_bounds__(kSortChunk) embedding_sort_kernel(const __grid_constant__ GradArgs g) {
+  __shared__ uint64_t other[2][kSortChunk];
   const GradTable& t = g.table[blockIdx.y];
   let_next_in();
   if (blockIdx.x == 0 && threadIdx.x == 0) *t.count = 0;
   if (t.ids == nullptr) return;
-  const uint32_t words = static_cast<uint32_t>((t.rows + 31) / 32);
-  for (uint32_t w = blockIdx.x * blockDim.x + threadIdx.x; w < words; w += gridDim.x * blockDim.x) t.present[w] = 0;
-  const uint32_t base = blockIdx.x * kSortChunk, n = min(g.tokens - base, static_cast<uint32_t>(kSortChunk));
-  uint32_t len = 64;
-  while (len < n) len *= 2;
-  for (uint32_t i = threadIdx.x; i < len; i += blockDim.x) {
-    uint64_t k = ~0ull;
-    if (i < n) {
-      const long long id = load_index(t.ids, base + i, t.wide);
-      const bool in = id >= 0 && id < t.rows;
-      if (!in) report_status(g.status, CCF_ERR_INDEX, static_cast<int>(base + i) & 0x7fffff);
-      k = static_cast<uint64_t>(in && id != t.skip ? static_cast<uint32_t>(id) : kNoRow) << 32 | (base + i);
-    }
-    key[i] = k;
+  const uint32_t tid = threadIdx.x, base = blockIdx.x * kSortChunk, n = min(g.tokens - base, static_cast<uint32_t>(kSortChunk));
+  uint64_t key = ~0ull;
+  if (tid < n) {
+    const long long id = load_index(t.ids, base + tid, t.wide);
+    const bool in = id >= 0 && id < t.rows;
+    if (!in) report_status(g.status, CCF_ERR_INDEX, static_cast<int>(base + tid) & 0x7fffff);
+    else t.slot[id] = base + tid;
+    key = static_cast<uint64_t>(in && id != t.skip ? static_cast<uint32_t>(id) : kNoRow) << 32 | (base + tid);
   }
-  for (uint32_t size = 2; size <= len; size *= 2) {
-    for (uint32_t j = size / 2; j > 0; j /= 2) {
+  int half = 0;
+#pragma unroll 1
+  for (uint32_t size = 2; size < 2 * n; size *= 2) {
+    const bool up = (tid & size) == 0;
+#pragma unroll 1
+    for (uint32_t j = size / 2; j >= 32; j /= 2, half ^= 1) {
+      other[half][tid] = key;
       __syncthreads();
-      if (threadIdx.x < len / 2) {
-        const uint32_t i = 2 * threadIdx.x - (threadIdx.x & (j - 1));
-        const uint64_t a = key[i], b = key[i + j];
-        if ((a > b) == ((i & size) == 0)) {
-          key[i] = b;
-          key[i + j] = a;
-        }
+      const uint64_t o = other[half][tid ^ j];
+      key = (((tid & j) == 0) == up) == (o < key) ? o : key;
+    }
+#pragma unroll
+    for (uint32_t j = 16; j > 0; j /= 2) {
+      if (j >= size) continue;
+      const uint64_t o = __shfl_xor_sync(0xffffffffu, key, j);
+      key = (((tid & j) == 0) == up) == (o < key) ? o : key;
+    }
+  }
+  if (tid < n) t.sorted_chunks[base + tid] = key;
+}
+
+// A key's place among all: its place in its own chunk and, for every other chunk, the keys there that are smaller: those of smaller ids and, in earlier
+// chunks, of the same. A block has a chunk's keys, one for each thread, and searches kSide chunks at a time, whose ids it brings into shared memory:
+// eleven steps there take less than one read from L2 (10 us with the searches in L2, ? now).
+constexpr int kSide = 8;
+__global__ void __launch_bounds__(kSortChunk) embedding_merge_kernel(const __grid_constant__ GradArgs g) {
+  __shared__ uint32_t ids[kSide][kSortChunk];
+  after_previous();
+  const GradTable& t = g.table[blockIdx.y];
+  if (t.ids == nullptr) return;
+  const uint32_t tid = threadIdx.x, own = blockIdx.x, i = own * kSortChunk + tid;
+  const uint64_t* src = t.sorted_chunks;
+  const uint64_t key = i < g.tokens ? src[i] : ~0ull;
+  const uint32_t id = id_of(key);
+  uint32_t place = tid;
+  for (uint32_t c = 0; c < g.chunks; c += kSide) {
+#pragma unroll
+    for (int u = 0; u < kSide; ++u) {
+      const uint32_t at = (c + u) * kSortChunk + tid;
+      ids[u][tid] = c + u != own && at < g.tokens ? id_of(src[at]) : 0xffffffffu;
+    }
+    __syncthreads();
+    uint32_t lo[kSide] = {};
+#pragma unroll
+    for (uint32_t step = kSortChunk; step > 0; step /= 2) {
+#pragma unroll
+      for (int u = 0; u < kSide; ++u) {
+        const uint32_t to = lo[u] + step;
+        if (to > kSortChunk) continue;
+        const uint32_t o = ids[u][to - 1];
+        if (o < id || (o == id && c + u < own)) lo[u] = to;
       }
     }
-  }
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-    t.sorted_chunks[base + i] = key[i];
-    if (g.chunks == 1) {
-      const uint32_t id = id_of(key[i]);
-      if (id != kNoRow && (i == 0 || id_of(key[i - 1]) != id)) atomicOr(t.present + id / 32, 1u << (id % 32));
+#pragma unroll
+    for (int u = 0; u < kSide; ++u) {
+      // tokens without a row carry the id of places that hold none: those do not count
+      const uint32_t n = c + u >= g.chunks || c + u == own ? 0 : min(g.tokens - (c + u) * kSortChunk, static_cast<uint32_t>(kSortChunk));
+      place += min(lo[u], n);
     }
+    __syncthreads();
   }
+  if (i < g.tokens) t.keys[place] = key;
 }
 
-// A key's place among all: its place in its own chunk and, for every other chunk, the keys there that are smaller. Keys differ.
-__global__ void __launch_bounds__(256) embedding_merge_kernel(const __grid_constant__ GradArgs g) {
-  after_previous();
-  const GradTable& t = g.table[blockIdx.y];
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-  if (t.ids == nullptr || i >= g.tokens) return;
-  const uint64_t* src = t.sorted_chunks;
-  const uint64_t k = src[i];
-  const uint32_t own = i / kSortChunk;
-  uint32_t place = i % kSortChunk;
-  for (uint32_t c = 0; c < g.chunks; ++c) {
-    if (c == own) continue;
-    const uint64_t* p = src + c * kSortChunk;
-    uint32_t lo = 0, hi = min(g.tokens - c * kSortChunk, static_cast<uint32_t>(kSortChunk));
-    while (lo < hi) {
-      const uint32_t mid = (lo + hi) / 2;
-      if (p[mid] < k) lo = mid + 1;
-      else hi = mid;
-    }
-    place += lo;
-  }
-  t.keys[place] = k;
-  const uint32_t id = id_of(k);
-  if (id != kNoRow && (i % kSortChunk == 0 || id_of(src[i - 1]) != id)) atomicOr(t.present + id / 32, 1u << (id % 32));
-}
-
-// The first blocks of a table sum: a warp takes one piece of the sorted tokens and one slice of the columns. The others write the zeros of
-// the rows that no token has, 32 rows each.
+// Sums, then zeros. Positions are summed first: their order is known, so these blocks do not wait for the sort, and they leave dy in L2 for the sums by id
+// behind them. A warp takes one piece of the sorted tokens and one slice of the columns. The last blocks write the zeros of the rows that no token has, 32
+// rows each; those need the sorting kernel's results only, not the merging one's, which has waited for it.
 template <int kType, bool kVec>
-__global__ void __launch_bounds__(32 * kEmbWarps) embedding_sum_kernel(const __grid_constant__ GradArgs g) {
+__global__ void __launch_bounds__(32 * kEmbWarps, 3) embedding_sum_kernel(const __grid_constant__ GradArgs g) {
   using S = Slice<kType, kVec>;
   constexpr int kUnroll = kVec ? 8 : 2;
-  after_previous();
-  const GradTable& t = g.table[blockIdx.y];
   const uint32_t warp = threadIdx.x >> 5, units = g.pieces * g.slices, sum_blocks = (units + kEmbWarps - 1) / kEmbWarps;
-  if (blockIdx.x >= sum_blocks) {
-    const uint32_t w = blockIdx.x - sum_blocks;
-    if (w >= (t.rows + 31) / 32) return;
-    uint32_t present = 0;
-    if (t.ids != nullptr) present = t.present[w];
-    else if (w < (g.seq + 31) / 32) present = g.seq - w * 32 >= 32 ? 0xffffffffu : (1u << (g.seq - w * 32)) - 1u;
-    const float zero[S::kE] = {};
-    for (uint32_t r = warp; r < 32; r += kEmbWarps) {
-      const long long row = static_cast<long long>(w) * 32 + r;
-      if ((present >> r & 1) || row >= t.rows) continue;
-      for (int c = 0; c < g.d; c += S::kCols) S::store(t.grad, static_cast<size_t>(row) * g.d + c, g.d - c, zero);
+  if (blockIdx.x >= sum_blocks * g.tables) {
+    uint32_t w = blockIdx.x - sum_blocks * g.tables;
+    int k = 0;
+    while (w >= (g.table[k].rows + 31) / 32) w -= static_cast<uint32_t>((g.table[k++].rows + 31) / 32);
+    const GradTable& t = g.table[k];
+    if (t.ids != nullptr && g.chunks == 1) wait_for_previous();
+    let_next_in();
+    const long long row = static_cast<long long>(w) * 32 + warp * 4 + lane_id();
+    bool used = true;
+    if (lane_id() < 4 && row < t.rows) {
+      if (t.ids == nullptr) {
+        used = row < g.seq;
+      } else {
+        const uint32_t at = __ldcg(t.slot + row);
+        used = row != t.skip && at < g.tokens &&
+               (t.wide ? __ldcg(reinterpret_cast<const long long*>(t.ids) + at) : __ldcg(reinterpret_cast<const int*>(t.ids) + at)) == row;
+      }
     }
+    const uint32_t unused = __ballot_sync(0xffffffffu, !used);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (!(unused >> r & 1)) continue;
+      const size_t at = (static_cast<size_t>(w) * 32 + warp * 4 + r) * g.d;
+      for (int c = 0; c < g.d; c += S::kCols) S::store_zero(t.grad, at + c, g.d - c);
+    }
+    wait_for_previous();   // every block waits before it ends, so that the end of this kernel is the end of those in front of it
     return;
   }
-  const uint32_t unit = blockIdx.x * kEmbWarps + warp;
-  if (unit >= units) return;
+  const GradTable& t = g.table[blockIdx.x / sum_blocks];
+  if (t.ids != nullptr) wait_for_previous();
+  let_next_in();
+  const uint32_t unit = blockIdx.x % sum_blocks * kEmbWarps + warp;
+  if (unit >= units) {
+    wait_for_previous();
+    return;
+  }
   const uint32_t piece = unit / g.slices, c = (unit - piece * g.slices) * S::kCols;
   const int left = g.d - static_cast<int>(c);
   const uint32_t begin = piece * g.piece, n = min(g.piece, g.tokens - begin);
@@ -263,7 +326,10 @@ __global__ void __launch_bounds__(32 * kEmbWarps) embedding_sum_kernel(const __g
         S::store_f32(t.head + static_cast<size_t>(piece) * g.d + c, left, acc);
       } else if (goes_on) {
         S::store_f32(t.tail + static_cast<size_t>(piece) * g.d + c, left, acc);
-        if (c == 0 && lane_id() == 0) t.list[atomicAdd(t.count, 1)] = static_cast<int>(piece);
+        if (c == 0 && lane_id() == 0) {
+          wait_for_previous();   // the sorting kernel zeroed the count
+          t.list[atomicAdd(t.count, 1)] = static_cast<int>(piece);
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < S::kE; ++i) acc[i] *= t.scale;
@@ -297,6 +363,7 @@ __global__ void __launch_bounds__(32 * kEmbWarps) embedding_sum_kernel(const __g
     }
   }
   finish(after == run);
+  wait_for_previous();
 }
 
 // Runs that cross pieces: tail of the piece where the run began, then the heads of those behind it. kJoinWarps warps take every
@@ -305,7 +372,7 @@ template <int kType, bool kVec>
 __global__ void __launch_bounds__(32 * kJoinWarps) embedding_join_kernel(const __grid_constant__ GradArgs g) {
   using S = Slice<kType, kVec>;
   constexpr int kUnroll = 4;
-  __shared__ float red[kJoinWarps][S::kCols];
+  __shared__ __align__(16) float red[kJoinWarps][S::kCols];
   after_previous();
   const GradTable& t = g.table[blockIdx.y];
   const uint32_t warp = threadIdx.x >> 5, items = static_cast<uint32_t>(*t.count) * g.slices;
@@ -362,7 +429,7 @@ static size_t lay_out(GradTable* t, void* base, long long tokens, long long rows
   x.head = reinterpret_cast<float*>(take(4 * pieces * d));
   x.tail = reinterpret_cast<float*>(take(4 * pieces * d));
   if (sorted) {
-    x.present = reinterpret_cast<uint32_t*>(take((static_cast<size_t>(rows) + 31) / 32 * 4));
+    x.slot = reinterpret_cast<uint32_t*>(take(4 * static_cast<size_t>(rows)));
     x.sorted_chunks = reinterpret_cast<uint64_t*>(take(8 * n));
     x.keys = n > kSortChunk ? reinterpret_cast<uint64_t*>(take(8 * n)) : x.sorted_chunks;
   }
@@ -371,7 +438,7 @@ static size_t lay_out(GradTable* t, void* base, long long tokens, long long rows
     t->list = x.list;
     t->head = x.head;
     t->tail = x.tail;
-    t->present = x.present;
+    t->slot = x.slot;
     t->sorted_chunks = x.sorted_chunks;
     t->keys = x.keys;
   }
@@ -405,9 +472,14 @@ static cudaError_t launch_behind(void (*kern)(KArgs...), dim3 grid, int threads,
 
 template <int kType, bool kVec>
 static int launch_fwd(const CcfEmbed& e, void* y, int* status, cudaStream_t st) {
-  const unsigned slices = (e.d + Slice<kType, kVec>::kCols - 1) / Slice<kType, kVec>::kCols, gy = (slices + kFwdSlices - 1) / kFwdSlices;
-  const long long need = (e.tokens + kEmbWarps - 1) / kEmbWarps, most = 1 + 16ll * sm_count() / gy;
-  embedding_fwd_kernel<kType, kVec><<<dim3(static_cast<unsigned>(need < most ? need : most), gy), 32 * kEmbWarps, 0, st>>>(e, y, status);
+  const uint32_t slices = (e.d + Slice<kType, kVec>::kCols - 1) / Slice<kType, kVec>::kCols;
+  uint32_t each = kFwdTokens;
+  while (each > 1 && (e.tokens + each - 1) / each * slices < 16 * 148) each /= 2;   // 16 warps an SM at least, while there are that many
+  const long long units = (e.tokens + each - 1) / each * slices, blocks = (units + kEmbWarps - 1) / kEmbWarps;
+  if (units > 0xffffffffll || blocks > 0x7fffffffll) return -2;
+  const auto kern = e.tables == 1 ? embedding_fwd_kernel<kType, kVec, 1> : e.tables == 2 ? embedding_fwd_kernel<kType, kVec, 2>
+                                                                                        : embedding_fwd_kernel<kType, kVec, 3>;
+  kern<<<static_cast<unsigned>(blocks), 32 * kEmbWarps, 0, st>>>(e, y, status, each, slices);
   return launch_result();
 }
 
@@ -415,24 +487,24 @@ template <int kType, bool kVec>
 static int launch_bwd(GradArgs& g, cudaStream_t st) {
   using S = Slice<kType, kVec>;
   g.slices = (g.d + S::kCols - 1) / S::kCols;
-  unsigned most = 0;
+  long long blocks = static_cast<long long>((static_cast<size_t>(g.pieces) * g.slices + kEmbWarps - 1) / kEmbWarps) * g.tables;
   bool sorted = false;
   for (int k = 0; k < g.tables; ++k) {
-    const unsigned blocks = (g.pieces * g.slices + kEmbWarps - 1) / kEmbWarps + static_cast<unsigned>((g.table[k].rows + 31) / 32);
-    most = blocks > most ? blocks : most;
+    blocks += (g.table[k].rows + 31) / 32;
     sorted = sorted || g.table[k].ids != nullptr;
   }
+  if (blocks > 0x7fffffffll || static_cast<long long>(g.pieces) * g.slices > 0xffffffffll) return -2;
   int launches = 2;
-  embedding_sort_kernel<<<dim3(sorted ? g.chunks : 1, g.tables), kSortChunk / 2, 0, st>>>(g);
+  embedding_sort_kernel<<<dim3(sorted ? g.chunks : 1, g.tables), kSortChunk, 0, st>>>(g);
   cudaError_t err = cudaGetLastError();
   if (err == cudaSuccess && sorted && g.chunks > 1) {
-    err = launch_behind(embedding_merge_kernel, dim3((g.tokens + 255) / 256, g.tables), 256, st, g);
+    err = launch_behind(embedding_merge_kernel, dim3(g.chunks, g.tables), kSortChunk, st, g);
     ++launches;
   }
-  if (err == cudaSuccess) err = launch_behind(embedding_sum_kernel<kType, kVec>, dim3(most, g.tables), 32 * kEmbWarps, st, g);
+  if (err == cudaSuccess) err = launch_behind(embedding_sum_kernel<kType, kVec>, dim3(static_cast<unsigned>(blocks)), 32 * kEmbWarps, st, g);
   if (err == cudaSuccess && g.pieces > 1) {
-    const unsigned blocks = g.pieces * g.slices, wave = 2 * sm_count();
-    err = launch_behind(embedding_join_kernel<kType, kVec>, dim3(blocks < wave ? blocks : wave, g.tables), 32 * kJoinWarps, st, g);
+    const unsigned items = g.pieces * g.slices, wave = 4 * sm_count();
+    err = launch_behind(embedding_join_kernel<kType, kVec>, dim3(items < wave ? items : wave, g.tables), 32 * kJoinWarps, st, g);
     ++launches;
   }
   return err == cudaSuccess ? launches : -static_cast<int>(err);
@@ -491,8 +563,12 @@ int ccf_embedding_bwd(const CcfEmbed* e, const void* dy, int* status, void* stre
   g.chunks = (g.tokens + kSortChunk - 1) / kSortChunk;
   g.tables = e->tables;
   g.d = e->d;
+  int order[CCF_EMBED_TABLES], n = 0;   // tables without ids first (embedding_sum_kernel)
+  for (int sorted = 0; sorted < 2; ++sorted)
+    for (int k = 0; k < e->tables; ++k)
+      if ((e->table[k].ids != nullptr) == (sorted != 0)) order[n++] = k;
   for (int k = 0; k < e->tables; ++k) {
-    const CcfEmbedTable& t = e->table[k];
+    const CcfEmbedTable& t = e->table[order[k]];
     if (t.grad == nullptr || t.scratch == nullptr || !on16(t.scratch)) return -2;
     vec = vec && on16(t.grad);
     GradTable& o = g.table[k];

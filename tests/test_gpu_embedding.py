@@ -39,7 +39,7 @@ def _run(ids, w, scale=1.0, dy=None, padding_idx=None, **kw):
 
 # tokens: one, a piece and around it, a sorted chunk and around it, several chunks; d: off and on 16 bytes, beyond one slice of a warp
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("tokens,rows,d", [(1, 1, 1), (1, 40, 8), (7, 3, 17), (8, 3, 64), (9, 100, 200), (33, 2, 1000), (2047, 5, 24), (2048, 700, 256),
+@pytest.mark.parametrize("tokens,rows,d", [(1, 1, 1), (1, 40, 8), (7, 3, 17), (8, 3, 64), (9, 100, 200), (33, 2, 1000), (1023, 5, 24), (1024, 700, 256), (1025, 1, 8),
                                            (2049, 33, 264), (5000, 64, 513), (6145, 6145, 40)])
 def test_sizes(dtype, tokens, rows, d):
     g, dt = _gen(tokens + d), TYPES[dtype]
