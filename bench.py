@@ -146,7 +146,9 @@ def classify_kernel(kname: str, scopes: str, shapes: str, vocab_padded: int, d_f
         if sum(1 for v in dims if v == str(d_ffn)) >= (2 if tokens == d_ffn else 1):
             return "dense_ffn_gemms"
         return "attention_projection_gemms"
-    if any(t in scopes for t in ("cross_entropy", "log_softmax", "nll_loss")) or "softmax" in k:
+    if "ccf::embedding_" in k:
+        return "embedding"
+    if any(t in scopes for t in ("cross_entropy", "log_softmax", "nll_loss")) or "softmax" in k or "ccf::logprobs_" in k:
         return "cross_entropy"
     if "layer_norm" in k or "layernorm" in scopes.lower():
         return "layernorm"

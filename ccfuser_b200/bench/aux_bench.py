@@ -1,6 +1,6 @@
 """Device-timed throughput of the memory-bound kernels around the grouped GEMMs on one GPU: router (forward and its
-GEMM-free backward), LayerNorm (forward / backward), grouped column sums, slot reduce, SGD step. Each case prints one
-JSON line with the achieved bytes per second against the measured copy bandwidth (MEASURED_PEAKS.json at the
+GEMM-free backward), LayerNorm (forward / backward), grouped column sums, slot reduce, SGD step, token embedding, log
+probabilities and dropout (forward / backward each). Each case prints one JSON line with the achieved bytes per second against the measured copy bandwidth (MEASURED_PEAKS.json at the
 repository root when present): these kernels read or write a [tokens, d] matrix once, so that is their roofline.
 
     python -m ccfuser_b200.bench.aux_bench --tokens 16384 --d-model 2048 --experts 64
@@ -23,7 +23,8 @@ def main():
     ap.add_argument("--d-ffn", type=int, default=8192)
     ap.add_argument("--experts", type=int, default=64)
     ap.add_argument("--top-k", type=int, default=2)
-    ap.add_argument("--cases", default="router,router_bwd,layernorm,colsum,reduce,sgd")
+    ap.add_argument("--cases", default="router,router_bwd,layernorm,colsum,reduce,sgd,embedding,logprobs,dropout")
+    ap.add_argument("--vocab", type=int, default=50304)
     ap.add_argument("--iters", type=int, default=10)
     args = ap.parse_args()
     _, hbm, src = measured_peaks()
@@ -103,6 +104,32 @@ def main():
         g = torch.randn(n, device=dev, dtype=torch.bfloat16)
         report("sgd_step", 3 * n * 2,
                lambda: N.check(lib.ccf_sgd_step(p.data_ptr(), g.data_ptr(), n, 1e-4, 0.0, 0, N.stream_ptr()), "ccf_sgd_step"))
+
+    v = args.vocab
+
+    def both(name, fwd_bytes, bwd_bytes, fn, inputs):
+        with torch.no_grad():
+            report(name + "_forward", fwd_bytes, fn)
+        out = fn()
+        up = torch.randn_like(out)
+        report(name + "_backward", bwd_bytes, lambda: torch.autograd.grad(out, inputs, up, retain_graph=True))
+    if "embedding" in cases:
+        from ..ops.embedding import embedding
+        table = (torch.randn(v, d, device=dev) * 0.02).bfloat16().requires_grad_(True)
+        ids = torch.randint(0, v, (t,), device=dev)
+        both("embedding", (min(t, v) + t) * d * 2, (t + v) * d * 2, lambda: embedding(ids, table), [table])
+    if "logprobs" in cases:
+        from ..ops.logprobs import token_logprobs
+        rows = min(t, 8192)
+        logits = torch.randn(rows, v, device=dev, dtype=torch.bfloat16).requires_grad_(True)
+        targets = torch.randint(0, v, (rows,), device=dev)
+        both("logprobs", rows * v * 2, rows * v * 4, lambda: token_logprobs(logits, targets).logprobs, [logits])
+        with torch.no_grad():
+            report("logprobs_top_5_forward", rows * v * 2, lambda: token_logprobs(logits, targets, top_k=5))
+    if "dropout" in cases:
+        from ..ops.dropout import dropout
+        xd, state = x.clone().requires_grad_(True), torch.tensor([1, 0], device=dev)
+        both("dropout_add", 3 * t * d * 2, 2 * t * d * 2, lambda: dropout(xd, 0.1, state, residual=x), [xd])
 
 
 if __name__ == "__main__":

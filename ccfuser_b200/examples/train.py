@@ -83,7 +83,7 @@ def build(args, world, dev, ep_group=None):
     else:
         b, s = args.batch or 16, args.seq or 512
         c = TransformerXLMoEConfig(router_dtype=torch.float32 if args.router_fp32 else None, aux_loss_coef=args.aux_loss_coef,
-                                   z_loss_coef=args.z_loss_coef, n_token=getattr(args, "n_token", 0) or 100, n_layer=args.layers or 12, tgt_len=s, mem_len=s, moe=moe,
+                                   z_loss_coef=args.z_loss_coef, dropout=getattr(args, "dropout", 0.0), n_token=getattr(args, "n_token", 0) or 100, n_layer=args.layers or 12, tgt_len=s, mem_len=s, moe=moe,
                                    num_experts=args.experts_per_gpu * world, top_k=args.top_k,
                                    capacity_factor=args.cf or None, ep_size=world, backend=backend, max_tokens=b * s, dtype=dtype)
         model = _TXLStep(TransformerXLMoE(c, ep_group=ep_group, device=dev))
@@ -113,6 +113,7 @@ def main():
     ap.add_argument("--fuse-expert-sgd", action="store_true",
                     help="fused variant with --optimizer sgd: expert weight matrices are updated inside the backward pass "
                          "(MoELayer.fuse_sgd; all of them when the experts live on one rank, the second projection otherwise)")
+    ap.add_argument("--dropout", type=float, default=0.0, help="txl only: dropout of the embedding, the residual branches and the output")
     ap.add_argument("--data", default="", help="txl only: training text file (word-level vocabulary built from it); "
                                                "default is a fixed synthetic batch")
     ap.add_argument("--valid", default="", help="txl only: validation text file, evaluated at the end")
@@ -226,6 +227,8 @@ def main():
     if corpus is not None and args.valid and corpus.data["valid"].numel() > (args.batch or 16) * ((args.seq or 512) + 1):
         from ..utils.data import evaluate_lm
         model.mems = None
+        if args.dropout > 0:
+            model.eval()
         val = evaluate_lm(lambda x, y: model({"ids": x, "labels": y}),
                           corpus.iterator("valid", args.batch or 16, args.seq or 512, device=dev), max_batches=50)
         if rank == 0:

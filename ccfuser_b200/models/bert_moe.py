@@ -17,6 +17,7 @@ import torch.nn.functional as F
 
 from ..config import MoEConfig
 from ..layers import MoELayer
+from ..ops.embedding import Embedding
 from ..ops.norm import LayerNorm
 
 
@@ -102,9 +103,9 @@ class BertMoEForQuestionAnswering(nn.Module):
     def __init__(self, c: BertMoEConfig, ep_group=None, device=None):
         super().__init__()
         self.config = c
-        self.word = nn.Embedding(c.vocab_size, c.d_model, device=device, dtype=c.dtype)
-        self.position = nn.Embedding(c.max_position, c.d_model, device=device, dtype=c.dtype)
-        self.token_type = nn.Embedding(c.type_vocab_size, c.d_model, device=device, dtype=c.dtype)
+        self.word = Embedding(c.vocab_size, c.d_model, device=device, dtype=c.dtype)
+        self.position = Embedding(c.max_position, c.d_model, device=device, dtype=c.dtype)
+        self.token_type = Embedding(c.type_vocab_size, c.d_model, device=device, dtype=c.dtype)
         self.ln_emb = LayerNorm(c.d_model, eps=c.layer_norm_eps, device=device, dtype=c.dtype)
         self.layer = nn.ModuleList([BertLayer(c, i in set(c.moe_layers), ep_group, device) for i in range(c.n_layer)])
         self.qa_outputs = nn.Linear(c.d_model, 2, device=device, dtype=c.dtype)
@@ -117,10 +118,8 @@ class BertMoEForQuestionAnswering(nn.Module):
                     nn.init.zeros_(m.bias)
 
     def forward(self, input_ids, attention_mask=None, token_type_ids=None, start_positions=None, end_positions=None):
-        b, s = input_ids.shape
-        pos = torch.arange(s, device=input_ids.device)
         tt = token_type_ids if token_type_ids is not None else torch.zeros_like(input_ids)
-        x = self.ln_emb(self.word(input_ids) + self.position(pos) + self.token_type(tt))
+        x = self.ln_emb(self.word(input_ids, position_weight=self.position.weight, type_weight=self.token_type.weight, type_ids=tt))
         mask = token_mask = None
         if attention_mask is not None:
             mask = attention_mask[:, None, None, :].to(torch.bool)

@@ -18,6 +18,8 @@ import torch.nn.functional as F
 
 from ..config import MoEConfig
 from ..layers import MoELayer
+from ..ops.embedding import Embedding
+from ..ops.logprobs import TokenLogprobs, cross_entropy, token_logprobs
 from ..ops.norm import LayerNorm
 
 
@@ -126,16 +128,17 @@ class Block(nn.Module):
 
 
 class GPTMoE(nn.Module):
-    """``forward(ids [B,S], labels=None)`` -> logits, or the mean next-token cross-entropy when labels are given."""
+    """``forward(ids [B,S], labels=None)`` -> logits, or the mean next-token cross-entropy when labels are given (labels of -100 are left
+    out). ``score(ids)`` -> log probabilities of the given tokens, entropies and best alternatives."""
 
     def __init__(self, c: GPTMoEConfig, ep_group=None, device=None):
         super().__init__()
         self.config = c
         # the embedding / LM-head matrix is padded to a multiple of 128 rows so the vocabulary GEMM runs on an
-        # aligned tensor-core kernel; the padding columns of the logits are masked out of the softmax
+        # aligned tensor-core kernel; the padding columns of the logits stay out of the softmax
         self.vocab_padded = (c.vocab_size + 127) // 128 * 128
-        self.wte = nn.Embedding(self.vocab_padded, c.d_model, device=device, dtype=c.dtype)
-        self.wpe = nn.Embedding(c.seq_len, c.d_model, device=device, dtype=c.dtype)
+        self.wte = Embedding(self.vocab_padded, c.d_model, device=device, dtype=c.dtype)
+        self.wpe = Embedding(c.seq_len, c.d_model, device=device, dtype=c.dtype)
         self.h = nn.ModuleList([Block(c, c.is_moe(i), ep_group, device) for i in range(c.n_layer)])
         self.ln_f = LayerNorm(c.d_model, device=device, dtype=c.dtype)
         self.apply(self._init)
@@ -156,19 +159,24 @@ class GPTMoE(nn.Module):
             if m.bias is not None:
                 nn.init.zeros_(m.bias)
 
-    def forward(self, ids: torch.Tensor, labels: Optional[torch.Tensor] = None):
-        b, s = ids.shape
-        pos = torch.arange(s, device=ids.device)
-        x = self.wte(ids) + self.wpe(pos)
+    def _logits(self, ids):
+        x = self.wte(ids, position_weight=self.wpe.weight)
         for blk in self.h:
             x = blk(x)
-        x = self.ln_f(x)
-        logits = F.linear(x, self.wte.weight)
-        if self.vocab_padded != self.config.vocab_size:
-            logits[..., self.config.vocab_size:] = float("-inf")
+        return F.linear(self.ln_f(x), self.wte.weight)
+
+    def forward(self, ids: torch.Tensor, labels: Optional[torch.Tensor] = None):
+        logits = self._logits(ids)
         if labels is None:
             return logits[..., :self.config.vocab_size]
-        return F.cross_entropy(logits.view(-1, logits.shape[-1]).float(), labels.reshape(-1))
+        return cross_entropy(logits, labels, self.config.vocab_size)
+
+    def score(self, ids: torch.Tensor, top_k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+        """For every token of ``ids [B,S]`` but the first, given those before it: log probability, the entropy of its distribution and the
+        ``top_k`` most probable tokens, each ``[B,S-1]`` (and ``top_k`` more columns)."""
+        targets = F.pad(ids[:, 1:], (0, 1), value=-100)      # all rows at once: the last place has no target
+        out = token_logprobs(self._logits(ids), targets, top_k, temperature, self.config.vocab_size)
+        return TokenLogprobs(*(None if t is None else t[:, :-1] for t in out))
 
     def moe_layers(self):
         return [blk.mlp for blk in self.h if blk.is_moe]

@@ -7,7 +7,8 @@ and replaces ``PositionwiseFF`` in every ``RelPartialLearnableDecoderLayer``
 over a 100-token vocabulary, 12 layers, d_model 512, 8 heads, d_inner 2048, tgt_len = mem_len = 512
 (mix_moe/ae/fig11_data.sh:52-92, mix_moe/mix_moe/examples/transformer-xl/train_ddp.py:228,360-361).
 This module is a compact re-implementation of that architecture: batch-first tensors, the standard
-``rel_shift`` formulation of (q + u) k^T + (q + v) r^T, cached hidden states as memory, plain or adaptive softmax.
+``rel_shift`` formulation of (q + u) k^T + (q + v) r^T, cached hidden states as memory, plain or adaptive softmax, dropout
+on the embedding, on what each sublayer adds to the residual stream and on the last layer's output.
 """
 from __future__ import annotations
 
@@ -15,11 +16,15 @@ import dataclasses
 from typing import List, Optional, Sequence
 
 import torch
+import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
 from ..config import MoEConfig
 from ..layers import MoELayer
+from ..ops.dropout import Dropout, DropoutState
+from ..ops.embedding import Embedding
+from ..ops.logprobs import cross_entropy
 from ..ops.norm import LayerNorm
 
 
@@ -46,6 +51,7 @@ class TransformerXLMoEConfig:
     pre_lnorm: bool = False
     adaptive_cutoffs: Sequence[int] = ()
     dropout: float = 0.0
+    dropout_seed: Optional[int] = None     # default: drawn from torch's generator; ranks of a job add their number
 
     router_dtype: Optional[torch.dtype] = None
     aux_loss_coef: float = 0.0
@@ -120,7 +126,7 @@ class RelPartialLearnableAttention(nn.Module):
 
 class DecoderLayer(nn.Module):
     """Attention with memory, then the position-wise FFN (dense or MoE)."""
-    def __init__(self, c: TransformerXLMoEConfig, ep_group=None, device=None):
+    def __init__(self, c: TransformerXLMoEConfig, ep_group=None, device=None, drop=None):
         super().__init__()
         self.attn = RelPartialLearnableAttention(c, device)
         self.ln1 = LayerNorm(c.d_model, device=device, dtype=c.dtype)
@@ -128,13 +134,17 @@ class DecoderLayer(nn.Module):
         self.is_moe = c.moe
         self.pos_ff = MoELayer(c.moe_config(), ep_group=ep_group, device=device) if c.moe else PositionwiseFF(c, device)
         self.pre_lnorm = c.pre_lnorm
+        self.drop = drop
+
+    def _add(self, x, branch):
+        return x + branch if self.drop is None else self.drop(branch, residual=x)
 
     def forward(self, x, r, r_w_bias, r_r_bias, mask, mem):
         if self.pre_lnorm:
-            x = x + self.attn(self.ln1(x), r, r_w_bias, r_r_bias, mask, None if mem is None else self.ln1(mem))
-            return x + self.pos_ff(self.ln2(x))
-        x = self.ln1(x + self.attn(x, r, r_w_bias, r_r_bias, mask, mem))
-        return self.ln2(x + self.pos_ff(x))
+            x = self._add(x, self.attn(self.ln1(x), r, r_w_bias, r_r_bias, mask, None if mem is None else self.ln1(mem)))
+            return self._add(x, self.pos_ff(self.ln2(x)))
+        x = self.ln1(self._add(x, self.attn(x, r, r_w_bias, r_r_bias, mask, mem)))
+        return self.ln2(self._add(x, self.pos_ff(x)))
 
 
 class TransformerXLMoE(nn.Module):
@@ -143,12 +153,15 @@ class TransformerXLMoE(nn.Module):
     def __init__(self, c: TransformerXLMoEConfig, ep_group=None, device=None):
         super().__init__()
         self.config = c
-        self.word_emb = nn.Embedding(c.n_token, c.d_model, device=device, dtype=c.dtype)
+        self.word_emb = Embedding(c.n_token, c.d_model, scale=c.d_model ** 0.5, device=device, dtype=c.dtype)
         self.pos_emb = PositionalEmbedding(c.d_model, device)
         self.r_w_bias = nn.Parameter(torch.zeros(c.n_head, c.d_head, device=device, dtype=c.dtype))
         self.r_r_bias = nn.Parameter(torch.zeros(c.n_head, c.d_head, device=device, dtype=c.dtype))
-        self.layers = nn.ModuleList([DecoderLayer(c, ep_group, device) for _ in range(c.n_layer)])
-        self.emb_scale = c.d_model ** 0.5
+        self.drop = None
+        if c.dropout > 0:
+            seed = int(torch.randint(2 ** 62, (1,))) if c.dropout_seed is None else c.dropout_seed
+            self.drop = Dropout(c.dropout, DropoutState(seed + (dist.get_rank() if dist.is_initialized() else 0), device))
+        self.layers = nn.ModuleList([DecoderLayer(c, ep_group, device, self.drop) for _ in range(c.n_layer)])
         if c.adaptive_cutoffs:
             self.crit = nn.AdaptiveLogSoftmaxWithLoss(c.d_model, c.n_token, list(c.adaptive_cutoffs), device=device)
         else:
@@ -185,7 +198,11 @@ class TransformerXLMoE(nn.Module):
             mems = self.init_mems(b, data.device)
         m_len = mems[0].shape[1] if mems is not None else 0
         k_len = m_len + q
-        x = self.word_emb(data) * self.emb_scale
+        x = self.word_emb(data)
+        if self.drop is not None:
+            if self.training:
+                self.drop.state.begin_step(data.device)
+            x = self.drop(x)
         pos_seq = torch.arange(k_len - 1, -1, -1.0, device=data.device)
         r = self.pos_emb(pos_seq).to(x.dtype)
         mask = torch.triu(torch.ones(q, k_len, device=data.device, dtype=torch.bool), diagonal=1 + m_len)[None, None]
@@ -194,13 +211,14 @@ class TransformerXLMoE(nn.Module):
             hids.append(x)
             x = layer(x, r, self.r_w_bias, self.r_r_bias, mask, None if mems is None else mems[i])
         new_mems = self._update_mems(hids, mems, q)
+        if self.drop is not None:
+            x = self.drop(x)
         if target is None:
             return x, new_mems
         if self.crit is not None:
             loss = self.crit(x.reshape(-1, x.shape[-1]).float(), target.reshape(-1)).loss
         else:
-            logits = F.linear(x, self.word_emb.weight).float()
-            loss = F.cross_entropy(logits.view(-1, logits.shape[-1]), target.reshape(-1))
+            loss = cross_entropy(F.linear(x, self.word_emb.weight), target)
         return loss, new_mems
 
     def moe_layers(self):

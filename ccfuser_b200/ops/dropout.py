@@ -113,6 +113,12 @@ class DropoutState:
     def advance(self):
         self.tensor[1:].add_(1)
 
+    def begin_step(self, device):
+        """The next step, its calls numbered from one again: the masks of a step follow from the seed and its number alone."""
+        self.on(device)
+        self.calls = 0
+        self.advance()
+
 
 class Dropout(nn.Module):
     """``dropout`` of a model: ``forward(x, residual=None)`` adds the residual, and in evaluation, or for ``p=0``, adds it alone."""

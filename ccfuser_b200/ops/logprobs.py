@@ -123,6 +123,12 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     return TokenLogprobs(out[0], out[1], *(out[2:] if top_k else (None, None)))
 
 
+def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, vocab_size: Optional[int] = None, ignore_index: int = -100) -> torch.Tensor:
+    """Mean of ``-token_logprobs`` over the targets that are not ignored: ``F.cross_entropy`` of the first ``vocab_size`` columns in fp32."""
+    lp = token_logprobs(logits, targets, vocab_size=vocab_size, ignore_index=ignore_index).logprobs
+    return -lp.sum() / (targets != ignore_index).sum()
+
+
 def _logprobs_torch(logits, targets, top_k, temperature, vocab, ignore):
     x = logits[..., :vocab]
     x = x if x.dtype == torch.float64 else x.float()
