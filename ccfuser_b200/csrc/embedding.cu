@@ -12,8 +12,11 @@ namespace ccf {
 
 constexpr int kSortChunk = 1024;     // keys that one block sorts in shared memory
 constexpr int kEmbWarps = 8;
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 16;
 constexpr uint32_t kNoRow = 0xffffffffu;   // id of a token without a gradient: skipped row, index out of range
+
+// a product that may pass 32 bits, in one instruction
+__device__ __forceinline__ uint64_t wide(uint32_t a, uint32_t b) { return static_cast<uint64_t>(a) * b; }
 
 // What the 32 lanes of a warp hold of a row: 32 * kE consecutive elements from a column on. kVec: 16 bytes per lane; otherwise (rows off
 // 16-byte boundaries) one element per lane and access.
@@ -33,6 +36,17 @@ struct Slice {
     } else {
 #pragma unroll
       for (int i = 0; i < kE; ++i) s[i] = on && col(i) < left ? load_elem<kType>(p, static_cast<long long>(at) + col(i)) : 0.f;
+    }
+  }
+  // f += scale * this, or with kFirst f = scale * this, in pairs
+  template <bool kFirst>
+  __device__ __forceinline__ void add_to(f32x2 (&f)[kE / 2], f32x2 scale) const {
+    float v[kE];
+    get(v);
+#pragma unroll
+    for (int i = 0; i < kE / 2; ++i) {
+      const f32x2 x = pk2(v[2 * i], v[2 * i + 1]);
+      f[i] = kFirst ? mul2(x, scale) : fma2(x, scale, f[i]);
     }
   }
   __device__ __forceinline__ void get(float (&f)[kE]) const {
@@ -64,20 +78,19 @@ struct Slice {
         if (col(i) < left) p[col(i)] = f[i];
     }
   }
-  static __device__ __forceinline__ void add_f32(const float* p, int left, bool on, float (&f)[kE]) {
+  static __device__ __forceinline__ void load_f32(const float* p, int left, float (&f)[kE]) {
     if constexpr (kVec) {
-      if (!on || lane_id() * kE >= left) return;
 #pragma unroll
       for (int i = 0; i < kE; i += 4) {
-        const float4 v = reinterpret_cast<const float4*>(p + col(i))[0];
-        f[i] += v.x;
-        f[i + 1] += v.y;
-        f[i + 2] += v.z;
-        f[i + 3] += v.w;
+        const float4 v = lane_id() * kE < left ? reinterpret_cast<const float4*>(p + col(i))[0] : make_float4(0.f, 0.f, 0.f, 0.f);
+        f[i] = v.x;
+        f[i + 1] = v.y;
+        f[i + 2] = v.z;
+        f[i + 3] = v.w;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kE; ++i) f[i] += on && col(i) < left ? p[col(i)] : 0.f;
+      for (int i = 0; i < kE; ++i) f[i] = col(i) < left ? p[col(i)] : 0.f;
     }
   }
   static __device__ __forceinline__ void store_zero(void* p, size_t at, int left) {   // past the L2 where it may: nobody reads it soon
@@ -92,58 +105,59 @@ struct Slice {
 };
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
-// A warp takes one slice of the columns for up to 8 consecutive tokens: their ids in one load, then kFwdRows tokens' rows of every table in flight. With a
-// token at a time the chain from an id to its row was walked for every kilobyte. Few tokens: fewer for each warp, so that they spread over the card.
-constexpr int kFwdTokens = 8, kFwdRows = 4;
+// A warp takes one slice of the columns for up to 16 consecutive tokens: their ids in one load, then kFwdRows tokens' rows of every table in flight (64
+// registers, four blocks an SM). With a token at a time the chain from an id to its row was walked for every kilobyte. Few tokens: fewer for each warp, so that
+// they spread over the card. 8192 tokens of 2048 bf16 with positions 14.8 us (52 MB from and to memory: 3.5 TB/s); tokens at one place of
+// several sequences, whose position then comes from L1, 16.4.
+constexpr int kFwdTokens = 16;
+template <int kTables>
+constexpr int kFwdRows = kTables <= 2 ? 4 : 2;
 
 template <int kType, bool kVec, int kTables>
-__global__ void __launch_bounds__(32 * kEmbWarps) embedding_fwd_kernel(const __grid_constant__ CcfEmbed e, void* __restrict__ y, int* status, uint32_t each,
-                                                                       uint32_t slices) {
+__global__ void __launch_bounds__(32 * kEmbWarps, 4) embedding_fwd_kernel(const __grid_constant__ CcfEmbed e, void* __restrict__ y, int* status, uint32_t each,
+                                                                          uint32_t slices) {
   using S = Slice<kType, kVec>;
+  constexpr int kRows = kFwdRows<kTables>;
   const uint32_t unit = blockIdx.x * kEmbWarps + (threadIdx.x >> 5), part = unit / slices, c = (unit - part * slices) * S::kCols;
   const uint32_t tokens = static_cast<uint32_t>(e.tokens), begin = part * each;
   if (begin >= tokens) return;
   const uint32_t n = min(each, tokens - begin);
   const int left = e.d - static_cast<int>(c);
-  long long id[kTables];
+  uint64_t at[kTables];   // where lane t finds token t's row
   bool in = true;
 #pragma unroll
   for (int k = 0; k < kTables; ++k) {
     const CcfEmbedTable& w = e.table[k];
     const uint32_t t = begin + min(static_cast<uint32_t>(lane_id()), n - 1);
-    id[k] = w.ids != nullptr ? load_index(w.ids, t, w.wide) : static_cast<long long>(t % static_cast<uint32_t>(e.seq));
-    const bool here = id[k] >= 0 && id[k] < w.rows;
+    const long long id = w.ids != nullptr ? load_index(w.ids, t, w.wide) : static_cast<long long>(t % static_cast<uint32_t>(e.seq));
+    const bool here = id >= 0 && id < w.rows;
     in = in && here;
-    id[k] = here ? id[k] : 0;
+    at[k] = here ? static_cast<uint64_t>(id) * w.ld + c : c;
   }
   const uint32_t good = __ballot_sync(0xffffffffu, in);
   if (c == 0 && !in && lane_id() < n) report_status(status, CCF_ERR_INDEX, static_cast<int>(begin + lane_id()) & 0x7fffff);
-  for (uint32_t t0 = 0; t0 < n; t0 += kFwdRows) {
-    S row[kTables][kFwdRows];
+  for (uint32_t t0 = 0; t0 < n; t0 += kRows) {
+    S row[kTables][kRows];
 #pragma unroll
-    for (int u = 0; u < kFwdRows; ++u) {
+    for (int u = 0; u < kRows; ++u) {
 #pragma unroll
-      for (int k = 0; k < kTables; ++k) {
-        const long long r = __shfl_sync(0xffffffffu, id[k], t0 + u);
-        row[k][u].load(e.table[k].weight, static_cast<size_t>(r) * e.table[k].ld + c, left, t0 + u < n);
-      }
+      for (int k = 0; k < kTables; ++k) row[k][u].load(e.table[k].weight, __shfl_sync(0xffffffffu, at[k], t0 + u), left, t0 + u < n);
     }
 #pragma unroll
-    for (int u = 0; u < kFwdRows; ++u) {
+    for (int u = 0; u < kRows; ++u) {
       if (t0 + u >= n) break;
+      f32x2 pairs[S::kE / 2];
+      row[0][u].template add_to<true>(pairs, bc2(e.table[0].scale));
+#pragma unroll
+      for (int k = 1; k < kTables; ++k) row[k][u].template add_to<false>(pairs, bc2(e.table[k].scale));
       float sum[S::kE];
 #pragma unroll
-      for (int k = 0; k < kTables; ++k) {
-        float f[S::kE];
-        row[k][u].get(f);
-#pragma unroll
-        for (int i = 0; i < S::kE; ++i) sum[i] = k == 0 ? f[i] * e.table[0].scale : fmaf(f[i], e.table[k].scale, sum[i]);
-      }
+      for (int i = 0; i < S::kE / 2; ++i) upk2(pairs[i], sum[2 * i], sum[2 * i + 1]);
       if (!(good >> (t0 + u) & 1)) {
 #pragma unroll
         for (int i = 0; i < S::kE; ++i) sum[i] = __int_as_float(0x7fc00000);
       }
-      S::store(y, static_cast<size_t>(begin + t0 + u) * e.d + c, left, sum);
+      S::store(y, wide(begin + t0 + u, e.d) + c, left, sum);
     }
   }
 }
@@ -156,6 +170,7 @@ struct GradTable {
   const void* ids;
   void* grad;
   uint64_t* sorted_chunks;
+  uint32_t* chunk_ids;   // the ids of sorted_chunks
   uint64_t* keys;
   uint32_t* slot;
   float* head;
@@ -166,13 +181,15 @@ struct GradTable {
   long long skip;
   float scale;
   int wide;
+  uint32_t piece, pieces, blocks;   // tokens of a piece, pieces, blocks that sum them
 };
 struct GradArgs {
   GradTable table[CCF_EMBED_TABLES];
   const void* dy;
   int* status;
   uint32_t tokens, seq, batch;
-  uint32_t piece, pieces, chunks, slices;
+  uint32_t chunks, slices;
+  uint32_t early, zeros_first, sums;   // blocks: sums by position, zeros in front of the sums by id, all sums
   int tables, d;
 };
 
@@ -222,27 +239,30 @@ __global__ void __launch_bounds__(kSortChunk) embedding_sort_kernel(const __grid
     }
   }
   if (tid < n) t.sorted_chunks[base + tid] = key;
+  if (g.chunks > 1) t.chunk_ids[base + tid] = tid < n ? id_of(key) : kNoRow;
 }
 
 // A key's place among all: its place in its own chunk and, for every other chunk, the keys there that are smaller: those of smaller ids and, in earlier
-// chunks, of the same. A block has a chunk's keys, one for each thread, and searches kSide chunks at a time, whose ids it brings into shared memory:
-// eleven steps there take less than one read from L2 (10 us with the searches in L2, ? now).
-constexpr int kSide = 8;
-__global__ void __launch_bounds__(kSortChunk) embedding_merge_kernel(const __grid_constant__ GradArgs g) {
-  __shared__ uint32_t ids[kSide][kSortChunk];
+// chunks, of the same. A block brings the ids of kSide chunks at a time into shared memory and searches them side by side for kMergeThreads keys of one
+// chunk: eleven steps there take less than one read from L2. Several blocks for each chunk: the searches' bank conflicts are what a block's time goes to.
+constexpr int kSide = 8, kMergeThreads = 256;
+__global__ void __launch_bounds__(kMergeThreads) embedding_merge_kernel(const __grid_constant__ GradArgs g) {
+  constexpr int kEach = kSide * kSortChunk / 4 / kMergeThreads;   // 16-byte pieces of ids for each thread
+  __shared__ uint4 staged[kSide * kSortChunk / 4];
+  const uint32_t* const ids = reinterpret_cast<const uint32_t*>(staged);
   after_previous();
   const GradTable& t = g.table[blockIdx.y];
   if (t.ids == nullptr) return;
-  const uint32_t tid = threadIdx.x, own = blockIdx.x, i = own * kSortChunk + tid;
-  const uint64_t* src = t.sorted_chunks;
-  const uint64_t key = i < g.tokens ? src[i] : ~0ull;
+  const uint32_t i = blockIdx.x * kMergeThreads + threadIdx.x, own = i / kSortChunk;
+  const uint64_t key = i < g.tokens ? t.sorted_chunks[i] : ~0ull;
   const uint32_t id = id_of(key);
-  uint32_t place = tid;
+  uint32_t place = i % kSortChunk;
   for (uint32_t c = 0; c < g.chunks; c += kSide) {
+    const uint32_t most = min(static_cast<uint32_t>(kSide), g.chunks - c) * (kSortChunk / 4);
 #pragma unroll
-    for (int u = 0; u < kSide; ++u) {
-      const uint32_t at = (c + u) * kSortChunk + tid;
-      ids[u][tid] = c + u != own && at < g.tokens ? id_of(src[at]) : 0xffffffffu;
+    for (int u = 0; u < kEach; ++u) {
+      const uint32_t at = u * kMergeThreads + threadIdx.x;
+      if (at < most) staged[at] = reinterpret_cast<const uint4*>(t.chunk_ids + c * kSortChunk)[at];
     }
     __syncthreads();
     uint32_t lo[kSide] = {};
@@ -251,32 +271,31 @@ __global__ void __launch_bounds__(kSortChunk) embedding_merge_kernel(const __gri
 #pragma unroll
       for (int u = 0; u < kSide; ++u) {
         const uint32_t to = lo[u] + step;
-        if (to > kSortChunk) continue;
-        const uint32_t o = ids[u][to - 1];
+        if (to > kSortChunk || c + u >= g.chunks) continue;
+        const uint32_t o = ids[u * kSortChunk + to - 1];
         if (o < id || (o == id && c + u < own)) lo[u] = to;
       }
     }
 #pragma unroll
-    for (int u = 0; u < kSide; ++u) {
-      // tokens without a row carry the id of places that hold none: those do not count
-      const uint32_t n = c + u >= g.chunks || c + u == own ? 0 : min(g.tokens - (c + u) * kSortChunk, static_cast<uint32_t>(kSortChunk));
-      place += min(lo[u], n);
-    }
+    for (int u = 0; u < kSide; ++u)   // behind the last token the ids are kNoRow, which only tokens without a row reach: those places do not count
+      if (c + u < g.chunks && c + u != own) place += min(lo[u], g.tokens - (c + u) * kSortChunk);
     __syncthreads();
   }
   if (i < g.tokens) t.keys[place] = key;
 }
 
-// Sums, then zeros. Positions are summed first: their order is known, so these blocks do not wait for the sort, and they leave dy in L2 for the sums by id
-// behind them. A warp takes one piece of the sorted tokens and one slice of the columns. The last blocks write the zeros of the rows that no token has, 32
-// rows each; those need the sorting kernel's results only, not the merging one's, which has waited for it.
+// Sums, and the zeros of the rows that no token has, 32 rows a block. A summing warp takes one piece of the sorted tokens and one slice of the columns.
+// Positions come first: their order is known, so these blocks do not wait for the sort, and they leave dy in L2 for the sums by id. Without positions
+// some of the zeros stand in front: they need the sorting kernel's results only, not the merging one's, which has waited for it. The other
+// zeros come last. Alternating sums and zeros was slower (59 us against 53: blocks that wait for the merge hold the places of blocks that could write).
 template <int kType, bool kVec>
-__global__ void __launch_bounds__(32 * kEmbWarps, 3) embedding_sum_kernel(const __grid_constant__ GradArgs g) {
+__global__ void __launch_bounds__(32 * kEmbWarps, 5) embedding_sum_kernel(const __grid_constant__ GradArgs g) {
   using S = Slice<kType, kVec>;
-  constexpr int kUnroll = kVec ? 8 : 2;
-  const uint32_t warp = threadIdx.x >> 5, units = g.pieces * g.slices, sum_blocks = (units + kEmbWarps - 1) / kEmbWarps;
-  if (blockIdx.x >= sum_blocks * g.tables) {
-    uint32_t w = blockIdx.x - sum_blocks * g.tables;
+  constexpr int kUnroll = kVec ? 4 : 2;   // 40 warps an SM with four rows in flight: 72 us a pass, 24 with eight 76
+  const uint32_t warp = threadIdx.x >> 5;
+  const bool front = blockIdx.x >= g.early && blockIdx.x < g.early + g.zeros_first;
+  if (front || blockIdx.x >= g.zeros_first + g.sums) {
+    uint32_t w = front ? blockIdx.x - g.early : blockIdx.x - g.sums;
     int k = 0;
     while (w >= (g.table[k].rows + 31) / 32) w -= static_cast<uint32_t>((g.table[k++].rows + 31) / 32);
     const GradTable& t = g.table[k];
@@ -288,56 +307,62 @@ __global__ void __launch_bounds__(32 * kEmbWarps, 3) embedding_sum_kernel(const 
       if (t.ids == nullptr) {
         used = row < g.seq;
       } else {
-        const uint32_t at = __ldcg(t.slot + row);
-        used = row != t.skip && at < g.tokens &&
-               (t.wide ? __ldcg(reinterpret_cast<const long long*>(t.ids) + at) : __ldcg(reinterpret_cast<const int*>(t.ids) + at)) == row;
+        const uint32_t token = __ldcg(t.slot + row);
+        used = row != t.skip && token < g.tokens &&
+               (t.wide ? __ldcg(reinterpret_cast<const long long*>(t.ids) + token) : __ldcg(reinterpret_cast<const int*>(t.ids) + token)) == row;
       }
     }
     const uint32_t unused = __ballot_sync(0xffffffffu, !used);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       if (!(unused >> r & 1)) continue;
-      const size_t at = (static_cast<size_t>(w) * 32 + warp * 4 + r) * g.d;
-      for (int c = 0; c < g.d; c += S::kCols) S::store_zero(t.grad, at + c, g.d - c);
+      const size_t first = wide(w * 32 + warp * 4 + r, g.d);
+      for (int c = 0; c < g.d; c += S::kCols) S::store_zero(t.grad, first + c, g.d - c);
     }
     wait_for_previous();   // every block waits before it ends, so that the end of this kernel is the end of those in front of it
     return;
   }
-  const GradTable& t = g.table[blockIdx.x / sum_blocks];
+  uint32_t at = blockIdx.x < g.early ? blockIdx.x : blockIdx.x - g.zeros_first;
+  int k = 0;
+  while (at >= g.table[k].blocks) at -= g.table[k++].blocks;
+  const GradTable& t = g.table[k];
   if (t.ids != nullptr) wait_for_previous();
   let_next_in();
-  const uint32_t unit = blockIdx.x % sum_blocks * kEmbWarps + warp;
-  if (unit >= units) {
+  const uint32_t unit = at * kEmbWarps + warp, piece = unit / g.slices, c = (unit - piece * g.slices) * S::kCols;
+  if (piece >= t.pieces) {
     wait_for_previous();
     return;
   }
-  const uint32_t piece = unit / g.slices, c = (unit - piece * g.slices) * S::kCols;
   const int left = g.d - static_cast<int>(c);
-  const uint32_t begin = piece * g.piece, n = min(g.piece, g.tokens - begin);
+  const uint32_t begin = piece * t.piece, n = min(t.piece, g.tokens - begin);
   const uint64_t mine = lane_id() < n ? key_at(g, t, begin + lane_id()) : ~0ull;
   const uint32_t before = begin > 0 ? id_of(key_at(g, t, begin - 1)) : kNoRow;
   const uint32_t after = begin + n < g.tokens ? id_of(key_at(g, t, begin + n)) : kNoRow;
-  float acc[S::kE] = {};
+  f32x2 acc[S::kE / 2] = {};
   uint32_t run = __shfl_sync(0xffffffffu, id_of(mine), 0);
   bool from_before = begin > 0 && run == before;
   auto finish = [&](bool goes_on) {
+    float f[S::kE];
+#pragma unroll
+    for (int i = 0; i < S::kE / 2; ++i) {
+      upk2(acc[i], f[2 * i], f[2 * i + 1]);
+      acc[i] = 0;
+    }
     if (run != kNoRow) {
       if (from_before) {
-        S::store_f32(t.head + static_cast<size_t>(piece) * g.d + c, left, acc);
+        S::store_f32(t.head + wide(piece, g.d) + c, left, f);
       } else if (goes_on) {
-        S::store_f32(t.tail + static_cast<size_t>(piece) * g.d + c, left, acc);
+        S::store_f32(t.tail + wide(piece, g.d) + c, left, f);
         if (c == 0 && lane_id() == 0) {
           wait_for_previous();   // the sorting kernel zeroed the count
           t.list[atomicAdd(t.count, 1)] = static_cast<int>(piece);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < S::kE; ++i) acc[i] *= t.scale;
-        S::store(t.grad, static_cast<size_t>(run) * g.d + c, left, acc);
+        for (int i = 0; i < S::kE; ++i) f[i] *= t.scale;
+        S::store(t.grad, wide(run, g.d) + c, left, f);
       }
     }
-#pragma unroll
-    for (int i = 0; i < S::kE; ++i) acc[i] = 0.f;
     from_before = false;
   };
   for (uint32_t j0 = 0; j0 < n; j0 += kUnroll) {
@@ -347,7 +372,7 @@ __global__ void __launch_bounds__(32 * kEmbWarps, 3) embedding_sum_kernel(const 
     for (int u = 0; u < kUnroll; ++u) {
       const uint64_t k = __shfl_sync(0xffffffffu, mine, (j0 + u) & 31);
       id[u] = j0 + u < n ? id_of(k) : kNoRow;
-      part[u].load(g.dy, static_cast<size_t>(static_cast<uint32_t>(k)) * g.d + c, left, id[u] != kNoRow);
+      part[u].load(g.dy, wide(static_cast<uint32_t>(k), g.d) + c, left, id[u] != kNoRow);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -359,63 +384,98 @@ __global__ void __launch_bounds__(32 * kEmbWarps, 3) embedding_sum_kernel(const 
       float f[S::kE];
       part[u].get(f);
 #pragma unroll
-      for (int i = 0; i < S::kE; ++i) acc[i] += f[i];
+      for (int i = 0; i < S::kE / 2; ++i) acc[i] = add2(acc[i], pk2(f[2 * i], f[2 * i + 1]));
     }
   }
   finish(after == run);
   wait_for_previous();
 }
 
-// Runs that cross pieces: tail of the piece where the run began, then the heads of those behind it. kJoinWarps warps take every
-// kJoinWarps-th piece each, and their sums are added in the warps' order.
+// Runs that cross pieces: the tail of the piece where the run began, then the heads of those behind it, in their order. Most runs go on for a few pieces:
+// a warp adds one up, four heads in flight, each read together with the key that says whether it counts. Runs of more than kShort further pieces are left to
+// the whole block, whose warps take every kJoinWarps-th piece each; their sums are added in the warps' order.
 template <int kType, bool kVec>
 __global__ void __launch_bounds__(32 * kJoinWarps) embedding_join_kernel(const __grid_constant__ GradArgs g) {
   using S = Slice<kType, kVec>;
-  constexpr int kUnroll = 4;
+  constexpr uint32_t kUnroll = 4, kShort = 4;
   __shared__ __align__(16) float red[kJoinWarps][S::kCols];
   after_previous();
   const GradTable& t = g.table[blockIdx.y];
   const uint32_t warp = threadIdx.x >> 5, items = static_cast<uint32_t>(*t.count) * g.slices;
-  for (uint32_t it = blockIdx.x; it < items; it += gridDim.x) {
+  auto add_heads = [&](uint32_t q, uint32_t step, uint32_t c, int left, uint32_t run, float (&acc)[S::kE]) {   // of pieces q, q + step, ...; whether all counted
+    float part[kUnroll][S::kE];
+    uint32_t id[kUnroll];
+#pragma unroll
+    for (uint32_t u = 0; u < kUnroll; ++u) {
+      const uint32_t p = min(q + u * step, t.pieces - 1);
+      id[u] = q + u * step < t.pieces ? id_of(key_at(g, t, p * t.piece)) : kNoRow;
+      S::load_f32(t.head + wide(p, g.d) + c, left, part[u]);
+    }
+    bool on = true;
+#pragma unroll
+    for (uint32_t u = 0; u < kUnroll; ++u) {
+      on = on && id[u] == run;   // the same id, so the run goes on: what the head's memory holds otherwise is not added
+#pragma unroll
+      for (int i = 0; i < S::kE; ++i) acc[i] = on ? acc[i] + part[u][i] : acc[i];
+    }
+    return on;
+  };
+  // a run with more than kShort pieces behind the one where it began
+  auto is_long = [&](uint32_t piece, uint32_t run) {
+    const uint32_t far = piece + kShort + 1;
+    return far < t.pieces && id_of(key_at(g, t, far * t.piece)) == run;
+  };
+  for (uint32_t it = blockIdx.x * kJoinWarps + warp; it < items; it += gridDim.x * kJoinWarps) {
     const uint32_t piece = static_cast<uint32_t>(t.list[it / g.slices]), c = it % g.slices * S::kCols;
     const int left = g.d - static_cast<int>(c);
-    const uint32_t run = id_of(key_at(g, t, (piece + 1) * g.piece - 1));
-    float acc[S::kE] = {};
-    bool on = true;
-    for (uint32_t q = piece + 1 + warp; on && q < g.pieces; q += kUnroll * kJoinWarps) {
+    const uint32_t run = id_of(key_at(g, t, (piece + 1) * t.piece - 1));
+    if (is_long(piece, run)) continue;
+    float acc[S::kE];
+    S::load_f32(t.tail + wide(piece, g.d) + c, left, acc);
+    for (uint32_t q = piece + 1; q <= piece + kShort && add_heads(q, 1, c, left, run, acc); q += kUnroll) {}
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const uint32_t p = q + u * kJoinWarps;
-        on = on && p < g.pieces && id_of(key_at(g, t, p * g.piece)) == run;
-        S::add_f32(t.head + static_cast<size_t>(on ? p : piece) * g.d + c, left, on, acc);
+    for (int i = 0; i < S::kE; ++i) acc[i] *= t.scale;
+    S::store(t.grad, wide(run, g.d) + c, left, acc);
+  }
+  for (uint32_t base = blockIdx.x; base < items; base += 32 * gridDim.x) {   // 32 items of this block looked through at a time, by every warp alike
+    const uint32_t mine = base + lane_id() * gridDim.x;
+    bool here = false;
+    if (mine < items) {
+      const uint32_t piece = static_cast<uint32_t>(t.list[mine / g.slices]);
+      here = is_long(piece, id_of(key_at(g, t, (piece + 1) * t.piece - 1)));
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, here); todo != 0; todo &= todo - 1) {
+      const uint32_t it = base + (__ffs(todo) - 1) * gridDim.x;
+      const uint32_t piece = static_cast<uint32_t>(t.list[it / g.slices]), c = it % g.slices * S::kCols;
+      const int left = g.d - static_cast<int>(c);
+      const uint32_t run = id_of(key_at(g, t, (piece + 1) * t.piece - 1));
+      float acc[S::kE] = {};
+      for (uint32_t q = piece + 1 + warp; q < t.pieces && add_heads(q, kJoinWarps, c, left, run, acc); q += kUnroll * kJoinWarps) {}
+      S::store_f32(red[warp], S::kCols, acc);
+      __syncthreads();
+      for (int j = threadIdx.x; j < S::kCols && j < left; j += 32 * kJoinWarps) {
+        float s = t.tail[wide(piece, g.d) + c + j];
+#pragma unroll
+        for (int k = 0; k < kJoinWarps; ++k) s += red[k][j];
+        store_elem<kType>(t.grad, static_cast<long long>(wide(run, g.d) + c + j), s * t.scale);
       }
+      __syncthreads();
     }
-    S::store_f32(red[warp], S::kCols, acc);
-    __syncthreads();
-    for (int j = threadIdx.x; j < S::kCols && j < left; j += 32 * kJoinWarps) {
-      float s = t.tail[static_cast<size_t>(piece) * g.d + c + j];
-#pragma unroll
-      for (int k = 0; k < kJoinWarps; ++k) s += red[k][j];
-      store_elem<kType>(t.grad, static_cast<long long>(static_cast<size_t>(run) * g.d + c + j), s * t.scale);
-    }
-    __syncthreads();
   }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
-static uint32_t piece_of(long long tokens, int d) {
-  // long enough that few runs are cut, short enough that the pieces fill the card: 148 SMs with 32 warps
-  const long long slices = (d + 127) / 128;
-  for (uint32_t p = 8; p < 32; p *= 2)
-    if ((tokens + p - 1) / p * slices <= 148 * 32) return p;
-  return 32;
+// Tokens of a piece of the sorted order: 16 (with 32 the pass of the GPT step takes 4 us more, with 8 10). Runs by position are all as long as there are
+// sequences: whole ones where they fit.
+static uint32_t piece_of(bool sorted, long long batch) {
+  return static_cast<uint32_t>(sorted || batch > 32 ? 16 : batch <= 16 ? 16 / batch * batch : batch);
 }
 
 static size_t up16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
 
 // Lays the scratch out; returns its size.
-static size_t lay_out(GradTable* t, void* base, long long tokens, long long rows, int d, bool sorted) {
-  const size_t n = static_cast<size_t>(tokens), piece = piece_of(tokens, d), pieces = (n + piece - 1) / piece;
+static size_t lay_out(GradTable* t, void* base, long long tokens, long long rows, int d, bool sorted, long long batch) {
+  const size_t n = static_cast<size_t>(tokens), piece = piece_of(sorted, batch), pieces = (n + piece - 1) / piece;
   uint8_t* p = static_cast<uint8_t*>(base);
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -431,9 +491,12 @@ static size_t lay_out(GradTable* t, void* base, long long tokens, long long rows
   if (sorted) {
     x.slot = reinterpret_cast<uint32_t*>(take(4 * static_cast<size_t>(rows)));
     x.sorted_chunks = reinterpret_cast<uint64_t*>(take(8 * n));
+    x.chunk_ids = reinterpret_cast<uint32_t*>(take(n > kSortChunk ? 4 * ((n + kSortChunk - 1) / kSortChunk) * kSortChunk : 0));
     x.keys = n > kSortChunk ? reinterpret_cast<uint64_t*>(take(8 * n)) : x.sorted_chunks;
   }
   if (t != nullptr) {
+    t->piece = static_cast<uint32_t>(piece);
+    t->pieces = static_cast<uint32_t>(pieces);
     t->count = x.count;
     t->list = x.list;
     t->head = x.head;
@@ -441,6 +504,7 @@ static size_t lay_out(GradTable* t, void* base, long long tokens, long long rows
     t->slot = x.slot;
     t->sorted_chunks = x.sorted_chunks;
     t->keys = x.keys;
+    t->chunk_ids = x.chunk_ids;
   }
   return at;
 }
@@ -476,7 +540,7 @@ static int launch_fwd(const CcfEmbed& e, void* y, int* status, cudaStream_t st) 
   uint32_t each = kFwdTokens;
   while (each > 1 && (e.tokens + each - 1) / each * slices < 16 * 148) each /= 2;   // 16 warps an SM at least, while there are that many
   const long long units = (e.tokens + each - 1) / each * slices, blocks = (units + kEmbWarps - 1) / kEmbWarps;
-  if (units > 0xffffffffll || blocks > 0x7fffffffll) return -2;
+  if (units > 0xffffff00ll || blocks > 0x7fffffffll) return -2;
   const auto kern = e.tables == 1 ? embedding_fwd_kernel<kType, kVec, 1> : e.tables == 2 ? embedding_fwd_kernel<kType, kVec, 2>
                                                                                         : embedding_fwd_kernel<kType, kVec, 3>;
   kern<<<static_cast<unsigned>(blocks), 32 * kEmbWarps, 0, st>>>(e, y, status, each, slices);
@@ -487,23 +551,36 @@ template <int kType, bool kVec>
 static int launch_bwd(GradArgs& g, cudaStream_t st) {
   using S = Slice<kType, kVec>;
   g.slices = (g.d + S::kCols - 1) / S::kCols;
-  long long blocks = static_cast<long long>((static_cast<size_t>(g.pieces) * g.slices + kEmbWarps - 1) / kEmbWarps) * g.tables;
+  long long sums = 0, zeros = 0, early = 0;
+  uint32_t most = 0;
   bool sorted = false;
   for (int k = 0; k < g.tables; ++k) {
-    blocks += (g.table[k].rows + 31) / 32;
-    sorted = sorted || g.table[k].ids != nullptr;
+    GradTable& t = g.table[k];
+    const long long units = static_cast<long long>(t.pieces) * g.slices, blocks = (units + kEmbWarps - 1) / kEmbWarps;
+    if (units > 0x7fffffffll) return -2;
+    t.blocks = static_cast<uint32_t>(blocks);
+    sums += blocks;
+    zeros += (t.rows + 31) / 32;
+    if (t.ids == nullptr) early += blocks;
+    else sorted = true;
+    most = t.pieces > most ? t.pieces : most;
   }
-  if (blocks > 0x7fffffffll || static_cast<long long>(g.pieces) * g.slices > 0xffffffffll) return -2;
+  if (sums + zeros > 0x7fffffffll) return -2;
+  g.sums = static_cast<uint32_t>(sums);
+  g.early = static_cast<uint32_t>(early);
+  const long long front = 2 * sm_count();   // about what is written while the merge runs
+  g.zeros_first = static_cast<uint32_t>(early > 0 || g.chunks == 1 ? 0 : zeros < front ? zeros : front);
+  const dim3 blocks(static_cast<unsigned>(sums + zeros));
   int launches = 2;
   embedding_sort_kernel<<<dim3(sorted ? g.chunks : 1, g.tables), kSortChunk, 0, st>>>(g);
   cudaError_t err = cudaGetLastError();
   if (err == cudaSuccess && sorted && g.chunks > 1) {
-    err = launch_behind(embedding_merge_kernel, dim3(g.chunks, g.tables), kSortChunk, st, g);
+    err = launch_behind(embedding_merge_kernel, dim3((g.tokens + kMergeThreads - 1) / kMergeThreads, g.tables), kMergeThreads, st, g);
     ++launches;
   }
-  if (err == cudaSuccess) err = launch_behind(embedding_sum_kernel<kType, kVec>, dim3(static_cast<unsigned>(blocks)), 32 * kEmbWarps, st, g);
-  if (err == cudaSuccess && g.pieces > 1) {
-    const unsigned items = g.pieces * g.slices, wave = 4 * sm_count();
+  if (err == cudaSuccess) err = launch_behind(embedding_sum_kernel<kType, kVec>, blocks, 32 * kEmbWarps, st, g);
+  if (err == cudaSuccess && most > 1) {
+    const unsigned items = most * g.slices, wave = 2 * sm_count();
     err = launch_behind(embedding_join_kernel<kType, kVec>, dim3(items < wave ? items : wave, g.tables), 32 * kJoinWarps, st, g);
     ++launches;
   }
@@ -539,9 +616,9 @@ int ccf_embedding_fwd(const CcfEmbed* e, void* y, int* status, void* stream) {
 }
 
 // Bytes of scratch that a table needs in ccf_embedding_bwd; sorted: it has ids. 0: a size out of range.
-long long ccf_embedding_scratch(long long tokens, long long rows, int d, int sorted) {
-  if (tokens < 1 || tokens > 0x7fffffffll || rows < 1 || rows > 0x7fffffffll || d < 1) return 0;
-  return static_cast<long long>(ccf::lay_out(nullptr, nullptr, tokens, rows, d, sorted != 0));
+long long ccf_embedding_scratch(long long tokens, long long seq, long long rows, int d, int sorted) {
+  if (tokens < 1 || tokens > 0x7fffffffll || seq < 1 || tokens % seq != 0 || rows < 1 || rows > 0x7fffffffll || d < 1) return 0;
+  return static_cast<long long>(ccf::lay_out(nullptr, nullptr, tokens, rows, d, sorted != 0, tokens / seq));
 }
 
 // grad [rows, d] of every table from dy [tokens, d]: all rows are written, those that no token has with zeros. `scratch` of each table on a
@@ -558,8 +635,6 @@ int ccf_embedding_bwd(const CcfEmbed* e, const void* dy, int* status, void* stre
   g.tokens = static_cast<uint32_t>(e->tokens);
   g.seq = static_cast<uint32_t>(e->seq);
   g.batch = g.tokens / g.seq;
-  g.piece = piece_of(e->tokens, e->d);
-  g.pieces = (g.tokens + g.piece - 1) / g.piece;
   g.chunks = (g.tokens + kSortChunk - 1) / kSortChunk;
   g.tables = e->tables;
   g.d = e->d;
@@ -572,7 +647,7 @@ int ccf_embedding_bwd(const CcfEmbed* e, const void* dy, int* status, void* stre
     if (t.grad == nullptr || t.scratch == nullptr || !on16(t.scratch)) return -2;
     vec = vec && on16(t.grad);
     GradTable& o = g.table[k];
-    lay_out(&o, t.scratch, e->tokens, t.rows, e->d, t.ids != nullptr);
+    lay_out(&o, t.scratch, e->tokens, t.rows, e->d, t.ids != nullptr, g.batch);
     o.ids = t.ids;
     o.grad = t.grad;
     o.rows = t.rows;

@@ -33,7 +33,7 @@ extern "C" {
 #endif
 int ccf_sizeof_embed();
 int ccf_embedding_fwd(const CcfEmbed* e, void* y, int* status, void* stream);
-long long ccf_embedding_scratch(long long tokens, long long rows, int d, int sorted);
+long long ccf_embedding_scratch(long long tokens, long long seq, long long rows, int d, int sorted);
 int ccf_embedding_bwd(const CcfEmbed* e, const void* dy, int* status, void* stream);
 #ifdef __cplusplus
 }

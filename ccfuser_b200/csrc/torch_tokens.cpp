@@ -44,12 +44,14 @@ void add_table(CcfEmbed& e, const at::Tensor& ids, int64_t rows, double scale, i
 
 // One gradient launch for up to three tables: grads[k] [rows, d] from dy [tokens, d].
 void run_grad(CcfEmbed& e, const at::Tensor& dy, const std::vector<at::Tensor>& grads, const at::Tensor& status) {
-  std::vector<at::Tensor> scratch;
-  bool sorted = false;
+  int64_t at[3] = {}, bytes = 0;
   for (int k = 0; k < e.tables; ++k) {
-    sorted = sorted || e.table[k].ids != nullptr;
-    scratch.push_back(at::empty({ccf_embedding_scratch(e.tokens, e.table[k].rows, e.d, e.table[k].ids != nullptr)}, dy.options().dtype(at::kByte)));
-    e.table[k].scratch = scratch.back().data_ptr();
+    at[k] = bytes;
+    bytes += ccf_embedding_scratch(e.tokens, e.seq, e.table[k].rows, e.d, e.table[k].ids != nullptr);   // a multiple of 16
+  }
+  const at::Tensor scratch = at::empty({bytes}, dy.options().dtype(at::kByte));
+  for (int k = 0; k < e.tables; ++k) {
+    e.table[k].scratch = static_cast<uint8_t*>(scratch.data_ptr()) + at[k];
     e.table[k].grad = grads[k].data_ptr();
   }
   const int launches = ccf_embedding_bwd(&e, dy.data_ptr(), status.data_ptr<int>(), stream());

@@ -284,7 +284,7 @@ def _declare(lib):
         "ccf_layernorm_bwd_parts": ([i, i], i),
         "ccf_layernorm_bwd": ([p, p, p, p, p, p, p, p, p, i, i, i, p, ull, p], i),
         "ccf_embedding_fwd": ([C.POINTER(Embed), p, p, p], i),
-        "ccf_embedding_scratch": ([ll, ll, i, i], ll),
+        "ccf_embedding_scratch": ([ll, ll, ll, i, i], ll),
         "ccf_embedding_bwd": ([C.POINTER(Embed), p, p, p], i),
         "ccf_logprobs_fwd": ([C.POINTER(Logprobs), p], i),
         "ccf_logprobs_bwd": ([C.POINTER(Logprobs), p], i),

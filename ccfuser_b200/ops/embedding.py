@@ -42,7 +42,7 @@ def _run_grad(e, dy, grads, status):
     scratch = []
     for k, g in enumerate(grads):
         t = e.table[k]
-        scratch.append(torch.empty(lib.ccf_embedding_scratch(e.tokens, t.rows, e.d, int(bool(t.ids))), dtype=torch.uint8, device=dy.device))
+        scratch.append(torch.empty(lib.ccf_embedding_scratch(e.tokens, e.seq, t.rows, e.d, int(bool(t.ids))), dtype=torch.uint8, device=dy.device))
         t.scratch, t.grad = scratch[-1].data_ptr(), g.data_ptr()
     n = lib.ccf_embedding_bwd(C.byref(e), dy.data_ptr(), status, N.stream_ptr())
     N.check(min(n, 0), "ccf_embedding_bwd")

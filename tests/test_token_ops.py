@@ -42,8 +42,8 @@ def test_embedding_entry_points_refuse_missing_memory():
     assert lib.ccf_embedding_bwd(C.byref(_embed(scratch=None)), A, A, None) == -2
     assert lib.ccf_embedding_bwd(C.byref(_embed(scratch=A + 8)), A, A, None) == -2
     assert lib.ccf_embedding_bwd(C.byref(_embed()), None, A, None) == -2
-    assert lib.ccf_embedding_scratch(0, 10, 64, 1) == 0 and lib.ccf_embedding_scratch(8, 0, 64, 1) == 0
-    assert lib.ccf_embedding_scratch(5000, 100, 64, 1) > lib.ccf_embedding_scratch(5000, 100, 64, 0) > 0
+    assert lib.ccf_embedding_scratch(0, 1, 10, 64, 1) == lib.ccf_embedding_scratch(8, 1, 0, 64, 1) == lib.ccf_embedding_scratch(8, 3, 5, 64, 1) == 0
+    assert lib.ccf_embedding_scratch(5000, 50, 100, 64, 1) > lib.ccf_embedding_scratch(5000, 50, 100, 64, 0) > 0
 
 
 def test_embedding_refuses():
