@@ -186,7 +186,7 @@ template <int kThreads>
 struct RowShared {
   RowStats part[kThreads / 32];
   RowStats all;
-  uint32_t group[kThreads < 128 ? kThreads : 128];   // largest element of a group of threads
+  __align__(16) uint32_t group[kThreads < 128 ? kThreads : 128];   // largest element of a group of threads
   uint64_t top[CCF_LOGPROBS_MAX_TOP];
   uint64_t best[kThreads / 32];
   uint64_t list[kListLen<kThreads>];
@@ -211,6 +211,7 @@ __device__ __forceinline__ void rank_list(RowShared<kThreads>& sh, int n, int k,
   for (int i = tid; i < n; i += kThreads) {
     const uint64_t key = sh.list[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += sh.list[j] > key;
     if (key != 0 && rank < k) sh.top[rank] = key;
   }
@@ -220,7 +221,7 @@ __device__ __forceinline__ void rank_list(RowShared<kThreads>& sh, int n, int k,
 template <int kThreads>
 __device__ __forceinline__ int log_group(int k) {   // log2 of the threads in a group
   constexpr int kLog = kThreads == 32 ? 5 : kThreads == 128 ? 7 : 8;
-  return max(0, min(5, kLog - 1 - (32 - __clz(k))));
+  return max(0, min(min(5, kLog - 2), kLog - 1 - (32 - __clz(k))));
 }
 
 // Before the row's first barrier: what select_top starts from.
@@ -253,10 +254,11 @@ __device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_
   if (tid < groups) {
     const uint32_t g = sh.group[tid];
     int above = 0, from = 0;
-    for (int i = 0; i < groups; ++i) {
-      const uint32_t o = sh.group[i];
-      above += o > g;
-      from += o >= g;
+#pragma unroll 2
+    for (int i = 0; i < groups; i += 4) {   // at least four groups
+      const uint4 o = *reinterpret_cast<const uint4*>(sh.group + i);
+      above += (o.x > g) + (o.y > g) + (o.z > g) + (o.w > g);
+      from += (o.x >= g) + (o.y >= g) + (o.z >= g) + (o.w >= g);
     }
     if (g != 0 && above < k && k <= from) sh.bound = g;   // the k-th largest; where there are fewer elements than that, every finite one counts
   }

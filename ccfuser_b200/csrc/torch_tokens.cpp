@@ -59,31 +59,40 @@ void run_grad(CcfEmbed& e, const at::Tensor& dy, const std::vector<at::Tensor>& 
   g_launches += launches;
 }
 
+// The sum of the lookups; `index`: the ids as the kernels read them.
+at::Tensor run_embedding(const at::Tensor& ids, const at::Tensor& weight, const OptTensor& position, const OptTensor& position_ids,
+                         const OptTensor& type, const OptTensor& type_ids, double scale, const at::Tensor& status, at::Tensor (&index)[3]) {
+  const c10::cuda::CUDAGuard guard(weight.device());
+  const at::Tensor tables[3] = {table_of(weight), position.has_value() ? table_of(*position) : at::Tensor(),
+                                type.has_value() ? table_of(*type) : at::Tensor()};
+  index[0] = ids.contiguous();
+  if (position_ids.has_value()) index[1] = position_ids->contiguous();
+  if (type_ids.has_value()) index[2] = type_ids->contiguous();
+  CcfEmbed e{};
+  e.tokens = ids.numel();
+  e.seq = ids.dim() > 0 ? ids.size(-1) : 1;
+  e.d = static_cast<int>(weight.size(1));
+  e.type = type_code(weight);
+  for (int k = 0; k < 3; ++k) {
+    if (!tables[k].defined()) continue;
+    add_table(e, index[k], tables[k].size(0), k == 0 ? scale : 1.0, -1);
+    e.table[e.tables - 1].weight = tables[k].data_ptr();
+    e.table[e.tables - 1].ld = tables[k].size(0) > 1 ? tables[k].stride(0) : e.d;
+  }
+  at::DimVector shape(ids.sizes());
+  shape.push_back(e.d);
+  const at::Tensor y = at::empty(shape, weight.options().requires_grad(false));
+  check(ccf_embedding_fwd(&e, y.data_ptr(), status.data_ptr<int>(), stream()), "ccf_embedding_fwd");
+  ++g_launches;
+  return y;
+}
+
 struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& ids, const at::Tensor& weight, const OptTensor& position,
                             const OptTensor& position_ids, const OptTensor& type, const OptTensor& type_ids, double scale, int64_t skip,
                             const at::Tensor& status) {
-    const c10::cuda::CUDAGuard guard(weight.device());
-    const at::Tensor tables[3] = {table_of(weight), position.has_value() ? table_of(*position) : at::Tensor(),
-                                  type.has_value() ? table_of(*type) : at::Tensor()};
-    const at::Tensor index[3] = {ids.contiguous(), position_ids.has_value() ? position_ids->contiguous() : at::Tensor(),
-                                 type_ids.has_value() ? type_ids->contiguous() : at::Tensor()};
-    CcfEmbed e{};
-    e.tokens = ids.numel();
-    e.seq = ids.dim() > 0 ? ids.size(-1) : 1;
-    e.d = static_cast<int>(weight.size(1));
-    e.type = type_code(weight);
-    for (int k = 0; k < 3; ++k) {
-      if (!tables[k].defined()) continue;
-      add_table(e, index[k], tables[k].size(0), k == 0 ? scale : 1.0, k == 0 ? skip : -1);
-      e.table[e.tables - 1].weight = tables[k].data_ptr();
-      e.table[e.tables - 1].ld = tables[k].size(0) > 1 ? tables[k].stride(0) : e.d;
-    }
-    auto shape = ids.sizes().vec();
-    shape.push_back(e.d);
-    const at::Tensor y = at::empty(shape, weight.options());
-    check(ccf_embedding_fwd(&e, y.data_ptr(), status.data_ptr<int>(), stream()), "ccf_embedding_fwd");
-    ++g_launches;
+    at::Tensor index[3];
+    const at::Tensor y = run_embedding(ids, weight, position, position_ids, type, type_ids, scale, status, index);
     ctx->save_for_backward({index[0], index[1], index[2]});
     ctx->saved_data["rows"] = std::vector<int64_t>{weight.size(0), position.has_value() ? position->size(0) : 0, type.has_value() ? type->size(0) : 0};
     // autograd counts the tensors that are there: ids, weight, position, its ids, type
@@ -136,59 +145,68 @@ at::Tensor embedding_grad(const at::Tensor& grad, const at::Tensor& ids, int64_t
 }
 
 // ---- log probabilities -------------------------------------------------------------------------------------------------
+// A call over the logits' rows as the kernels read them.
+struct Scored {
+  at::Tensor x, targets, logprobs, entropy, top, top_ids, stats;
+  int64_t ld;
+};
+Scored run_logprobs(const at::Tensor& logits, const at::Tensor& targets, int64_t top_k, double temperature, int64_t vocab, int64_t ignore,
+                    const at::Tensor& status, bool training) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t width = logits.size(-1), rows = targets.numel();
+  Scored r;
+  r.x = logits.dim() == 2 ? logits : logits.reshape({rows, width});
+  if (r.x.stride(1) != 1 || (rows > 1 && r.x.stride(0) < width)) r.x = r.x.contiguous();
+  if (reinterpret_cast<uintptr_t>(r.x.data_ptr()) % 16 != 0) r.x = r.x.clone(at::MemoryFormat::Contiguous);
+  r.targets = targets.contiguous();
+  r.ld = rows > 1 ? r.x.stride(0) : width;
+  const auto f32 = at::TensorOptions(logits.device()).dtype(at::kFloat);
+  r.logprobs = at::empty(targets.sizes(), f32);
+  r.entropy = at::empty(targets.sizes(), f32);
+  CcfLogprobs a{};
+  a.x = r.x.data_ptr();
+  a.targets = r.targets.data_ptr();
+  a.wide = r.targets.scalar_type() == at::kLong;
+  a.logprobs = r.logprobs.data_ptr<float>();
+  a.entropy = r.entropy.data_ptr<float>();
+  a.status = status.data_ptr<int>();
+  a.rows = rows;
+  a.ld = r.ld;
+  a.ignore = ignore;
+  a.vocab = static_cast<int>(vocab);
+  a.width = static_cast<int>(width);
+  a.top_k = static_cast<int>(top_k);
+  a.type = type_code(r.x);
+  a.inv_t = static_cast<float>(1.0 / temperature);
+  if (top_k > 0) {
+    at::DimVector wide(targets.sizes());
+    wide.push_back(top_k);
+    r.top = at::empty(wide, f32);
+    r.top_ids = at::empty(wide, f32.dtype(at::kLong));
+    a.top_logprobs = r.top.data_ptr<float>();
+    a.top_ids = reinterpret_cast<long long*>(r.top_ids.data_ptr<int64_t>());
+  }
+  if (training) {
+    r.stats = at::empty({rows, 3}, f32);
+    a.stats = r.stats.data_ptr<float>();
+  }
+  check(ccf_logprobs_fwd(&a, stream()), "ccf_logprobs_fwd");
+  ++g_launches;
+  return r;
+}
+
 struct LogprobsFn : torch::autograd::Function<LogprobsFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& targets, int64_t top_k, double temperature,
                                int64_t vocab, int64_t ignore, const at::Tensor& status) {
-    const c10::cuda::CUDAGuard guard(logits.device());
-    const int64_t width = logits.size(-1), rows = targets.numel();
-    at::Tensor x = logits.reshape({rows, width});
-    if (x.stride(1) != 1 || (rows > 1 && x.stride(0) < width)) x = x.contiguous();
-    if (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) x = x.clone(at::MemoryFormat::Contiguous);
-    const at::Tensor t = targets.contiguous();
-    const auto f32 = logits.options().dtype(at::kFloat);
-    const auto shape = targets.sizes();
-    const at::Tensor lp = at::empty(shape, f32), entropy = at::empty(shape, f32);
-    at::Tensor top, top_ids, stats;
-    CcfLogprobs a{};
-    a.x = x.data_ptr();
-    a.targets = t.data_ptr();
-    a.wide = t.scalar_type() == at::kLong;
-    a.logprobs = lp.data_ptr<float>();
-    a.entropy = entropy.data_ptr<float>();
-    a.status = status.data_ptr<int>();
-    a.rows = rows;
-    a.ld = rows > 1 ? x.stride(0) : width;
-    a.ignore = ignore;
-    a.vocab = static_cast<int>(vocab);
-    a.width = static_cast<int>(width);
-    a.top_k = static_cast<int>(top_k);
-    a.type = type_code(x);
-    a.inv_t = static_cast<float>(1.0 / temperature);
-    if (top_k > 0) {
-      auto wide = shape.vec();
-      wide.push_back(top_k);
-      top = at::empty(wide, f32);
-      top_ids = at::empty(wide, f32.dtype(at::kLong));
-      a.top_logprobs = top.data_ptr<float>();
-      a.top_ids = reinterpret_cast<long long*>(top_ids.data_ptr<int64_t>());
-    }
-    const bool training = logits.requires_grad();
-    if (training) {
-      stats = at::empty({rows, 3}, f32);
-      a.stats = stats.data_ptr<float>();
-    }
-    check(ccf_logprobs_fwd(&a, stream()), "ccf_logprobs_fwd");
-    ++g_launches;
-    if (training) {
-      ctx->save_for_backward({x, t, stats, top_ids});
-      ctx->saved_data["args"] = std::vector<int64_t>{top_k, vocab, ignore, a.ld};
-      ctx->saved_data["inv_t"] = 1.0 / temperature;
-      ctx->saved_data["shape"] = logits.sizes();
-    }
+    const Scored r = run_logprobs(logits, targets, top_k, temperature, vocab, ignore, status, true);
+    ctx->save_for_backward({r.x, r.targets, r.stats, r.top_ids});
+    ctx->saved_data["args"] = std::vector<int64_t>{top_k, vocab, ignore, r.ld};
+    ctx->saved_data["inv_t"] = 1.0 / temperature;
+    ctx->saved_data["shape"] = logits.sizes();
     ctx->set_materialize_grads(false);
-    if (top_k == 0) return {lp, entropy};
-    ctx->mark_non_differentiable({top_ids});
-    return {lp, entropy, top, top_ids};
+    if (top_k == 0) return {r.logprobs, r.entropy};
+    ctx->mark_non_differentiable({r.top_ids});
+    return {r.logprobs, r.entropy, r.top, r.top_ids};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -266,6 +284,10 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
   }
 };
 
+// Without a graph to build, the kernels alone: the function around them costs the host about 2 us.
+// A forward-mode tangent goes to the function as well, which refuses it.
+bool needs_graph(const at::Tensor& t) { return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined(); }
+
 }  // namespace
 
 void ccf_torch::add_token_ops(py::module_& m) {
@@ -273,19 +295,33 @@ void ccf_torch::add_token_ops(py::module_& m) {
       "embedding",
       [](const at::Tensor& ids, const at::Tensor& weight, const OptTensor& position, const OptTensor& position_ids, const OptTensor& type,
          const OptTensor& type_ids, double scale, int64_t skip, const at::Tensor& status) {
-        return EmbeddingFn::apply(ids, weight, position, position_ids, type, type_ids, scale, skip, status);
+        if (needs_graph(weight) || (position.has_value() && needs_graph(*position)) || (type.has_value() && needs_graph(*type)))
+          return EmbeddingFn::apply(ids, weight, position, position_ids, type, type_ids, scale, skip, status);
+        const at::AutoDispatchBelowADInplaceOrView below;
+        at::Tensor index[3];
+        return run_embedding(ids, weight, position, position_ids, type, type_ids, scale, status, index);
       },
       py::call_guard<py::gil_scoped_release>());
   m.def("embedding_grad", &embedding_grad, py::call_guard<py::gil_scoped_release>());
   m.def(
       "token_logprobs",
       [](const at::Tensor& logits, const at::Tensor& targets, int64_t top_k, double temperature, int64_t vocab, int64_t ignore,
-         const at::Tensor& status) { return LogprobsFn::apply(logits, targets, top_k, temperature, vocab, ignore, status); },
+         const at::Tensor& status) -> variable_list {
+        if (needs_graph(logits)) return LogprobsFn::apply(logits, targets, top_k, temperature, vocab, ignore, status);
+        const at::AutoDispatchBelowADInplaceOrView below;
+        const Scored r = run_logprobs(logits, targets, top_k, temperature, vocab, ignore, status, false);
+        if (top_k == 0) return {r.logprobs, r.entropy};
+        return {r.logprobs, r.entropy, r.top, r.top_ids};
+      },
       py::call_guard<py::gil_scoped_release>());
   m.def(
       "dropout",
       [](const at::Tensor& x, const OptTensor& residual, const at::Tensor& state, int64_t call, int64_t drop) {
-        return DropoutFn::apply(x, residual, state, call, drop);
+        if (needs_graph(x) || (residual.has_value() && needs_graph(*residual))) return DropoutFn::apply(x, residual, state, call, drop);
+        const c10::cuda::CUDAGuard guard(x.device());
+        const at::AutoDispatchBelowADInplaceOrView below;
+        return run_dropout(packed(x), residual.has_value() ? packed(*residual) : at::Tensor(),
+                           reinterpret_cast<const long long*>(state.data_ptr<int64_t>()), nullptr, call, drop);
       },
       py::call_guard<py::gil_scoped_release>());
 }

@@ -161,3 +161,37 @@ def test_through_the_fused_layers():
     assert torch.equal(scores.top_ids[..., 0], logits[:, :-1].argmax(-1))
     for layer in (*m.moe_layers(), *g.moe_layers()):
         layer.release()
+
+
+def test_transforms_are_refused():
+    import torch.autograd.forward_ad as fwd
+    from ccfuser_b200.ops.dropout import dropout
+    from ccfuser_b200.ops.embedding import embedding
+    from ccfuser_b200.ops.logprobs import token_logprobs
+    x, ids, state = torch.randn(4, 3, 64, device="cuda"), torch.arange(3, device="cuda"), torch.tensor([1, 2], device="cuda")
+    calls = (lambda t: embedding(ids, t), lambda t: token_logprobs(t, ids).logprobs, lambda t: dropout(t, 0.5, state))
+    for f in calls:
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(x)
+        with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+            f(fwd.make_dual(x[0], torch.ones_like(x[0])))
+
+
+def test_a_traced_graph_replays_the_kernels():
+    """torch.jit.trace records the operations, not only the allocation of their outputs: on other inputs the graph gives what the functions give."""
+    from ccfuser_b200.ops.dropout import dropout
+    from ccfuser_b200.ops.embedding import embedding
+    from ccfuser_b200.ops.logprobs import token_logprobs
+    w, state = torch.randn(50, 64, device="cuda"), torch.tensor([1, 2], device="cuda")
+
+    def chain(ids, targets):
+        y = dropout(embedding(ids, w, 2.0), 0.3, state)
+        out = token_logprobs(y, targets, top_k=3)
+        return out.logprobs, out.entropy, out.top_logprobs, out.top_ids
+    one = (torch.arange(10, device="cuda"), torch.arange(10, device="cuda"))
+    two = (torch.arange(10, device="cuda") + 7, torch.arange(10, device="cuda") + 20)
+    with torch.no_grad():
+        traced = torch.jit.trace(chain, one, check_trace=False)
+        for args in (one, two):
+            for a, b in zip(traced(*args), chain(*args)):
+                assert torch.equal(a, b)
