@@ -272,21 +272,28 @@ __device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_
     if (v != neg_inf() && order_of(v) >= bound) list(v, index);
   };
   if (edge_index >= 0) consider(edge, edge_index);
-  uint32_t owners = __ballot_sync(0xffffffffu, largest >= bound);
-  const uint32_t wide = __ballot_sync(0xffffffffu, run.second != neg_inf() && order_of(run.second) >= bound);
-  while (owners != 0) {
-    const int owner = __ffs(owners) - 1;
-    owners &= owners - 1;
-    if (wide >> owner & 1) {
-      for (int v = first + tid - lane + owner + lane * kThreads; v < last; v += 32 * kThreads) {
-        float f[kE];
-        unpack16<kType>(__ldg(pieces + v), f);
+  uint32_t wide = __ballot_sync(0xffffffffu, run.second != neg_inf() && order_of(run.second) >= bound);
+  uint32_t owners = __ballot_sync(0xffffffffu, largest >= bound) & ~wide;
+  while (owners != 0) {   // four of them at a time, so that their elements come together
+    float f[4];
+    int index[4];
 #pragma unroll
-        for (int i = 0; i < kE; ++i) consider(f[i], shape.head + v * kE + i);
-      }
-    } else {
-      const int v = __shfl_sync(0xffffffffu, run.at, owner) + lane / kE * kThreads, index = shape.head + v * kE + lane % kE;
-      if (lane < kUnroll * kE && v < last) consider(load_elem<kType>(p, index), index);
+    for (int u = 0; u < 4; ++u) {
+      const int owner = __ffs(owners) - 1;
+      const int v = __shfl_sync(0xffffffffu, run.at, owner & 31) + lane / kE * kThreads;
+      index[u] = shape.head + v * kE + lane % kE;
+      f[u] = owner >= 0 && lane < kUnroll * kE && v < last ? load_elem<kType>(p, index[u]) : neg_inf();
+      owners &= owners - 1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) consider(f[u], index[u]);
+  }
+  for (; wide != 0; wide &= wide - 1) {
+    for (int v = first + tid - lane + __ffs(wide) - 1 + lane * kThreads; v < last; v += 32 * kThreads) {
+      float f[kE];
+      unpack16<kType>(__ldg(pieces + v), f);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) consider(f[i], shape.head + v * kE + i);
     }
   }
   row_sync<kThreads>();
@@ -344,7 +351,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
   Shared& sh = shared[kThreads == 32 ? warp : 0];
   const uint8_t* p = reinterpret_cast<const uint8_t*>(a.x) + static_cast<size_t>(row) * a.ld * kElemBytes<kType>;
   const RowShape<kType> shape(p, a.vocab);
-  const int first = static_cast<int>(static_cast<unsigned>(shape.pieces) * rank >> log_split);   // at most 2^28 pieces and 8 blocks
+  const int first = static_cast<int>(static_cast<unsigned>(shape.pieces) * rank >> log_split);   // at most 2^28 pieces and 4 blocks
   const int last = static_cast<int>(static_cast<unsigned>(shape.pieces) * (rank + 1) >> log_split);
   const uint4* pieces = reinterpret_cast<const uint4*>(p + shape.head * kElemBytes<kType>);
   const float c = a.inv_t * kLog2e;
@@ -598,10 +605,11 @@ static int launch_fwd(const CcfLogprobs& a, int log_split, cudaStream_t st) {
 
 template <int kType, bool kTop>
 static int choose_fwd(const CcfLogprobs& a, cudaStream_t st) {
-  if (a.vocab <= 1024) return launch_fwd<kType, 32, kTop>(a, 0, st);
-  if (a.rows >= 4 * sm_count()) return launch_fwd<kType, 128, kTop>(a, 0, st);
+  const bool many = a.rows >= 4 * sm_count();
+  if (a.vocab <= 1024 || (many && a.vocab <= 4096)) return launch_fwd<kType, 32, kTop>(a, 0, st);
+  if (many) return launch_fwd<kType, 128, kTop>(a, 0, st);
   int log_split = 0;
-  while (log_split < 3 && a.rows << log_split < 2 * sm_count() && a.vocab >> log_split > 8192) ++log_split;
+  while (log_split < 2 && a.rows << log_split < 2 * sm_count() && a.vocab >> log_split > 8192) ++log_split;
   return launch_fwd<kType, 256, kTop>(a, log_split, st);
 }
 

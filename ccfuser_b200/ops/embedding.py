@@ -8,8 +8,8 @@ the same bits every time. The autograd function is C++ (csrc/torch_tokens.cpp); 
 while a graph is traced.
 
 An id outside its table does not fault the GPU: its row is NaN, it adds nothing to a gradient, and it is recorded in the device's status word, which
-``ops.gemm.Workspace.get(device).check()`` raises as ``TokenIndexError``. On the CPU, and for other types than bf16, fp16 and fp32, the same
-sums run on torch's operations, which raise ``IndexError``.
+``ops.gemm.Workspace.get(device).check()`` raises as ``TokenIndexError``. On the CPU the same sums run on torch's operations, which raise
+``IndexError``.
 """
 from __future__ import annotations
 
@@ -138,7 +138,13 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *, po
         _check_ids("type_ids", type_ids, weight.device)
         if type_ids.shape != ids.shape:
             type_ids = type_ids.expand(ids.shape)
-    if not (weight.is_cuda and weight.dtype in N.DTYPE_CODE and ids.numel() > 0 and weight.numel() > 0):
+    if ids.numel() == 0 or weight.shape[1] == 0:
+        return weight.new_zeros(*ids.shape, weight.shape[1])
+    if any(t is not None and t.shape[0] == 0 for t in (weight, position_weight, type_weight)):
+        raise ValueError("a table without rows")
+    if weight.is_cuda and weight.dtype not in N.DTYPE_CODE:
+        raise TypeError(f"tables on a GPU are bf16, fp16 or fp32, not {weight.dtype}")
+    if not weight.is_cuda:
         return _embedding_torch(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx)
     if ids.numel() > MAX_TOKENS:
         raise ValueError(f"{ids.numel()} tokens: at most 2^31 - 1 in one call")
@@ -169,7 +175,9 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
     if num_rows < 1 or grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
         raise ValueError(f"grad: {list(ids.shape)} + [d] and at least one row, got {list(grad.shape)} and {num_rows} rows")
     skip = _skip(padding_idx, num_rows)
-    if not (grad.is_cuda and grad.dtype in N.DTYPE_CODE and grad.numel() > 0):
+    if grad.is_cuda and grad.dtype not in N.DTYPE_CODE:
+        raise TypeError(f"gradients on a GPU are bf16, fp16 or fp32, not {grad.dtype}")
+    if not grad.is_cuda or grad.numel() == 0:
         grad = grad.detach()
         out = torch.zeros(num_rows, grad.shape[-1], dtype=grad.dtype if grad.dtype == torch.float64 else torch.float32, device=grad.device)
         out.index_add_(0, ids.reshape(-1).long(), grad.reshape(-1, grad.shape[-1]).to(out.dtype))
