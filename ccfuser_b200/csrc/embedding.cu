@@ -522,16 +522,15 @@ static bool valid(const CcfEmbed* e) {
   return true;
 }
 
-template <typename... KArgs>
-static cudaError_t launch_behind(void (*kern)(KArgs...), dim3 grid, int threads, cudaStream_t st, KArgs... args) {
+static cudaError_t launch_behind(void (*kern)(GradArgs), dim3 grid, int threads, cudaStream_t st, int early, const GradArgs& g) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.stream = st;
   cudaLaunchAttribute attr = early_attribute();
   cfg.attrs = &attr;
-  cfg.numAttrs = early_launches(0, st);
-  return cudaLaunchKernelEx(&cfg, kern, args...);
+  cfg.numAttrs = early;
+  return cudaLaunchKernelEx(&cfg, kern, g);
 }
 
 template <int kType, bool kVec>
@@ -571,17 +570,18 @@ static int launch_bwd(GradArgs& g, cudaStream_t st) {
   const long long front = 2 * sm_count();   // about what is written while the merge runs
   g.zeros_first = static_cast<uint32_t>(early > 0 || g.chunks == 1 ? 0 : zeros < front ? zeros : front);
   const dim3 blocks(static_cast<unsigned>(sums + zeros));
+  const int may_overlap = early_launches(0, st);
   int launches = 2;
   embedding_sort_kernel<<<dim3(sorted ? g.chunks : 1, g.tables), kSortChunk, 0, st>>>(g);
   cudaError_t err = cudaGetLastError();
   if (err == cudaSuccess && sorted && g.chunks > 1) {
-    err = launch_behind(embedding_merge_kernel, dim3((g.tokens + kMergeThreads - 1) / kMergeThreads, g.tables), kMergeThreads, st, g);
+    err = launch_behind(embedding_merge_kernel, dim3((g.tokens + kMergeThreads - 1) / kMergeThreads, g.tables), kMergeThreads, st, may_overlap, g);
     ++launches;
   }
-  if (err == cudaSuccess) err = launch_behind(embedding_sum_kernel<kType, kVec>, blocks, 32 * kEmbWarps, st, g);
+  if (err == cudaSuccess) err = launch_behind(embedding_sum_kernel<kType, kVec>, blocks, 32 * kEmbWarps, st, may_overlap, g);
   if (err == cudaSuccess && most > 1) {
     const unsigned items = most * g.slices, wave = 2 * sm_count();
-    err = launch_behind(embedding_join_kernel<kType, kVec>, dim3(items < wave ? items : wave, g.tables), 32 * kJoinWarps, st, g);
+    err = launch_behind(embedding_join_kernel<kType, kVec>, dim3(items < wave ? items : wave, g.tables), 32 * kJoinWarps, st, may_overlap, g);
     ++launches;
   }
   return err == cudaSuccess ? launches : -static_cast<int>(err);
