@@ -5,6 +5,8 @@
 // Both directions are bound by bytes. Forward: the used rows in, y out. Backward: dW[v] = scale * sum of dy_t over the tokens with id v, in
 // fp32, rounded once; dy is read once and every row of the gradient written once. The tokens are sorted by (id, place) first, so that a
 // row's sum runs over its tokens in their order: no atomics on values, the same bits every time.
+#include <cooperative_groups.h>
+
 #include "elements.cuh"
 #include "embedding.h"
 
@@ -13,6 +15,7 @@ namespace ccf {
 constexpr int kSortChunk = 1024;     // keys that one block sorts in shared memory
 constexpr int kEmbWarps = 8;
 constexpr int kJoinWarps = 16;
+constexpr uint32_t kShort = 4;       // further pieces of a run that a warp adds up by itself
 constexpr uint32_t kNoRow = 0xffffffffu;   // id of a token without a gradient: skipped row, index out of range
 
 // a product that may pass 32 bits, in one instruction
@@ -165,7 +168,8 @@ __global__ void __launch_bounds__(32 * kEmbWarps, 4) embedding_fwd_kernel(const 
 // ---- backward ----------------------------------------------------------------------------------------------------------
 // Scratch of one table. `keys`: (id << 32 | token), sorted. `slot`: for a row that some token has, one of its tokens. A run of equal ids is cut where
 // a piece of the sorted tokens ends: a piece leaves the sum of a run that came from the piece before in `head`, of one that began in it and goes on in
-// `tail`; `list` holds the pieces that left a tail.
+// `tail`; `list` holds the pieces that left a tail, with the run's id: from the front
+// those of runs with at most kShort further pieces, from the back the others; `count` says how many of each.
 struct GradTable {
   const void* ids;
   void* grad;
@@ -175,7 +179,7 @@ struct GradTable {
   uint32_t* slot;
   float* head;
   float* tail;
-  int* list;
+  uint2* list;
   int* count;
   long long rows;
   long long skip;
@@ -202,23 +206,60 @@ __device__ __forceinline__ uint64_t key_at(const GradArgs& g, const GradTable& t
   return static_cast<uint64_t>(s) << 32 | ((i - s * g.batch) * g.seq + s);
 }
 
+// The place of a key among all: its place in its own chunk and, for every other chunk, the keys there that are smaller: those of smaller ids and, in
+// earlier chunks, of the same. `ids`: those of kSide chunks from chunk c on, in order, kNoRow where there is none; searched side by side, three instructions a
+// step (with bounds and both comparisons in it eight, and 7.7 us for 8192 tokens in eight blocks instead of 4).
+constexpr int kSide = 8;
+__device__ __forceinline__ uint32_t smaller_elsewhere(const GradArgs& g, const uint32_t* ids, uint32_t c, uint32_t own, uint32_t id) {
+  uint32_t lo[kSide], below[kSide], n = 0;
+#pragma unroll
+  for (int u = 0; u < kSide; ++u) {
+    lo[u] = 0;
+    below[u] = c + u < own ? id + 1 : id;
+  }
+#pragma unroll
+  for (uint32_t step = kSortChunk / 2; step > 0; step /= 2) {
+#pragma unroll
+    for (int u = 0; u < kSide; ++u)
+      if (ids[u * kSortChunk + lo[u] + step - 1] < below[u]) lo[u] += step;
+  }
+#pragma unroll
+  for (int u = 0; u < kSide; ++u) {
+    lo[u] += ids[u * kSortChunk + lo[u]] < below[u];
+    // a token without a row stands behind all of an earlier chunk (its id + 1 is 0)
+    if (id == kNoRow && c + u < own) lo[u] = kSortChunk;
+    if (c + u != own) n += lo[u];
+  }
+  return n;
+}
+
 // Each block sorts one chunk of keys, one for each thread: bitonic, with exchanges inside a warp by shuffles and the others through shared memory.
+// Up to kSide chunks are one cluster, whose blocks then read each other's ids and put every key in its place among all: 8192 tokens in one launch.
 // Every token also leaves its place in `slot` at its id, whichever of equal ids comes last: a row is used if the token named there has its id. So
-// `slot` needs no zeros beforehand, and what it says is the same whoever won. 17 us with 2048 keys in shared memory alone, ? now.
+// `slot` needs no zeros beforehand, and what it says is the same whoever won. 8192 tokens 10.7 us, 1024 5; a chunk of 2048 64-bit keys sorted in shared
+// memory alone took 17, and the merge as a launch of its own 9 more.
+// Key: (id, place in the chunk) in 32 bits for tables of less than kShortRows rows, in 64 for larger ones.
+constexpr uint32_t kShortRows = (1u << 22) - 1;
+template <typename Key>
 __global__ void __launch_bounds__(kSortChunk) embedding_sort_kernel(const __grid_constant__ GradArgs g) {
-  __shared__ uint64_t other[2][kSortChunk];
+  namespace cg = cooperative_groups;
+  constexpr int kPlaceBits = sizeof(Key) == 4 ? 10 : 32;
+  constexpr uint32_t kLast = sizeof(Key) == 4 ? kShortRows : kNoRow;   // the id of a token without a row
+  __shared__ Key other[2][kSortChunk];
+  __shared__ uint32_t ids[kSide * kSortChunk];
   const GradTable& t = g.table[blockIdx.y];
   let_next_in();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *t.count = 0;
+  if (blockIdx.x == 0 && threadIdx.x < 2) t.count[threadIdx.x] = 0;
   if (t.ids == nullptr) return;
-  const uint32_t tid = threadIdx.x, base = blockIdx.x * kSortChunk, n = min(g.tokens - base, static_cast<uint32_t>(kSortChunk));
-  uint64_t key = ~0ull;
+  const uint32_t tid = threadIdx.x, own = blockIdx.x, base = own * kSortChunk;
+  const uint32_t n = own < g.chunks ? min(g.tokens - base, static_cast<uint32_t>(kSortChunk)) : 0;
+  Key key = ~static_cast<Key>(0);
   if (tid < n) {
     const long long id = load_index(t.ids, base + tid, t.wide);
     const bool in = id >= 0 && id < t.rows;
     if (!in) report_status(g.status, CCF_ERR_INDEX, static_cast<int>(base + tid) & 0x7fffff);
     else t.slot[id] = base + tid;
-    key = static_cast<uint64_t>(in && id != t.skip ? static_cast<uint32_t>(id) : kNoRow) << 32 | (base + tid);
+    key = static_cast<Key>(in && id != t.skip ? static_cast<uint32_t>(id) : kLast) << kPlaceBits | tid;
   }
   int half = 0;
 #pragma unroll 1
@@ -228,57 +269,58 @@ __global__ void __launch_bounds__(kSortChunk) embedding_sort_kernel(const __grid
     for (uint32_t j = size / 2; j >= 32; j /= 2, half ^= 1) {
       other[half][tid] = key;
       __syncthreads();
-      const uint64_t o = other[half][tid ^ j];
+      const Key o = other[half][tid ^ j];
       key = (((tid & j) == 0) == up) == (o < key) ? o : key;
     }
 #pragma unroll
     for (uint32_t j = 16; j > 0; j /= 2) {
       if (j >= size) continue;
-      const uint64_t o = __shfl_xor_sync(0xffffffffu, key, j);
+      const Key o = __shfl_xor_sync(0xffffffffu, key, j);
       key = (((tid & j) == 0) == up) == (o < key) ? o : key;
     }
   }
-  if (tid < n) t.sorted_chunks[base + tid] = key;
-  if (g.chunks > 1) t.chunk_ids[base + tid] = tid < n ? id_of(key) : kNoRow;
+  uint32_t id = static_cast<uint32_t>(key >> kPlaceBits);
+  if (tid >= n || id == kLast) id = kNoRow;
+  const uint64_t full = static_cast<uint64_t>(id) << 32 | (base + (static_cast<uint32_t>(key) & (kSortChunk - 1)));
+  if (g.chunks == 1) {
+    if (tid < n) t.keys[tid] = full;
+    return;
+  }
+  if (g.chunks > kSide) {   // the merging kernel goes on
+    if (tid < n) t.sorted_chunks[base + tid] = full;
+    t.chunk_ids[base + tid] = id;
+    return;
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  if (own < g.chunks) ids[own * kSortChunk + tid] = id;
+  cluster.sync();
+#pragma unroll
+  for (uint32_t u = 0; u < kSide; ++u)
+    if (u != own) ids[u * kSortChunk + tid] = u < g.chunks ? cluster.map_shared_rank(ids, u)[u * kSortChunk + tid] : kNoRow;
+  cluster.sync();   // nobody leaves while its shared memory is read
+  if (tid < n) t.keys[tid + smaller_elsewhere(g, ids, 0, own, id)] = full;
 }
 
-// A key's place among all: its place in its own chunk and, for every other chunk, the keys there that are smaller: those of smaller ids and, in earlier
-// chunks, of the same. A block brings the ids of kSide chunks at a time into shared memory and searches them side by side for kMergeThreads keys of one
-// chunk: eleven steps there take less than one read from L2. Several blocks for each chunk: the searches' bank conflicts are what a block's time goes to.
-constexpr int kSide = 8, kMergeThreads = 256;
+// More chunks than a cluster has blocks: kMergeThreads keys of one chunk a block, the ids of kSide chunks at a time in shared memory.
+constexpr int kMergeThreads = 256;
 __global__ void __launch_bounds__(kMergeThreads) embedding_merge_kernel(const __grid_constant__ GradArgs g) {
   constexpr int kEach = kSide * kSortChunk / 4 / kMergeThreads;   // 16-byte pieces of ids for each thread
   __shared__ uint4 staged[kSide * kSortChunk / 4];
-  const uint32_t* const ids = reinterpret_cast<const uint32_t*>(staged);
   after_previous();
   const GradTable& t = g.table[blockIdx.y];
   if (t.ids == nullptr) return;
   const uint32_t i = blockIdx.x * kMergeThreads + threadIdx.x, own = i / kSortChunk;
   const uint64_t key = i < g.tokens ? t.sorted_chunks[i] : ~0ull;
-  const uint32_t id = id_of(key);
   uint32_t place = i % kSortChunk;
   for (uint32_t c = 0; c < g.chunks; c += kSide) {
-    const uint32_t most = min(static_cast<uint32_t>(kSide), g.chunks - c) * (kSortChunk / 4);
+    const uint32_t most = min(static_cast<uint32_t>(kSide), g.chunks - c) * (kSortChunk / 4);   // the rest: no chunks
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
       const uint32_t at = u * kMergeThreads + threadIdx.x;
-      if (at < most) staged[at] = reinterpret_cast<const uint4*>(t.chunk_ids + c * kSortChunk)[at];
+      staged[at] = at < most ? reinterpret_cast<const uint4*>(t.chunk_ids + c * kSortChunk)[at] : make_uint4(kNoRow, kNoRow, kNoRow, kNoRow);
     }
     __syncthreads();
-    uint32_t lo[kSide] = {};
-#pragma unroll
-    for (uint32_t step = kSortChunk; step > 0; step /= 2) {
-#pragma unroll
-      for (int u = 0; u < kSide; ++u) {
-        const uint32_t to = lo[u] + step;
-        if (to > kSortChunk || c + u >= g.chunks) continue;
-        const uint32_t o = ids[u * kSortChunk + to - 1];
-        if (o < id || (o == id && c + u < own)) lo[u] = to;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kSide; ++u)   // behind the last token the ids are kNoRow, which only tokens without a row reach: those places do not count
-      if (c + u < g.chunks && c + u != own) place += min(lo[u], g.tokens - (c + u) * kSortChunk);
+    place += smaller_elsewhere(g, reinterpret_cast<const uint32_t*>(staged), c, own, id_of(key));
     __syncthreads();
   }
   if (i < g.tokens) t.keys[place] = key;
@@ -286,7 +328,7 @@ __global__ void __launch_bounds__(kMergeThreads) embedding_merge_kernel(const __
 
 // Sums, and the zeros of the rows that no token has, 32 rows a block. A summing warp takes one piece of the sorted tokens and one slice of the columns.
 // Positions come first: their order is known, so these blocks do not wait for the sort, and they leave dy in L2 for the sums by id. Without positions
-// some of the zeros stand in front: they need the sorting kernel's results only, not the merging one's, which has waited for it. The other
+// some of the zeros stand in front where a merging kernel runs: they need the sorting kernel's results only, which that one has waited for. The other
 // zeros come last. Alternating sums and zeros was slower (59 us against 53: blocks that wait for the merge hold the places of blocks that could write).
 template <int kType, bool kVec>
 __global__ void __launch_bounds__(32 * kEmbWarps, 5) embedding_sum_kernel(const __grid_constant__ GradArgs g) {
@@ -299,7 +341,7 @@ __global__ void __launch_bounds__(32 * kEmbWarps, 5) embedding_sum_kernel(const 
     int k = 0;
     while (w >= (g.table[k].rows + 31) / 32) w -= static_cast<uint32_t>((g.table[k++].rows + 31) / 32);
     const GradTable& t = g.table[k];
-    if (t.ids != nullptr && g.chunks == 1) wait_for_previous();
+    if (t.ids != nullptr && g.chunks <= kSide) wait_for_previous();
     let_next_in();
     const long long row = static_cast<long long>(w) * 32 + warp * 4 + lane_id();
     bool used = true;
@@ -354,8 +396,11 @@ __global__ void __launch_bounds__(32 * kEmbWarps, 5) embedding_sum_kernel(const 
       } else if (goes_on) {
         S::store_f32(t.tail + wide(piece, g.d) + c, left, f);
         if (c == 0 && lane_id() == 0) {
-          wait_for_previous();   // the sorting kernel zeroed the count
-          t.list[atomicAdd(t.count, 1)] = static_cast<int>(piece);
+          wait_for_previous();   // the sorting kernel zeroed the counts
+          const uint32_t far = piece + kShort + 1;
+          const bool is_long = far < t.pieces && id_of(key_at(g, t, far * t.piece)) == run;
+          const int at = atomicAdd(t.count + is_long, 1);
+          t.list[is_long ? t.pieces - 1 - at : at] = make_uint2(piece, run);
         }
       } else {
 #pragma unroll
@@ -392,75 +437,60 @@ __global__ void __launch_bounds__(32 * kEmbWarps, 5) embedding_sum_kernel(const 
 }
 
 // Runs that cross pieces: the tail of the piece where the run began, then the heads of those behind it, in their order. Most runs go on for a few pieces:
-// a warp adds one up, four heads in flight, each read together with the key that says whether it counts. Runs of more than kShort further pieces are left to
-// the whole block, whose warps take every kJoinWarps-th piece each; their sums are added in the warps' order.
+// a warp adds one up, all of its heads in flight, each read together with the key that says whether it counts. Runs of more than kShort further pieces are for
+// a whole block, whose warps take every kJoinWarps-th piece each; their sums are added in the warps' order. Those come first: they take longest.
 template <int kType, bool kVec>
 __global__ void __launch_bounds__(32 * kJoinWarps) embedding_join_kernel(const __grid_constant__ GradArgs g) {
   using S = Slice<kType, kVec>;
-  constexpr uint32_t kUnroll = 4, kShort = 4;
   __shared__ __align__(16) float red[kJoinWarps][S::kCols];
   after_previous();
   const GradTable& t = g.table[blockIdx.y];
-  const uint32_t warp = threadIdx.x >> 5, items = static_cast<uint32_t>(*t.count) * g.slices;
-  auto add_heads = [&](uint32_t q, uint32_t step, uint32_t c, int left, uint32_t run, float (&acc)[S::kE]) {   // of pieces q, q + step, ...; whether all counted
-    float part[kUnroll][S::kE];
-    uint32_t id[kUnroll];
+  const uint32_t warp = threadIdx.x >> 5, shorts = static_cast<uint32_t>(t.count[0]) * g.slices, longs = static_cast<uint32_t>(t.count[1]) * g.slices;
+  auto add_heads = [&](uint32_t q, uint32_t step, uint32_t c, int left, uint32_t run, float (&acc)[S::kE]) {   // of kShort pieces; whether all counted
+    float part[kShort][S::kE];
+    uint32_t id[kShort];
 #pragma unroll
-    for (uint32_t u = 0; u < kUnroll; ++u) {
+    for (uint32_t u = 0; u < kShort; ++u) {
       const uint32_t p = min(q + u * step, t.pieces - 1);
       id[u] = q + u * step < t.pieces ? id_of(key_at(g, t, p * t.piece)) : kNoRow;
       S::load_f32(t.head + wide(p, g.d) + c, left, part[u]);
     }
     bool on = true;
 #pragma unroll
-    for (uint32_t u = 0; u < kUnroll; ++u) {
+    for (uint32_t u = 0; u < kShort; ++u) {
       on = on && id[u] == run;   // the same id, so the run goes on: what the head's memory holds otherwise is not added
 #pragma unroll
       for (int i = 0; i < S::kE; ++i) acc[i] = on ? acc[i] + part[u][i] : acc[i];
     }
     return on;
   };
-  // a run with more than kShort pieces behind the one where it began
-  auto is_long = [&](uint32_t piece, uint32_t run) {
-    const uint32_t far = piece + kShort + 1;
-    return far < t.pieces && id_of(key_at(g, t, far * t.piece)) == run;
-  };
-  for (uint32_t it = blockIdx.x * kJoinWarps + warp; it < items; it += gridDim.x * kJoinWarps) {
-    const uint32_t piece = static_cast<uint32_t>(t.list[it / g.slices]), c = it % g.slices * S::kCols;
+  for (uint32_t it = blockIdx.x; it < longs; it += gridDim.x) {
+    const uint2 what = t.list[t.pieces - 1 - it / g.slices];
+    const uint32_t c = it % g.slices * S::kCols;
     const int left = g.d - static_cast<int>(c);
-    const uint32_t run = id_of(key_at(g, t, (piece + 1) * t.piece - 1));
-    if (is_long(piece, run)) continue;
+    float acc[S::kE] = {};
+    for (uint32_t q = what.x + 1 + warp; q < t.pieces && add_heads(q, kJoinWarps, c, left, what.y, acc); q += kShort * kJoinWarps) {}
+    S::store_f32(red[warp], S::kCols, acc);
+    __syncthreads();
+    for (int j = threadIdx.x; j < S::kCols && j < left; j += 32 * kJoinWarps) {
+      float s = t.tail[wide(what.x, g.d) + c + j];
+#pragma unroll
+      for (int k = 0; k < kJoinWarps; ++k) s += red[k][j];
+      store_elem<kType>(t.grad, static_cast<long long>(wide(what.y, g.d) + c + j), s * t.scale);
+    }
+    __syncthreads();
+  }
+  // from the other end of the grid
+  for (uint32_t it = (gridDim.x - 1 - blockIdx.x) * kJoinWarps + warp; it < shorts; it += gridDim.x * kJoinWarps) {
+    const uint2 what = t.list[it / g.slices];
+    const uint32_t c = it % g.slices * S::kCols;
+    const int left = g.d - static_cast<int>(c);
     float acc[S::kE];
-    S::load_f32(t.tail + wide(piece, g.d) + c, left, acc);
-    for (uint32_t q = piece + 1; q <= piece + kShort && add_heads(q, 1, c, left, run, acc); q += kUnroll) {}
+    S::load_f32(t.tail + wide(what.x, g.d) + c, left, acc);
+    add_heads(what.x + 1, 1, c, left, what.y, acc);
 #pragma unroll
     for (int i = 0; i < S::kE; ++i) acc[i] *= t.scale;
-    S::store(t.grad, wide(run, g.d) + c, left, acc);
-  }
-  for (uint32_t base = blockIdx.x; base < items; base += 32 * gridDim.x) {   // 32 items of this block looked through at a time, by every warp alike
-    const uint32_t mine = base + lane_id() * gridDim.x;
-    bool here = false;
-    if (mine < items) {
-      const uint32_t piece = static_cast<uint32_t>(t.list[mine / g.slices]);
-      here = is_long(piece, id_of(key_at(g, t, (piece + 1) * t.piece - 1)));
-    }
-    for (uint32_t todo = __ballot_sync(0xffffffffu, here); todo != 0; todo &= todo - 1) {
-      const uint32_t it = base + (__ffs(todo) - 1) * gridDim.x;
-      const uint32_t piece = static_cast<uint32_t>(t.list[it / g.slices]), c = it % g.slices * S::kCols;
-      const int left = g.d - static_cast<int>(c);
-      const uint32_t run = id_of(key_at(g, t, (piece + 1) * t.piece - 1));
-      float acc[S::kE] = {};
-      for (uint32_t q = piece + 1 + warp; q < t.pieces && add_heads(q, kJoinWarps, c, left, run, acc); q += kUnroll * kJoinWarps) {}
-      S::store_f32(red[warp], S::kCols, acc);
-      __syncthreads();
-      for (int j = threadIdx.x; j < S::kCols && j < left; j += 32 * kJoinWarps) {
-        float s = t.tail[wide(piece, g.d) + c + j];
-#pragma unroll
-        for (int k = 0; k < kJoinWarps; ++k) s += red[k][j];
-        store_elem<kType>(t.grad, static_cast<long long>(wide(run, g.d) + c + j), s * t.scale);
-      }
-      __syncthreads();
-    }
+    S::store(t.grad, wide(what.y, g.d) + c, left, acc);
   }
 }
 
@@ -484,15 +514,16 @@ static size_t lay_out(GradTable* t, void* base, long long tokens, long long rows
     return r;
   };
   GradTable x{};
-  x.count = reinterpret_cast<int*>(take(4));
-  x.list = reinterpret_cast<int*>(take(4 * pieces));
+  x.count = reinterpret_cast<int*>(take(8));
+  x.list = reinterpret_cast<uint2*>(take(8 * pieces));
   x.head = reinterpret_cast<float*>(take(4 * pieces * d));
   x.tail = reinterpret_cast<float*>(take(4 * pieces * d));
   if (sorted) {
+    const size_t chunks = (n + kSortChunk - 1) / kSortChunk;
     x.slot = reinterpret_cast<uint32_t*>(take(4 * static_cast<size_t>(rows)));
-    x.sorted_chunks = reinterpret_cast<uint64_t*>(take(8 * n));
-    x.chunk_ids = reinterpret_cast<uint32_t*>(take(n > kSortChunk ? 4 * ((n + kSortChunk - 1) / kSortChunk) * kSortChunk : 0));
-    x.keys = n > kSortChunk ? reinterpret_cast<uint64_t*>(take(8 * n)) : x.sorted_chunks;
+    x.keys = reinterpret_cast<uint64_t*>(take(8 * n));
+    x.sorted_chunks = reinterpret_cast<uint64_t*>(take(chunks > kSide ? 8 * n : 0));
+    x.chunk_ids = reinterpret_cast<uint32_t*>(take(chunks > kSide ? 4 * chunks * kSortChunk : 0));
   }
   if (t != nullptr) {
     t->piece = static_cast<uint32_t>(piece);
@@ -550,7 +581,7 @@ template <int kType, bool kVec>
 static int launch_bwd(GradArgs& g, cudaStream_t st) {
   using S = Slice<kType, kVec>;
   g.slices = (g.d + S::kCols - 1) / S::kCols;
-  long long sums = 0, zeros = 0, early = 0;
+  long long sums = 0, zeros = 0, early = 0, largest = 0;
   uint32_t most = 0;
   bool sorted = false;
   for (int k = 0; k < g.tables; ++k) {
@@ -562,19 +593,29 @@ static int launch_bwd(GradArgs& g, cudaStream_t st) {
     zeros += (t.rows + 31) / 32;
     if (t.ids == nullptr) early += blocks;
     else sorted = true;
+    largest = t.rows > largest ? t.rows : largest;
     most = t.pieces > most ? t.pieces : most;
   }
   if (sums + zeros > 0x7fffffffll) return -2;
   g.sums = static_cast<uint32_t>(sums);
   g.early = static_cast<uint32_t>(early);
   const long long front = 2 * sm_count();   // about what is written while the merge runs
-  g.zeros_first = static_cast<uint32_t>(early > 0 || g.chunks == 1 ? 0 : zeros < front ? zeros : front);
+  g.zeros_first = static_cast<uint32_t>(early > 0 || g.chunks <= kSide ? 0 : zeros < front ? zeros : front);
   const dim3 blocks(static_cast<unsigned>(sums + zeros));
   const int may_overlap = early_launches(0, st);
   int launches = 2;
-  embedding_sort_kernel<<<dim3(sorted ? g.chunks : 1, g.tables), kSortChunk, 0, st>>>(g);
-  cudaError_t err = cudaGetLastError();
-  if (err == cudaSuccess && sorted && g.chunks > 1) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  while (g.chunks <= kSide && attr.val.clusterDim.x < g.chunks) attr.val.clusterDim.x *= 2;
+  cfg.gridDim = dim3(!sorted ? 1 : g.chunks <= kSide ? attr.val.clusterDim.x : g.chunks, g.tables);
+  cfg.blockDim = dim3(kSortChunk);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = sorted && attr.val.clusterDim.x > 1 ? 1 : 0;
+  cudaError_t err = cudaLaunchKernelEx(&cfg, largest < kShortRows ? embedding_sort_kernel<uint32_t> : embedding_sort_kernel<uint64_t>, g);
+  if (err == cudaSuccess && sorted && g.chunks > kSide) {
     err = launch_behind(embedding_merge_kernel, dim3((g.tokens + kMergeThreads - 1) / kMergeThreads, g.tables), kMergeThreads, st, may_overlap, g);
     ++launches;
   }
