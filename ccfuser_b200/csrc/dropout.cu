@@ -5,13 +5,15 @@
 // (mix_moe/mix_moe/examples/transformer-xl/mem_transformer_mix_moe.py).
 //
 // Bound by reading x (and the residual) and writing y once. 16 bits an element, eight elements a block of the generator: ten integer operations an
-// element next to 4 or 6 bytes. p is rounded to a multiple of 2^-16, and 1 / (1 - p) is that of the rounded p, so that the mean stays.
+// element next to 4 or 6 bytes. p is rounded to a multiple of 2^-16, and 1 / (1 - p) is that of the rounded p, so that the mean stays. One rounding, of
+// the sum in fp32. 16384 x 4096 bf16 with the residual 66 us (6.1 TB/s), without 51 (5.3 TB/s; with one round of the generator instead of ten 48).
 #include "dropout.h"
 #include "elements.cuh"
 
 namespace ccf {
 
-constexpr int kDropThreads = 256, kDropBlocks = 4;   // blocks per SM: one wave, each thread walks the groups a grid apart
+// Blocks per SM: one wave, each thread walks the groups a grid apart. Sum of both passes at that size with 3, 4, 5 and 6 blocks: 124, 118, 122 and 121 us.
+constexpr int kDropThreads = 256, kDropBlocks = 4;
 template <int kType, bool kResidual>
 constexpr int kDropGroups = kType != kFp32 && !kResidual ? 4 : 2;   // groups that a thread has in flight: 64 bytes
 

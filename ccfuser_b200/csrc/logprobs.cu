@@ -6,7 +6,8 @@
 //   lp_j = (x_j - M) / T - ln S        H = ln S - ln 2 * Q / S        (both terms of H are >= 0: nothing cancels)
 //   dx_j = 1/T * ( g [j = t] + sum_k g_k [j = top_k] - p_j (g + sum_k g_k + g_H (lp_j + H)) ),   p_j = 2^u_j / S
 // One pass over the logits with running M, S and Q forward; one pass that reads them and writes the gradient backward. Both are bound by those
-// bytes; next to them stand one exponential and about five more instructions an element. Statistics in fp32.
+// bytes; next to them stand one exponential and about five more instructions an element. Statistics in fp32: a sum of V terms has V / 512 to V / 64
+// additions in a row, and the terms' relative error of 2^-22 averages out; the gradient is rounded once, to the logits' type.
 #include <cooperative_groups.h>
 
 #include "elements.cuh"
@@ -190,7 +191,6 @@ struct RowShared {
   uint64_t top[CCF_LOGPROBS_MAX_TOP];
   uint64_t best[kThreads / 32];
   uint64_t list[kListLen<kThreads>];
-  uint32_t bound;
   int listed;
 };
 template <int kThreads>
@@ -206,9 +206,9 @@ __device__ __forceinline__ void row_sync() {
 }
 
 // sh.list[0, n) by rank into sh.top, the k largest
-template <int kThreads>
-__device__ __forceinline__ void rank_list(RowShared<kThreads>& sh, int n, int k, int tid) {
-  for (int i = tid; i < n; i += kThreads) {
+template <int kStep, typename Shared>
+__device__ __forceinline__ void rank_list(Shared& sh, int n, int k, int first) {
+  for (int i = first; i < n; i += kStep) {
     const uint64_t key = sh.list[i];
     int rank = 0;
 #pragma unroll 8
@@ -232,10 +232,7 @@ __device__ __forceinline__ uint32_t group_maxima(RowShared<kThreads>& sh, float 
   uint32_t g = mine;
   for (int o = 1 << log >> 1; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
   if ((tid & ((1 << log) - 1)) == 0) sh.group[tid >> log] = g;
-  if (tid == 0) {
-    sh.listed = 0;
-    sh.bound = 1;
-  }
+  if (tid == 0) sh.listed = 0;
   if (tid < CCF_LOGPROBS_MAX_TOP) sh.top[tid] = 0;
   return mine;
 }
@@ -251,8 +248,9 @@ __device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_
   const int tid = kThreads == 32 ? lane_id() : threadIdx.x, lane = lane_id();
   const uint4* pieces = reinterpret_cast<const uint4*>(p + shape.head * kElemBytes<kType>);
   const int groups = kThreads >> log_group<kThreads>(k);
-  if (tid < groups) {
-    const uint32_t g = sh.group[tid];
+  uint32_t bound = 0;   // every warp finds it by itself: cheaper than a barrier
+  for (int j = lane; j < groups; j += 32) {
+    const uint32_t g = sh.group[j];
     int above = 0, from = 0;
 #pragma unroll 2
     for (int i = 0; i < groups; i += 4) {   // at least four groups
@@ -260,10 +258,9 @@ __device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_
       above += (o.x > g) + (o.y > g) + (o.z > g) + (o.w > g);
       from += (o.x >= g) + (o.y >= g) + (o.z >= g) + (o.w >= g);
     }
-    if (g != 0 && above < k && k <= from) sh.bound = g;   // the k-th largest; where there are fewer elements than that, every finite one counts
+    if (above < k && k <= from) bound = g;   // the k-th largest
   }
-  row_sync<kThreads>();
-  const uint32_t bound = sh.bound;
+  bound = max(1u, __reduce_max_sync(0xffffffffu, bound));   // fewer elements than that: every finite one counts
   auto list = [&](float v, int index) {
     const int at = atomicAdd(&sh.listed, 1);
     if (at < kListLen<kThreads>) sh.list[at] = top_key(v, index);
@@ -298,9 +295,9 @@ __device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_
   }
   row_sync<kThreads>();
   const int n = sh.listed;
-  if (n <= kListLen<kThreads>) {
-    rank_list<kThreads>(sh, n, k, tid);
-    row_sync<kThreads>();
+  if (n <= kListLen<kThreads>) {   // the first warp's work, and what is written from it too
+    if (tid < 32) rank_list<32>(sh, n, k, lane);
+    __syncwarp();
     return;
   }
   uint64_t below = ~0ull;
@@ -336,8 +333,11 @@ __device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_
   row_sync<kThreads>();
 }
 
-// kThreads per row; a warp per row, eight rows a block, where rows are short. Rows of wide vocabularies may be shared by a cluster of `split` blocks,
+// kThreads per row; a warp per row, eight rows a block, where rows are short. Rows of wide vocabularies may be shared by a cluster of 2^log_split blocks,
 // each with its part of the columns, whose statistics and alternatives the first one joins: a few rows would leave most of the card idle.
+// 8192 rows of 50257 bf16 131 us (6.3 TB/s), 4099 with five alternatives 84 (4.9 TB/s: choosing them takes a tenth more instructions), 4 rows with twenty 10.
+// Bound by the memory in the first, by the arithmetic's latency in the second (55 % of the issue slots). Rows by bulk copies into shared memory, over the ends
+// of rows, took 167 to 230 us: what their buffers leave room for is too few warps.
 template <int kType, int kThreads, bool kTop>
 __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_kernel(const __grid_constant__ CcfLogprobs a, int log_split) {
   namespace cg = cooperative_groups;
@@ -429,6 +429,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
       cluster.sync();   // nobody leaves while its shared memory is read
       if (rank != 0) return;
     }
+    if (tid >= 32) return;   // the first warp has what is left
   }
   const float log_s = logf(st.s), mc = st.m * c;
   // lp_j = (x_j - M) / T - log_sum: the sum stands relative to the rounded M c, so the rounding is taken out of it
@@ -492,7 +493,8 @@ __device__ __forceinline__ RowGrad row_grad(const CcfLogprobs& a, long long row,
   return r;
 }
 
-// kThreads per row and part of its columns (blockIdx.y of gridDim.y), a warp per row where rows are short.
+// kThreads per row and part of its columns (blockIdx.y of gridDim.y), a warp per row where rows are short. Bound by reading the logits and writing
+// the gradient once: 8192 rows of 50304 bf16 254 us, 6.5 TB/s.
 template <int kType, int kThreads>
 __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_bwd_kernel(const __grid_constant__ CcfLogprobs a) {
   constexpr int kE = kElemsPer16<kType>;
@@ -605,6 +607,9 @@ static int launch_fwd(const CcfLogprobs& a, int log_split, cudaStream_t st) {
 
 template <int kType, bool kTop>
 static int choose_fwd(const CcfLogprobs& a, cudaStream_t st) {
+  // us, 0 and 5 alternatives. A warp a row against more threads: 8192 x 1000 12 and 16 / 18 and 35, 4096 x 4000 14 and 18 / 14 and 21, 300 x 4000
+  // 12 / 7. 128 threads against 256: 8192 x 50257 131 / 144, 2000 x 2000 8 / 12, 300 x 20000 10 / 8, 1000 x 20000 equal. Four blocks a row against one:
+  // 64 x 50257 8 and 10 / 12 and 14; eight: 4 x 50257 with 20 alternatives 10 / 12.
   const bool many = a.rows >= 4 * sm_count();
   if (a.vocab <= 1024 || (many && a.vocab <= 4096)) return launch_fwd<kType, 32, kTop>(a, 0, st);
   if (many) return launch_fwd<kType, 128, kTop>(a, 0, st);
@@ -616,10 +621,11 @@ static int choose_fwd(const CcfLogprobs& a, cudaStream_t st) {
 template <int kType>
 static int choose_bwd(const CcfLogprobs& a, cudaStream_t st) {
   const unsigned rows = static_cast<unsigned>(a.rows);
-  if (a.width <= 1024) {
+  // us, a warp a row against 256 threads: 8192 x 1000 10 / 29, 2000 x 2000 7.6 / 10.3, 300 x 1000 5.4 / 4.4, 16 x 4000 8 / 4
+  if (a.width <= 1024 || (a.width <= 2048 && a.rows >= 4 * sm_count())) {
     logprobs_bwd_kernel<kType, 32><<<(rows + 7) / 8, 256, 0, st>>>(a);
   } else {
-    int split = 1;
+    int split = 1;   // of a row's columns. 64 x 50257 6 us, unsplit 12; with half or twice the blocks 1025 x 30522 takes 28.7 instead of 26.7
     const int pieces = a.width / kElemsPer16<kType>;
     while (split < 64 && a.rows * split < 8 * sm_count() && pieces / split > 256 * kUnroll) split *= 2;
     logprobs_bwd_kernel<kType, 256><<<dim3(rows, split), 256, 0, st>>>(a);
