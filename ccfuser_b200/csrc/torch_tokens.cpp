@@ -151,7 +151,7 @@ at::Tensor embedding(const at::Tensor& ids, const at::Tensor& weight, const OptT
   const c10::cuda::CUDAGuard guard(weight.device());
   at::Tensor index[3], y;
   {
-    const at::AutoDispatchBelowADInplaceOrView below;
+    const at::NoGradGuard no_graph;   // views still share their base's version: a change before the backward pass is noticed
     y = run_embedding(ids, weight, position, or_none(position_ids), type, or_none(type_ids), scale, status, index);
   }
   if (builds_graph(weight, position, type)) {
@@ -283,7 +283,7 @@ variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& targets
   const bool training = builds_graph(logits);
   Scored r;
   {
-    const at::AutoDispatchBelowADInplaceOrView below;
+    const at::NoGradGuard no_graph;   // views still share their base's version: a change before the backward pass is noticed
     r = run_logprobs(logits, targets, top_k, temperature, vocab, ignore, status, training);
   }
   if (training) {
@@ -333,7 +333,7 @@ at::Tensor dropout(const at::Tensor& x, const OptTensor& residual_, const at::Te
   const bool training = builds_graph(x, residual);
   at::Tensor y, used;
   {
-    const at::AutoDispatchBelowADInplaceOrView below;
+    const at::NoGradGuard no_graph;   // views still share their base's version: a change before the backward pass is noticed
     if (training) used = at::empty({2}, state.options());   // the seed and step of this pass: the state may move on before the backward pass
     y = run_dropout(packed(x), residual.defined() ? packed(residual) : at::Tensor(), reinterpret_cast<const long long*>(state.data_ptr<int64_t>()),
                     training ? reinterpret_cast<long long*>(used.data_ptr<int64_t>()) : nullptr, call, drop);

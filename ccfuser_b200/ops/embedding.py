@@ -24,7 +24,8 @@ from torch.autograd.function import once_differentiable
 from .. import native as N
 from . import gemm as G
 
-MAX_TOKENS = 2 ** 31 - 1
+MAX_TOKENS = 2 ** 26
+MAX_ROWS = 2 ** 31 - 1
 _INDEX = (torch.int64, torch.int32)
 
 
@@ -147,7 +148,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *, po
     if not weight.is_cuda:
         return _embedding_torch(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx)
     if ids.numel() > MAX_TOKENS:
-        raise ValueError(f"{ids.numel()} tokens: at most 2^31 - 1 in one call")
+        raise ValueError(f"{ids.numel()} tokens: at most 2^26 in one call")
     module = N.torch_module()
     if module is None or torch.jit.is_tracing():
         return _EmbeddingFn.apply(ids, weight, position_weight, position_ids, type_weight, type_ids, float(scale), skip)
@@ -184,8 +185,8 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
         if skip >= 0:
             out[skip] = 0.0
         return out.mul_(scale).to(grad.dtype)
-    if ids.numel() > MAX_TOKENS or num_rows > MAX_TOKENS:
-        raise ValueError("at most 2^31 - 1 tokens and rows in one call")
+    if ids.numel() > MAX_TOKENS or num_rows > MAX_ROWS:
+        raise ValueError("at most 2^26 tokens and 2^31 - 1 rows in one call")
     module = N.torch_module()
     with torch.no_grad():
         if module is not None and not torch.jit.is_tracing():

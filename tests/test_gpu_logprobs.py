@@ -220,6 +220,11 @@ def test_an_input_changed_in_between_is_noticed():
     x.add_(1)
     with pytest.raises(RuntimeError, match="modified"):
         out.logprobs.sum().backward()
+    x = (w * 2)[None]                       # seen as rows by a view
+    out = token_logprobs(x, torch.arange(3, device="cuda")[None])
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified"):
+        out.logprobs.sum().backward()
 
 
 def test_other_streams_and_a_captured_step():

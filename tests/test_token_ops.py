@@ -24,7 +24,7 @@ def _embed(**kw):
     return e
 
 
-@pytest.mark.parametrize("bad", [dict(tables=0), dict(tables=4), dict(type=3), dict(type=-1), dict(d=0), dict(tokens=0), dict(tokens=2 ** 31),
+@pytest.mark.parametrize("bad", [dict(tables=0), dict(tables=4), dict(type=3), dict(type=-1), dict(d=0), dict(tokens=0), dict(tokens=2 ** 26 + 4), dict(tokens=2 ** 31),
                                  dict(seq=0), dict(seq=3), dict(rows=0), dict(rows=2 ** 31), dict(ids=None, rows=3)])
 def test_embedding_entry_points_refuse(bad):
     lib = N.load()

@@ -117,11 +117,11 @@ class Scores:
 
 
 # ---- dropout -----------------------------------------------------------------------------------------------------------
-def philox_bits(seed, step, call, n):
-    """16 bits an element from Philox4x32-10, in Python's whole numbers."""
+def philox_bits(seed, step, call, n, first=0):
+    """16 bits an element from Philox4x32-10, in Python's whole numbers, of n elements from group `first` of eight on."""
     low = 0xFFFFFFFF
     out = []
-    for group in range((n + 7) // 8):
+    for group in range(first, first + (n + 7) // 8):
         c = [group & low, group >> 32, call & low, step & low]
         k0, k1 = seed & low, (seed >> 32) & low
         for _ in range(10):
