@@ -1,5 +1,6 @@
-// The autograd functions around embedding.cu, logprobs.cu and dropout.cu. ops/embedding.py, ops/logprobs.py and ops/dropout.py check the
-// arguments, and hold the same functions in Python for where this module is missing or a graph is being traced.
+// The autograd functions around embedding.cu, logprobs.cu and dropout.cu, with the checks of their arguments (in Python they took 2 of a small call's 9 us).
+// ops/embedding.py, ops/logprobs.py and ops/dropout.py hold both in Python as well, for where this module is missing, a graph is being traced or
+// the tensors are not on a GPU.
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -9,6 +10,8 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
+#include <cmath>
 #include <optional>
 
 #include "dropout.h"
@@ -145,9 +148,51 @@ struct EmbeddingNode : TokenNode {
   }
 };
 
-at::Tensor embedding(const at::Tensor& ids, const at::Tensor& weight, const OptTensor& position_, const OptTensor& position_ids, const OptTensor& type_,
-                     const OptTensor& type_ids, double scale, int64_t skip, const at::Tensor& status) {
+void check_index(const char* name, const at::Tensor& ids, const at::Tensor& of) {
+  TORCH_CHECK_TYPE(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, name, " are int64 or int32, not ", ids.scalar_type());
+  TORCH_CHECK_VALUE(ids.device() == of.device(), name, " are on ", ids.device(), ", the tensor beside them on ", of.device());
+}
+void check_table(const char* name, const at::Tensor& t, const at::Tensor& w) {
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) > 0 && t.size(1) == w.size(1) && t.scalar_type() == w.scalar_type() && t.device() == w.device(), name, ": [rows, ",
+                    w.size(1), "] of ", w.scalar_type(), " on ", w.device(), ", got ", t.sizes(), " of ", t.scalar_type(), " on ", t.device());
+}
+void check_type(const at::Tensor& t) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat,
+                   "on a GPU bf16, fp16 or fp32, not ", t.scalar_type());
+}
+int64_t skipped(const std::optional<int64_t>& padding, int64_t rows) {
+  if (!padding.has_value()) return -1;
+  TORCH_CHECK_VALUE(-rows <= *padding && *padding < rows, "padding_idx ", *padding, " lies outside the table's ", rows, " rows");
+  return *padding < 0 ? *padding + rows : *padding;
+}
+void check_count(int64_t tokens) { TORCH_CHECK_VALUE(tokens <= CCF_EMBED_MAX_TOKENS, tokens, " tokens: at most 2^26 in one call"); }
+// as many as the ids
+OptTensor spread(const OptTensor& t, const at::Tensor& ids) {
+  return !t.has_value() || t->sizes() == ids.sizes() ? t : OptTensor(t->expand(ids.sizes()));
+}
+
+at::Tensor embedding(const at::Tensor& ids, const at::Tensor& weight, const OptTensor& position_, const OptTensor& position_ids_, const OptTensor& type_,
+                     const OptTensor& type_ids_, double scale, const std::optional<int64_t>& padding, const at::Tensor& status) {
   const at::Tensor &position = or_none(position_), &type = or_none(type_);
+  TORCH_CHECK_VALUE(weight.dim() == 2, "weight: [rows, d], got ", weight.sizes());
+  check_type(weight);
+  check_index("ids", ids, weight);
+  check_count(ids.numel());
+  const int64_t skip = skipped(padding, weight.size(0));
+  if (position.defined()) {
+    check_table("position_weight", position, weight);
+    if (position_ids_.has_value()) check_index("position_ids", *position_ids_, weight);
+    const int64_t seq = ids.dim() > 0 ? ids.size(-1) : 1;
+    TORCH_CHECK_VALUE(position_ids_.has_value() || seq <= position.size(0), seq, " positions, and ", position.size(0), " rows in position_weight");
+  } else {
+    TORCH_CHECK_VALUE(!position_ids_.has_value(), "position_ids without position_weight");
+  }
+  TORCH_CHECK_VALUE(type.defined() == type_ids_.has_value(), "type_weight and type_ids go together");
+  if (type.defined()) {
+    check_table("type_weight", type, weight);
+    check_index("type_ids", *type_ids_, weight);
+  }
+  const OptTensor position_ids = spread(position_ids_, ids), type_ids = spread(type_ids_, ids);
   const c10::cuda::CUDAGuard guard(weight.device());
   at::Tensor index[3], y;
   {
@@ -168,7 +213,14 @@ at::Tensor embedding(const at::Tensor& ids, const at::Tensor& weight, const OptT
   return y;
 }
 
-at::Tensor embedding_grad(const at::Tensor& grad, const at::Tensor& ids, int64_t rows, double scale, int64_t skip, const at::Tensor& status) {
+at::Tensor embedding_grad(const at::Tensor& grad, const at::Tensor& ids, int64_t rows, double scale, const std::optional<int64_t>& padding,
+                          const at::Tensor& status) {
+  check_index("ids", ids, grad);
+  check_type(grad);
+  check_count(ids.numel());
+  TORCH_CHECK_VALUE(rows >= 1 && rows <= 0x7fffffff && grad.dim() == ids.dim() + 1 && grad.sizes().slice(0, ids.dim()) == ids.sizes(), "grad: ", ids.sizes(),
+                    " + [d] and 1 to 2^31 - 1 rows, got ", grad.sizes(), " and ", rows, " rows");
+  const int64_t skip = skipped(padding, rows);
   const c10::cuda::CUDAGuard guard(grad.device());
   const at::Tensor dy = packed(grad), index = ids.contiguous();
   CcfEmbed e{};
@@ -277,8 +329,18 @@ struct LogprobsNode : TokenNode {
   }
 };
 
-variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& targets, int64_t top_k, double temperature, int64_t vocab, int64_t ignore,
-                             const at::Tensor& status) {
+variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& targets, int64_t top_k, double temperature,
+                             const std::optional<int64_t>& vocab_size, int64_t ignore, const at::Tensor& status) {
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && targets.sizes() == logits.sizes().slice(0, logits.dim() - 1), "targets: one per row of the logits, ",
+                    logits.sizes(), ", got ", targets.sizes());
+  check_type(logits);
+  check_index("targets", targets, logits);
+  const int64_t width = logits.size(-1), vocab = vocab_size.value_or(width);
+  TORCH_CHECK_VALUE(1 <= vocab && vocab <= width, "vocab_size: 1 to the ", width, " columns of the logits, got ", vocab);
+  const int64_t most = std::min<int64_t>(CCF_LOGPROBS_MAX_TOP, vocab);
+  TORCH_CHECK_VALUE(0 <= top_k && top_k <= most, "top_k: 0 to ", most, ", got ", top_k);
+  TORCH_CHECK_VALUE(1e-37 <= temperature && temperature <= 1e37, "temperature: a positive number that fp32 holds, got ", temperature);
+  TORCH_CHECK_VALUE(width <= (1 << 30) && targets.numel() < (1 << 28), "at most 2^30 columns and 2^28 - 1 rows in one call");
   const c10::cuda::CUDAGuard guard(logits.device());
   const bool training = builds_graph(logits);
   Scored r;
@@ -327,8 +389,16 @@ struct DropoutNode : TokenNode {
   }
 };
 
-at::Tensor dropout(const at::Tensor& x, const OptTensor& residual_, const at::Tensor& state, int64_t call, int64_t drop) {
+at::Tensor dropout(const at::Tensor& x, const OptTensor& residual_, const at::Tensor& state, int64_t call, double p) {
   const at::Tensor& residual = or_none(residual_);
+  TORCH_CHECK_VALUE(0.0 <= p && p <= 1.0, "p: 0 to 1, got ", p);
+  TORCH_CHECK_VALUE(0 <= call && call <= 0xffffffffll, "call: 0 to 2^32 - 1, got ", call);
+  TORCH_CHECK_VALUE(state.scalar_type() == at::kLong && state.dim() == 1 && state.size(0) == 2 && state.device() == x.device() && state.is_contiguous(),
+                    "state: two int64 next to each other on ", x.device(), ", got ", state.sizes(), " of ", state.scalar_type(), " on ", state.device());
+  check_type(x);
+  TORCH_CHECK_VALUE(!residual.defined() || (residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type() && residual.device() == x.device()),
+                    "residual: ", x.sizes(), " of ", x.scalar_type(), " on ", x.device(), ", got ", residual.defined() ? residual.sizes() : x.sizes());
+  const int64_t drop = std::llrint(p * 65536.0);   // to even, as Python's round
   const c10::cuda::CUDAGuard guard(x.device());
   const bool training = builds_graph(x, residual);
   at::Tensor y, used;

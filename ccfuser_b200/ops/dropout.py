@@ -71,6 +71,10 @@ def dropout(x: torch.Tensor, p: float, state: torch.Tensor, call: int = 0, resid
 
     ``state``: int64 tensor [seed, step] on the device of ``x``. Calls of one step need different numbers ``call`` (0 to 2^32 - 1) for different
     masks; the low 32 bits of the step count. ``residual`` has the shape and type of ``x``. A dropped element is 0 whatever it was."""
+    if x.is_cuda and x.dtype in N.DTYPE_CODE and x.numel():
+        module = N.torch_module()
+        if module is not None and not torch.jit.is_tracing():      # checks its arguments as below
+            return module.dropout(x, residual, state, call, p)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"p: 0 to 1, got {p}")
     if not 0 <= call <= _LOW:
@@ -87,10 +91,7 @@ def dropout(x: torch.Tensor, p: float, state: torch.Tensor, call: int = 0, resid
         wide = x if x.dtype == torch.float64 else x.float()
         y = torch.where(keep_mask(x.shape, p, state, call), wide * (65536 / max(1, 65536 - drop)), torch.zeros_like(wide))
         return (y if residual is None else y + residual.to(y.dtype)).to(x.dtype)
-    module = N.torch_module()
-    if module is None or torch.jit.is_tracing():
-        return _DropoutFn.apply(x, residual, state, call, drop)
-    return module.dropout(x, residual, state, call, drop)
+    return _DropoutFn.apply(x, residual, state, call, drop)
 
 
 class DropoutState:

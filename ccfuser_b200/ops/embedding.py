@@ -118,6 +118,11 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *, po
 
     ``position_ids`` (broadcast to the shape of ``ids``) default to the index along the last dimension of ``ids``. The tables are ``[rows, d]`` of one
     type. ``padding_idx``: that row of ``weight`` gets no gradient (it is looked up like any other). The result cannot be differentiated twice."""
+    if weight.is_cuda and weight.numel() and ids.numel():
+        module = N.torch_module()
+        if module is not None and not torch.jit.is_tracing():      # checks its arguments as below
+            return module.embedding(ids, weight, position_weight, position_ids, type_weight, type_ids, scale, padding_idx,
+                                    G.Workspace.of(weight).status)
     if weight.dim() != 2:
         raise ValueError(f"weight: [rows, d], got {tuple(weight.shape)}")
     _check_ids("ids", ids, weight.device)
@@ -139,20 +144,15 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *, po
         _check_ids("type_ids", type_ids, weight.device)
         if type_ids.shape != ids.shape:
             type_ids = type_ids.expand(ids.shape)
-    if ids.numel() == 0 or weight.shape[1] == 0:
-        return weight.new_zeros(*ids.shape, weight.shape[1])
-    if any(t is not None and t.shape[0] == 0 for t in (weight, position_weight, type_weight)):
+    if ids.numel() and any(t is not None and t.shape[0] == 0 for t in (weight, position_weight, type_weight)):
         raise ValueError("a table without rows")
     if weight.is_cuda and weight.dtype not in N.DTYPE_CODE:
         raise TypeError(f"tables on a GPU are bf16, fp16 or fp32, not {weight.dtype}")
-    if not weight.is_cuda:
+    if not weight.is_cuda or ids.numel() == 0 or weight.shape[1] == 0:
         return _embedding_torch(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx)
     if ids.numel() > MAX_TOKENS:
         raise ValueError(f"{ids.numel()} tokens: at most 2^26 in one call")
-    module = N.torch_module()
-    if module is None or torch.jit.is_tracing():
-        return _EmbeddingFn.apply(ids, weight, position_weight, position_ids, type_weight, type_ids, float(scale), skip)
-    return module.embedding(ids, weight, position_weight, position_ids, type_weight, type_ids, scale, skip, G.Workspace.of(weight).status)
+    return _EmbeddingFn.apply(ids, weight, position_weight, position_ids, type_weight, type_ids, float(scale), skip)
 
 
 def _embedding_torch(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx):
@@ -172,6 +172,10 @@ def _embedding_torch(ids, weight, scale, position_weight, position_ids, type_wei
 def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """The dense gradient ``[num_rows, d]`` of a table from the gradient ``[*ids.shape, d]`` of its lookups: what ``embedding`` does in its
     backward pass, without a graph."""
+    if grad.is_cuda and grad.numel():
+        module = N.torch_module()
+        if module is not None and not torch.jit.is_tracing():
+            return module.embedding_grad(grad, ids, num_rows, scale, padding_idx, G.Workspace.of(grad).status)
     _check_ids("ids", ids, grad.device)
     if num_rows < 1 or grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
         raise ValueError(f"grad: {list(ids.shape)} + [d] and at least one row, got {list(grad.shape)} and {num_rows} rows")
@@ -187,10 +191,7 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
         return out.mul_(scale).to(grad.dtype)
     if ids.numel() > MAX_TOKENS or num_rows > MAX_ROWS:
         raise ValueError("at most 2^26 tokens and 2^31 - 1 rows in one call")
-    module = N.torch_module()
     with torch.no_grad():
-        if module is not None and not torch.jit.is_tracing():
-            return module.embedding_grad(grad, ids, num_rows, scale, skip, G.Workspace.of(grad).status)
         dy, index = G.packed(grad), ids.contiguous()
         e = N.Embed(tokens=index.numel(), seq=1, d=dy.shape[-1], type=N.DTYPE_CODE[dy.dtype])
         _fill(e, index, num_rows, float(scale), skip)

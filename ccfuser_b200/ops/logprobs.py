@@ -97,6 +97,11 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     no gradient from their log probability. Alternatives come by value, equal ones by index; ``top_k`` is at most 32 and the vocabulary. A column at -inf has
     no probability: where fewer than ``top_k`` others are left, the id is -1 and the log probability -inf. A row without a finite logit gives -inf, entropy 0
     and a zero gradient; a row with NaN or +inf gives NaN. Log probabilities, entropy and the alternatives' log probabilities are differentiable, once."""
+    if logits.is_cuda and logits.dtype in N.DTYPE_CODE and targets.numel():
+        module = N.torch_module()
+        if module is not None and not torch.jit.is_tracing():      # checks its arguments as below
+            out = module.token_logprobs(logits, targets, top_k, temperature, vocab_size, ignore_index, G.Workspace.of(logits).status)
+            return TokenLogprobs(*out) if top_k else TokenLogprobs(out[0], out[1], None, None)
     if logits.dim() < 1 or targets.shape != logits.shape[:-1]:
         raise ValueError(f"targets: one per row of the logits, {tuple(logits.shape[:-1])}, got {tuple(targets.shape)}")
     if targets.dtype not in (torch.int64, torch.int32):
@@ -115,11 +120,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
         return _logprobs_torch(logits, targets, top_k, temperature, vocab, ignore_index)
     if width > MAX_WIDTH or targets.numel() > MAX_ROWS:
         raise ValueError("at most 2^30 columns and 2^28 - 1 rows in one call")
-    module = N.torch_module()
-    if module is None or torch.jit.is_tracing():
-        out = _LogprobsFn.apply(logits, targets, top_k, float(temperature), vocab, ignore_index)
-    else:
-        out = module.token_logprobs(logits, targets, top_k, temperature, vocab, ignore_index, G.Workspace.of(logits).status)
+    out = _LogprobsFn.apply(logits, targets, top_k, float(temperature), vocab, ignore_index)
     return TokenLogprobs(out[0], out[1], *(out[2:] if top_k else (None, None)))
 
 

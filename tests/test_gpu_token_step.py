@@ -195,3 +195,64 @@ def test_a_traced_graph_replays_the_kernels():
         for args in (one, two):
             for a, b in zip(traced(*args), chain(*args)):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("function", ["C++", "Python"])
+def test_refusals_on_the_gpu(monkeypatch, function):
+    """The checks beside the kernels, in both forms of the functions."""
+    from ccfuser_b200 import native as N
+    from ccfuser_b200.ops.dropout import dropout
+    from ccfuser_b200.ops.embedding import embedding, embedding_grad
+    from ccfuser_b200.ops.logprobs import token_logprobs
+    if function == "Python":
+        monkeypatch.setattr(N, "torch_module", lambda: None)
+    w, ids = torch.randn(10, 8, device="cuda"), torch.tensor([[1, 2, 3]], device="cuda")
+    for kw in (dict(position_ids=ids), dict(type_weight=w), dict(type_ids=ids), dict(padding_idx=10), dict(padding_idx=-11), dict(position_weight=w[:2]),
+               dict(position_weight=w[:, :4]), dict(position_weight=w.half()), dict(position_weight=w.cpu()), dict(position_weight=w[:0], position_ids=ids)):
+        with pytest.raises(ValueError):
+            embedding(ids, w, **kw)
+    for bad, error in ((ids.float(), TypeError), (ids.bool(), TypeError), (ids.cpu(), ValueError)):
+        with pytest.raises(error):
+            embedding(bad, w)
+        with pytest.raises(error):
+            embedding_grad(torch.randn(1, 3, 8, device="cuda"), bad, 10)
+    with pytest.raises(TypeError):
+        embedding(ids, w.double())
+    with pytest.raises(ValueError):
+        embedding(ids, w[0])
+    with pytest.raises(ValueError):
+        embedding(ids, w[:0])
+    with pytest.raises(RuntimeError):
+        embedding(ids, w, position_weight=w, position_ids=torch.zeros(2, 2, dtype=torch.long, device="cuda"))
+    for grad, rows in ((torch.randn(2, 8, device="cuda"), 10), (torch.randn(1, 3, 8, device="cuda"), 0)):
+        with pytest.raises(ValueError):
+            embedding_grad(grad, ids, rows)
+    x, t = torch.randn(3, 10, device="cuda"), torch.tensor([1, 2, 3], device="cuda")
+    for kw in (dict(top_k=-1), dict(top_k=11), dict(top_k=33), dict(vocab_size=0), dict(vocab_size=11), dict(vocab_size=4, top_k=5),
+               dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("inf")), dict(temperature=float("nan"))):
+        with pytest.raises(ValueError):
+            token_logprobs(x, t, **kw)
+    for bad, error in ((t[:2], ValueError), (t[:, None], ValueError), (t.cpu(), ValueError), (t.float(), TypeError)):
+        with pytest.raises(error):
+            token_logprobs(x, bad)
+    s = torch.tensor([1, 2], device="cuda")
+    for kw in (dict(p=-0.1), dict(p=1.1), dict(p=float("nan")), dict(call=-1), dict(call=2 ** 32), dict(state=s.int()), dict(state=s[:1]),
+               dict(state=torch.zeros(4, dtype=torch.int64, device="cuda")[::2]), dict(state=s.cpu()), dict(residual=x[:2]), dict(residual=x.half())):
+        with pytest.raises(ValueError):
+            dropout(**{"x": x, "p": 0.5, "state": s, **kw})
+    # nothing to do
+    assert embedding(ids[:0], w).shape == (0, 3, 8) and embedding(ids, w[:, :0]).shape == (1, 3, 0)
+    assert token_logprobs(x[:0], t[:0]).logprobs.shape == (0,) and dropout(x[:0], 0.5, s).shape == (0, 10)
+
+
+def test_ids_of_other_shapes():
+    """A single id, positions and types given for all sequences at once."""
+    from ccfuser_b200.ops.embedding import embedding
+    w, p = torch.randn(10, 8, device="cuda"), torch.randn(6, 8, device="cuda")
+    one = embedding(torch.tensor(3, device="cuda"), w, 2.0, position_weight=p)
+    assert torch.equal(one, w[3] * 2 + p[0])
+    ids = torch.arange(6, device="cuda").int().view(2, 3)
+    for shape in ((3,), (1, 3), (2, 1), (2, 3), ()):
+        at = torch.full(shape, 4, device="cuda", dtype=torch.int32) if shape != (3,) else torch.tensor([5, 0, 2], device="cuda")
+        y = embedding(ids, w, position_weight=p, position_ids=at, type_weight=p, type_ids=at.long())
+        assert torch.equal(y, w[ids.long()] + p[at.long()].expand(2, 3, 8) + p[at.long()].expand(2, 3, 8))
