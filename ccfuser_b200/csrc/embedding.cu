@@ -22,21 +22,22 @@ constexpr uint32_t kNoRow = 0xffffffffu;   // id of a token without a gradient: 
 // a product that may pass 32 bits, in one instruction
 __device__ __forceinline__ uint64_t wide(uint32_t a, uint32_t b) { return static_cast<uint64_t>(a) * b; }
 
-// What the 32 lanes of a warp hold of a row: 32 * kE consecutive elements from a column on. kVec: 16 bytes per lane; otherwise (rows off
+// What a warp, or kLanes of its lanes, hold of a row: kLanes * kE consecutive elements from a column on. kVec: 16 bytes per lane; otherwise (rows off
 // 16-byte boundaries) one element per lane and access.
-template <int kType, bool kVec>
+template <int kType, bool kVec, int kLanes = 32>
 struct Slice {
   static constexpr int kE = kElemsPer16<kType>;
-  static constexpr int kCols = 32 * kE;
+  static constexpr int kCols = kLanes * kE;
   uint4 q;
   float s[kVec ? 1 : kE];
 
-  static __device__ __forceinline__ int col(int i) { return kVec ? lane_id() * kE + i : lane_id() + 32 * i; }
+  static __device__ __forceinline__ int lane() { return lane_id() & (kLanes - 1); }
+  static __device__ __forceinline__ int col(int i) { return kVec ? lane() * kE + i : lane() + kLanes * i; }
   __device__ __forceinline__ void load(const void* p, size_t at, int left, bool on) {
     if constexpr (kVec) {
       q = make_uint4(0, 0, 0, 0);
-      if (on && lane_id() * kE < left)
-        q = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p) + at * kElemBytes<kType>) + lane_id());
+      if (on && lane() * kE < left)
+        q = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p) + at * kElemBytes<kType>) + lane());
     } else {
 #pragma unroll
       for (int i = 0; i < kE; ++i) s[i] = on && col(i) < left ? load_elem<kType>(p, static_cast<long long>(at) + col(i)) : 0.f;
@@ -63,8 +64,8 @@ struct Slice {
   }
   static __device__ __forceinline__ void store(void* p, size_t at, int left, const float (&f)[kE]) {
     if constexpr (kVec) {
-      if (lane_id() * kE < left)
-        reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p) + at * kElemBytes<kType>)[lane_id()] = pack16<kType>(f);
+      if (lane() * kE < left)
+        reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p) + at * kElemBytes<kType>)[lane()] = pack16<kType>(f);
     } else {
 #pragma unroll
       for (int i = 0; i < kE; ++i)
@@ -73,7 +74,7 @@ struct Slice {
   }
   static __device__ __forceinline__ void store_f32(float* p, int left, const float (&f)[kE]) {
     if constexpr (kVec) {
-      if (lane_id() * kE >= left) return;
+      if (lane() * kE >= left) return;
 #pragma unroll
       for (int i = 0; i < kE; i += 4) reinterpret_cast<float4*>(p + col(i))[0] = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
     } else {
@@ -86,7 +87,7 @@ struct Slice {
     if constexpr (kVec) {
 #pragma unroll
       for (int i = 0; i < kE; i += 4) {
-        const float4 v = lane_id() * kE < left ? reinterpret_cast<const float4*>(p + col(i))[0] : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 v = lane() * kE < left ? reinterpret_cast<const float4*>(p + col(i))[0] : make_float4(0.f, 0.f, 0.f, 0.f);
         f[i] = v.x;
         f[i + 1] = v.y;
         f[i + 2] = v.z;
@@ -99,7 +100,7 @@ struct Slice {
   }
   static __device__ __forceinline__ void store_zero(void* p, size_t at, int left) {   // past the L2 where it may: nobody reads it soon
     if constexpr (kVec) {
-      if (lane_id() * kE < left) __stcs(reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p) + at * kElemBytes<kType>) + lane_id(), make_uint4(0, 0, 0, 0));
+      if (lane() * kE < left) __stcs(reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p) + at * kElemBytes<kType>) + lane(), make_uint4(0, 0, 0, 0));
     } else {
 #pragma unroll
       for (int i = 0; i < kE; ++i)
@@ -234,34 +235,22 @@ __device__ __forceinline__ uint32_t smaller_elsewhere(const GradArgs& g, const u
   return n;
 }
 
-// Each block sorts one chunk of keys, one for each thread: bitonic, with exchanges inside a warp by shuffles and the others through shared memory.
-// Up to kSide chunks are one cluster, whose blocks then read each other's ids and put every key in its place among all: 8192 tokens in one launch.
-// Every token also leaves its place in `slot` at its id, whichever of equal ids comes last: a row is used if the token named there has its id. So
-// `slot` needs no zeros beforehand, and what it says is the same whoever won. 8192 tokens 10.7 us, 1024 5; a chunk of 2048 64-bit keys sorted in shared
-// memory alone took 17, and the merge as a launch of its own 9 more.
-// Key: (id, place in the chunk) in 32 bits for tables of less than kShortRows rows, in 64 for larger ones.
+// Key of the sort: (id, place in the chunk) in 32 bits for tables of less than kShortRows rows, in 64 for larger ones.
 constexpr uint32_t kShortRows = (1u << 22) - 1;
 template <typename Key>
-__global__ void __launch_bounds__(kSortChunk) embedding_sort_kernel(const __grid_constant__ GradArgs g) {
-  namespace cg = cooperative_groups;
-  constexpr int kPlaceBits = sizeof(Key) == 4 ? 10 : 32;
-  constexpr uint32_t kLast = sizeof(Key) == 4 ? kShortRows : kNoRow;   // the id of a token without a row
-  __shared__ Key other[2][kSortChunk];
-  __shared__ uint32_t ids[kSide * kSortChunk];
-  const GradTable& t = g.table[blockIdx.y];
-  let_next_in();
-  if (blockIdx.x == 0 && threadIdx.x < 2) t.count[threadIdx.x] = 0;
-  if (t.ids == nullptr) return;
-  const uint32_t tid = threadIdx.x, own = blockIdx.x, base = own * kSortChunk;
-  const uint32_t n = own < g.chunks ? min(g.tokens - base, static_cast<uint32_t>(kSortChunk)) : 0;
-  Key key = ~static_cast<Key>(0);
-  if (tid < n) {
-    const long long id = load_index(t.ids, base + tid, t.wide);
-    const bool in = id >= 0 && id < t.rows;
-    if (!in) report_status(g.status, CCF_ERR_INDEX, static_cast<int>(base + tid) & 0x7fffff);
-    else t.slot[id] = base + tid;
-    key = static_cast<Key>(in && id != t.skip ? static_cast<uint32_t>(id) : kLast) << kPlaceBits | tid;
-  }
+constexpr int kPlaceBits = sizeof(Key) == 4 ? 10 : 32;
+template <typename Key>
+constexpr uint32_t kLast = sizeof(Key) == 4 ? kShortRows : kNoRow;   // the id of a token without a row
+template <typename Key>
+__device__ __forceinline__ uint32_t key_id(Key key) {
+  const uint32_t id = static_cast<uint32_t>(key >> kPlaceBits<Key>);
+  return id == kLast<Key> ? kNoRow : id;
+}
+
+// n keys of a block of kSortChunk threads, one each, in order: bitonic, with exchanges inside a warp by shuffles and the others through shared memory.
+template <typename Key>
+__device__ __forceinline__ Key sort_keys(Key key, Key (&other)[2][kSortChunk], uint32_t n) {
+  const uint32_t tid = threadIdx.x;
   int half = 0;
 #pragma unroll 1
   for (uint32_t size = 2; size < 2 * n; size *= 2) {
@@ -280,13 +269,36 @@ __global__ void __launch_bounds__(kSortChunk) embedding_sort_kernel(const __grid
       key = (((tid & j) == 0) == up) == (o < key) ? o : key;
     }
   }
-  uint32_t id = static_cast<uint32_t>(key >> kPlaceBits);
-  if (tid >= n || id == kLast) id = kNoRow;
-  const uint64_t full = static_cast<uint64_t>(id) << 32 | (base + (static_cast<uint32_t>(key) & (kSortChunk - 1)));
-  if (g.chunks == 1) {
-    if (tid < n) t.keys[tid] = full;
-    return;
+  return key;
+}
+
+// Each block sorts one chunk of keys, one for each thread.
+// Up to kSide chunks are one cluster, whose blocks then read each other's ids and put every key in its place among all: 8192 tokens in one launch.
+// Every token also leaves its place in `slot` at its id, whichever of equal ids comes last: a row is used if the token named there has its id. So
+// `slot` needs no zeros beforehand, and what it says is the same whoever won. 8192 tokens 10.7 us; a chunk of 2048 64-bit keys sorted in shared
+// memory alone took 17, and the merge as a launch of its own 9 more.
+template <typename Key>
+__global__ void __launch_bounds__(kSortChunk) embedding_sort_kernel(const __grid_constant__ GradArgs g) {
+  namespace cg = cooperative_groups;
+  __shared__ Key other[2][kSortChunk];
+  __shared__ uint32_t ids[kSide * kSortChunk];
+  const GradTable& t = g.table[blockIdx.y];
+  let_next_in();
+  if (blockIdx.x == 0 && threadIdx.x < 2) t.count[threadIdx.x] = 0;
+  if (t.ids == nullptr) return;
+  const uint32_t tid = threadIdx.x, own = blockIdx.x, base = own * kSortChunk;
+  const uint32_t n = own < g.chunks ? min(g.tokens - base, static_cast<uint32_t>(kSortChunk)) : 0;
+  Key key = ~static_cast<Key>(0);
+  if (tid < n) {
+    const long long id = load_index(t.ids, base + tid, t.wide);
+    const bool in = id >= 0 && id < t.rows;
+    if (!in) report_status(g.status, CCF_ERR_INDEX, static_cast<int>(base + tid) & 0x7fffff);
+    else t.slot[id] = base + tid;
+    key = static_cast<Key>(in && id != t.skip ? static_cast<uint32_t>(id) : kLast<Key>) << kPlaceBits<Key> | tid;
   }
+  key = sort_keys(key, other, n);
+  const uint32_t id = tid < n ? key_id(key) : kNoRow;
+  const uint64_t full = static_cast<uint64_t>(id) << 32 | (base + (static_cast<uint32_t>(key) & (kSortChunk - 1)));
   if (g.chunks > kSide) {   // the merging kernel goes on
     if (tid < n) t.sorted_chunks[base + tid] = full;
     t.chunk_ids[base + tid] = id;
@@ -325,6 +337,121 @@ __global__ void __launch_bounds__(kMergeThreads) embedding_merge_kernel(const __
     __syncthreads();
   }
   if (i < g.tokens) t.keys[place] = key;
+}
+
+// Up to kSortChunk tokens: one launch. A block for each table and narrow slice of the columns sorts the tokens by itself (every block the same ones: cheaper than
+// waiting for one that did). kFewLanes lanes sum a piece of as many tokens, and what runs leave at the pieces' ends meets in shared memory. The other blocks look
+// through the ids for those of their kFewRows rows and write zeros into the rest. 1000 tokens of 512, 10000 rows: 12.3 us (with whole warps, so a quarter of
+// the blocks, 20.5), in three launches 17.8 and 6 us more of the host's time; 1024 of 4096 with one word in half of the places 13.7 and 16.4.
+constexpr uint32_t kFewRows = 128, kFewLanes = 8;
+template <int kType, bool kVec, typename Key>
+__global__ void __launch_bounds__(kSortChunk) embedding_few_kernel(const __grid_constant__ GradArgs g) {
+  using S = Slice<kType, kVec, kFewLanes>;
+  using Row = Slice<kType, kVec>;
+  constexpr int kUnroll = kVec ? 4 : 2;
+  extern __shared__ __align__(16) float ends[];   // [pieces][head, tail][kCols]
+  __shared__ Key other[2][kSortChunk];
+  __shared__ uint32_t sid[kSortChunk + 1], token[kSortChunk], tail_run[kSortChunk / kFewLanes];
+  const uint32_t tid = threadIdx.x, piece = tid / kFewLanes, n = g.tokens;
+  auto id_at = [&](const GradTable& t, uint32_t i) { return t.ids != nullptr ? load_index(t.ids, i, t.wide) : static_cast<long long>(i % g.seq); };
+  if (blockIdx.x >= g.sums) {
+    uint32_t w = blockIdx.x - g.sums;
+    int k = 0;
+    while (w >= (g.table[k].rows + kFewRows - 1) / kFewRows) w -= static_cast<uint32_t>((g.table[k++].rows + kFewRows - 1) / kFewRows);
+    const GradTable& t = g.table[k];
+    const long long first = static_cast<long long>(w) * kFewRows;
+    if (tid < kFewRows) sid[tid] = 0;
+    __syncthreads();
+    if (tid < n) {
+      const long long id = id_at(t, tid);
+      if (id >= first && id < first + kFewRows && id != t.skip) sid[id - first] = 1;
+    }
+    __syncthreads();
+    for (uint32_t r = tid >> 5; r < kFewRows && first + r < t.rows; r += kSortChunk / 32) {
+      if (sid[r]) continue;
+      const size_t at = wide(static_cast<uint32_t>(first) + r, g.d);
+      for (int c = 0; c < g.d; c += Row::kCols) Row::store_zero(t.grad, at + c, g.d - c);
+    }
+    return;
+  }
+  const GradTable& t = g.table[blockIdx.x / g.slices];
+  const uint32_t c = blockIdx.x % g.slices * S::kCols;
+  const int left = g.d - static_cast<int>(c);
+  Key key = ~static_cast<Key>(0);
+  if (tid < n) {
+    const long long id = id_at(t, tid);
+    const bool in = id >= 0 && id < t.rows;
+    if (!in && c == 0) report_status(g.status, CCF_ERR_INDEX, static_cast<int>(tid));
+    key = static_cast<Key>(in && id != t.skip ? static_cast<uint32_t>(id) : kLast<Key>) << kPlaceBits<Key> | tid;
+  }
+  key = sort_keys(key, other, n);
+  sid[tid] = tid < n ? key_id(key) : kNoRow;
+  token[tid] = static_cast<uint32_t>(key) & (kSortChunk - 1);
+  if (tid == 0) sid[kSortChunk] = kNoRow;
+  if (S::lane() == 0) tail_run[piece] = kNoRow;
+  __syncthreads();
+  const uint32_t begin = piece * kFewLanes;
+  float* const head = ends + piece * 2 * S::kCols;
+  if (begin < n) {
+    uint32_t run = sid[begin];
+    bool from_before = begin > 0 && run == sid[begin - 1];
+    f32x2 acc[S::kE / 2] = {};
+    auto finish = [&](bool goes_on) {
+      float f[S::kE];
+#pragma unroll
+      for (int i = 0; i < S::kE / 2; ++i) {
+        upk2(acc[i], f[2 * i], f[2 * i + 1]);
+        acc[i] = 0;
+      }
+      if (run != kNoRow) {
+        if (from_before || goes_on) {
+          S::store_f32(from_before ? head : head + S::kCols, S::kCols, f);
+          if (!from_before && S::lane() == 0) tail_run[piece] = run;
+        } else {
+#pragma unroll
+          for (int i = 0; i < S::kE; ++i) f[i] *= t.scale;
+          S::store(t.grad, wide(run, g.d) + c, left, f);
+        }
+      }
+      from_before = false;
+    };
+    const uint32_t m = min(kFewLanes, n - begin);
+    for (uint32_t j0 = 0; j0 < m; j0 += kUnroll) {
+      S part[kUnroll];
+      uint32_t id[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        id[u] = j0 + u < m ? sid[begin + j0 + u] : kNoRow;
+        part[u].load(g.dy, id[u] != kNoRow ? wide(token[begin + j0 + u], g.d) + c : c, left, id[u] != kNoRow);
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (j0 + u >= m) break;
+        if (id[u] != run) {
+          finish(false);
+          run = id[u];
+        }
+        float f[S::kE];
+        part[u].get(f);
+#pragma unroll
+        for (int i = 0; i < S::kE / 2; ++i) acc[i] = add2(acc[i], pk2(f[2 * i], f[2 * i + 1]));
+      }
+    }
+    finish(sid[begin + m] == run);
+  }
+  __syncthreads();
+  const uint32_t run = tail_run[piece];
+  if (run == kNoRow) return;
+  float acc[S::kE], part[S::kE];
+  S::load_f32(head + S::kCols, S::kCols, acc);
+  for (uint32_t q = piece + 1; q * kFewLanes < n && sid[q * kFewLanes] == run; ++q) {
+    S::load_f32(ends + q * 2 * S::kCols, S::kCols, part);
+#pragma unroll
+    for (int i = 0; i < S::kE; ++i) acc[i] += part[i];
+  }
+#pragma unroll
+  for (int i = 0; i < S::kE; ++i) acc[i] *= t.scale;
+  S::store(t.grad, wide(run, g.d) + c, left, acc);
 }
 
 // Sums, then the zeros of the rows that no token has, 32 rows a block. A summing warp takes one piece of the sorted tokens and one slice of the columns.
@@ -577,9 +704,36 @@ static int launch_fwd(const CcfEmbed& e, void* y, int* status, cudaStream_t st) 
 }
 
 template <int kType, bool kVec>
+static int launch_few(GradArgs& g, cudaStream_t st) {
+  using S = Slice<kType, kVec, kFewLanes>;
+  long long zeros = 0, largest = 0;
+  for (int k = 0; k < g.tables; ++k) {
+    zeros += (g.table[k].rows + kFewRows - 1) / kFewRows;
+    largest = g.table[k].rows > largest ? g.table[k].rows : largest;
+  }
+  g.slices = (g.d + S::kCols - 1) / S::kCols;
+  g.sums = g.slices * g.tables;
+  constexpr int kSmem = kSortChunk / kFewLanes * 2 * S::kCols * 4;
+  const bool narrow = largest < kShortRows;
+  const auto kern = narrow ? embedding_few_kernel<kType, kVec, uint32_t> : embedding_few_kernel<kType, kVec, uint64_t>;
+  static bool configured[64][2] = {};   // per device: the attribute belongs to the (function, device) pair
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!configured[dev & 63][narrow]) {
+    const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (err != cudaSuccess) return -static_cast<int>(err);
+    configured[dev & 63][narrow] = true;
+  }
+  kern<<<static_cast<unsigned>(g.sums + zeros), kSortChunk, kSmem, st>>>(g);
+  const int rc = launch_result();
+  return rc == 0 ? 1 : rc;
+}
+
+template <int kType, bool kVec>
 static int launch_bwd(GradArgs& g, cudaStream_t st) {
   using S = Slice<kType, kVec>;
   g.slices = (g.d + S::kCols - 1) / S::kCols;
+  if (g.chunks == 1) return launch_few<kType, kVec>(g, st);
   long long sums = 0, zeros = 0, largest = 0;
   uint32_t most = 0;
   bool sorted = false;
@@ -653,9 +807,10 @@ int ccf_embedding_fwd(const CcfEmbed* e, void* y, int* status, void* stream) {
   }
 }
 
-// Bytes of scratch that a table needs in ccf_embedding_bwd; sorted: it has ids. 0: a size out of range.
+// Bytes of scratch that a table needs in ccf_embedding_bwd; sorted: it has ids. None (0) for up to 1024 tokens. -1: a size out of range.
 long long ccf_embedding_scratch(long long tokens, long long seq, long long rows, int d, int sorted) {
-  if (tokens < 1 || tokens > CCF_EMBED_MAX_TOKENS || seq < 1 || tokens % seq != 0 || rows < 1 || rows > 0x7fffffffll || d < 1) return 0;
+  if (tokens < 1 || tokens > CCF_EMBED_MAX_TOKENS || seq < 1 || tokens % seq != 0 || rows < 1 || rows > 0x7fffffffll || d < 1) return -1;
+  if (tokens <= ccf::kSortChunk) return 0;
   return static_cast<long long>(ccf::lay_out(nullptr, nullptr, tokens, rows, d, sorted != 0, tokens / seq));
 }
 
@@ -682,10 +837,10 @@ int ccf_embedding_bwd(const CcfEmbed* e, const void* dy, int* status, void* stre
       if ((e->table[k].ids != nullptr) == (sorted != 0)) order[n++] = k;
   for (int k = 0; k < e->tables; ++k) {
     const CcfEmbedTable& t = e->table[order[k]];
-    if (t.grad == nullptr || t.scratch == nullptr || !on16(t.scratch)) return -2;
+    if (t.grad == nullptr || (g.chunks > 1 && (t.scratch == nullptr || !on16(t.scratch)))) return -2;
     vec = vec && on16(t.grad);
     GradTable& o = g.table[k];
-    lay_out(&o, t.scratch, e->tokens, t.rows, e->d, t.ids != nullptr, g.batch);
+    if (g.chunks > 1) lay_out(&o, t.scratch, e->tokens, t.rows, e->d, t.ids != nullptr, g.batch);
     o.ids = t.ids;
     o.grad = t.grad;
     o.rows = t.rows;

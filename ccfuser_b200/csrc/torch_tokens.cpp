@@ -87,8 +87,11 @@ void run_grad(CcfEmbed& e, const at::Tensor& dy, const at::Tensor& status) {
     at[k] = bytes;
     bytes += ccf_embedding_scratch(e.tokens, e.seq, e.table[k].rows, e.d, e.table[k].ids != nullptr);   // a multiple of 16
   }
-  const at::Tensor scratch = at::empty({bytes}, dy.options().dtype(at::kByte));
-  for (int k = 0; k < e.tables; ++k) e.table[k].scratch = static_cast<uint8_t*>(scratch.data_ptr()) + at[k];
+  at::Tensor scratch;
+  if (bytes > 0) {
+    scratch = at::empty({bytes}, dy.options().dtype(at::kByte));
+    for (int k = 0; k < e.tables; ++k) e.table[k].scratch = static_cast<uint8_t*>(scratch.data_ptr()) + at[k];
+  }
   const int launches = ccf_embedding_bwd(&e, dy.data_ptr(), status.data_ptr<int>(), current_stream());
   TORCH_CHECK(launches > 0, "ccf_embedding_bwd failed with code ", launches);
   g_launches += launches;

@@ -39,10 +39,11 @@ def test_embedding_entry_points_refuse_missing_memory():
     assert lib.ccf_embedding_fwd(C.byref(_embed(ld=63)), A, A, None) == -2
     assert lib.ccf_embedding_fwd(C.byref(_embed()), None, A, None) == -2
     assert lib.ccf_embedding_bwd(C.byref(_embed(grad=None)), A, A, None) == -2
-    assert lib.ccf_embedding_bwd(C.byref(_embed(scratch=None)), A, A, None) == -2
-    assert lib.ccf_embedding_bwd(C.byref(_embed(scratch=A + 8)), A, A, None) == -2
+    assert lib.ccf_embedding_bwd(C.byref(_embed(tokens=1028, scratch=None)), A, A, None) == -2
+    assert lib.ccf_embedding_bwd(C.byref(_embed(tokens=1028, scratch=A + 8)), A, A, None) == -2
     assert lib.ccf_embedding_bwd(C.byref(_embed()), None, A, None) == -2
-    assert lib.ccf_embedding_scratch(0, 1, 10, 64, 1) == lib.ccf_embedding_scratch(8, 1, 0, 64, 1) == lib.ccf_embedding_scratch(8, 3, 5, 64, 1) == 0
+    assert lib.ccf_embedding_scratch(0, 1, 10, 64, 1) == lib.ccf_embedding_scratch(8, 1, 0, 64, 1) == lib.ccf_embedding_scratch(8, 3, 5, 64, 1) == -1
+    assert lib.ccf_embedding_scratch(1024, 1, 10, 64, 1) == 0
     assert lib.ccf_embedding_scratch(5000, 50, 100, 64, 1) > lib.ccf_embedding_scratch(5000, 50, 100, 64, 0) > 0
 
 
