@@ -669,7 +669,7 @@ static size_t lay_out(GradTable* t, void* base, long long tokens, long long rows
 static bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 static bool valid(const CcfEmbed* e) {
-  if (e == nullptr || e->tables < 1 || e->tables > CCF_EMBED_TABLES || e->type < 0 || e->type > 2 || e->d < 1 || e->tokens < 1 ||
+  if (e == nullptr || e->tables < 1 || e->tables > CCF_EMBED_TABLES || e->type < 0 || e->type > 2 || e->d < 1 || e->d > CCF_EMBED_MAX_D || e->tokens < 1 ||
       e->tokens > CCF_EMBED_MAX_TOKENS || e->seq < 1 || e->tokens % e->seq != 0)
     return false;
   for (int k = 0; k < e->tables; ++k) {
@@ -786,7 +786,7 @@ extern "C" {
 int ccf_sizeof_embed() { return static_cast<int>(sizeof(CcfEmbed)); }
 
 // y [tokens, d] = the sum over the tables of scale * weight[id]. An index out of range is recorded in `status` (code 5, the token) and gives a row
-// of NaN. At most 2^26 tokens and 2^31 - 1 rows; tokens is a multiple of seq.
+// of NaN. At most 2^26 tokens, 2^31 - 1 rows and 2^24 columns; tokens is a multiple of seq.
 int ccf_embedding_fwd(const CcfEmbed* e, void* y, int* status, void* stream) {
   using namespace ccf;
   if (!valid(e) || y == nullptr) return -2;
@@ -809,7 +809,7 @@ int ccf_embedding_fwd(const CcfEmbed* e, void* y, int* status, void* stream) {
 
 // Bytes of scratch that a table needs in ccf_embedding_bwd; sorted: it has ids. None (0) for up to 1024 tokens. -1: a size out of range.
 long long ccf_embedding_scratch(long long tokens, long long seq, long long rows, int d, int sorted) {
-  if (tokens < 1 || tokens > CCF_EMBED_MAX_TOKENS || seq < 1 || tokens % seq != 0 || rows < 1 || rows > 0x7fffffffll || d < 1) return -1;
+  if (tokens < 1 || tokens > CCF_EMBED_MAX_TOKENS || seq < 1 || tokens % seq != 0 || rows < 1 || rows > 0x7fffffffll || d < 1 || d > CCF_EMBED_MAX_D) return -1;
   if (tokens <= ccf::kSortChunk) return 0;
   return static_cast<long long>(ccf::lay_out(nullptr, nullptr, tokens, rows, d, sorted != 0, tokens / seq));
 }

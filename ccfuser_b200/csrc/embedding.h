@@ -2,6 +2,7 @@
 #pragma once
 
 #define CCF_EMBED_TABLES 3
+#define CCF_EMBED_MAX_D (1 << 24)
 #define CCF_EMBED_MAX_TOKENS (1 << 26)   // merging sorted chunks takes time with the square of their number: seconds there
 
 // One table of a sum of lookups. `ids`: an index per token (32 or 64 bits), or null for the token's place in its sequence

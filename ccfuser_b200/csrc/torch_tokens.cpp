@@ -159,6 +159,10 @@ void check_table(const char* name, const at::Tensor& t, const at::Tensor& w) {
   TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) > 0 && t.size(1) == w.size(1) && t.scalar_type() == w.scalar_type() && t.device() == w.device(), name, ": [rows, ",
                     w.size(1), "] of ", w.scalar_type(), " on ", w.device(), ", got ", t.sizes(), " of ", t.scalar_type(), " on ", t.device());
 }
+// what the kernels count in 32 bits
+void check_size(const at::Tensor& w) {
+  TORCH_CHECK_VALUE(w.size(0) <= 0x7fffffff && w.size(1) <= CCF_EMBED_MAX_D, "a table of at most 2^31 - 1 rows and 2^24 columns, got ", w.sizes());
+}
 void check_type(const at::Tensor& t) {
   TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat,
                    "on a GPU bf16, fp16 or fp32, not ", t.scalar_type());
@@ -179,11 +183,13 @@ at::Tensor embedding(const at::Tensor& ids, const at::Tensor& weight, const OptT
   const at::Tensor &position = or_none(position_), &type = or_none(type_);
   TORCH_CHECK_VALUE(weight.dim() == 2, "weight: [rows, d], got ", weight.sizes());
   check_type(weight);
+  check_size(weight);
   check_index("ids", ids, weight);
   check_count(ids.numel());
   const int64_t skip = skipped(padding, weight.size(0));
   if (position.defined()) {
     check_table("position_weight", position, weight);
+    check_size(position);
     if (position_ids_.has_value()) check_index("position_ids", *position_ids_, weight);
     const int64_t seq = ids.dim() > 0 ? ids.size(-1) : 1;
     TORCH_CHECK_VALUE(position_ids_.has_value() || seq <= position.size(0), seq, " positions, and ", position.size(0), " rows in position_weight");
@@ -193,6 +199,7 @@ at::Tensor embedding(const at::Tensor& ids, const at::Tensor& weight, const OptT
   TORCH_CHECK_VALUE(type.defined() == type_ids_.has_value(), "type_weight and type_ids go together");
   if (type.defined()) {
     check_table("type_weight", type, weight);
+    check_size(type);
     check_index("type_ids", *type_ids_, weight);
   }
   const OptTensor position_ids = spread(position_ids_, ids), type_ids = spread(type_ids_, ids);
@@ -221,8 +228,9 @@ at::Tensor embedding_grad(const at::Tensor& grad, const at::Tensor& ids, int64_t
   check_index("ids", ids, grad);
   check_type(grad);
   check_count(ids.numel());
-  TORCH_CHECK_VALUE(rows >= 1 && rows <= 0x7fffffff && grad.dim() == ids.dim() + 1 && grad.sizes().slice(0, ids.dim()) == ids.sizes(), "grad: ", ids.sizes(),
-                    " + [d] and 1 to 2^31 - 1 rows, got ", grad.sizes(), " and ", rows, " rows");
+  TORCH_CHECK_VALUE(rows >= 1 && rows <= 0x7fffffff && grad.dim() == ids.dim() + 1 && grad.sizes().slice(0, ids.dim()) == ids.sizes() &&
+                        grad.size(-1) <= CCF_EMBED_MAX_D,
+                    "grad: ", ids.sizes(), " + [d], 1 to 2^31 - 1 rows and at most 2^24 columns, got ", grad.sizes(), " and ", rows, " rows");
   const int64_t skip = skipped(padding, rows);
   const c10::cuda::CUDAGuard guard(grad.device());
   const at::Tensor dy = packed(grad), index = ids.contiguous();

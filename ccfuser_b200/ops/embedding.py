@@ -26,6 +26,7 @@ from . import gemm as G
 
 MAX_TOKENS = 2 ** 26
 MAX_ROWS = 2 ** 31 - 1
+MAX_COLUMNS = 2 ** 24
 _INDEX = (torch.int64, torch.int32)
 
 
@@ -152,6 +153,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *, po
         return _embedding_torch(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx)
     if ids.numel() > MAX_TOKENS:
         raise ValueError(f"{ids.numel()} tokens: at most 2^26 in one call")
+    if weight.shape[1] > MAX_COLUMNS or any(t is not None and t.shape[0] > MAX_ROWS for t in (weight, position_weight, type_weight)):
+        raise ValueError("a table of at most 2^31 - 1 rows and 2^24 columns")
     return _EmbeddingFn.apply(ids, weight, position_weight, position_ids, type_weight, type_ids, float(scale), skip)
 
 
@@ -189,8 +192,8 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
         if skip >= 0:
             out[skip] = 0.0
         return out.mul_(scale).to(grad.dtype)
-    if ids.numel() > MAX_TOKENS or num_rows > MAX_ROWS:
-        raise ValueError("at most 2^26 tokens and 2^31 - 1 rows in one call")
+    if ids.numel() > MAX_TOKENS or num_rows > MAX_ROWS or grad.shape[-1] > MAX_COLUMNS:
+        raise ValueError("at most 2^26 tokens, 2^31 - 1 rows and 2^24 columns in one call")
     with torch.no_grad():
         dy, index = G.packed(grad), ids.contiguous()
         e = N.Embed(tokens=index.numel(), seq=1, d=dy.shape[-1], type=N.DTYPE_CODE[dy.dtype])

@@ -60,3 +60,13 @@ def test_activations_beyond_32_bits():
     assert torch.equal(y[first:].cpu() != 0, bits >= 32768)
     bits = R.philox_bits(3, 4, 6, 800, 2 ** 28 - 50)       # around 2^31 elements
     assert torch.equal(y[2 ** 31 - 400:2 ** 31 + 400].cpu() != 0, bits >= 32768)
+
+
+def test_the_widest_rows():
+    from ccfuser_b200.ops.embedding import embedding, embedding_grad
+    w = (torch.arange(2 ** 25, device="cuda") % 251).bfloat16().view(2, 2 ** 24)
+    ids = torch.tensor([1, 0, 1], device="cuda")
+    y = embedding(ids, w)
+    assert torch.equal(y, w[ids])
+    grad = embedding_grad(y, ids, 3)
+    assert torch.equal(grad[0], w[0]) and torch.equal(grad[1], w[1] + w[1]) and not grad[2].any()

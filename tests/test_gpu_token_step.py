@@ -245,6 +245,30 @@ def test_refusals_on_the_gpu(monkeypatch, function):
     assert token_logprobs(x[:0], t[:0]).logprobs.shape == (0,) and dropout(x[:0], 0.5, s).shape == (0, 10)
 
 
+@pytest.mark.parametrize("function", ["C++", "Python"])
+def test_tables_beyond_32_bits_are_refused(monkeypatch, function):
+    """Numbers of rows and columns that the kernels' 32 bits would wrap: refused before anything is read or copied."""
+    from ccfuser_b200 import native as N
+    from ccfuser_b200.ops.embedding import embedding, embedding_grad
+    if function == "Python":
+        monkeypatch.setattr(N, "torch_module", lambda: None)
+    ids, one = torch.tensor([0, 0], device="cuda"), torch.ones(1, 1, device="cuda")
+    for rows, cols in ((1, 2 ** 24 + 1), (1, 2 ** 32 + 8), (2 ** 31, 1), (2 ** 32 + 1, 1)):
+        with pytest.raises(ValueError):
+            embedding(ids, one.expand(rows, cols))
+        w = torch.ones(2, min(cols, 2 ** 24), device="cuda")
+        if cols == 1:
+            with pytest.raises(ValueError):
+                embedding(ids, w, position_weight=one.expand(rows, 1))
+            with pytest.raises(ValueError):
+                embedding(ids, w, type_weight=one.expand(rows, 1), type_ids=ids)
+            with pytest.raises(ValueError):
+                embedding_grad(torch.ones(2, 1, device="cuda"), ids, rows)
+        else:
+            with pytest.raises(ValueError):
+                embedding_grad(one.expand(2, cols), ids, 1)
+
+
 def test_ids_of_other_shapes():
     """A single id, positions and types given for all sequences at once."""
     from ccfuser_b200.ops.embedding import embedding

@@ -47,6 +47,13 @@ def test_embedding_entry_points_refuse_missing_memory():
     assert lib.ccf_embedding_scratch(5000, 50, 100, 64, 1) > lib.ccf_embedding_scratch(5000, 50, 100, 64, 0) > 0
 
 
+def test_embedding_entry_points_refuse_wide_tables():
+    lib = N.load()
+    e = _embed(d=2 ** 24 + 1, ld=2 ** 24 + 1)
+    assert lib.ccf_embedding_fwd(C.byref(e), A, A, None) == lib.ccf_embedding_bwd(C.byref(e), A, A, None) == -2
+    assert lib.ccf_embedding_scratch(5000, 50, 100, 2 ** 24 + 1, 1) == -1 < lib.ccf_embedding_scratch(5000, 50, 100, 2 ** 24, 1)
+
+
 def test_embedding_refuses():
     w, ids = torch.randn(10, 8), torch.tensor([[1, 2, 3]])
     for kw in (dict(position_ids=ids), dict(type_weight=w), dict(type_ids=ids), dict(padding_idx=10), dict(padding_idx=-11),
