@@ -502,9 +502,8 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_bwd_
   const long long row = kThreads == 32 ? blockIdx.x * 8ll + warp : static_cast<long long>(blockIdx.x);
   if (kThreads == 32 && row >= a.rows) return;
   const int split = static_cast<int>(gridDim.y), rank = static_cast<int>(blockIdx.y);
-  const size_t at = static_cast<size_t>(row) * a.ld * kElemBytes<kType>;
-  const uint8_t* p = reinterpret_cast<const uint8_t*>(a.x) + at;
-  uint8_t* o = reinterpret_cast<uint8_t*>(a.dx) + at;
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(a.x) + static_cast<size_t>(row) * a.ld * kElemBytes<kType>;
+  uint8_t* o = reinterpret_cast<uint8_t*>(a.dx) + static_cast<size_t>(row) * a.dx_ld * kElemBytes<kType>;
   const RowShape<kType> shape(p, a.width);
   const int first = static_cast<int>(static_cast<long long>(shape.pieces) * rank / split);
   const int last = static_cast<int>(static_cast<long long>(shape.pieces) * (rank + 1) / split);
@@ -652,12 +651,13 @@ int ccf_logprobs_fwd(const CcfLogprobs* a, void* stream) {
   return top ? choose_fwd<kFp32, true>(*a, st) : choose_fwd<kFp32, false>(*a, st);
 }
 
-// dx [rows, width] in the layout of x from the gradients of the outputs that are given: zeros behind the vocabulary and in rows without a gradient.
+// dx [rows, width], `dx_ld` elements between rows, from the gradients of the outputs that are given: zeros behind the vocabulary and in rows without a gradient.
 int ccf_logprobs_bwd(const CcfLogprobs* a, void* stream) {
   using namespace ccf;
   if (!valid(a) || a->dx == nullptr || (reinterpret_cast<uintptr_t>(a->dx) & 15) != 0 || a->stats == nullptr ||
       (a->d_top != nullptr && (a->top_k == 0 || a->top_ids == nullptr)))
     return -2;
+  if (a->rows > 1 && (a->dx_ld < a->width || (a->dx_ld - a->ld) % (a->type == kFp32 ? 4 : 8) != 0)) return -2;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (a->type == kBf16) return choose_bwd<kBf16>(*a, st);
   if (a->type == kFp16) return choose_bwd<kFp16>(*a, st);

@@ -4,7 +4,8 @@
 #define CCF_LOGPROBS_MAX_TOP 32
 
 // One call over logits [rows, width] (`ld` elements between rows) of which the first `vocab` columns count. `stats`: three floats per row
-// (largest logit, sum, entropy) that the backward pass reads. The gradients may be null; `dx` has the layout of `x`.
+// (largest logit, sum, entropy) that the backward pass reads. The gradients may be null. The rows of `dx`
+// begin as far from a 16-byte boundary as those of `x` do: `dx_ld` differs from `ld` by a multiple of 16 bytes where there are several.
 struct CcfLogprobs {
   const void* x;
   const void* targets;
@@ -20,6 +21,7 @@ struct CcfLogprobs {
   int* status;
   long long rows;
   long long ld;
+  long long dx_ld;
   long long ignore;
   int vocab;
   int width;

@@ -314,7 +314,8 @@ struct LogprobsNode : TokenNode {
       any = true;
     }
     if (!any) return out;
-    const at::Tensor whole = at::empty({rows, ld}, x.options());   // rows lie as those of the logits do
+    const int64_t dx_ld = width + (ld - width) % (type_code(x) == 2 ? 4 : 8);   // rows begin where those of the logits do in their 16 bytes
+    const at::Tensor whole = at::empty({rows, dx_ld}, x.options());
     CcfLogprobs a{};
     a.x = x.data_ptr();
     a.targets = t.data_ptr();
@@ -327,6 +328,7 @@ struct LogprobsNode : TokenNode {
     a.dx = whole.data_ptr();
     a.rows = rows;
     a.ld = ld;
+    a.dx_ld = dx_ld;
     a.top_k = static_cast<int>(top_k);
     a.vocab = static_cast<int>(vocab);
     a.ignore = ignore;
@@ -335,7 +337,7 @@ struct LogprobsNode : TokenNode {
     a.inv_t = static_cast<float>(inv_t);
     check(ccf_logprobs_bwd(&a, current_stream()), "ccf_logprobs_bwd");
     ++g_launches;
-    out[0] = (ld == width ? whole : whole.narrow(1, 0, width)).view(shape);
+    out[0] = (dx_ld == width ? whole : whole.narrow(1, 0, width)).view(shape);
     return out;
   }
 };

@@ -144,7 +144,7 @@ class Logprobs(C.Structure):
     """Mirror of CcfLogprobs (csrc/logprobs.h)."""
     _fields_ = [("x", _vp), ("targets", _vp), ("logprobs", _vp), ("entropy", _vp), ("top_logprobs", _vp), ("top_ids", _vp), ("stats", _vp),
                 ("d_logprobs", _vp), ("d_entropy", _vp), ("d_top", _vp), ("dx", _vp), ("status", _vp), ("rows", C.c_longlong),
-                ("ld", C.c_longlong), ("ignore", C.c_longlong), ("vocab", C.c_int), ("width", C.c_int), ("top_k", C.c_int),
+                ("ld", C.c_longlong), ("dx_ld", C.c_longlong), ("ignore", C.c_longlong), ("vocab", C.c_int), ("width", C.c_int), ("top_k", C.c_int),
                 ("type", C.c_int), ("wide", C.c_int), ("inv_t", C.c_float)]
 
 

@@ -79,7 +79,8 @@ class _LogprobsFn(torch.autograd.Function):
         if all(v is None for v in g):
             return (None,) * 6
         a = _args(x, t, *ctx.args, 0)
-        whole = torch.empty(x.shape[0], a.ld, dtype=x.dtype, device=x.device)     # rows lie as those of the logits do
+        a.dx_ld = a.width + (a.ld - a.width) % (16 // x.element_size())       # rows begin where those of the logits do in their 16 bytes
+        whole = torch.empty(x.shape[0], a.dx_ld, dtype=x.dtype, device=x.device)
         a.stats, a.top_ids, a.dx = stats.data_ptr(), N.ptr(ids), whole.data_ptr()
         a.d_logprobs, a.d_entropy, a.d_top = N.ptr(g[0]), N.ptr(g[1]), N.ptr(g[2])
         with torch.cuda.device(x.device):

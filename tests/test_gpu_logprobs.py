@@ -143,6 +143,21 @@ def test_shapes_strides_and_alignment():
     assert empty.logprobs.shape == (0, 10) and empty.top_ids.shape == (0, 10, 2)
 
 
+@pytest.mark.parametrize("function", ["C++", "Python"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_rows_far_apart(monkeypatch, dtype, function):
+    """The logits of one place of every sequence: a gradient of their own size, not of the sequences'."""
+    from ccfuser_b200 import native as N
+    if function == "Python":
+        monkeypatch.setattr(N, "torch_module", lambda: None)
+    g = _gen(5)
+    for seq, width, vocab in ((7, 1001, 1001), (50, 1004, 990), (3, 9003, 9000), (200, 57, 57)):
+        base = (_randn(g, 5, seq, width) * 2).to(TYPES[dtype])
+        t = torch.randint(0, vocab, (5,), generator=g, device="cuda")
+        _, dx = _check(base[:, 0], t, vocab, top_k=2)
+        assert dx.stride(0) < width + 8 and dx.untyped_storage().nbytes() <= 5 * (width + 7) * dx.element_size()
+
+
 def test_each_gradient_alone_and_rows_without_one():
     from ccfuser_b200.ops.logprobs import token_logprobs
     g = _gen(2)

@@ -123,6 +123,12 @@ def test_logprobs_entry_points_refuse_missing_memory():
         assert lib.ccf_logprobs_bwd(C.byref(_scores(**bad)), None) == -2
 
 
+def test_logprobs_entry_point_refuses_rows_of_another_alignment():
+    lib = N.load()
+    for bad in (dict(dx_ld=0), dict(dx_ld=63), dict(dx_ld=65), dict(dx_ld=68), dict(dx_ld=66, type=2), dict(dx_ld=-64), dict(ld=65, dx_ld=64)):
+        assert lib.ccf_logprobs_bwd(C.byref(_scores(**bad)), None) == -2
+
+
 def test_logprobs_refuses():
     x, t = torch.randn(3, 10), torch.tensor([1, 2, 3])
     for kw in (dict(top_k=-1), dict(top_k=11), dict(top_k=33), dict(vocab_size=0), dict(vocab_size=11), dict(vocab_size=4, top_k=5),
