@@ -94,15 +94,63 @@ def dropout(x: torch.Tensor, p: float, state: torch.Tensor, call: int = 0, resid
     return _DropoutFn.apply(x, residual, state, call, drop)
 
 
+class _First:
+    """Notes where a pass begins."""
+
+    def __init__(self, state, start):
+        self.state, self.start = state, start
+
+    def __enter__(self):
+        self.start[:] = [(self.state.tensor.clone(), self.state.calls)]
+
+    def __exit__(self, *_):
+        pass
+
+
+class _Again:
+    """Goes back there, once for every repetition."""
+
+    def __init__(self, state, start):
+        self.state, self.start, self.now = state, start, []
+
+    def __enter__(self):
+        s = self.state
+        self.now.append((s.tensor.clone(), s.calls))
+        s.tensor.copy_(self.start[0][0])
+        s.calls = self.start[0][1]
+        s._again += 1
+
+    def __exit__(self, *_):
+        s = self.state
+        tensor, s.calls = self.now.pop()
+        s.tensor.copy_(tensor)
+        s._again -= 1
+
+
 class DropoutState:
     """Seed, step and call counter that the dropouts of one model share. ``advance()`` begins the next step's masks: an addition on the device, so
-    that a captured one advances with every replay."""
+    that a captured one advances with every replay. ``tensor`` is what a checkpoint file has to keep for later steps to go on with their masks.
+
+    A forward pass that the backward pass repeats (``torch.utils.checkpoint``) needs the numbers that its calls had, which
+    ``checkpoint(..., use_reentrant=False, context_fn=state.recomputed)`` gives them; without that, a call inside a backward pass is an error."""
 
     def __init__(self, seed: int, device=None):
         self.tensor = torch.tensor([seed, 0], dtype=torch.int64, device=device)
         self.calls = 0
+        self._again = 0
+
+    def _not_repeated(self):
+        if not self._again and torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("a DropoutState used inside a backward pass would draw other masks than the forward pass did: give checkpoint() "
+                               "use_reentrant=False and context_fn=state.recomputed, or call dropout() with numbers of your own")
+
+    def recomputed(self):
+        """The contexts of a checkpointed forward pass and of its repetition, in which step and call numbers are those of the first one."""
+        start = []
+        return _First(self, start), _Again(self, start)
 
     def next_call(self) -> int:
+        self._not_repeated()
         self.calls = (self.calls + 1) & _LOW
         return self.calls
 
@@ -112,6 +160,7 @@ class DropoutState:
         return self.tensor
 
     def advance(self):
+        self._not_repeated()
         self.tensor[1:].add_(1)
 
     def begin_step(self, device):

@@ -248,3 +248,37 @@ def test_dropout_on_the_host():
     assert not torch.equal(one, two) and torch.equal(m.eval()(one), one)
     rng.advance()
     assert rng.tensor.tolist() == [3, 1] and rng.calls == 2
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_a_repeated_forward_pass_draws_the_same_masks(device):
+    """Activation checkpointing: the gradients of the same pass without it, also where the state has moved on; refused where the masks would differ."""
+    from torch.utils.checkpoint import checkpoint
+    w = torch.arange(1.0, 65.0, device=device)
+
+    def run(wrap, later):
+        rng = D.DropoutState(5, device)
+        drop = D.Dropout(0.5, rng)
+        x = w.clone().requires_grad_(True)
+
+        def block(h):
+            return drop(drop(h * w).sin(), residual=h)
+
+        rng.begin_step(x.device)
+        y = wrap(rng, block, wrap(rng, block, x))
+        if later:
+            rng.begin_step(x.device)
+            drop(w)
+        y.sum().backward(retain_graph=True)
+        one = x.grad.clone()
+        y.sum().backward()
+        assert torch.equal(x.grad, one + one)
+        return y.detach(), one, rng.tensor.tolist(), rng.calls
+
+    for later in (False, True):
+        plain = run(lambda rng, f, h: f(h), later)
+        again = run(lambda rng, f, h: checkpoint(f, h, use_reentrant=False, context_fn=rng.recomputed), later)
+        assert torch.equal(plain[0], again[0]) and torch.equal(plain[1], again[1]) and plain[2:] == again[2:]
+        for reentrant in (False, True):
+            with pytest.raises(RuntimeError, match="other masks"):
+                run(lambda rng, f, h: checkpoint(f, h, use_reentrant=reentrant), later)
