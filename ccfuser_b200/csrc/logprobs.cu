@@ -104,28 +104,36 @@ struct RowShape {
 
 // u_j = x_j c - m c, with m c rounded once and the same for all of a row: one fused operation, whose rounding of m c cancels in every quotient. That
 // holds where m c is finite and raised elements vanish; elsewhere (rows of the type's lowest value, an extreme temperature) u_j = (x_j - m) c.
+// Products are rounded where they are taken (__fmul_rn): one that the compiler drew into a following subtraction would be another number.
+constexpr float kMostMc = 1e37f;
 template <int kType>
 __device__ __forceinline__ bool fused_ok(float mc, float c) {
-  const float low = kFloor<kType> * c;
-  return low - mc < -200.f && fabsf(mc) < 1e37f && low > -1e38f;
+  const float low = __fmul_rn(kFloor<kType>, c), least = low > -1e38f ? fmaxf(low + 200.f, -kMostMc) : kMostMc;
+  return mc > least && mc < kMostMc;
 }
+// The exponents are relative to m c, rounded where they come from the fused operation and exact elsewhere: m c and what its rounding left out of it. Sums under several
+// maxima meet by the difference of both: without the second, fp32 logits around 1e6 would be a hundredth off.
+template <int kType>
+__device__ __forceinline__ float rest_of(float m, float mc, float c) { return fused_ok<kType>(mc, c) ? 0.f : fmaf(m, c, -mc); }
 
 struct RowStats {
   float m, s, q;
 };
 // the same sums relative to a larger m
+template <int kType>
 __device__ __forceinline__ void rescale(RowStats& a, float m, float c) {
-  const float d = a.m == m ? 0.f : fmaxf(a.m * c - m * c, kFloorU), f = exp2_fast(d);
-  a.q = fmaf(a.s, d, a.q) * f;
+  const float from = __fmul_rn(a.m, c), to = __fmul_rn(m, c), d = (from - to) + (rest_of<kType>(a.m, from, c) - rest_of<kType>(m, to, c));
+  const float u = a.m == m ? 0.f : fmaxf(d, kFloorU), f = exp2_fast(u);
+  a.q = fmaf(a.s, u, a.q) * f;
   a.s *= f;
   a.m = m;
 }
-template <int kLanes>
+template <int kType, int kLanes>
 __device__ __forceinline__ void reduce_lanes(RowStats& a, float c) {
   float m = a.m;
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  rescale(a, m, c);
+  rescale<kType>(a, m, c);
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o /= 2) {
     a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
@@ -136,7 +144,7 @@ __device__ __forceinline__ void reduce_lanes(RowStats& a, float c) {
 // running statistics of one thread; with kTop also the place of the turn that holds its largest element, and the largest of the other turns
 template <int kType, bool kTop>
 struct Running {
-  float m = neg_inf(), mc = neg_inf(), second = neg_inf();
+  float m = neg_inf(), mc = neg_inf(), rest = 0.f, second = neg_inf();
   int at = 0;
   f32x2 s = 0, q = 0;
   __device__ __forceinline__ void turn(float largest, int v, float c) {
@@ -149,10 +157,12 @@ struct Running {
   __device__ __forceinline__ void raise(float to, float c) {   // before elements up to `to`
     if (to <= m) return;
     m = max_nan(m, to);
-    const float next = m * c, d = fmaxf(mc - next, kFloorU), f = exp2_fast(d);   // m has changed: the two products differ, or both are infinite
+    const float next = __fmul_rn(m, c), next_rest = rest_of<kType>(m, next, c);
+    const float d = fmaxf((mc - next) + (rest - next_rest), kFloorU), f = exp2_fast(d);   // NaN, from infinite products: the floor
     q = mul2(fma2(s, bc2(d), q), bc2(f));
     s = mul2(s, bc2(f));
     mc = next;
+    rest = next_rest;
   }
   __device__ __forceinline__ void add(f32x2 u) {
     float u0, u1;
@@ -396,13 +406,13 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
   RowStats st = run.done();
   uint32_t largest = 0;
   if constexpr (kTop) largest = group_maxima<kThreads>(sh, own, tid, a.top_k);
-  reduce_lanes<32>(st, c);
+  reduce_lanes<kType, 32>(st, c);
   if constexpr (kThreads > 32) {
     constexpr int kWarps = kThreads / 32;
     if (lane == 0) sh.part[warp] = st;
     __syncthreads();
     st = sh.part[lane % kWarps];
-    reduce_lanes<kWarps>(st, c);
+    reduce_lanes<kType, kWarps>(st, c);
   } else {
     __syncwarp();
   }
@@ -415,7 +425,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
       if (rank == 0) {
         st = RowStats{neg_inf(), 0.f, 0.f};
         if (lane < split) st = *cluster.map_shared_rank(&sh.all, lane);
-        reduce_lanes<32>(st, c);
+        reduce_lanes<kType, 32>(st, c);
         if constexpr (kTop) {
           const int n = split * a.top_k;
           for (int i = tid; i < n; i += kThreads) sh.list[i] = cluster.map_shared_rank(sh.top, i / a.top_k)[i % a.top_k];
@@ -431,7 +441,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
     }
     if (tid >= 32) return;   // the first warp has what is left
   }
-  const float log_s = logf(st.s), mc = st.m * c;
+  const float log_s = logf(st.s), mc = __fmul_rn(st.m, c);
   // lp_j = (x_j - M) / T - log_sum: the sum stands relative to the rounded M c, so the rounding is taken out of it
   const float log_sum = fused_ok<kType>(mc, c) ? fmaf(-kLn2, fmaf(st.m, c, -mc), log_s) : log_s;
   const bool none = st.m == neg_inf(), bad = !(st.m < __int_as_float(0x7f800000));
@@ -520,7 +530,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_bwd_
     if (edge_index >= 0) store_elem<kType>(o, edge_index, 0.f);
     return;
   }
-  const float mc = r.m * c;
+  const float mc = __fmul_rn(r.m, c);
   const bool fused = fused_ok<kType>(mc, c);
   auto grad = [&](float x) {
     const float u = fmaxf(fused ? fmaf(x, c, -mc) : (x - r.m) * c, kFloorU);
