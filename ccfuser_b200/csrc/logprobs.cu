@@ -103,9 +103,10 @@ struct RowShape {
 };
 
 // u_j = x_j c - m c, with m c rounded once and the same for all of a row: one fused operation, whose rounding of m c cancels in every quotient. That
-// holds where m c is finite and raised elements vanish; elsewhere (rows of the type's lowest value, an extreme temperature) u_j = (x_j - m) c.
+// holds where raised elements vanish and where m c is at most 2^20: the largest element's u is what the rounding left out, here at most 2^-5, but 256 at
+// 2^33, and 2^256 is no number. Elsewhere (rows of the type's lowest value, large logits, an extreme temperature) u_j = (x_j - m) c.
 // Products are rounded where they are taken (__fmul_rn): one that the compiler drew into a following subtraction would be another number.
-constexpr float kMostMc = 1e37f;
+constexpr float kMostMc = 1048576.f;
 template <int kType>
 __device__ __forceinline__ bool fused_ok(float mc, float c) {
   const float low = __fmul_rn(kFloor<kType>, c), least = low > -1e38f ? fmaxf(low + 200.f, -kMostMc) : kMostMc;
