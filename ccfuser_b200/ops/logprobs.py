@@ -135,8 +135,9 @@ def _logprobs_torch(logits, targets, top_k, temperature, vocab, ignore):
     x = logits[..., :vocab]
     x = x if x.dtype == torch.float64 else x.float()
     none = (x == -math.inf).all(dim=-1, keepdim=True)
-    # a row without a finite logit gets zeros in its place, which give it no gradient
-    lp = torch.log_softmax(torch.where(none, torch.zeros_like(x), x / temperature), dim=-1)
+    # a row without a finite logit gets zeros in its place, which give it no gradient. The largest is taken off before the division, which may pass the type's range
+    largest = x.detach().amax(dim=-1, keepdim=True)
+    lp = torch.log_softmax(torch.where(none, torch.zeros_like(x), (x - largest) / temperature), dim=-1)
     lp = torch.where(none, torch.full_like(lp, -math.inf), lp)
     gone = lp == -math.inf
     entropy = -torch.where(gone, torch.zeros_like(lp), lp.exp() * torch.where(gone, torch.zeros_like(lp), lp)).sum(dim=-1)
