@@ -128,8 +128,8 @@ class Block(nn.Module):
 
 
 class GPTMoE(nn.Module):
-    """``forward(ids [B,S], labels=None)`` -> logits, or the mean next-token cross-entropy when labels are given (labels of -100 are left
-    out). ``score(ids)`` -> log probabilities of the given tokens, entropies and best alternatives."""
+    """``forward(ids [B,S], labels=None)`` -> logits, or the mean next-token cross-entropy when labels are given (one per token, in any
+    shape; those of -100 are left out). ``score(ids)`` -> log probabilities of the given tokens, entropies and best alternatives."""
 
     def __init__(self, c: GPTMoEConfig, ep_group=None, device=None):
         super().__init__()
@@ -169,7 +169,7 @@ class GPTMoE(nn.Module):
         logits = self._logits(ids)
         if labels is None:
             return logits[..., :self.config.vocab_size]
-        return cross_entropy(logits, labels, self.config.vocab_size)
+        return cross_entropy(logits, labels.reshape(logits.shape[:-1]), self.config.vocab_size)
 
     def score(self, ids: torch.Tensor, top_k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
         """For every token of ``ids [B,S]`` but the first, given those before it: log probability, the entropy of its distribution and the

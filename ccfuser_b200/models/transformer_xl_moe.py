@@ -218,7 +218,7 @@ class TransformerXLMoE(nn.Module):
         if self.crit is not None:
             loss = self.crit(x.reshape(-1, x.shape[-1]).float(), target.reshape(-1)).loss
         else:
-            loss = cross_entropy(F.linear(x, self.word_emb.weight), target)
+            loss = cross_entropy(F.linear(x, self.word_emb.weight), target.reshape(x.shape[:-1]))
         return loss, new_mems
 
     def moe_layers(self):
