@@ -119,6 +119,8 @@ class BertMoEForQuestionAnswering(nn.Module):
 
     def forward(self, input_ids, attention_mask=None, token_type_ids=None, start_positions=None, end_positions=None):
         tt = token_type_ids if token_type_ids is not None else torch.zeros_like(input_ids)
+        if tt.shape != input_ids.shape:
+            input_ids, tt = torch.broadcast_tensors(input_ids, tt)
         x = self.ln_emb(self.word(input_ids, position_weight=self.position.weight, type_weight=self.token_type.weight, type_ids=tt))
         mask = token_mask = None
         if attention_mask is not None:
