@@ -221,5 +221,14 @@ class TransformerXLMoE(nn.Module):
             loss = cross_entropy(F.linear(x, self.word_emb.weight), target.reshape(x.shape[:-1]))
         return loss, new_mems
 
+    @property
+    def emb_scale(self):
+        """Factor of the word embedding."""
+        return self.word_emb.scale
+
+    @emb_scale.setter
+    def emb_scale(self, scale):
+        self.word_emb.scale = scale
+
     def moe_layers(self):
         return [l.pos_ff for l in self.layers if l.is_moe]

@@ -29,3 +29,13 @@ def test_bert_token_types_broadcast(ids_shape, types_shape):
     want = F.embedding(ids, m.word.weight) + F.embedding(torch.arange(9), m.position.weight) + F.embedding(tt, m.token_type.weight)
     torch.testing.assert_close(seen[0], want)
     assert start.shape == (3, 9)
+
+
+def test_the_embedding_factor_of_transformer_xl():
+    m, ids = _txl(), torch.randint(0, 50, (2, 8))
+    assert m.emb_scale == 32 ** 0.5
+    seen = []
+    m.layers[0].register_forward_pre_hook(lambda mod, args: seen.append(args[0]))
+    m.emb_scale = 2.0
+    m(ids)
+    torch.testing.assert_close(seen[0], F.embedding(ids, m.word_emb.weight) * 2.0)
