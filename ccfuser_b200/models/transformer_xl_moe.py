@@ -160,7 +160,7 @@ class TransformerXLMoE(nn.Module):
         self.drop = None
         if c.dropout > 0:
             seed = int(torch.randint(2 ** 62, (1,))) if c.dropout_seed is None else c.dropout_seed
-            self.drop = Dropout(c.dropout, DropoutState(seed + (dist.get_rank() if dist.is_initialized() else 0), device))
+            self.drop = Dropout(c.dropout, DropoutState(seed, device, rank=dist.get_rank() if dist.is_initialized() else 0))
         self.layers = nn.ModuleList([DecoderLayer(c, ep_group, device, self.drop) for _ in range(c.n_layer)])
         if c.adaptive_cutoffs:
             self.crit = nn.AdaptiveLogSoftmaxWithLoss(c.d_model, c.n_token, list(c.adaptive_cutoffs), device=device)

@@ -129,15 +129,32 @@ class _Again:
 
 class DropoutState:
     """Seed, step and call counter that the dropouts of one model share. ``advance()`` begins the next step's masks: an addition on the device, so
-    that a captured one advances with every replay. ``tensor`` is what a checkpoint file has to keep for later steps to go on with their masks.
+    that a captured one advances with every replay. ``rank`` is added to the seed: ranks of a job give the same seed and draw masks of their own.
+    ``state_dict()`` is what a checkpoint has to keep for later steps to go on with their masks, the same on every rank
+    (``utils.checkpoint.save_ep_checkpoint`` keeps it for the ``Dropout`` modules of a model).
 
     A forward pass that the backward pass repeats (``torch.utils.checkpoint``) needs the numbers that its calls had, which
     ``checkpoint(..., use_reentrant=False, context_fn=state.recomputed)`` gives them; without that, a call inside a backward pass is an error."""
 
-    def __init__(self, seed: int, device=None):
-        self.tensor = torch.tensor([seed, 0], dtype=torch.int64, device=device)
+    def __init__(self, seed: int, device=None, rank: int = 0):
+        self.rank = rank
+        self.tensor = torch.tensor([self._wrapped(seed + rank), 0], dtype=torch.int64, device=device)
         self.calls = 0
         self._again = 0
+
+    @staticmethod
+    def _wrapped(seed):
+        """As 64 bits with a sign hold it."""
+        return (seed + 2 ** 63) % 2 ** 64 - 2 ** 63
+
+    def state_dict(self) -> dict:
+        seed, step = self.tensor.tolist()
+        return {"seed": self._wrapped(seed - self.rank), "step": step, "calls": self.calls}
+
+    def load_state_dict(self, state: dict):
+        """In place: captured graphs go on with it."""
+        self.tensor.copy_(torch.tensor([self._wrapped(state["seed"] + self.rank), state["step"]]))
+        self.calls = state["calls"]
 
     def _not_repeated(self):
         if not self._again and torch._C._current_graph_task_id() != -1:

@@ -22,6 +22,12 @@ def expert_keys(model: nn.Module) -> List[str]:
     return [n for n, p in model.named_parameters() if getattr(p, "skip_allreduce", False)]
 
 
+def dropout_states(model: nn.Module) -> list:
+    """The dropout states (``ops.dropout.DropoutState``) of a model's modules, each once, in the order of the modules."""
+    from ..ops.dropout import Dropout
+    return list({id(m.state): m.state for m in model.modules() if isinstance(m, Dropout)}.values())
+
+
 def ep_state_dict(model: nn.Module) -> Dict[str, Dict[str, torch.Tensor]]:
     """Split the model state into {'experts': local expert tensors, 'replicated': everything else} (on CPU)."""
     ek = set(expert_keys(model))
@@ -34,7 +40,8 @@ def save_ep_checkpoint(model: nn.Module, prefix: str, ep_rank: int, ep_size: int
                        optimizer: Optional[torch.optim.Optimizer] = None):
     """Every rank writes ``<prefix>.ep<rank>of<size>.pt``; rank 0 also writes the replicated part and a manifest. With
     ``optimizer`` every rank also writes its optimizer state (``<prefix>.opt<rank>of<size>.pt``: it covers this rank's
-    experts and its copy of the replicated parameters; it is reloaded only at the same expert-parallel degree)."""
+    experts and its copy of the replicated parameters; it is reloaded only at the same expert-parallel degree). The manifest
+    also keeps seed, step and call number of the model's dropouts."""
     os.makedirs(os.path.dirname(os.path.abspath(prefix)) or ".", exist_ok=True)
     parts = ep_state_dict(model)
     torch.save(parts["experts"], f"{prefix}.ep{ep_rank}of{ep_size}.pt")
@@ -45,7 +52,7 @@ def save_ep_checkpoint(model: nn.Module, prefix: str, ep_rank: int, ep_size: int
         e_loc = {k: int(v.shape[0]) for k, v in parts["experts"].items()}
         with open(f"{prefix}.manifest.json", "w") as f:
             json.dump({"ep_size": ep_size, "experts_per_rank": e_loc, "expert_keys": sorted(parts["experts"]),
-                       "extra": extra or {}}, f, indent=1)
+                       "dropout": [d.state_dict() for d in dropout_states(model)], "extra": extra or {}}, f, indent=1)
 
 
 def reshard_expert_state(shards: List[Dict[str, torch.Tensor]], new_ep_size: int) -> List[Dict[str, torch.Tensor]]:
@@ -64,7 +71,8 @@ def load_ep_checkpoint(model: nn.Module, prefix: str, ep_rank: int, ep_size: int
                        optimizer: Optional[torch.optim.Optimizer] = None) -> dict:
     """Load a checkpoint written at any EP degree into a model sharded over ``ep_size`` ranks. ``optimizer`` state is
     restored when the checkpoint has it for this degree; after a change of degree the optimizer starts fresh (the
-    returned manifest then carries ``"optimizer_restored": False``)."""
+    returned manifest then carries ``"optimizer_restored": False``). Dropouts go on with the masks that the writing job would have
+    drawn next; a checkpoint without their states, or with those of another number of them, leaves them as they are (``"dropout_restored": False``)."""
     with open(f"{prefix}.manifest.json") as f:
         manifest = json.load(f)
     old = int(manifest["ep_size"])
@@ -76,6 +84,11 @@ def load_ep_checkpoint(model: nn.Module, prefix: str, ep_rank: int, ep_size: int
     state = dict(torch.load(f"{prefix}.replicated.pt", map_location="cpu"))
     state.update(experts)
     model.load_state_dict(state, strict=strict)
+    states, kept = dropout_states(model), manifest.get("dropout", [])
+    manifest["dropout_restored"] = len(states) == len(kept)
+    if manifest["dropout_restored"]:
+        for d, s in zip(states, kept):
+            d.load_state_dict(s)
     if optimizer is not None:
         path = f"{prefix}.opt{ep_rank}of{ep_size}.pt"
         restored = old == ep_size and os.path.exists(path)
