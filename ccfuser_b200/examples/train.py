@@ -22,6 +22,7 @@ import torch.nn as nn
 from ..models.bert_moe import BertMoEConfig, BertMoEForQuestionAnswering
 from ..models.gpt_moe import GPTMoE, GPTMoEConfig
 from ..models.transformer_xl_moe import TransformerXLMoE, TransformerXLMoEConfig
+from ..ops.gemm import IdCheck
 from ..parallel.ddp import wrap_ddp
 from ..utils.dist import init_distributed
 
@@ -191,10 +192,15 @@ def main():
                     extra = m.gate.get_loss()
                     if extra is not None and extra.requires_grad:
                         loss = loss + extra.to(loss.dtype).sum()
+        ids_ok = IdCheck(dev) if dev.type == "cuda" else None
+        if ids_ok is not None and args.fuse_expert_sgd:    # the backward pass changes weights
+            ids_ok.wait(f"step {i}")
         loss.backward()
         if expert_dp_group is not None and args.variant != "dense":
             from ..parallel.ddp import reduce_expert_grads
             reduce_expert_grads(model, expert_dp_group, scale=1.0 / world)   # replicas of an expert agree again
+        if ids_ok is not None:
+            ids_ok.wait(f"step {i}")
         opt.step()
         if args.rebalance_every > 0 and args.variant != "dense" and (i + 1) % args.rebalance_every == 0:
             from ..layers import MoELayer
@@ -231,6 +237,8 @@ def main():
             model.eval()
         val = evaluate_lm(lambda x, y: model({"ids": x, "labels": y}),
                           corpus.iterator("valid", args.batch or 16, args.seq or 512, device=dev), max_batches=50)
+        if dev.type == "cuda":
+            IdCheck(dev).wait("validation")
         if rank == 0:
             print(json.dumps({"bench": "e2e", "model": args.model, "valid_loss": round(val, 4), "vocab": len(corpus.vocab)}))
     if args.save:

@@ -23,6 +23,7 @@ ACT_CODE = {"gelu": ACT_GELU, "relu": ACT_RELU, "none": ACT_NONE, "swiglu": ACT_
 
 ERR_NAMES = {1: "pipeline barrier timeout", 2: "peer flag timeout", 3: "bounds check", 4: "receive buffer overflow",
              5: "index out of range"}
+ERR_INDEX = 5
 
 _vp = C.c_void_p
 

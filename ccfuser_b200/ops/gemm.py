@@ -100,6 +100,25 @@ class Workspace:
             raise MoECommError(msg)
 
 
+class IdCheck:
+    """Ids out of range in what has been issued on a device's current stream so far: the status word is copied to the host behind that work, and
+    ``wait()`` raises ``TokenIndexError`` for one as soon as the copy is there, while later work goes on. Taken behind a forward pass and waited for before its
+    gradients change a weight, it stops a training loop that a bad id would otherwise fill with NaN. Other codes are left for ``Workspace.check``."""
+
+    def __init__(self, device):
+        self.ws = Workspace.get(device)
+        self.host = torch.zeros(2, dtype=torch.int32, pin_memory=True)
+        self.done = torch.cuda.Event()
+        with torch.cuda.device(self.ws.status.device):
+            self.host.copy_(self.ws.status, non_blocking=True)
+            self.done.record()
+
+    def wait(self, what: str = "training step"):
+        self.done.synchronize()
+        if int(self.host[0]) & 0xff == N.ERR_INDEX:
+            self.ws.check(what)
+
+
 _MBAR_SITES = {1: "tile scheduler slot (producer)", 2: "free pipeline stage (producer)", 3: "tile index (MMA warp)",
                4: "free accumulator (MMA warp)", 5: "operands of a stage (MMA warp)", 6: "tile index (epilogue)",
                7: "finished accumulator (epilogue)", 0x22: "free pipeline stage (producer, CTA-pair kernel)",

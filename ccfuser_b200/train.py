@@ -13,6 +13,7 @@ import torch
 import torch.distributed as dist
 import torch.nn as nn
 
+from .ops.gemm import IdCheck
 from .parallel.ddp import allreduce_replicated_grads, reduce_expert_grads, wrap_ddp
 
 
@@ -54,7 +55,11 @@ class TrainStep:
         self._ids = self._labels = None
 
     def step_device(self, ids: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
-        """One optimisation step on device tensors; returns the loss tensor (no host sync)."""
+        """One optimisation step on device tensors; returns the loss tensor (no host sync). An id outside its table makes it NaN, gradients and weights
+        with it, until ``ops.gemm.Workspace.check`` is asked; ``step`` asks in time."""
+        return self._step(ids, labels, False)
+
+    def _step(self, ids, labels, check_ids):
         self.opt.zero_grad(set_to_none=True)
         if self.fuse_expert_sgd:
             group = self.opt.param_groups[0]
@@ -66,17 +71,25 @@ class TrainStep:
             aux = self.raw_model.aux_loss()
             if aux is not None:
                 loss = loss + aux.to(loss.dtype).sum()
+        check = None
+        if check_ids and self.device.type == "cuda":
+            check = IdCheck(self.device)
+            if self.fuse_expert_sgd:       # the backward pass changes weights
+                check.wait()
         loss.backward()
         if self.distributed and not self.use_ddp:
             allreduce_replicated_grads(self.raw_model, self.dp_group)
         if self.expert_dp_group is not None or self.mean_expert_grads:
             scale = 1.0 / dist.get_world_size(self.dp_group) if (self.mean_expert_grads and dist.is_initialized()) else None
             reduce_expert_grads(self.raw_model, self.expert_dp_group, scale)
+        if check is not None:
+            check.wait()
         self.opt.step()
         return loss.detach()
 
     def step(self, ids: torch.Tensor, labels: Optional[torch.Tensor] = None) -> float:
-        """ids/labels: host tensors (pinned for an asynchronous copy). Returns the loss."""
+        """ids/labels: host tensors (pinned for an asynchronous copy). Returns the loss. An id outside its table raises
+        ``TokenIndexError`` before any weight has changed."""
         if labels is None:
             labels = ids
         if self._ids is None or self._ids.shape != ids.shape:
@@ -84,4 +97,4 @@ class TrainStep:
             self._labels = torch.empty(labels.shape, dtype=labels.dtype, device=self.device)
         self._ids.copy_(ids, non_blocking=True)
         self._labels.copy_(labels, non_blocking=True)
-        return float(self.step_device(self._ids, self._labels).item())
+        return float(self._step(self._ids, self._labels, True).item())
