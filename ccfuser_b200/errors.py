@@ -23,5 +23,5 @@ class MoEOverflow(MoECommError):
     """More rows were routed to a rank than its receive buffer was sized for."""
 
 
-class TokenIndexError(MoECommError, IndexError):
-    """A token, position, type or target id lay outside its table; its row of the output is NaN."""
+class TokenIndexError(RuntimeError, IndexError):
+    """A token, position, type or target id lay outside its table; its row of the output is NaN. Not a ``MoECommError``: no peer is lost."""

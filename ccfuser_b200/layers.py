@@ -183,7 +183,8 @@ class MoELayer(nn.Module):
         return self._fused.routing_stats() if self._fused is not None else {}
 
     def check_status(self):
-        """Host read of the fused kernels' status word; raises MoECommTimeout / MoEOverflow / MoECommError. With
+        """Host read of the fused kernels' status word; raises MoECommTimeout / MoEOverflow / MoECommError, or
+        TokenIndexError for what the kernels in front of or behind the layers recorded there. With
         CCFUSER_CANARY=1 the guard regions around the symmetric buffers are verified as well."""
         if self._fused is not None:
             self._fused.ctx.check_status("MoELayer")
