@@ -73,6 +73,11 @@ __device__ __forceinline__ long long load_index(const void* p, long long i, int 
   return wide ? __ldg(reinterpret_cast<const long long*>(p) + i) : static_cast<long long>(__ldg(reinterpret_cast<const int*>(p) + i));
 }
 
+// An id out of its table, at this token (or row of logits). The status word has 23 bits for it: the last number stands for all from there on.
+__device__ __forceinline__ void report_index(int* status, uint32_t token) {
+  report_status(status, CCF_ERR_INDEX, static_cast<int>(min(token, 0x7fffffu)));
+}
+
 inline int sm_count() {
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);

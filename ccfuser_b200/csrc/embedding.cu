@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(32 * kEmbWarps, 4) embedding_fwd_kernel(const 
     at[k] = here ? static_cast<uint64_t>(id) * w.ld + c : c;
   }
   const uint32_t good = __ballot_sync(0xffffffffu, in);
-  if (c == 0 && !in && lane_id() < n) report_status(status, CCF_ERR_INDEX, static_cast<int>(begin + lane_id()) & 0x7fffff);
+  if (c == 0 && !in && lane_id() < n) report_index(status, begin + lane_id());
   for (uint32_t t0 = 0; t0 < n; t0 += kRows) {
     S row[kTables][kRows];
 #pragma unroll
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kSortChunk) embedding_sort_kernel(const __grid
   if (tid < n) {
     const long long id = load_index(t.ids, base + tid, t.wide);
     const bool in = id >= 0 && id < t.rows;
-    if (!in) report_status(g.status, CCF_ERR_INDEX, static_cast<int>(base + tid) & 0x7fffff);
+    if (!in) report_index(g.status, base + tid);
     else t.slot[id] = base + tid;
     key = static_cast<Key>(in && id != t.skip ? static_cast<uint32_t>(id) : kLast<Key>) << kPlaceBits<Key> | tid;
   }
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kSortChunk) embedding_few_kernel(const __grid_
   if (tid < n) {
     const long long id = id_at(t, tid);
     const bool in = id >= 0 && id < t.rows;
-    if (!in && c == 0) report_status(g.status, CCF_ERR_INDEX, static_cast<int>(tid));
+    if (!in && c == 0) report_index(g.status, tid);
     key = static_cast<Key>(in && id != t.skip ? static_cast<uint32_t>(id) : kLast<Key>) << kPlaceBits<Key> | tid;
   }
   key = sort_keys(key, other, n);

@@ -26,7 +26,7 @@ enum CcfStatus {
   CCF_ERR_FLAG_TIMEOUT = 2,   // a peer's arrival flag / counter never reached its target
   CCF_ERR_BOUNDS = 3,         // an index failed a debug bounds check; the access was skipped
   CCF_ERR_OVERFLOW = 4,       // more rows routed to a rank than its receive buffer holds
-  CCF_ERR_INDEX = 5           // a token or target id outside its table; detail: the token
+  CCF_ERR_INDEX = 5           // a token or target id outside its table; detail: the token, 2^23 - 1 for all from there on
 };
 
 // Rows pushed by the dispatch role. All peer_* pointers are addresses in *this* process' address space

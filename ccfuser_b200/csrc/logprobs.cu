@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_fwd_
     if (target == a.ignore) {
       lp = 0.f;
     } else if (target < 0 || target >= a.vocab) {
-      report_status(a.status, CCF_ERR_INDEX, static_cast<int>(row) & 0x7fffff);
+      report_index(a.status, static_cast<uint32_t>(row));
       lp = nan;
     }
     a.logprobs[row] = lp;

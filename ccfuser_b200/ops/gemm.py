@@ -151,7 +151,8 @@ def describe_status(code: int, detail: int) -> str:
     if code == 4:
         return f"receive buffer of rank {detail} too small for the rows routed to it"
     if code == 5:
-        return f"an id of token {detail} lies outside its table (its row is NaN, and it adds nothing to a gradient)"
+        token = str(detail) if detail < 0x7fffff else f"{detail} or a later one"
+        return f"an id of token {token} lies outside its table (its row is NaN, and it adds nothing to a gradient)"
     return f"unknown code {code}, detail {detail:#x}"
 
 

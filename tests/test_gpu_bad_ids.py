@@ -54,3 +54,21 @@ def test_the_training_example_stops(monkeypatch, model):
     torch.cuda.synchronize()
     (m, before), = made
     assert all(torch.equal(a, b) for a, b in zip(before, _weights(m)))
+
+
+@pytest.mark.parametrize("at", [3, 2 ** 23 - 2, 2 ** 23 - 1, 2 ** 23 + 1])
+def test_the_number_of_a_late_token(at):
+    """The status word has 23 bits for it: behind them no other token is named."""
+    from ccfuser_b200 import TokenIndexError
+    from ccfuser_b200.ops.embedding import embedding, embedding_grad
+    from ccfuser_b200.ops.gemm import Workspace
+    from ccfuser_b200.ops.logprobs import token_logprobs
+    n = 2 ** 23 + 2
+    ids = torch.zeros(n, dtype=torch.int32, device="cuda")
+    ids[at] = 2
+    w = torch.ones(2, 8, device="cuda", dtype=torch.bfloat16)
+    calls = [lambda: embedding(ids, w), lambda: token_logprobs(w[:1].expand(n, 8)[:, :2], ids), lambda: embedding_grad(w[:1].expand(n, 8), ids, 2)]
+    for call in calls:
+        call()
+        with pytest.raises(TokenIndexError, match=f"token {at} lies" if at < 2 ** 23 - 1 else "token 8388607 or a later one"):
+            Workspace.get("cuda").check("test")

@@ -20,3 +20,8 @@ def test_a_bad_id_is_no_lost_peer():
     assert isinstance(e, TokenIndexError) and isinstance(e, IndexError) and isinstance(e, RuntimeError)
     assert not isinstance(e, MoECommError) and "token 7 " in str(e)
     assert isinstance(_raised(2), MoECommError)
+
+
+def test_the_number_of_a_late_token():
+    assert "token 8388606 lies" in str(_raised(8388606 << 8 | 5))
+    assert "token 8388607 or a later one" in str(_raised(8388607 << 8 | 5))
