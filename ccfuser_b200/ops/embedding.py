@@ -119,7 +119,12 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *, po
 
     ``position_ids`` (broadcast to the shape of ``ids``) default to the index along the last dimension of ``ids``. The tables are ``[rows, d]`` of one
     type. ``padding_idx``: that row of ``weight`` gets no gradient (it is looked up like any other). The result cannot be differentiated twice."""
-    if weight.is_cuda and weight.numel() and ids.numel():
+    return _embedding(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx)
+
+
+def _embedding(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx, plain=False):
+    """plain: by torch's operations on a GPU too."""
+    if weight.is_cuda and weight.numel() and ids.numel() and not plain:
         module = N.torch_module()
         if module is not None and not torch.jit.is_tracing():      # checks its arguments as below
             return module.embedding(ids, weight, position_weight, position_ids, type_weight, type_ids, scale, padding_idx,
@@ -147,9 +152,10 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *, po
             type_ids = type_ids.expand(ids.shape)
     if ids.numel() and any(t is not None and t.shape[0] == 0 for t in (weight, position_weight, type_weight)):
         raise ValueError("a table without rows")
-    if weight.is_cuda and weight.dtype not in N.DTYPE_CODE:
+    plain = plain or not weight.is_cuda
+    if not plain and weight.dtype not in N.DTYPE_CODE:
         raise TypeError(f"tables on a GPU are bf16, fp16 or fp32, not {weight.dtype}")
-    if not weight.is_cuda or ids.numel() == 0 or weight.shape[1] == 0:
+    if plain or ids.numel() == 0 or weight.shape[1] == 0:
         return _embedding_torch(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx)
     if ids.numel() > MAX_TOKENS:
         raise ValueError(f"{ids.numel()} tokens: at most 2^26 in one call")
@@ -206,6 +212,7 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
 
 class Embedding(nn.Embedding):
     """``nn.Embedding`` (same parameters, same state-dict keys) on ``embedding``, with a factor ``scale`` and the other tables as arguments of its call.
+    What the kernels do not take (fp64 tables, more than 2^26 tokens, 2^31 - 1 rows or 2^24 columns) runs on torch's operations.
     ``max_norm``, ``scale_grad_by_freq`` and ``sparse`` are refused."""
 
     def __init__(self, *args, scale: float = 1.0, **kw):
@@ -215,5 +222,7 @@ class Embedding(nn.Embedding):
         self.scale = scale
 
     def forward(self, ids, position_weight=None, position_ids=None, type_weight=None, type_ids=None):
-        return embedding(ids, self.weight, self.scale, position_weight=position_weight, position_ids=position_ids, type_weight=type_weight,
-                         type_ids=type_ids, padding_idx=self.padding_idx)
+        w = self.weight
+        rows = max(t.shape[0] for t in (w, position_weight, type_weight) if t is not None)
+        plain = w.dtype not in N.DTYPE_CODE or ids.numel() > MAX_TOKENS or rows > MAX_ROWS or w.shape[1] > MAX_COLUMNS
+        return _embedding(ids, w, self.scale, position_weight, position_ids, type_weight, type_ids, self.padding_idx, plain)
