@@ -40,7 +40,12 @@ struct TokenNode : torch::autograd::Node {
     for (SavedVariable& v : saved) v.reset_data();
   }
   void keep(const at::Tensor& t) { saved.emplace_back(t, false); }
+  // the i-th kept tensor: hooks on saved tensors may hand it back in memory of their own, with other strides
   at::Tensor kept(int i) { return saved[i].unpack(shared_from_this()); }
+  at::Tensor kept_contiguous(int i) {
+    const at::Tensor t = kept(i);
+    return t.defined() ? t.contiguous() : t;
+  }
   variable_list apply(variable_list&& grads) final {
     TORCH_CHECK(!at::GradMode::is_enabled(), "ccfuser_b200: this operator's gradient cannot be differentiated again (create_graph=True)");
     const std::lock_guard<std::mutex> lock(mutex_);
@@ -132,7 +137,7 @@ struct EmbeddingNode : TokenNode {
   variable_list gradients(const variable_list& grads) override {
     variable_list out(3);
     if (!grads[0].defined()) return out;
-    const at::Tensor index[3] = {kept(0), kept(1), kept(2)};
+    const at::Tensor index[3] = {kept_contiguous(0), kept_contiguous(1), kept_contiguous(2)};
     const c10::cuda::CUDAGuard guard(grads[0].device());
     const at::Tensor dy = packed(grads[0]);
     CcfEmbed e{};
@@ -247,20 +252,25 @@ at::Tensor embedding_grad(const at::Tensor& grad, const at::Tensor& ids, int64_t
 }
 
 // ---- log probabilities -------------------------------------------------------------------------------------------------
-// A call over the logits' rows as the kernels read them.
+// The logits as the kernels read them: rows with any distance, the first on a 16-byte boundary, their elements next to each other.
+at::Tensor rows_of(const at::Tensor& logits, int64_t rows, int64_t width) {
+  at::Tensor x = logits.dim() == 2 ? logits : logits.reshape({rows, width});
+  if (x.stride(1) != 1 || (rows > 1 && x.stride(0) < width)) x = x.contiguous();
+  if (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) x = x.clone(at::MemoryFormat::Contiguous);
+  return x;
+}
+int64_t distance_of(const at::Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+// A call over the logits' rows.
 struct Scored {
   at::Tensor x, targets, logprobs, entropy, top, top_ids, stats;
-  int64_t ld;
 };
 Scored run_logprobs(const at::Tensor& logits, const at::Tensor& targets, int64_t top_k, double temperature, int64_t vocab, int64_t ignore,
                     const at::Tensor& status, bool training) {
   const int64_t width = logits.size(-1), rows = targets.numel();
   Scored r;
-  r.x = logits.dim() == 2 ? logits : logits.reshape({rows, width});
-  if (r.x.stride(1) != 1 || (rows > 1 && r.x.stride(0) < width)) r.x = r.x.contiguous();
-  if (reinterpret_cast<uintptr_t>(r.x.data_ptr()) % 16 != 0) r.x = r.x.clone(at::MemoryFormat::Contiguous);
+  r.x = rows_of(logits, rows, width);
   r.targets = targets.contiguous();
-  r.ld = rows > 1 ? r.x.stride(0) : width;
   const auto f32 = at::TensorOptions(logits.device()).dtype(at::kFloat);
   r.logprobs = at::empty(targets.sizes(), f32);
   r.entropy = at::empty(targets.sizes(), f32);
@@ -272,7 +282,7 @@ Scored run_logprobs(const at::Tensor& logits, const at::Tensor& targets, int64_t
   a.entropy = r.entropy.data_ptr<float>();
   a.status = status.data_ptr<int>();
   a.rows = rows;
-  a.ld = r.ld;
+  a.ld = distance_of(r.x);
   a.ignore = ignore;
   a.vocab = static_cast<int>(vocab);
   a.width = static_cast<int>(width);
@@ -297,15 +307,17 @@ Scored run_logprobs(const at::Tensor& logits, const at::Tensor& targets, int64_t
 }
 
 struct LogprobsNode : TokenNode {
-  int64_t top_k, vocab, ignore, ld;
+  int64_t top_k, vocab, ignore;
   double inv_t;
   std::vector<int64_t> shape;
   std::string name() const override { return "CcfTokenLogprobsBackward"; }
   variable_list gradients(const variable_list& grads) override {
     variable_list out(1);
-    const at::Tensor x = kept(0), t = kept(1), stats = kept(2), top_ids = kept(3);
-    const c10::cuda::CUDAGuard guard(x.device());
-    const int64_t rows = x.size(0), width = x.size(1);
+    const at::Tensor saved_x = kept(0), t = kept_contiguous(1), stats = kept_contiguous(2), top_ids = kept_contiguous(3);
+    const c10::cuda::CUDAGuard guard(saved_x.device());
+    const int64_t rows = saved_x.size(0), width = saved_x.size(1);
+    const at::Tensor x = rows_of(saved_x, rows, width);
+    const int64_t ld = distance_of(x);
     at::Tensor g[3];
     bool any = false;
     for (int i = 0; i < static_cast<int>(grads.size()); ++i) {
@@ -367,7 +379,6 @@ variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& targets
     node->top_k = top_k;
     node->vocab = vocab;
     node->ignore = ignore;
-    node->ld = r.ld;
     node->inv_t = 1.0 / temperature;
     node->shape = logits.sizes().vec();
     torch::autograd::set_history(r.logprobs, node);
@@ -396,8 +407,10 @@ struct DropoutNode : TokenNode {
     if (!grads[0].defined()) return out;
     const c10::cuda::CUDAGuard guard(grads[0].device());
     out[1] = grads[0];
-    if (task_should_compute_output(0))
-      out[0] = run_dropout(packed(grads[0]), at::Tensor(), reinterpret_cast<const long long*>(kept(0).data_ptr<int64_t>()), nullptr, call, drop);
+    if (task_should_compute_output(0)) {
+      const at::Tensor used = kept_contiguous(0);
+      out[0] = run_dropout(packed(grads[0]), at::Tensor(), reinterpret_cast<const long long*>(used.data_ptr<int64_t>()), nullptr, call, drop);
+    }
     return out;
   }
 };

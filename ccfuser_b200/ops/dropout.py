@@ -44,7 +44,7 @@ class _DropoutFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         used, = ctx.saved_tensors
-        dx = _run(G.packed(dy), None, used, None, ctx.call, ctx.drop) if ctx.needs_input_grad[0] else None
+        dx = _run(G.packed(dy), None, used.contiguous(), None, ctx.call, ctx.drop) if ctx.needs_input_grad[0] else None
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
 
 

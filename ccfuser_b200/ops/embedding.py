@@ -77,7 +77,7 @@ class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        index, out, grads = ctx.saved_tensors, [None] * 8, []
+        index, out, grads = [None if i is None else i.contiguous() for i in ctx.saved_tensors], [None] * 8, []   # hooks may have other strides
         dy = G.packed(dy)
         e = N.Embed(tokens=index[0].numel(), seq=index[0].shape[-1] if index[0].dim() else 1, d=dy.shape[-1], type=N.DTYPE_CODE[dy.dtype])
         for k, at in enumerate((1, 2, 4)):

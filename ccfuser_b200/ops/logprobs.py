@@ -40,18 +40,21 @@ def _args(x, t, top_k, temperature, vocab, ignore, status):
                       type=N.DTYPE_CODE[x.dtype], inv_t=1.0 / temperature)
 
 
+def _rows_of(logits, rows, width):
+    """The logits as the kernels read them: rows with any distance, the first on a 16-byte boundary, their elements next to each other."""
+    x = logits.reshape(rows, width)
+    if x.stride(1) != 1 or (rows > 1 and x.stride(0) < width):
+        x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
+
+
 class _LogprobsFn(torch.autograd.Function):
     """The C++ function in Python."""
 
     @staticmethod
     def forward(ctx, logits, targets, top_k, temperature, vocab, ignore):
         rows, width = targets.numel(), logits.shape[-1]
-        x = logits.reshape(rows, width)
-        if x.stride(1) != 1 or (rows > 1 and x.stride(0) < width):
-            x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone(memory_format=torch.contiguous_format)
-        t = targets.contiguous()
+        x, t = _rows_of(logits, rows, width), targets.contiguous()
         f32 = dict(dtype=torch.float32, device=logits.device)
         lp, entropy, stats = torch.empty(targets.shape, **f32), torch.empty(targets.shape, **f32), torch.empty(rows, 3, **f32)
         a = _args(x, t, top_k, temperature, vocab, ignore, G.Workspace.status_of(x))
@@ -74,7 +77,8 @@ class _LogprobsFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        x, t, stats, ids = ctx.saved_tensors
+        x, t, stats, ids = ctx.saved_tensors       # hooks may have put them into memory of their own, with other strides
+        x, t, stats, ids = _rows_of(x, *x.shape), t.contiguous(), stats.contiguous(), None if ids is None else ids.contiguous()
         g = [None if v is None else v.contiguous() for v in grads[:3]] + [None]
         if all(v is None for v in g):
             return (None,) * 6
