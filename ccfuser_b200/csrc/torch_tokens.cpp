@@ -47,11 +47,15 @@ struct TokenNode : torch::autograd::Node {
     return t.defined() ? t.contiguous() : t;
   }
   variable_list apply(variable_list&& grads) final {
-    TORCH_CHECK(!at::GradMode::is_enabled(), "ccfuser_b200: this operator's gradient cannot be differentiated again (create_graph=True)");
+    const bool again = at::GradMode::is_enabled();   // the gradient is to be differentiated in its turn
+    TORCH_CHECK(!again || twice, "ccfuser_b200: this operator's gradient cannot be differentiated again (create_graph=True)");
     const std::lock_guard<std::mutex> lock(mutex_);
-    return gradients(grads);
+    return again ? torch_gradients(grads) : gradients(grads);
   }
   virtual variable_list gradients(const variable_list& grads) = 0;
+  // the same by operations of torch, which record a graph; for nodes with `twice`: those that models make
+  virtual variable_list torch_gradients(const variable_list&) { return {}; }
+  bool twice = false;
 };
 template <typename T, typename... Inputs>
 std::shared_ptr<T> make_node(const Inputs&... inputs) {
@@ -154,6 +158,23 @@ struct EmbeddingNode : TokenNode {
     if (e.tables > 0) run_grad(e, dy, status);
     return out;
   }
+  variable_list torch_gradients(const variable_list& grads) override {
+    variable_list out(3);
+    if (!grads[0].defined()) return out;
+    const at::Tensor index[3] = {kept(0), kept(1), kept(2)};
+    const int64_t tokens = index[0].numel(), seq = index[0].dim() > 0 ? index[0].size(-1) : 1;
+    const at::Tensor dy = grads[0].reshape({tokens, grads[0].size(-1)}).to(at::kFloat);
+    for (int k = 0; k < 3; ++k) {
+      if (rows[k] == 0 || !task_should_compute_output(k)) continue;
+      const at::Tensor ids =
+          index[k].defined() ? index[k].reshape({tokens}).to(at::kLong) : at::arange(tokens, index[0].options().dtype(at::kLong)).remainder(seq);
+      at::Tensor off = ids.lt(0).logical_or(ids.ge(rows[k]));   // adds nothing
+      if (k == 0) off = off.logical_or(ids.eq(skip));
+      const at::Tensor g = at::embedding_dense_backward(dy.masked_fill(off.unsqueeze(1), 0), ids.masked_fill(off, 0), rows[k], -1, false);
+      out[k] = g.mul(k == 0 ? scale : 1.0).to(grads[0].scalar_type());
+    }
+    return out;
+  }
 };
 
 void check_index(const char* name, const at::Tensor& ids, const at::Tensor& of) {
@@ -184,7 +205,7 @@ OptTensor spread(const OptTensor& t, const at::Tensor& ids) {
 }
 
 at::Tensor embedding(const at::Tensor& ids, const at::Tensor& weight, const OptTensor& position_, const OptTensor& position_ids_, const OptTensor& type_,
-                     const OptTensor& type_ids_, double scale, const std::optional<int64_t>& padding, const at::Tensor& status) {
+                     const OptTensor& type_ids_, double scale, const std::optional<int64_t>& padding, const at::Tensor& status, bool twice) {
   const at::Tensor &position = or_none(position_), &type = or_none(type_);
   TORCH_CHECK_VALUE(weight.dim() == 2, "weight: [rows, d], got ", weight.sizes());
   check_type(weight);
@@ -223,6 +244,7 @@ at::Tensor embedding(const at::Tensor& ids, const at::Tensor& weight, const OptT
     node->scale = scale;
     node->skip = skip;
     node->status = status;
+    node->twice = twice;
     torch::autograd::set_history(y, node);
   }
   return y;
@@ -313,10 +335,10 @@ struct LogprobsNode : TokenNode {
   std::string name() const override { return "CcfTokenLogprobsBackward"; }
   variable_list gradients(const variable_list& grads) override {
     variable_list out(1);
-    const at::Tensor saved_x = kept(0), t = kept_contiguous(1), stats = kept_contiguous(2), top_ids = kept_contiguous(3);
-    const c10::cuda::CUDAGuard guard(saved_x.device());
-    const int64_t rows = saved_x.size(0), width = saved_x.size(1);
-    const at::Tensor x = rows_of(saved_x, rows, width);
+    const at::Tensor logits = kept(0), t = kept_contiguous(1), stats = kept_contiguous(2), top_ids = kept_contiguous(3);
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const int64_t rows = t.numel(), width = shape.back();
+    const at::Tensor x = rows_of(logits, rows, width);
     const int64_t ld = distance_of(x);
     at::Tensor g[3];
     bool any = false;
@@ -352,10 +374,26 @@ struct LogprobsNode : TokenNode {
     out[0] = (dx_ld == width ? whole : whole.narrow(1, 0, width)).view(shape);
     return out;
   }
+  // of the log probabilities alone
+  variable_list torch_gradients(const variable_list& grads) override {
+    variable_list out(1);
+    TORCH_CHECK(top_k == 0 && !grads[1].defined(), "ccfuser_b200: only the gradient of the log probabilities can be differentiated again");
+    if (!grads[0].defined()) return out;
+    const at::Tensor logits = kept(0), t = kept(1).reshape({-1}).to(at::kLong);
+    const int64_t rows = t.numel(), width = shape.back();
+    const at::Tensor z = logits.reshape({rows, width}).narrow(1, 0, vocab).to(at::kFloat).mul(inv_t);
+    const at::Tensor none = z.detach().isneginf().all(1, true);
+    const at::Tensor p = at::softmax(z.masked_fill(none, 0), 1);
+    const at::Tensor off = t.eq(ignore).logical_or(t.lt(0)).logical_or(t.ge(vocab)).logical_or(none.squeeze(1));
+    const at::Tensor g = grads[0].reshape({rows}).masked_fill(off, 0).unsqueeze(1);
+    const at::Tensor d = p.mul(g.neg()).scatter_add(1, t.masked_fill(off, 0).unsqueeze(1), g).mul(inv_t);
+    out[0] = at::constant_pad_nd(d, {0, width - vocab}).to(logits.scalar_type()).reshape(shape);
+    return out;
+  }
 };
 
 variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& targets, int64_t top_k, double temperature,
-                             const std::optional<int64_t>& vocab_size, int64_t ignore, const at::Tensor& status) {
+                             const std::optional<int64_t>& vocab_size, int64_t ignore, const at::Tensor& status, bool twice) {
   TORCH_CHECK_VALUE(logits.dim() >= 1 && targets.sizes() == logits.sizes().slice(0, logits.dim() - 1), "targets: one per row of the logits, ",
                     logits.sizes(), ", got ", targets.sizes());
   check_type(logits);
@@ -375,7 +413,8 @@ variable_list token_logprobs(const at::Tensor& logits, const at::Tensor& targets
   }
   if (training) {
     const auto node = make_node<LogprobsNode>(logits);
-    for (const at::Tensor& t : {r.x, r.targets, r.stats, r.top_ids}) node->keep(t);
+    for (const at::Tensor& t : {twice ? logits : r.x, r.targets, r.stats, r.top_ids}) node->keep(t);   // r.x has no history
+    node->twice = twice;
     node->top_k = top_k;
     node->vocab = vocab;
     node->ignore = ignore;

@@ -410,6 +410,14 @@ def current_raw_stream(device_index: int) -> int:
     return torch.cuda.current_stream(device_index).cuda_stream
 
 
+def transformed() -> bool:
+    """Whether a transform of torch.func (vmap, grad, jvp) or a forward-mode derivative is under way, in which kernels take no part."""
+    return torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0
+
+
+REFUSED_TWICE = "ccfuser_b200: this operator's gradient cannot be differentiated again (create_graph=True)"
+
+
 def stream_ptr() -> int:
     """Handle of the current stream of the current device (0 without a GPU: host-side dry runs)."""
     global _gpu_seen

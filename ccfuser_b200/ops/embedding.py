@@ -19,7 +19,6 @@ from typing import Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from .. import native as N
 from . import gemm as G
@@ -55,7 +54,7 @@ class _EmbeddingFn(torch.autograd.Function):
     """The C++ function in Python."""
 
     @staticmethod
-    def forward(ctx, ids, weight, position, position_ids, types, type_ids, scale, skip):
+    def forward(ctx, ids, weight, position, position_ids, types, type_ids, scale, skip, twice):
         index = [None if t is None else t.contiguous() for t in (ids, position_ids, type_ids)]
         e = N.Embed(tokens=ids.numel(), seq=ids.shape[-1] if ids.dim() else 1, d=weight.shape[1], type=N.DTYPE_CODE[weight.dtype])
         held = []
@@ -71,13 +70,25 @@ class _EmbeddingFn(torch.autograd.Function):
         N.count(1)
         ctx.save_for_backward(*index)
         ctx.rows = [0 if w is None else w.shape[0] for w in (weight, position, types)]
-        ctx.scale, ctx.skip = scale, skip
+        ctx.scale, ctx.skip, ctx.twice = scale, skip, twice
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        index, out, grads = [None if i is None else i.contiguous() for i in ctx.saved_tensors], [None] * 8, []   # hooks may have other strides
+        index, out, grads = [None if i is None else i.contiguous() for i in ctx.saved_tensors], [None] * 9, []   # hooks may have other strides
+        if torch.is_grad_enabled():      # the gradient is to be differentiated in its turn: by operations of torch
+            if not ctx.twice:
+                raise RuntimeError(N.REFUSED_TWICE)
+            dy32 = dy.reshape(-1, dy.shape[-1]).float()
+            for k, at in enumerate((1, 2, 4)):
+                if not (ctx.rows[k] and ctx.needs_input_grad[at]):
+                    continue
+                seq = index[0].shape[-1] if index[0].dim() else 1
+                i = torch.arange(index[0].numel(), device=dy.device) % seq if index[k] is None else index[k].reshape(-1).long()
+                off = (i < 0) | (i >= ctx.rows[k]) | ((i == ctx.skip) if k == 0 else False)
+                g = torch.ops.aten.embedding_dense_backward(dy32.masked_fill(off[:, None], 0), i.masked_fill(off, 0), ctx.rows[k], -1, False)
+                out[at] = (g * (ctx.scale if k == 0 else 1.0)).to(dy.dtype)
+            return tuple(out)
         dy = G.packed(dy)
         e = N.Embed(tokens=index[0].numel(), seq=index[0].shape[-1] if index[0].dim() else 1, d=dy.shape[-1], type=N.DTYPE_CODE[dy.dtype])
         for k, at in enumerate((1, 2, 4)):
@@ -122,13 +133,13 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *, po
     return _embedding(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx)
 
 
-def _embedding(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx, plain=False):
-    """plain: by torch's operations on a GPU too."""
+def _embedding(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx, plain=False, twice=False):
+    """plain: by torch's operations on a GPU too. twice: the gradient can be differentiated again, then by torch's operations."""
     if weight.is_cuda and weight.numel() and ids.numel() and not plain:
         module = N.torch_module()
         if module is not None and not torch.jit.is_tracing():      # checks its arguments as below
             return module.embedding(ids, weight, position_weight, position_ids, type_weight, type_ids, scale, padding_idx,
-                                    G.Workspace.of(weight).status)
+                                    G.Workspace.of(weight).status, twice)
     if weight.dim() != 2:
         raise ValueError(f"weight: [rows, d], got {tuple(weight.shape)}")
     _check_ids("ids", ids, weight.device)
@@ -161,7 +172,7 @@ def _embedding(ids, weight, scale, position_weight, position_ids, type_weight, t
         raise ValueError(f"{ids.numel()} tokens: at most 2^26 in one call")
     if weight.shape[1] > MAX_COLUMNS or any(t is not None and t.shape[0] > MAX_ROWS for t in (weight, position_weight, type_weight)):
         raise ValueError("a table of at most 2^31 - 1 rows and 2^24 columns")
-    return _EmbeddingFn.apply(ids, weight, position_weight, position_ids, type_weight, type_ids, float(scale), skip)
+    return _EmbeddingFn.apply(ids, weight, position_weight, position_ids, type_weight, type_ids, float(scale), skip, twice)
 
 
 def _embedding_torch(ids, weight, scale, position_weight, position_ids, type_weight, type_ids, padding_idx):
@@ -212,7 +223,8 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
 
 class Embedding(nn.Embedding):
     """``nn.Embedding`` (same parameters, same state-dict keys) on ``embedding``, with a factor ``scale`` and the other tables as arguments of its call.
-    What the kernels do not take (fp64 tables, more than 2^26 tokens, 2^31 - 1 rows or 2^24 columns) runs on torch's operations.
+    What the kernels do not take (fp64 tables, more than 2^26 tokens, 2^31 - 1 rows or 2^24 columns, transforms of torch.func, derivatives in
+    forward mode, second derivatives) runs on torch's operations.
     ``max_norm``, ``scale_grad_by_freq`` and ``sparse`` are refused."""
 
     def __init__(self, *args, scale: float = 1.0, **kw):
@@ -224,5 +236,5 @@ class Embedding(nn.Embedding):
     def forward(self, ids, position_weight=None, position_ids=None, type_weight=None, type_ids=None):
         w = self.weight
         rows = max(t.shape[0] for t in (w, position_weight, type_weight) if t is not None)
-        plain = w.dtype not in N.DTYPE_CODE or ids.numel() > MAX_TOKENS or rows > MAX_ROWS or w.shape[1] > MAX_COLUMNS
-        return _embedding(ids, w, self.scale, position_weight, position_ids, type_weight, type_ids, self.padding_idx, plain)
+        plain = N.transformed() or w.dtype not in N.DTYPE_CODE or ids.numel() > MAX_TOKENS or rows > MAX_ROWS or w.shape[1] > MAX_COLUMNS
+        return _embedding(ids, w, self.scale, position_weight, position_ids, type_weight, type_ids, self.padding_idx, plain, True)

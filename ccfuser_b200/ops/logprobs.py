@@ -15,7 +15,6 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import native as N
 from . import gemm as G
@@ -52,7 +51,7 @@ class _LogprobsFn(torch.autograd.Function):
     """The C++ function in Python."""
 
     @staticmethod
-    def forward(ctx, logits, targets, top_k, temperature, vocab, ignore):
+    def forward(ctx, logits, targets, top_k, temperature, vocab, ignore, twice):
         rows, width = targets.numel(), logits.shape[-1]
         x, t = _rows_of(logits, rows, width), targets.contiguous()
         f32 = dict(dtype=torch.float32, device=logits.device)
@@ -66,8 +65,8 @@ class _LogprobsFn(torch.autograd.Function):
         with torch.cuda.device(logits.device):
             N.check(N.load().ccf_logprobs_fwd(C.byref(a), N.stream_ptr()), "ccf_logprobs_fwd")
         N.count(1)
-        ctx.save_for_backward(x, t, stats, ids)
-        ctx.args, ctx.shape = (top_k, temperature, vocab, ignore), logits.shape
+        ctx.save_for_backward(logits if twice else x, t, stats, ids)      # x has no history
+        ctx.args, ctx.shape, ctx.twice = (top_k, temperature, vocab, ignore), logits.shape, twice
         ctx.set_materialize_grads(False)
         if not top_k:
             return lp, entropy
@@ -75,13 +74,17 @@ class _LogprobsFn(torch.autograd.Function):
         return lp, entropy, top, ids
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):
         x, t, stats, ids = ctx.saved_tensors       # hooks may have put them into memory of their own, with other strides
-        x, t, stats, ids = _rows_of(x, *x.shape), t.contiguous(), stats.contiguous(), None if ids is None else ids.contiguous()
+        if torch.is_grad_enabled():      # the gradient is to be differentiated in its turn: by operations of torch
+            if not ctx.twice or ids is not None or grads[1] is not None:
+                raise RuntimeError(N.REFUSED_TWICE)
+            return (None if grads[0] is None else _grad_torch(x, t, grads[0], *ctx.args[1:]),) + (None,) * 6
+        x = _rows_of(x, t.numel(), x.shape[-1])
+        t, stats, ids = t.contiguous(), stats.contiguous(), None if ids is None else ids.contiguous()
         g = [None if v is None else v.contiguous() for v in grads[:3]] + [None]
         if all(v is None for v in g):
-            return (None,) * 6
+            return (None,) * 7
         a = _args(x, t, *ctx.args, 0)
         a.dx_ld = a.width + (a.ld - a.width) % (16 // x.element_size())       # rows begin where those of the logits do in their 16 bytes
         whole = torch.empty(x.shape[0], a.dx_ld, dtype=x.dtype, device=x.device)
@@ -90,7 +93,19 @@ class _LogprobsFn(torch.autograd.Function):
         with torch.cuda.device(x.device):
             N.check(N.load().ccf_logprobs_bwd(C.byref(a), N.stream_ptr()), "ccf_logprobs_bwd")
         N.count(1)
-        return (whole[:, :x.shape[1]].view(ctx.shape),) + (None,) * 5
+        return (whole[:, :x.shape[1]].view(ctx.shape),) + (None,) * 6
+
+
+def _grad_torch(logits, targets, g, temperature, vocab, ignore):
+    """The gradient of the log probabilities with respect to the logits."""
+    z = logits[..., :vocab].float() / temperature
+    none = (z.detach() == -math.inf).all(dim=-1, keepdim=True)
+    p = torch.softmax(z.masked_fill(none, 0.0), dim=-1)
+    t = targets.long()
+    off = (t == ignore) | (t < 0) | (t >= vocab) | none[..., 0]
+    g = g.masked_fill(off, 0.0)[..., None]
+    d = (p * -g).scatter_add(-1, t.masked_fill(off, 0)[..., None], g) / temperature
+    return torch.nn.functional.pad(d, (0, logits.shape[-1] - vocab)).to(logits.dtype)
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, temperature: float = 1.0, vocab_size: Optional[int] = None,
@@ -102,11 +117,27 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     no gradient from their log probability. Alternatives come by value, equal ones by index; ``top_k`` is at most 32 and the vocabulary. A column at -inf has
     no probability: where fewer than ``top_k`` others are left, the id is -1 and the log probability -inf. A row without a finite logit gives -inf, entropy 0
     and a zero gradient; a row with NaN or +inf gives NaN. Log probabilities, entropy and the alternatives' log probabilities are differentiable, once."""
+    return _token_logprobs(logits, targets, top_k, temperature, vocab_size, ignore_index, False)
+
+
+def _token_logprobs(logits, targets, top_k, temperature, vocab_size, ignore_index, twice):
+    """twice: the gradient of the log probabilities can be differentiated again, then by torch's operations."""
     if logits.is_cuda and logits.dtype in N.DTYPE_CODE and targets.numel():
         module = N.torch_module()
         if module is not None and not torch.jit.is_tracing():      # checks its arguments as below
-            out = module.token_logprobs(logits, targets, top_k, temperature, vocab_size, ignore_index, G.Workspace.of(logits).status)
+            out = module.token_logprobs(logits, targets, top_k, temperature, vocab_size, ignore_index, G.Workspace.of(logits).status, twice)
             return TokenLogprobs(*out) if top_k else TokenLogprobs(out[0], out[1], None, None)
+    vocab = _check(logits, targets, top_k, temperature, vocab_size)
+    if not (logits.is_cuda and logits.dtype in N.DTYPE_CODE and targets.numel() > 0):
+        return _logprobs_torch(logits, targets, top_k, temperature, vocab, ignore_index)
+    if logits.shape[-1] > MAX_WIDTH or targets.numel() > MAX_ROWS:
+        raise ValueError("at most 2^30 columns and 2^28 - 1 rows in one call")
+    out = _LogprobsFn.apply(logits, targets, top_k, float(temperature), vocab, ignore_index, twice)
+    return TokenLogprobs(out[0], out[1], *(out[2:] if top_k else (None, None)))
+
+
+def _check(logits, targets, top_k, temperature, vocab_size):
+    """The number of columns that count."""
     if logits.dim() < 1 or targets.shape != logits.shape[:-1]:
         raise ValueError(f"targets: one per row of the logits, {tuple(logits.shape[:-1])}, got {tuple(targets.shape)}")
     if targets.dtype not in (torch.int64, torch.int32):
@@ -121,36 +152,56 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
         raise ValueError(f"top_k: 0 to {min(MAX_TOP, vocab)}, got {top_k}")
     if not 1e-37 <= temperature <= 1e37:       # it and its inverse are normal in fp32
         raise ValueError(f"temperature: a positive number that fp32 holds, got {temperature}")
-    if not (logits.is_cuda and logits.dtype in N.DTYPE_CODE and targets.numel() > 0):
-        return _logprobs_torch(logits, targets, top_k, temperature, vocab, ignore_index)
-    if width > MAX_WIDTH or targets.numel() > MAX_ROWS:
-        raise ValueError("at most 2^30 columns and 2^28 - 1 rows in one call")
-    out = _LogprobsFn.apply(logits, targets, top_k, float(temperature), vocab, ignore_index)
-    return TokenLogprobs(out[0], out[1], *(out[2:] if top_k else (None, None)))
+    return vocab
 
 
 def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, vocab_size: Optional[int] = None, ignore_index: int = -100) -> torch.Tensor:
-    """Mean of ``-token_logprobs`` over the targets that are not ignored: ``F.cross_entropy`` of the first ``vocab_size`` columns in fp32."""
-    lp = token_logprobs(logits, targets, vocab_size=vocab_size, ignore_index=ignore_index).logprobs
+    """Mean of ``-token_logprobs`` over the targets that are not ignored: ``F.cross_entropy`` of the first ``vocab_size`` columns in fp32. What the
+    kernels do not take (fp64 logits, more than 2^28 - 1 rows or 2^30 columns, transforms of torch.func, derivatives in forward mode, second derivatives)
+    runs on torch's operations."""
+    if N.transformed() or logits.dtype not in N.DTYPE_CODE or not logits.is_cuda or targets.numel() > MAX_ROWS or logits.shape[-1] > MAX_WIDTH:
+        vocab = _check(logits, targets, 0, 1.0, vocab_size)
+        lp = _picked(_log_softmax(logits, 1.0, vocab)[1], targets, vocab, ignore_index)
+    else:
+        lp = _token_logprobs(logits, targets, 0, 1.0, vocab_size, ignore_index, True).logprobs
     return -lp.sum() / (targets != ignore_index).sum()
 
 
-def _logprobs_torch(logits, targets, top_k, temperature, vocab, ignore):
+def _log_softmax(logits, temperature, vocab):
     x = logits[..., :vocab]
     x = x if x.dtype == torch.float64 else x.float()
-    none = (x == -math.inf).all(dim=-1, keepdim=True)
-    # a row without a finite logit gets zeros in its place, which give it no gradient. The largest is taken off before the division, which may pass the type's range
     largest = x.detach().amax(dim=-1, keepdim=True)
-    lp = torch.log_softmax(torch.where(none, torch.zeros_like(x), (x - largest) / temperature), dim=-1)
-    lp = torch.where(none, torch.full_like(lp, -math.inf), lp)
+    z = x if temperature == 1.0 else (x - largest) / temperature      # without the largest: the quotient may pass the type's range
+    none = largest == -math.inf
+    if _host_may_look(x) and not bool(none.any()):
+        return x, torch.log_softmax(z, dim=-1)
+    # a row without a finite logit gets zeros in its place, which give it no gradient
+    lp = torch.log_softmax(torch.where(none, torch.zeros_like(x), z), dim=-1)
+    return x, torch.where(none, torch.full_like(lp, -math.inf), lp)
+
+
+def _host_may_look(t):
+    """Not in transforms and captures."""
+    return not N.transformed() and not (t.is_cuda and torch.cuda.is_current_stream_capturing())
+
+
+def _picked(lp, targets, vocab, ignore):
+    """The targets' log probabilities. One outside the vocabulary raises, or gives NaN where the host may not look."""
+    kept = targets != ignore
+    outside = kept & ((targets < 0) | (targets >= vocab))
+    if _host_may_look(lp) and bool(outside.any()):
+        raise IndexError(f"a target lies outside the vocabulary of {vocab}")
+    at = torch.where(kept & ~outside, targets, torch.zeros_like(targets)).long()
+    picked = lp.gather(-1, at[..., None])[..., 0]
+    picked = torch.where(outside, torch.full_like(picked, math.nan), picked)
+    return torch.where(kept, picked, torch.zeros_like(picked))
+
+
+def _logprobs_torch(logits, targets, top_k, temperature, vocab, ignore):
+    x, lp = _log_softmax(logits, temperature, vocab)
     gone = lp == -math.inf
     entropy = -torch.where(gone, torch.zeros_like(lp), lp.exp() * torch.where(gone, torch.zeros_like(lp), lp)).sum(dim=-1)
-    kept = targets != ignore
-    if bool(((targets < 0) | (targets >= vocab))[kept].any()):
-        raise IndexError(f"a target lies outside the vocabulary of {vocab}")
-    at = torch.where(kept, targets, torch.zeros_like(targets)).long()
-    picked = lp.gather(-1, at[..., None])[..., 0]
-    picked = torch.where(kept, picked, torch.zeros_like(picked))
+    picked = _picked(lp, targets, vocab, ignore)
     if not top_k:
         return TokenLogprobs(picked, entropy, None, None)
     ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k]
