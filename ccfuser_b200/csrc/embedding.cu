@@ -694,7 +694,8 @@ template <int kType, bool kVec>
 static int launch_fwd(const CcfEmbed& e, void* y, int* status, cudaStream_t st) {
   const uint32_t slices = (e.d + Slice<kType, kVec>::kCols - 1) / Slice<kType, kVec>::kCols;
   uint32_t each = kFwdTokens;
-  while (each > 1 && (e.tokens + each - 1) / each * slices < 16 * 148) each /= 2;   // 16 warps an SM at least, while there are that many
+  const int least = 16 * sm_count();
+  while (each > 1 && (e.tokens + each - 1) / each * slices < least) each /= 2;   // 16 warps an SM at least, while there are that many
   const long long units = (e.tokens + each - 1) / each * slices, blocks = (units + kEmbWarps - 1) / kEmbWarps;
   if (units > 0xffffff00ll || blocks > 0x7fffffffll) return -2;
   const auto kern = e.tables == 1 ? embedding_fwd_kernel<kType, kVec, 1> : e.tables == 2 ? embedding_fwd_kernel<kType, kVec, 2>
