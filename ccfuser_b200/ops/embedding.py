@@ -235,6 +235,6 @@ class Embedding(nn.Embedding):
 
     def forward(self, ids, position_weight=None, position_ids=None, type_weight=None, type_ids=None):
         w = self.weight
-        rows = max(t.shape[0] for t in (w, position_weight, type_weight) if t is not None)
-        plain = N.transformed() or w.dtype not in N.DTYPE_CODE or ids.numel() > MAX_TOKENS or rows > MAX_ROWS or w.shape[1] > MAX_COLUMNS
+        plain = (N.transformed() or w.dtype not in N.DTYPE_CODE or ids.numel() > MAX_TOKENS or w.shape[1] > MAX_COLUMNS or w.shape[0] > MAX_ROWS
+                 or (position_weight is not None and position_weight.shape[0] > MAX_ROWS) or (type_weight is not None and type_weight.shape[0] > MAX_ROWS))
         return _embedding(ids, w, self.scale, position_weight, position_ids, type_weight, type_ids, self.padding_idx, plain, True)
