@@ -410,9 +410,14 @@ def current_raw_stream(device_index: int) -> int:
     return torch.cuda.current_stream(device_index).cuda_stream
 
 
-def transformed() -> bool:
-    """Whether a transform of torch.func (vmap, grad, jvp) or a forward-mode derivative is under way, in which kernels take no part."""
-    return torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0
+_NO_DISPATCH = torch.Tensor.__torch_dispatch__
+
+
+def transformed(t: torch.Tensor) -> bool:
+    """Whether operations on ``t`` are more than work on memory, so that kernels take no part in them: torch.compile and torch.export, transforms of torch.func
+    (vmap, grad, jvp), derivatives in forward mode, dispatch modes and tensors of their own kind (fake ones)."""
+    return (torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active() or torch.autograd.forward_ad._current_level >= 0
+            or torch._C._len_torch_dispatch_stack() > 0 or type(t).__torch_dispatch__ is not _NO_DISPATCH)
 
 
 REFUSED_TWICE = "ccfuser_b200: this operator's gradient cannot be differentiated again (create_graph=True)"

@@ -223,8 +223,8 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
 
 class Embedding(nn.Embedding):
     """``nn.Embedding`` (same parameters, same state-dict keys) on ``embedding``, with a factor ``scale`` and the other tables as arguments of its call.
-    What the kernels do not take (fp64 tables, more than 2^26 tokens, 2^31 - 1 rows or 2^24 columns, transforms of torch.func, derivatives in
-    forward mode, second derivatives) runs on torch's operations.
+    What the kernels do not take (fp64 tables, more than 2^26 tokens, 2^31 - 1 rows or 2^24 columns, ``native.transformed`` ones, second
+    derivatives) runs on torch's operations.
     ``max_norm``, ``scale_grad_by_freq`` and ``sparse`` are refused."""
 
     def __init__(self, *args, scale: float = 1.0, **kw):
@@ -235,6 +235,6 @@ class Embedding(nn.Embedding):
 
     def forward(self, ids, position_weight=None, position_ids=None, type_weight=None, type_ids=None):
         w = self.weight
-        plain = (N.transformed() or w.dtype not in N.DTYPE_CODE or ids.numel() > MAX_TOKENS or w.shape[1] > MAX_COLUMNS or w.shape[0] > MAX_ROWS
+        plain = (N.transformed(w) or w.dtype not in N.DTYPE_CODE or ids.numel() > MAX_TOKENS or w.shape[1] > MAX_COLUMNS or w.shape[0] > MAX_ROWS
                  or (position_weight is not None and position_weight.shape[0] > MAX_ROWS) or (type_weight is not None and type_weight.shape[0] > MAX_ROWS))
         return _embedding(ids, w, self.scale, position_weight, position_ids, type_weight, type_ids, self.padding_idx, plain, True)

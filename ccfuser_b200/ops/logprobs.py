@@ -157,9 +157,8 @@ def _check(logits, targets, top_k, temperature, vocab_size):
 
 def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, vocab_size: Optional[int] = None, ignore_index: int = -100) -> torch.Tensor:
     """Mean of ``-token_logprobs`` over the targets that are not ignored: ``F.cross_entropy`` of the first ``vocab_size`` columns in fp32. What the
-    kernels do not take (fp64 logits, more than 2^28 - 1 rows or 2^30 columns, transforms of torch.func, derivatives in forward mode, second derivatives)
-    runs on torch's operations."""
-    if N.transformed() or logits.dtype not in N.DTYPE_CODE or not logits.is_cuda or targets.numel() > MAX_ROWS or logits.shape[-1] > MAX_WIDTH:
+    kernels do not take (fp64 logits, more than 2^28 - 1 rows or 2^30 columns, ``native.transformed`` ones, second derivatives) runs on torch's operations."""
+    if N.transformed(logits) or logits.dtype not in N.DTYPE_CODE or not logits.is_cuda or targets.numel() > MAX_ROWS or logits.shape[-1] > MAX_WIDTH:
         vocab = _check(logits, targets, 0, 1.0, vocab_size)
         lp = _picked(_log_softmax(logits, 1.0, vocab)[1], targets, vocab, ignore_index)
     else:
@@ -181,8 +180,8 @@ def _log_softmax(logits, temperature, vocab):
 
 
 def _host_may_look(t):
-    """Not in transforms and captures."""
-    return not N.transformed() and not (t.is_cuda and torch.cuda.is_current_stream_capturing())
+    """Not where there is no memory to look at, and not in captures."""
+    return not N.transformed(t) and t.device.type != "meta" and not (t.is_cuda and torch.cuda.is_current_stream_capturing())
 
 
 def _picked(lp, targets, vocab, ignore):

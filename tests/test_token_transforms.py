@@ -117,3 +117,67 @@ def test_what_counts_for_nothing_counts_for_nothing_again(monkeypatch, function)
     for b, c in zip(second, want2):
         torch.testing.assert_close(b.double(), c, rtol=2.0 ** -16, atol=2.0 ** -24 * 256)
     assert not bool(first[0][3].any())
+
+
+def _small(name, device):
+    m, x, y, _ = _model(name, torch.float32, device)
+    return m, x, y
+
+
+@pytest.mark.parametrize("name", ["gpt", "txl"])
+@pytest.mark.parametrize("device", ["meta", *DEVICES])
+def test_without_memory(name, device):
+    """Shapes alone: the meta device and fake tensors, forward and backward."""
+    import contextlib
+
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from ccfuser_b200.models.gpt_moe import GPTMoE, GPTMoEConfig
+    from ccfuser_b200.models.transformer_xl_moe import TransformerXLMoE, TransformerXLMoEConfig
+    with contextlib.nullcontext() if device == "meta" else FakeTensorMode():      # where a module cannot be moved
+        if name == "gpt":
+            m = GPTMoE(GPTMoEConfig(vocab_size=50, n_layer=1, n_head=2, d_model=32, d_ffn=64, seq_len=8, moe_every=0, dtype=torch.float32), device=device)
+        else:
+            m = TransformerXLMoE(TransformerXLMoEConfig(n_token=50, n_layer=1, n_head=2, d_model=32, d_head=16, d_inner=64, tgt_len=8, mem_len=8, moe=False,
+                                                        dtype=torch.float32), device=device)
+        x = torch.zeros(4, 8, dtype=torch.long, device=device)
+        loss = _loss(m, x, x)
+        loss.backward()
+    assert loss.shape == () and loss.device.type == device
+    assert all(p.grad is not None and p.grad.shape == p.shape for p in m.parameters())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("how", ["compile", "export", "make_fx"])
+def test_graphs_of_a_whole_model(how, device):
+    """One graph of a step's loss, which gives on other inputs what the model gives."""
+    m, x, y = _small("gpt", device)
+    u, v = y.clamp_min(0), x.roll(1, 1)
+    with torch.no_grad():
+        if how == "compile":
+            f = torch.compile(m, backend="eager", fullgraph=True)
+            f(x, y)
+        elif how == "export":
+            f = torch.export.export(m, (x, y)).module()
+        else:
+            from torch.fx.experimental.proxy_tensor import make_fx
+            f = make_fx(lambda a, b: m(a, b), tracing_mode="real")(x, y)
+        want = m(u, v)
+        assert abs(float(f(u, v)) - float(want)) <= TOL * float(want)
+
+
+@pytest.mark.gpu
+def test_kernels_serve_what_is_not_transformed():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from ccfuser_b200 import native as N
+    from ccfuser_b200.ops.logprobs import cross_entropy
+    m, x, _ = _small("gpt", "cuda")
+    before = N.LAUNCHES[0]
+    y = m.wte(x, position_weight=m.wpe.weight)
+    loss = cross_entropy(y, x % 32)
+    assert y.grad_fn.name() == "CcfEmbeddingBackward" and N.LAUNCHES[0] == before + 2
+    loss.backward()
+    assert m.wte.weight.grad is not None
+    with FakeTensorMode(), pytest.raises(Exception):
+        torch.zeros(3, device="cuda").tolist()
+    assert not N.transformed(m.wte.weight) and not N.transformed(y)
