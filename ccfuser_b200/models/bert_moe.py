@@ -17,7 +17,7 @@ import torch.nn.functional as F
 
 from ..config import MoEConfig
 from ..layers import MoELayer
-from ..ops.embedding import Embedding
+from ..ops.embedding import Embedding, look_up
 from ..ops.norm import LayerNorm
 
 
@@ -121,7 +121,7 @@ class BertMoEForQuestionAnswering(nn.Module):
         tt = token_type_ids if token_type_ids is not None else torch.zeros_like(input_ids)
         if tt.shape != input_ids.shape:
             input_ids, tt = torch.broadcast_tensors(input_ids, tt)
-        x = self.ln_emb(self.word(input_ids, position_weight=self.position.weight, type_weight=self.token_type.weight, type_ids=tt))
+        x = self.ln_emb(look_up(self.word, input_ids, position=self.position, types=self.token_type, type_ids=tt))
         mask = token_mask = None
         if attention_mask is not None:
             mask = attention_mask[:, None, None, :].to(torch.bool)

@@ -18,7 +18,7 @@ import torch.nn.functional as F
 
 from ..config import MoEConfig
 from ..layers import MoELayer
-from ..ops.embedding import Embedding
+from ..ops.embedding import Embedding, look_up
 from ..ops.logprobs import TokenLogprobs, cross_entropy, token_logprobs
 from ..ops.norm import LayerNorm
 
@@ -160,7 +160,7 @@ class GPTMoE(nn.Module):
                 nn.init.zeros_(m.bias)
 
     def _logits(self, ids):
-        x = self.wte(ids, position_weight=self.wpe.weight)
+        x = look_up(self.wte, ids, position=self.wpe)
         for blk in self.h:
             x = blk(x)
         return F.linear(self.ln_f(x), self.wte.weight)

@@ -23,7 +23,7 @@ import torch.nn.functional as F
 from ..config import MoEConfig
 from ..layers import MoELayer
 from ..ops.dropout import Dropout, DropoutState
-from ..ops.embedding import Embedding
+from ..ops.embedding import Embedding, look_up
 from ..ops.logprobs import cross_entropy
 from ..ops.norm import LayerNorm
 
@@ -153,7 +153,8 @@ class TransformerXLMoE(nn.Module):
     def __init__(self, c: TransformerXLMoEConfig, ep_group=None, device=None):
         super().__init__()
         self.config = c
-        self.word_emb = Embedding(c.n_token, c.d_model, scale=c.d_model ** 0.5, device=device, dtype=c.dtype)
+        self.word_emb = Embedding(c.n_token, c.d_model, device=device, dtype=c.dtype)
+        self.emb_scale = c.d_model ** 0.5
         self.pos_emb = PositionalEmbedding(c.d_model, device)
         self.r_w_bias = nn.Parameter(torch.zeros(c.n_head, c.d_head, device=device, dtype=c.dtype))
         self.r_r_bias = nn.Parameter(torch.zeros(c.n_head, c.d_head, device=device, dtype=c.dtype))
@@ -198,7 +199,7 @@ class TransformerXLMoE(nn.Module):
             mems = self.init_mems(b, data.device)
         m_len = mems[0].shape[1] if mems is not None else 0
         k_len = m_len + q
-        x = self.word_emb(data)
+        x = look_up(self.word_emb, data, self.emb_scale)
         if self.drop is not None:
             if self.training:
                 self.drop.state.begin_step(data.device)
@@ -220,15 +221,6 @@ class TransformerXLMoE(nn.Module):
         else:
             loss = cross_entropy(F.linear(x, self.word_emb.weight), target.reshape(x.shape[:-1]))
         return loss, new_mems
-
-    @property
-    def emb_scale(self):
-        """Factor of the word embedding."""
-        return self.word_emb.scale
-
-    @emb_scale.setter
-    def emb_scale(self, scale):
-        self.word_emb.scale = scale
 
     def moe_layers(self):
         return [l.pos_ff for l in self.layers if l.is_moe]

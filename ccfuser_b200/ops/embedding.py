@@ -233,8 +233,28 @@ class Embedding(nn.Embedding):
             raise ValueError("max_norm, scale_grad_by_freq and sparse are not supported")
         self.scale = scale
 
-    def forward(self, ids, position_weight=None, position_ids=None, type_weight=None, type_ids=None):
+    def forward(self, ids, position_weight=None, position_ids=None, type_weight=None, type_ids=None, scale: float = 1.0):
+        """``scale`` multiplies the module's own."""
         w = self.weight
         plain = (N.transformed(w) or w.dtype not in N.DTYPE_CODE or ids.numel() > MAX_TOKENS or w.shape[1] > MAX_COLUMNS or w.shape[0] > MAX_ROWS
                  or (position_weight is not None and position_weight.shape[0] > MAX_ROWS) or (type_weight is not None and type_weight.shape[0] > MAX_ROWS))
-        return _embedding(ids, w, self.scale, position_weight, position_ids, type_weight, type_ids, self.padding_idx, plain, True)
+        return _embedding(ids, w, self.scale * scale, position_weight, position_ids, type_weight, type_ids, self.padding_idx, plain, True)
+
+
+def _untouched(m):
+    return type(m) is Embedding and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
+def look_up(word: nn.Module, ids: torch.Tensor, scale: float = 1.0, position: Optional[nn.Module] = None, types: Optional[nn.Module] = None,
+            type_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The sum of what a model's embedding modules give for tokens, their places and their types: one pass over their tables where all of them are ``Embedding``; module
+    after module where one has been replaced (another vocabulary, an adapter) or carries hooks."""
+    others = [m for m in (position, types) if m is not None]
+    if _untouched(word) and all(_untouched(m) and m.scale == 1.0 and m.padding_idx is None for m in others):
+        return word(ids, None if position is None else position.weight, None, None if types is None else types.weight, type_ids, scale)
+    x = word(ids)
+    if scale != 1.0:
+        x = x * scale
+    if position is not None:
+        x = x + position(torch.arange(ids.shape[-1], device=ids.device))
+    return x if types is None else x + types(type_ids)

@@ -39,3 +39,61 @@ def test_the_embedding_factor_of_transformer_xl():
     m.emb_scale = 2.0
     m(ids)
     torch.testing.assert_close(seen[0], F.embedding(ids, m.word_emb.weight) * 2.0)
+
+
+class _Adapter(torch.nn.Module):
+    """A low-rank addition to a table, which keeps the table's name for its weight."""
+
+    def __init__(self, base):
+        super().__init__()
+        self.base = base
+        self.a, self.b = torch.nn.Parameter(torch.randn(base.num_embeddings, 2)), torch.nn.Parameter(torch.randn(2, base.embedding_dim))
+
+    @property
+    def weight(self):
+        return self.base.weight
+
+    def forward(self, ids):
+        return self.base(ids) + F.embedding(ids, self.a) @ self.b
+
+
+def _tables(name):
+    """A model, the call that runs it, its embedding modules and what the sum of their outputs goes through."""
+    torch.manual_seed(0)
+    ids, tt = torch.randint(0, 40, (2, 8)), torch.randint(0, 2, (2, 8))
+    if name == "gpt":
+        m = _gpt()
+        return m, lambda: m(ids), {"wte": ids, "wpe": torch.arange(8)}, m.h[0], 1.0
+    if name == "bert":
+        m = BertMoEForQuestionAnswering(BertMoEConfig(vocab_size=60, n_layer=1, n_head=2, d_model=32, d_ffn=64, max_position=20, moe_layers=(),
+                                                      dtype=torch.float32))
+        return m, lambda: m(ids, None, tt), {"word": ids, "position": torch.arange(8), "token_type": tt}, m.ln_emb, 1.0
+    m = _txl()
+    return m, lambda: m(ids), {"word_emb": ids}, m.layers[0], 32 ** 0.5
+
+
+@pytest.mark.parametrize("name,table", [("gpt", "wte"), ("gpt", "wpe"), ("bert", "word"), ("bert", "position"), ("bert", "token_type"), ("txl", "word_emb")])
+@pytest.mark.parametrize("change", ["replaced", "adapter", "hook", "pre_hook"])
+def test_replaced_and_hooked_tables(name, table, change):
+    """An embedding module is what it does when called: another module, an adapter around it or a hook counts as it did."""
+    m, call, places, first, scale = _tables(name)
+    calls = []
+    if change == "replaced":
+        old = getattr(m, table)
+        setattr(m, table, torch.nn.Embedding(old.num_embeddings, old.embedding_dim))
+    elif change == "adapter":
+        setattr(m, table, _Adapter(getattr(m, table)))
+    elif change == "hook":
+        getattr(m, table).register_forward_hook(lambda mod, args, out: calls.append(1) or out * 3.0)
+    else:
+        getattr(m, table).register_forward_pre_hook(lambda mod, args: calls.append(1))
+    want = 0.0
+    for i, (n, at) in enumerate(places.items()):
+        part = getattr(m, n)(at)
+        want = want + (part * scale if i == 0 else part)
+    del calls[:]
+    seen = []
+    first.register_forward_pre_hook(lambda mod, args: seen.append(args[0]))
+    call()
+    torch.testing.assert_close(seen[0], want)
+    assert len(calls) == ("hook" in change)
