@@ -251,7 +251,8 @@ __device__ __forceinline__ uint32_t group_maxima(RowShared<kThreads>& sh, float 
 // The k largest elements of this block's share of a row, in order, into sh.top. The largest elements of groups of threads are elements themselves: the k-th
 // largest of those bounds the k-th largest element from below. Only threads whose own largest element reaches the bound look at elements again (a few more than
 // k), for most of them those of the one turn that held it, an element a lane; and only elements that reach the bound are listed. Should they
-// not fit the list (many equal elements), they are taken one after the other instead, each the largest below the one before.
+// not fit the list (many equal elements), they are taken one after the other instead, each the largest below the one before: 4 rows of 50257 with five columns above
+// the type's lowest value and twenty alternatives 113 us, not 10.
 template <int kType, int kThreads>
 __device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_t* p, const RowShape<kType>& shape, int first, int last,
                                            const Running<kType, true>& run, uint32_t largest, float edge, int edge_index, int k) {
@@ -346,7 +347,7 @@ __device__ __forceinline__ void select_top(RowShared<kThreads>& sh, const uint8_
 
 // kThreads per row; a warp per row, eight rows a block, where rows are short. Rows of wide vocabularies may be shared by a cluster of 2^log_split blocks,
 // each with its part of the columns, whose statistics and alternatives the first one joins: a few rows would leave most of the card idle.
-// 8192 rows of 50257 bf16 131 us (6.3 TB/s), 4099 with five alternatives 84 (4.9 TB/s: choosing them takes a tenth more instructions), 4 rows with twenty 10.
+// 8192 rows of 50257 bf16 133 us (6.2 TB/s), 4099 with five alternatives 84 (4.9 TB/s: choosing them takes a quarter more instructions), 4 rows with twenty 10.
 // Bound by the memory in the first, by the arithmetic's latency in the second (55 % of the issue slots). Rows by bulk copies into shared memory, over the ends
 // of rows, took 167 to 230 us: what their buffers leave room for is too few warps.
 template <int kType, int kThreads, bool kTop>
@@ -505,7 +506,7 @@ __device__ __forceinline__ RowGrad row_grad(const CcfLogprobs& a, long long row,
 }
 
 // kThreads per row and part of its columns (blockIdx.y of gridDim.y), a warp per row where rows are short. Bound by reading the logits and writing
-// the gradient once: 8192 rows of 50304 bf16 254 us, 6.5 TB/s.
+// the gradient once: 8192 rows of 50304 bf16 258 us, 6.4 TB/s.
 template <int kType, int kThreads>
 __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) logprobs_bwd_kernel(const __grid_constant__ CcfLogprobs a) {
   constexpr int kE = kElemsPer16<kType>;
