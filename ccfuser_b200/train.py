@@ -53,13 +53,11 @@ class TrainStep:
             raise ValueError("fuse_expert_sgd needs plain SGD and expert gradients that nothing else uses")
         self.aux_loss = aux_loss
         self._ids = self._labels = None
+        self._check_ids = False
 
     def step_device(self, ids: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
         """One optimisation step on device tensors; returns the loss tensor (no host sync). An id outside its table makes it NaN, gradients and weights
         with it, until ``ops.gemm.Workspace.check`` is asked; ``step`` asks in time."""
-        return self._step(ids, labels, False)
-
-    def _step(self, ids, labels, check_ids):
         self.opt.zero_grad(set_to_none=True)
         if self.fuse_expert_sgd:
             group = self.opt.param_groups[0]
@@ -72,7 +70,7 @@ class TrainStep:
             if aux is not None:
                 loss = loss + aux.to(loss.dtype).sum()
         check = None
-        if check_ids and self.device.type == "cuda":
+        if self._check_ids and self.device.type == "cuda":
             check = IdCheck(self.device)
             if self.fuse_expert_sgd:       # the backward pass changes weights
                 check.wait()
@@ -97,4 +95,8 @@ class TrainStep:
             self._labels = torch.empty(labels.shape, dtype=labels.dtype, device=self.device)
         self._ids.copy_(ids, non_blocking=True)
         self._labels.copy_(labels, non_blocking=True)
-        return float(self._step(self._ids, self._labels, True).item())
+        self._check_ids = True
+        try:
+            return float(self.step_device(self._ids, self._labels).item())
+        finally:
+            self._check_ids = False

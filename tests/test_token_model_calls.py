@@ -97,3 +97,23 @@ def test_replaced_and_hooked_tables(name, table, change):
     call()
     torch.testing.assert_close(seen[0], want)
     assert len(calls) == ("hook" in change)
+
+
+def test_a_step_of_its_own_in_a_subclass():
+    from ccfuser_b200.train import TrainStep
+
+    class Counted(TrainStep):
+        steps = 0
+
+        def step_device(self, ids, labels):
+            self.steps += 1
+            return super().step_device(ids, labels)
+    trainer = Counted(_gpt())
+    ids = torch.randint(0, 200, (2, 16))
+    before = [p.detach().clone() for p in trainer.raw_model.parameters()]
+    assert trainer.step(ids) > 0 and trainer.steps == 1
+    assert not all(torch.equal(a, b) for a, b in zip(before, trainer.raw_model.parameters()))
+    before = [p.detach().clone() for p in trainer.raw_model.parameters()]
+    with pytest.raises(IndexError):
+        trainer.step(ids + 256)
+    assert all(torch.equal(a, b) for a, b in zip(before, trainer.raw_model.parameters()))
