@@ -17,10 +17,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libccfuser_b200.so")
-TORCH_SOURCES = [os.path.join(CSRC, f) for f in ("torch_norm.cpp", "torch_tokens.cpp", "torch_ops.h", "norm.h", "embedding.h", "logprobs.h",
-                                                 "dropout.h")]
+TORCH_SOURCES = [os.path.join(CSRC, f) for f in ("torch_norm.cpp", "torch_tokens.cpp", "torch_training.cpp", "torch_ops.h", "torch_nodes.h", "norm.h",
+                                                 "embedding.h", "logprobs.h", "dropout.h", "expert_sort.h", "adamw.h")]
 SOURCES = ["gemm.cu", "gemm2.cu", "gemm_swap.cu", "gemm_wgrad.cu", "moe_kernels.cu", "route.cu", "combine.cu", "router.cu", "runtime.cu",
-           "no_alloc.cu", "norm.cu", "embedding.cu", "logprobs.cu", "dropout.cu"]
+           "no_alloc.cu", "norm.cu", "embedding.cu", "logprobs.cu", "dropout.cu", "expert_sort.cu", "adamw.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 

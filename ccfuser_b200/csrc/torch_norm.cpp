@@ -77,5 +77,6 @@ PYBIND11_MODULE(_ccf_torch, m) {
          int64_t wait_ns) { return LayerNormFn::apply(x, weight, bias, status, eps, wait_ns); },
       py::call_guard<py::gil_scoped_release>());
   ccf_torch::add_token_ops(m);
+  ccf_torch::add_training_ops(m);
   m.def("launches", [] { return g_launches.load(); });
 }

@@ -1,4 +1,4 @@
-// What the autograd functions of the module built against torch share (torch_norm.cpp, torch_tokens.cpp).
+// What the autograd functions of the module built against torch share (torch_norm.cpp, torch_tokens.cpp, torch_training.cpp).
 #pragma once
 #include <ATen/ATen.h>
 #include <torch/csrc/utils/pybind.h>
@@ -18,5 +18,6 @@ inline at::Tensor packed(const at::Tensor& t) {
 }
 
 void add_token_ops(py::module_& m);
+void add_training_ops(py::module_& m);
 
 }  // namespace ccf_torch

@@ -149,6 +149,30 @@ class Logprobs(C.Structure):
                 ("type", C.c_int), ("wide", C.c_int), ("inv_t", C.c_float)]
 
 
+class Order(C.Structure):
+    """Mirror of CcfOrder (csrc/expert_sort.h)."""
+    _fields_ = [("idx", _vp), ("slot_row", _vp), ("row_slot", _vp), ("counts", _vp), ("base", _vp), ("scratch", _vp), ("slots", C.c_longlong),
+                ("rows", C.c_longlong), ("capacity", C.c_longlong), ("experts", C.c_int), ("align", C.c_int), ("wide", C.c_int), ("pad0", C.c_int)]
+
+
+class Rows(C.Structure):
+    """Mirror of CcfRows (csrc/expert_sort.h)."""
+    _fields_ = [("tokens_in", _vp), ("rows_in", _vp), ("tokens_out", _vp), ("rows_out", _vp), ("slot_row", _vp), ("row_slot", _vp), ("weights", _vp),
+                ("d_weights", _vp), ("tokens", C.c_longlong), ("rows", C.c_longlong), ("ld", C.c_longlong), ("top_k", C.c_int), ("d", C.c_int),
+                ("type", C.c_int), ("weight_type", C.c_int)]
+
+
+class AdamwTensor(C.Structure):
+    """Mirror of CcfAdamwTensor (csrc/adamw.h)."""
+    _fields_ = [("p", _vp), ("g", _vp), ("m", _vp), ("v", _vp), ("e", _vp), ("n", C.c_longlong), ("rows", C.c_longlong), ("number", C.c_longlong)]
+
+
+class Adamw(C.Structure):
+    """Mirror of CcfAdamw (csrc/adamw.h)."""
+    _fields_ = [("tensors", _vp), ("count", C.c_int), ("type", C.c_int), ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("weight_decay", C.c_double), ("seed", C.c_ulonglong), ("step", C.c_longlong), ("scalars", _vp)]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -189,7 +213,7 @@ def _build_locked(needed, make):
 
 
 def torch_module():
-    """The autograd functions in C++ (csrc/torch_norm.cpp, csrc/torch_tokens.cpp), or None where this torch has no module and none can be
+    """The autograd functions in C++ (csrc/torch_norm.cpp, csrc/torch_tokens.cpp, csrc/torch_training.cpp), or None where this torch has no module and none can be
     built: the kernels do not need it (ops/norm.py and its neighbours have the functions in Python). Tried once; says so once."""
     global _torch_module, _torch_module_tried
     if _torch_module is not None or _torch_module_tried:
@@ -212,7 +236,7 @@ def torch_module():
             except Exception as e:  # noqa: BLE001
                 import warnings
                 warnings.warn(f"ccfuser_b200: {_build.torch_path()} could not be built or loaded ({e}); the autograd functions "
-                              "of LayerNorm, embeddings, log probabilities and dropout run in Python, on the same kernels")
+                              "of LayerNorm, embeddings, log probabilities, dropout and sorted tokens run in Python, on the same kernels")
             _torch_module_tried = True
     return _torch_module
 
@@ -240,7 +264,8 @@ def load(build_if_missing: bool = True):
         for name, struct in (("gemm_args", GemmArgs), ("dispatch_args", DispatchArgs),
                              ("gemm_launch", GemmLaunch), ("plan_args", PlanArgs), ("layer", Layer),
                              ("layer_grads", LayerGrads), ("barrier_args", BarrierArgs),
-                             ("sgd_multi", SgdMulti), ("embed", Embed), ("logprobs", Logprobs)):
+                             ("sgd_multi", SgdMulti), ("embed", Embed), ("logprobs", Logprobs), ("order", Order), ("rows", Rows),
+                             ("adamw", Adamw), ("adamw_tensor", AdamwTensor)):
             want = getattr(lib, "ccf_sizeof_" + name)()
             if want != C.sizeof(struct):
                 raise RuntimeError(f"ctypes mirror of {name} is {C.sizeof(struct)} bytes, library has {want}")
@@ -290,6 +315,15 @@ def _declare(lib):
         "ccf_logprobs_fwd": ([C.POINTER(Logprobs), p], i),
         "ccf_logprobs_bwd": ([C.POINTER(Logprobs), p], i),
         "ccf_dropout": ([p, p, p, p, p, C.c_uint, C.c_uint, ll, i, p], i),
+        "ccf_order_rows": ([ll, i, ll, i], ll),
+        "ccf_order_scratch": ([ll, i], ll),
+        "ccf_order": ([C.POINTER(Order), p], i),
+        "ccf_sort_rows": ([C.POINTER(Rows), i, p], i),
+        "ccf_return_rows": ([C.POINTER(Rows), p], i),
+        "ccf_return_rows_bwd": ([C.POINTER(Rows), p], i),
+        "ccf_adamw": ([C.POINTER(Adamw), p], i),
+        "ccf_adamw_scalars": ([C.POINTER(Adamw), p, p, p, p], i),
+        "ccf_state_values": ([p, p, p, ll, ll, i, i, p], i),
         "ccf_symm_alloc": ([ull, C.POINTER(p)], i),
         "ccf_symm_free": ([p], i),
         "ccf_symm_handle_bytes": ([], i),

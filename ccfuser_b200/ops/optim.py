@@ -2,6 +2,8 @@
 from __future__ import annotations
 
 import ctypes as C
+import math
+from typing import Optional, Sequence
 
 import torch
 
@@ -74,3 +76,348 @@ class FusedSGD(torch.optim.Optimizer):
                     with torch.cuda.device(device):
                         self._launch(lib, batch, lr, wd, int(dtype == torch.float16), N.stream_ptr())
         return loss
+
+
+# ---- AdamW -----------------------------------------------------------------------------------------------------------------
+STATE_BLOCK = 256          # weights that share the exponents of their 8-bit moments (csrc/adamw.h)
+STATE8_LEAST = 4096        # weights from which on a tensor's moments are worth 8 bits
+_M32, _M64 = 0xFFFFFFFF, 0xFFFFFFFFFFFFFFFF
+
+
+def state8(p: torch.Tensor, rows: int = 1):
+    """Empty 8-bit moments of a tensor: codes of the first and the second (uint8, of ``p``'s shape), and the exponents of their blocks, ``[rows, blocks of a row,
+    2]``. ``rows``: parts of equal size that no block crosses, such as the experts of a weight ``[experts, out, in]``."""
+    if rows < 1 or p.numel() % rows:
+        raise ValueError(f"rows: a divisor of the {p.numel()} weights, got {rows}")
+    blocks = -(-(p.numel() // rows) // STATE_BLOCK)
+    return (torch.zeros(p.shape, dtype=torch.uint8, device=p.device), torch.zeros(p.shape, dtype=torch.uint8, device=p.device),
+            torch.full((rows, blocks, 2), 40, dtype=torch.uint8, device=p.device))
+
+
+def state_values(codes: torch.Tensor, exponents: torch.Tensor, second: bool = False, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """What 8-bit moments stand for: ``codes`` (uint8) with the exponents ``[rows, blocks of a row, 2]`` (or ``[blocks, 2]``) of their blocks; ``second``: they are
+    second moments. bf16 and fp32 hold every value as it is (fp16 only those of its range)."""
+    if codes.dtype != torch.uint8 or exponents.dtype != torch.uint8:
+        raise TypeError(f"codes and exponents are uint8, not {codes.dtype} and {exponents.dtype}")
+    if dtype not in N.DTYPE_CODE:
+        raise TypeError(f"values in bf16, fp16 or fp32, not {dtype}")
+    _check_exponents(codes, exponents if exponents.dim() != 2 else exponents.unsqueeze(0), "codes")
+    rows = exponents.shape[0] if exponents.dim() == 3 else 1
+    if codes.device != exponents.device:
+        raise ValueError(f"codes are on {codes.device}, their exponents on {exponents.device}")
+    if not codes.is_cuda or codes.numel() == 0 or N.transformed(codes):
+        return _decode(codes, exponents.reshape(rows, -1, 2), second).to(dtype)
+    codes, exponents = codes.contiguous(), exponents.contiguous()
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    with torch.cuda.device(codes.device):
+        N.check(N.load().ccf_state_values(codes.data_ptr(), exponents.data_ptr(), out.data_ptr(), codes.numel(), rows, int(second), N.DTYPE_CODE[dtype],
+                                          N.stream_ptr()), "ccf_state_values")
+    N.count(1)
+    return out
+
+
+def _check_exponents(p, e, name):
+    rows = e.shape[0] if e.dim() == 3 else 0
+    if rows < 1 or p.numel() % rows or tuple(e.shape[1:]) != (-(-(p.numel() // rows) // STATE_BLOCK), 2):
+        raise ValueError(f"exponents of {name}: [rows, blocks of a row, 2] for {p.numel()} weights, got {tuple(e.shape)}")
+
+
+def _check_state(p, g, m, v, e, i):
+    if g.layout != torch.strided or g.dtype != p.dtype:
+        raise TypeError(f"grads: tensor {i} is {g.layout} of {g.dtype}, its parameter {p.dtype}")
+    if not p.is_floating_point():
+        raise TypeError(f"params: tensor {i} is {p.dtype}")
+    kind = torch.uint8 if e is not None else torch.float64 if p.dtype == torch.float64 else torch.float32
+    if m.dtype != kind or v.dtype != kind or (e is not None and e.dtype != kind):
+        raise TypeError(f"moments of tensor {i} are {kind}, not {m.dtype} and {v.dtype}")
+    if e is not None and p.dtype == torch.float64:
+        raise TypeError(f"params: tensor {i} is of fp64, whose moments have no 8-bit form")
+    if g.shape != p.shape or m.shape != p.shape or v.shape != p.shape:
+        raise ValueError(f"tensor {i}: {tuple(p.shape)}, its gradient and moments {tuple(g.shape)}, {tuple(m.shape)} and {tuple(v.shape)}")
+    if any(t is not None and t.device != p.device for t in (g, m, v, e)):
+        raise ValueError(f"tensor {i} and what belongs to it lie on several devices")
+    if e is not None:
+        _check_exponents(p, e, f"tensor {i}")
+
+
+@torch.no_grad()
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor],
+               step: Optional[int] = None, *, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+               exponents: Optional[Sequence[torch.Tensor]] = None, seed: int = 0, counter: Optional[torch.Tensor] = None) -> None:
+    """One AdamW step of every tensor in place, by one launch for up to 400 tensors of a type (csrc/adamw.cu).
+
+    Gradients have their parameters' types (bf16, fp16, fp32); the arithmetic is fp32 whatever they are. Moments are fp32, or uint8 codes with ``exponents``
+    (``state8``), which are rounded up or down by a hash of (``seed``, step, place of the tensor in the list, weight), so that their mean is right. ``step`` is the number of this step,
+    from 1. With ``counter``, an int64 tensor of one element on the tensors' device, that is raised by one instead and read on the device, so that a captured
+    call counts its replays; then ``lr`` may be an fp32 tensor of one element there. Values that are not finite make a weight NaN as in torch, and with 8-bit moments from the
+    next step on all weights of its block. Tensors on a CPU, of fp64 or not contiguous take torch's operations, to the same codes."""
+    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    exponents = None if exponents is None else list(exponents)
+    if any(len(t) != len(params) for t in (grads, exp_avgs, exp_avg_sqs) + (() if exponents is None else (exponents,))):
+        raise ValueError(f"{len(params)} params, and other numbers of gradients, moments or exponents")
+    if (step is None) == (counter is None):
+        raise ValueError("either step or counter")
+    if counter is None and step < 1:
+        raise ValueError(f"step: from 1, got {step}")
+    device_lr = lr if torch.is_tensor(lr) else None
+    if counter is not None and (counter.dtype != torch.int64 or counter.numel() != 1):
+        raise ValueError(f"counter: one int64, got {tuple(counter.shape)} of {counter.dtype}")
+    if device_lr is not None and (counter is None or lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != counter.device):
+        raise ValueError("lr: a number, or with counter one fp32 beside it")
+    lr = 0.0 if device_lr is not None else float(lr)
+    beta1, beta2 = (float(b) for b in betas)
+    if not (0.0 <= lr and 0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0 and 0.0 <= eps and 0.0 <= weight_decay):
+        raise ValueError(f"lr, eps and weight_decay are at least 0, betas in [0, 1), got {lr}, {eps}, {weight_decay}, {beta1, beta2}")
+    seed = (int(seed) + (1 << 63)) % (1 << 64) - (1 << 63)      # as C's 64 bits
+    if not params:
+        return
+    rates = (lr, beta1, beta2, float(eps), float(weight_decay), seed)
+    module = N.torch_module() if params[0].is_cuda else None
+    if module is not None and module.adamw_step(params, grads, exp_avgs, exp_avg_sqs, exponents, *rates, 0 if step is None else int(step), counter, device_lr):
+        return
+    tensors = list(zip(params, grads, exp_avgs, exp_avg_sqs, [None] * len(params) if exponents is None else exponents))
+    seen = set()
+    for i, t in enumerate(tensors):
+        _check_state(*t, i)
+        if counter is not None and t[0].device != counter.device:
+            raise ValueError(f"counter: on {counter.device}, the tensors beside it on {t[0].device}")
+        if t[0].numel() and t[0].data_ptr() in seen:
+            raise ValueError(f"params: tensor {i} is there twice")
+        seen.add(t[0].data_ptr())
+    _adamw_each(tensors, rates, step, counter, device_lr)
+
+
+def _adamw_each(tensors, rates, step, counter, device_lr):
+    """The step without the C++ module, or with tensors that the kernels do not take."""
+    lr, beta1, beta2, eps, wd, seed = rates
+    by_kind, others = {}, []
+    for i, (p, g, m, v, e) in enumerate(tensors):
+        if p.numel() == 0:
+            continue
+        if p.is_cuda and p.dtype in N.DTYPE_CODE and all(t is None or t.is_contiguous() for t in (p, m, v, e)):
+            by_kind.setdefault((p.device, p.dtype), []).append((i, p, g.contiguous(), m, v, e))
+        else:
+            others.append((i, p, g, m, v, e))
+    a = N.Adamw(lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=wd, seed=seed & _M64, step=step or 0)
+    scalars = None
+    if counter is not None and counter.is_cuda:
+        scalars = torch.empty(32, dtype=torch.uint8, device=counter.device)
+        with torch.cuda.device(counter.device):
+            N.check(N.load().ccf_adamw_scalars(C.byref(a), counter.data_ptr(), N.ptr(device_lr), scalars.data_ptr(), N.stream_ptr()), "ccf_adamw_scalars")
+        N.count(1)
+        a.scalars = scalars.data_ptr()
+    elif counter is not None:
+        counter += 1
+    for (device, dtype), batch in by_kind.items():
+        table = (N.AdamwTensor * len(batch))(*(N.AdamwTensor(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), N.ptr(e), p.numel(), 1 if e is None else e.shape[0], i)
+                                               for i, p, g, m, v, e in batch))
+        a.tensors, a.count, a.type = C.addressof(table), len(batch), N.DTYPE_CODE[dtype]
+        with torch.cuda.device(device):
+            launches = N.load().ccf_adamw(C.byref(a), N.stream_ptr())
+        N.check(min(launches, 0), "ccf_adamw")
+        N.count(launches)
+        for _, p, _, m, v, e in batch:
+            for t in (p, m, v) + (() if e is None else (e,)):
+                if not t.is_inference():
+                    torch.autograd.graph.increment_version(t)
+    if others:
+        if counter is not None:      # the number of the step is needed on the host
+            step, lr = int(counter), lr if device_lr is None else float(device_lr)
+        key = _split_mix(_split_mix(seed & _M64) ^ step) >> 32
+        for i, p, g, m, v, e in others:
+            _adamw_torch(p, g, m, v, e, (key + i * 0x9E3779B9) & _M32, lr, beta1, beta2, eps, wd, step)
+
+
+def _adamw_torch(p, g, m, v, e, key, lr, beta1, beta2, eps, wd, step):
+    """One tensor by torch's operations."""
+    wide = torch.float64 if p.dtype == torch.float64 else torch.float32
+    first, second, g = (m, v, g.to(wide)) if e is None else (_decode(m, e, False), _decode(v, e, True), g.to(wide))
+    first = first * beta1 + g * (1 - beta1)
+    second = second * beta2 + g * g * (1 - beta2)
+    update = first / (second.sqrt() / math.sqrt(1 - beta2 ** step) + eps)
+    p.copy_(p.to(wide) * (1 - lr * wd) - update * (lr / (1 - beta1 ** step)))
+    if e is None:
+        m.copy_(first)
+        v.copy_(second)
+        return
+    at = torch.arange(p.numel(), device=p.device)
+    h = _mix((at + key) & _M32).view(p.shape)
+    for codes, x, bits, k in ((m, first, h & 0xFFFFF, 0), (v, second, h >> 12, 1)):
+        c, e[..., k] = _encode(x, e.shape[0], bits.int(), k == 1)
+        codes.copy_(c)
+
+
+def _mix(h):
+    """MurmurHash3's last step, on int64 that hold 32 bits."""
+    h = h ^ (h >> 16)
+    h = (h * 0x85EBCA6B) & _M32
+    h = h ^ (h >> 13)
+    h = (h * 0xC2B2AE35) & _M32
+    return h ^ (h >> 16)
+
+
+def _split_mix(x):
+    x = (x + 0x9E3779B97F4A7C15) & _M64
+    x = (x ^ x >> 30) * 0xBF58476D1CE4E5B9 & _M64
+    x = (x ^ x >> 27) * 0x94D049BB133111EB & _M64
+    return x ^ x >> 31
+
+
+def _blocks(x, rows):
+    """[rows, blocks, STATE_BLOCK], the last block of a row filled up with zeros."""
+    x = x.reshape(rows, -1)
+    return torch.nn.functional.pad(x, (0, -x.shape[1] % STATE_BLOCK)).view(rows, -1, STATE_BLOCK)
+
+
+def _unblocks(x, shape):
+    n = math.prod(shape)
+    return x.reshape(x.shape[0], -1)[:, :n // x.shape[0]].reshape(shape)
+
+
+def _power(exponent):
+    """2 to the given int32, from -126 to 127, in fp32."""
+    return ((exponent + 127) << 23).view(torch.float32)
+
+
+# a code is the upper bits of a float: its exponent is that far below the block's, and its block's factor is split in two for the range of fp32
+_FIRST, _SECOND = (120, 8), (100, 4)
+
+
+def _decode(codes, e, second):
+    down, near = _SECOND if second else _FIRST
+    c, x = _blocks(codes, e.shape[0]).int(), e[..., int(second)].int().unsqueeze(-1)
+    bits = c << 20 if second else ((c & 0x7F) << 20) | ((c & 0x80) << 24)
+    finite = x < 255
+    values = bits.view(torch.float32) * 2.0 ** down * _power(torch.where(finite, x.clamp(min=40) - 127 - near, 0))
+    return _unblocks(torch.where(finite, values, math.nan), codes.shape)
+
+
+def _encode(x, rows, bits, second):
+    """Codes and their blocks' exponents."""
+    down, near = _SECOND if second else _FIRST
+    b = _blocks(x, rows)
+    a = b.abs()
+    top = a.view(torch.int32).amax(dim=-1, keepdim=True)
+    e = torch.where(top < 0x7F800000, (top + 0xFFFFF) >> 23, 255).clamp(min=40)
+    finite = e < 255
+    y = a * _power(torch.where(finite, 127 + near - e, 0)) * 2.0 ** -down
+    code = (y.view(torch.int32) + _blocks(bits, rows)) >> 20
+    code = torch.where(a > 0, code.clamp(min=1), code) if second else code | (b.view(torch.int32) >> 24) & 0x80
+    return _unblocks(torch.where(finite, code, 0).to(torch.uint8), x.shape), e.squeeze(-1).to(torch.uint8)
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` on ``adamw_step``: all tensors of a step in one launch per type (400 of them at most), moments in fp32 whatever the weights' type
+    or, with ``state_bits=8``, in 8 bits (2 bytes a weight instead of 8; tensors of fewer than 4096 weights and fp64 ones keep theirs in full). The mean of what
+    8 bits hold is right, so that moments go on following changes of a fraction of their steps; ``seed`` chooses the hash that decides.
+
+    ``capturable=True``: for steps captured in a CUDA graph. The number of the step then lies on the device, one for all parameters of a group and device, and ``lr`` may be an fp32 tensor of
+    one element there; the first step is taken before the capture. ``state_dict`` has the names of torch's (``step``, ``exp_avg``, ``exp_avg_sq``, and ``exponents`` for 8 bits), and
+    loads those of ``torch.optim.AdamW``. Expert weights (and the router's) share exponents inside an expert only, so that ``rebalance_experts`` moves their moments with them."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32, seed: int = 0,
+                 capturable: bool = False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits: 8 or 32, got {state_bits}")
+        if torch.is_tensor(lr) and not capturable:
+            raise ValueError("lr: a tensor with capturable=True only")
+        if not (torch.is_tensor(lr) or lr >= 0.0) or eps < 0.0 or weight_decay < 0.0 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"lr, eps and weight_decay are at least 0, betas in [0, 1), got {lr}, {eps}, {weight_decay}, {betas}")
+        self._counters = {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed, capturable=capturable))
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:
+            for k, v in (("state_bits", 32), ("seed", 0), ("capturable", False)):
+                group.setdefault(k, v)
+        self._counters = {}
+
+    def __getstate__(self):
+        return {k: v for k, v in super().__getstate__().items() if k != "_counters"}
+
+    def _counter(self, k, p):
+        """The number of the last step of group ``k`` on the parameter's device."""
+        key = (k, p.device)
+        if key not in self._counters:
+            steps = [self.state[q]["step"] for q in self.param_groups[k]["params"] if q.device == p.device and "step" in self.state.get(q, {})]
+            known = max((int(s) for s in steps), default=0)
+            self._counters[key] = torch.full((1,), known, dtype=torch.int64, device=p.device)
+            for q in self.param_groups[k]["params"]:
+                if q.device == p.device and "step" in self.state.get(q, {}):
+                    self.state[q]["step"] = self._counters[key]
+        return self._counters[key]
+
+    def _start(self, k, group, p):
+        state = self.state[p]
+        if group["state_bits"] == 8 and p.numel() >= STATE8_LEAST and p.dtype in N.DTYPE_CODE:
+            # rows that move between ranks (parallel/placement.py) take their blocks along
+            moves = p.dim() >= 2 and (getattr(p, "skip_allreduce", False) or hasattr(p, "dp_comm"))
+            state["exp_avg"], state["exp_avg_sq"], state["exponents"] = state8(p, p.shape[0] if moves else 1)
+        else:
+            kind = torch.float64 if p.dtype == torch.float64 else torch.float32
+            state["exp_avg"], state["exp_avg_sq"] = (torch.zeros(p.shape, dtype=kind, device=p.device) for _ in range(2))
+        state["step"] = self._counter(k, p) if group["capturable"] else 0
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        for k, group in enumerate(self.param_groups):
+            batches = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if capturing and not (group["capturable"] and "step" in state):
+                    raise RuntimeError("FusedAdamW: a step in a CUDA graph needs capturable=True and a step before the capture")
+                if "step" not in state:
+                    state = self._start(k, group, p)
+                if group["capturable"]:
+                    key = (p.device, "exponents" in state)
+                else:
+                    state["step"] += 1
+                    key = (state["step"], "exponents" in state)
+                batches.setdefault(key, []).append((p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("exponents")))
+            raised = set()
+            for n, ((number, eight), batch) in enumerate(batches.items()):
+                p, g, m, v, e = zip(*batch)
+                counter = None
+                if group["capturable"]:
+                    number, counter = None, self._counter(k, p[0])
+                    if counter.device in raised:      # raised by the batch before
+                        counter -= 1
+                    raised.add(counter.device)
+                adamw_step(p, g, m, v, number, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                           exponents=e if eight else None, seed=group["seed"] + (k << 32) + n, counter=counter)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """Moments keep the types that they were saved in: torch's own loading casts them to the weights'."""
+        seen = []
+        handle = self.register_load_state_dict_pre_hook(lambda _, d: seen.append(d))      # behind the hooks that change it
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            handle.remove()
+        saved = seen[-1]
+        ids = [i for group in saved["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(ids, params):
+            state = saved["state"].get(i)
+            if not state:
+                continue
+            kind = torch.uint8 if "exponents" in state else torch.float64 if p.dtype == torch.float64 else torch.float32
+            for name in ("exp_avg", "exp_avg_sq", "exponents"):
+                if name in state:
+                    self.state[p][name] = state[name].detach().to(device=p.device, dtype=torch.uint8 if name == "exponents" else kind, copy=True).contiguous()
+            self.state[p]["step"] = int(state["step"])
+        for k, group in enumerate(self.param_groups):
+            if group["capturable"]:
+                for p in group["params"]:
+                    if "step" in self.state.get(p, {}):
+                        self._counter(k, p)
