@@ -45,6 +45,8 @@ int ccf_order(const CcfOrder* o, void* stream);
 // rows_out[slot_row[t, j]] = tokens_in[t], zeros in rows without a slot. `behind_order`: right behind ccf_order on the same stream, which nothing but it
 // wrote row numbers for
 int ccf_sort_rows(const CcfRows* r, int behind_order, void* stream);
+// Both, `r` with the order's slot_row and row_slot; launches made, or a negative code
+int ccf_sort_by_expert(const CcfOrder* o, const CcfRows* r, void* stream);
 // tokens_out[t] = sum over j of weights[t, j] * rows_in[slot_row[t, j]]; without weights, of the rows alone
 int ccf_return_rows(const CcfRows* r, void* stream);
 // its gradients: rows_out[slot_row[t, j]] = weights[t, j] * tokens_in[t], zeros elsewhere; d_weights[t, j] = <tokens_in[t], rows_in[slot_row[t, j]]>.

@@ -32,9 +32,16 @@ void check_idx(const at::Tensor& idx, int64_t experts, const std::optional<int64
   TORCH_CHECK_VALUE(idx.numel() <= CCF_SORT_MAX_SLOTS, idx.numel(), " slots: at most 2^30 in one call");
 }
 
-Order run_order(const at::Tensor& idx_, int64_t experts, const std::optional<int64_t>& capacity, int64_t align) {
-  const at::Tensor idx = idx_.contiguous();
-  CcfOrder o{};
+// a tensor of its own in the memory of another; without the dispatcher, which takes longer than the launches of a small call
+at::Tensor part_of(const at::Tensor& t, int64_t first, at::IntArrayRef sizes) {
+  at::Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), t.dtype());
+  r.unsafeGetTensorImpl()->set_storage_offset(first);
+  r.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return r;
+}
+
+// Memory for the order of idx, contiguous, and the arguments of its kernels.
+Order new_order(CcfOrder& o, const at::Tensor& idx, int64_t experts, const std::optional<int64_t>& capacity, int64_t align) {
   o.idx = idx.data_ptr();
   o.slots = idx.numel();
   o.capacity = capacity.value_or(o.slots);
@@ -43,19 +50,15 @@ Order run_order(const at::Tensor& idx_, int64_t experts, const std::optional<int
   o.wide = idx.scalar_type() == at::kLong;
   o.rows = ccf_order_rows(o.slots, o.experts, o.capacity, o.align);
   TORCH_CHECK_VALUE(o.rows >= 0, "at most 2^31 - 1 rows in one call");
-  const auto i32 = at::TensorOptions(idx.device()).dtype(at::kInt);
-  const int64_t scratch = ccf_order_scratch(o.slots, o.experts) / 4;
-  // small arrays from one allocation: counts, base and the blocks' counts
-  const at::Tensor small = at::empty({2 * experts + 1 + scratch}, i32);
-  const Order r = {at::empty(idx.sizes(), i32), at::empty({o.rows}, i32), small.narrow(0, 0, experts), small.narrow(0, experts, experts + 1)};
+  const int64_t scratch = ccf_order_scratch(o.slots, o.experts) / 4, small = 2 * experts + 1;
+  const at::Tensor all = at::empty({o.slots + o.rows + small + scratch}, at::TensorOptions(idx.device()).dtype(at::kInt));
+  const Order r = {part_of(all, 0, idx.sizes()), part_of(all, o.slots, {o.rows}), part_of(all, o.slots + o.rows, {experts}),
+                   part_of(all, o.slots + o.rows + experts, {experts + 1})};
   o.slot_row = r.slot_row.data_ptr<int>();
   o.row_slot = r.row_slot.data_ptr<int>();
   o.counts = r.counts.data_ptr<int>();
   o.base = r.base.data_ptr<int>();
-  o.scratch = small.data_ptr<int>() + 2 * experts + 1;
-  const int launches = ccf_order(&o, current_stream());
-  TORCH_CHECK(launches > 0, "ccf_order failed with code ", launches);
-  g_launches += launches;
+  o.scratch = all.data_ptr<int>() + o.slots + o.rows + small;
   return r;
 }
 
@@ -77,7 +80,8 @@ CcfRows rows_args(const at::Tensor& slot_row, int64_t rows, int64_t d, const at:
   return a;
 }
 
-at::Tensor run_sort(const at::Tensor& x_, const at::Tensor& slot_row, const at::Tensor& row_slot, bool behind_order) {
+// The rows of an order; with `o` the order is made as well, of what lies in `o`.
+at::Tensor run_sort(const at::Tensor& x_, const at::Tensor& slot_row, const at::Tensor& row_slot, const CcfOrder* o) {
   const int64_t d = x_.size(-1);
   CcfRows a = rows_args(slot_row, row_slot.numel(), d, x_);
   const at::Tensor x = token_rows(x_, a.tokens, d);
@@ -86,8 +90,14 @@ at::Tensor run_sort(const at::Tensor& x_, const at::Tensor& slot_row, const at::
   if (a.tokens > 1) a.ld = x.stride(0);
   a.row_slot = row_slot.data_ptr<int>();
   a.rows_out = rows.data_ptr();
-  check(ccf_sort_rows(&a, behind_order, current_stream()), "ccf_sort_rows");
-  ++g_launches;
+  if (o == nullptr) {
+    check(ccf_sort_rows(&a, 0, current_stream()), "ccf_sort_rows");
+    ++g_launches;
+  } else {
+    const int launches = ccf_sort_by_expert(o, &a, current_stream());
+    TORCH_CHECK(launches > 0, "ccf_sort_by_expert failed with code ", launches);
+    g_launches += launches;
+  }
   return rows;
 }
 
@@ -200,8 +210,8 @@ void check_order(const at::Tensor& slot_row, const at::Tensor& row_slot) {
   TORCH_CHECK_VALUE(slot_row.numel() <= CCF_SORT_MAX_SLOTS && row_slot.numel() <= 0x7fffffff, "at most 2^30 slots and 2^31 - 1 rows in one call");
 }
 
-at::Tensor sorted(const at::Tensor& x, const at::Tensor& slot_row, const at::Tensor& row_slot, bool behind_order, bool training) {
-  const at::Tensor rows = run_sort(x, slot_row, row_slot, behind_order);
+at::Tensor sorted(const at::Tensor& x, const at::Tensor& slot_row, const at::Tensor& row_slot, const CcfOrder* o, bool training) {
+  const at::Tensor rows = run_sort(x, slot_row, row_slot, o);
   if (training) {
     const auto node = make_node<SortNode>(x);
     node->keep(slot_row);
@@ -214,7 +224,12 @@ at::Tensor sorted(const at::Tensor& x, const at::Tensor& slot_row, const at::Ten
 variable_list expert_order(const at::Tensor& idx, int64_t experts, const std::optional<int64_t>& capacity, int64_t align) {
   check_idx(idx, experts, capacity, align);
   const c10::cuda::CUDAGuard guard(idx.device());
-  const Order o = run_order(idx, experts, capacity, align);
+  CcfOrder a{};
+  const at::Tensor packed_idx = idx.contiguous();
+  const Order o = new_order(a, packed_idx, experts, capacity, align);
+  const int launches = ccf_order(&a, current_stream());
+  TORCH_CHECK(launches > 0, "ccf_order failed with code ", launches);
+  g_launches += launches;
   return {o.slot_row, o.row_slot, o.counts, o.base};
 }
 
@@ -224,8 +239,10 @@ variable_list sort_by_expert(const at::Tensor& x, const at::Tensor& idx, int64_t
   const c10::cuda::CUDAGuard guard(x.device());
   const bool training = builds_graph(x);
   const at::NoGradGuard no_graph;   // views still share their base's version: a change before the backward pass is noticed
-  const Order o = run_order(idx, experts, capacity, align);
-  return {sorted(x, o.slot_row, o.row_slot, true, training), o.slot_row, o.row_slot, o.counts, o.base};
+  CcfOrder a{};
+  const at::Tensor packed_idx = idx.contiguous();
+  const Order o = new_order(a, packed_idx, experts, capacity, align);
+  return {sorted(x, o.slot_row, o.row_slot, &a, training), o.slot_row, o.row_slot, o.counts, o.base};
 }
 
 at::Tensor sort_rows(const at::Tensor& x, const at::Tensor& slot_row, const at::Tensor& row_slot) {
@@ -234,7 +251,7 @@ at::Tensor sort_rows(const at::Tensor& x, const at::Tensor& slot_row, const at::
   const c10::cuda::CUDAGuard guard(x.device());
   const bool training = builds_graph(x);
   const at::NoGradGuard no_graph;
-  return sorted(x, slot_row.contiguous(), row_slot.contiguous(), false, training);
+  return sorted(x, slot_row.contiguous(), row_slot.contiguous(), nullptr, training);
 }
 
 at::Tensor return_rows(const at::Tensor& rows, const at::Tensor& slot_row_, const at::Tensor& row_slot_, const OptTensor& weights_) {
@@ -369,6 +386,17 @@ bool adamw_step(const std::vector<at::Tensor>& params, const std::vector<at::Ten
   return true;
 }
 
+at::Tensor state_values(const at::Tensor& codes_, const at::Tensor& exponents_, bool second, int64_t type) {
+  const at::Tensor codes = codes_.contiguous(), exponents = exponents_.contiguous();
+  const c10::cuda::CUDAGuard guard(codes.device());
+  const at::Tensor out = at::empty(codes.sizes(), codes.options().dtype(type == 0 ? at::kBFloat16 : type == 1 ? at::kHalf : at::kFloat));
+  check(ccf_state_values(codes.data_ptr(), exponents.data_ptr<uint8_t>(), out.data_ptr(), codes.numel(), exponents.dim() == 3 ? exponents.size(0) : 1, second,
+                         static_cast<int>(type), current_stream()),
+        "ccf_state_values");
+  ++g_launches;
+  return out;
+}
+
 }  // namespace
 
 void ccf_torch::add_training_ops(py::module_& m) {
@@ -378,4 +406,5 @@ void ccf_torch::add_training_ops(py::module_& m) {
   m.def("sort_rows", &sort_rows, free);
   m.def("return_rows", &return_rows, free);
   m.def("adamw_step", &adamw_step, free);
+  m.def("state_values", &state_values, free);
 }

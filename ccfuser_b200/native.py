@@ -319,6 +319,7 @@ def _declare(lib):
         "ccf_order_scratch": ([ll, i], ll),
         "ccf_order": ([C.POINTER(Order), p], i),
         "ccf_sort_rows": ([C.POINTER(Rows), i, p], i),
+        "ccf_sort_by_expert": ([C.POINTER(Order), C.POINTER(Rows), p], i),
         "ccf_return_rows": ([C.POINTER(Rows), p], i),
         "ccf_return_rows_bwd": ([C.POINTER(Rows), p], i),
         "ccf_adamw": ([C.POINTER(Adamw), p], i),

@@ -90,10 +90,10 @@ def _check_return(rows, order, weights):
             raise TypeError(f"weights: a floating type, got {weights.dtype}")
 
 
-def _on_kernels(*tensors) -> bool:
-    """Whether the kernels take these tensors (None: nothing); the first says whether there is anything to do."""
-    first = tensors[0]
-    return first.is_cuda and first.numel() > 0 and not N.transformed(first) and all(t is None or t.dtype in N.DTYPE_CODE for t in tensors)
+def _on_kernels(x, weights=None) -> bool:
+    """Whether the kernels take these tensors, and have anything to do."""
+    return (x.is_cuda and x.dtype in N.DTYPE_CODE and x.numel() > 0 and not N.transformed(x)
+            and (weights is None or (weights.dtype in N.DTYPE_CODE and not N.transformed(weights))))
 
 
 def _module():

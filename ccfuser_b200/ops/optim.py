@@ -107,6 +107,9 @@ def state_values(codes: torch.Tensor, exponents: torch.Tensor, second: bool = Fa
         raise ValueError(f"codes are on {codes.device}, their exponents on {exponents.device}")
     if not codes.is_cuda or codes.numel() == 0 or N.transformed(codes):
         return _decode(codes, exponents.reshape(rows, -1, 2), second).to(dtype)
+    module = N.torch_module()
+    if module is not None:
+        return module.state_values(codes, exponents, second, N.DTYPE_CODE[dtype])
     codes, exponents = codes.contiguous(), exponents.contiguous()
     out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
     with torch.cuda.device(codes.device):
