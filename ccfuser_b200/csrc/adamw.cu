@@ -3,7 +3,7 @@
 // in fp32 whatever the weights' type, rounded once. Moments lie in fp32 or in 8 bits.
 //
 // 8 bits: CCF_ADAMW_BLOCK weights share a power of two 2^E per moment, the binade of the block's largest value (one byte, E + 127, at least 40; 255: the block
-// holds something that is not finite, and all of it is NaN from then on). A code is a small float relative to it: sign, 4 bits of exponent and 3 of mantissa
+// holds something that is not finite, or above 1.875 2^127, and all of it is NaN from then on). A code is a small float relative to it: sign, 4 bits of exponent and 3 of mantissa
 // for m (17 binades down to the smallest), 5 and 3 for v (33 binades), with gradual underflow. A scale that is a power of two makes a code the upper
 // bits of a float, so that coding is an integer addition and a shift. What counts for training is the rounding: with b2 = 0.999 a step changes v by 0.1 %
 // where codes lie 6 to 12 % apart, and rounding to nearest would lose every such change. A value is rounded up or down by 20 bits of a hash, up as often as

@@ -308,7 +308,7 @@ void check_state(const at::Tensor& p, const at::Tensor& g, const at::Tensor& m, 
 // One step; false, with nothing changed, where a tensor is not one for the kernels (another type or device, not contiguous).
 bool adamw_step(const std::vector<at::Tensor>& params, const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& first, const std::vector<at::Tensor>& second,
                 const std::optional<std::vector<at::Tensor>>& exponents, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t seed, int64_t step,
-                const OptTensor& counter, const OptTensor& device_lr) {
+                const OptTensor& counter, const OptTensor& device_lr, const std::optional<std::vector<int64_t>>& numbers) {
   const size_t n = params.size();
   std::vector<at::Tensor> packed_grads;      // lives until the launches
   std::vector<AdamwCall> calls;
@@ -337,7 +337,7 @@ bool adamw_step(const std::vector<at::Tensor>& params, const std::vector<at::Ten
     t.v = v.data_ptr();
     t.n = p.numel();
     t.rows = 1;
-    t.number = static_cast<int64_t>(i);
+    t.number = numbers.has_value() ? (*numbers)[i] : static_cast<int64_t>(i);
     if (e != nullptr) {
       t.e = e->data_ptr<uint8_t>();
       t.rows = e->size(0);

@@ -106,7 +106,8 @@ def main():
     ap.add_argument("--moe-every", type=int, default=1)
     ap.add_argument("--cf", type=float, default=0.0)
     ap.add_argument("--dtype", default="bf16")
-    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "adamw"])
+    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "adamw", "fused_adamw", "fused_adamw8"],
+                    help="fused_adamw: the library's AdamW, moments in fp32; fused_adamw8: in 8 bits")
     ap.add_argument("--lr", type=float, default=1e-4)
     ap.add_argument("--aux-loss-coef", type=float, default=0.0, help="weight of the router load-balance loss")
     ap.add_argument("--z-loss-coef", type=float, default=0.0, help="weight of the router z-loss")
@@ -145,7 +146,11 @@ def main():
     model, batch, tokens = build(args, ep_size, dev, ep_group)
     wrapped = wrap_ddp(model) if world > 1 else model
     params = [p for p in model.parameters() if p.requires_grad]
-    opt = torch.optim.SGD(params, lr=args.lr) if args.optimizer == "sgd" else torch.optim.AdamW(params, lr=args.lr)
+    if args.optimizer.startswith("fused_adamw"):
+        from ..ops.optim import FusedAdamW
+        opt = FusedAdamW(params, lr=args.lr, state_bits=8 if args.optimizer == "fused_adamw8" else 32)
+    else:
+        opt = torch.optim.SGD(params, lr=args.lr) if args.optimizer == "sgd" else torch.optim.AdamW(params, lr=args.lr)
     if args.fuse_expert_sgd:
         if args.variant != "fused" or args.optimizer != "sgd" or expert_dp_group is not None:
             raise SystemExit("--fuse-expert-sgd needs --variant fused, --optimizer sgd and experts that are not replicated")

@@ -146,18 +146,20 @@ def _check_state(p, g, m, v, e, i):
 @torch.no_grad()
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor],
                step: Optional[int] = None, *, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
-               exponents: Optional[Sequence[torch.Tensor]] = None, seed: int = 0, counter: Optional[torch.Tensor] = None) -> None:
+               exponents: Optional[Sequence[torch.Tensor]] = None, seed: int = 0, numbers: Optional[Sequence[int]] = None,
+               counter: Optional[torch.Tensor] = None) -> None:
     """One AdamW step of every tensor in place, by one launch for up to 400 tensors of a type (csrc/adamw.cu).
 
     Gradients have their parameters' types (bf16, fp16, fp32); the arithmetic is fp32 whatever they are. Moments are fp32, or uint8 codes with ``exponents``
-    (``state8``), which are rounded up or down by a hash of (``seed``, step, place of the tensor in the list, weight), so that their mean is right. ``step`` is the number of this step,
-    from 1. With ``counter``, an int64 tensor of one element on the tensors' device, that is raised by one instead and read on the device, so that a captured
+    (``state8``), which are rounded up or down by a hash of (``seed``, step, tensor, weight), so that their mean is right; a tensor's number there is that in ``numbers``, or its place in
+    the list. ``step`` is the number of this step, from 1. With ``counter``, an int64 tensor of one element on the tensors' device, that is raised by one instead and read on the device, so that a captured
     call counts its replays; then ``lr`` may be an fp32 tensor of one element there. Values that are not finite make a weight NaN as in torch, and with 8-bit moments from the
     next step on all weights of its block. Tensors on a CPU, of fp64 or not contiguous take torch's operations, to the same codes."""
     params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     exponents = None if exponents is None else list(exponents)
-    if any(len(t) != len(params) for t in (grads, exp_avgs, exp_avg_sqs) + (() if exponents is None else (exponents,))):
-        raise ValueError(f"{len(params)} params, and other numbers of gradients, moments or exponents")
+    numbers = None if numbers is None else [int(n) for n in numbers]
+    if any(t is not None and len(t) != len(params) for t in (grads, exp_avgs, exp_avg_sqs, exponents, numbers)):
+        raise ValueError(f"{len(params)} params need as many gradients, moments, exponents and numbers")
     if (step is None) == (counter is None):
         raise ValueError("either step or counter")
     if counter is None and step < 1:
@@ -175,8 +177,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if not params:
         return
     rates = (lr, beta1, beta2, float(eps), float(weight_decay), seed)
-    module = N.torch_module() if params[0].is_cuda else None
-    if module is not None and module.adamw_step(params, grads, exp_avgs, exp_avg_sqs, exponents, *rates, 0 if step is None else int(step), counter, device_lr):
+    traced = N.transformed(params[0])      # no memory to look at
+    module = N.torch_module() if params[0].is_cuda and not traced else None
+    if module is not None and module.adamw_step(params, grads, exp_avgs, exp_avg_sqs, exponents, *rates, 0 if step is None else int(step), counter, device_lr, numbers):
         return
     tensors = list(zip(params, grads, exp_avgs, exp_avg_sqs, [None] * len(params) if exponents is None else exponents))
     seen = set()
@@ -184,26 +187,27 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         _check_state(*t, i)
         if counter is not None and t[0].device != counter.device:
             raise ValueError(f"counter: on {counter.device}, the tensors beside it on {t[0].device}")
-        if t[0].numel() and t[0].data_ptr() in seen:
+        place = id(t[0]) if traced else t[0].data_ptr()
+        if t[0].numel() and place in seen:
             raise ValueError(f"params: tensor {i} is there twice")
-        seen.add(t[0].data_ptr())
-    _adamw_each(tensors, rates, step, counter, device_lr)
+        seen.add(place)
+    _adamw_each(tensors, numbers or range(len(params)), rates, step, counter, device_lr, traced)
 
 
-def _adamw_each(tensors, rates, step, counter, device_lr):
+def _adamw_each(tensors, numbers, rates, step, counter, device_lr, traced):
     """The step without the C++ module, or with tensors that the kernels do not take."""
     lr, beta1, beta2, eps, wd, seed = rates
     by_kind, others = {}, []
-    for i, (p, g, m, v, e) in enumerate(tensors):
+    for i, (p, g, m, v, e) in zip(numbers, tensors):
         if p.numel() == 0:
             continue
-        if p.is_cuda and p.dtype in N.DTYPE_CODE and all(t is None or t.is_contiguous() for t in (p, m, v, e)):
+        if p.is_cuda and not traced and p.dtype in N.DTYPE_CODE and all(t is None or t.is_contiguous() for t in (p, m, v, e)):
             by_kind.setdefault((p.device, p.dtype), []).append((i, p, g.contiguous(), m, v, e))
         else:
             others.append((i, p, g, m, v, e))
     a = N.Adamw(lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=wd, seed=seed & _M64, step=step or 0)
     scalars = None
-    if counter is not None and counter.is_cuda:
+    if counter is not None and counter.is_cuda and not traced:
         scalars = torch.empty(32, dtype=torch.uint8, device=counter.device)
         with torch.cuda.device(counter.device):
             N.check(N.load().ccf_adamw_scalars(C.byref(a), counter.data_ptr(), N.ptr(device_lr), scalars.data_ptr(), N.stream_ptr()), "ccf_adamw_scalars")
@@ -372,7 +376,8 @@ class FusedAdamW(torch.optim.Optimizer):
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         for k, group in enumerate(self.param_groups):
             batches = {}
-            for p in group["params"]:
+            # a parameter's number is its place in the group, whether or not those before it have gradients: replicas on several ranks round alike
+            for number, p in enumerate(group["params"]):
                 if p.grad is None:
                     continue
                 state = self.state[p]
@@ -385,18 +390,18 @@ class FusedAdamW(torch.optim.Optimizer):
                 else:
                     state["step"] += 1
                     key = (state["step"], "exponents" in state)
-                batches.setdefault(key, []).append((p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("exponents")))
+                batches.setdefault(key, []).append((p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("exponents"), number))
             raised = set()
-            for n, ((number, eight), batch) in enumerate(batches.items()):
-                p, g, m, v, e = zip(*batch)
+            for (step, eight), batch in batches.items():
+                p, g, m, v, e, numbers = zip(*batch)
                 counter = None
                 if group["capturable"]:
-                    number, counter = None, self._counter(k, p[0])
+                    step, counter = None, self._counter(k, p[0])
                     if counter.device in raised:      # raised by the batch before
                         counter -= 1
                     raised.add(counter.device)
-                adamw_step(p, g, m, v, number, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                           exponents=e if eight else None, seed=group["seed"] + (k << 32) + n, counter=counter)
+                adamw_step(p, g, m, v, step, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                           exponents=e if eight else None, seed=group["seed"] + (k << 32), numbers=numbers, counter=counter)
         return loss
 
     def load_state_dict(self, state_dict):

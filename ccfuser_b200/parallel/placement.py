@@ -201,7 +201,12 @@ def _state_tensors(optimizer, p: nn.Parameter):
     if optimizer is None:
         return []
     st = optimizer.state.get(p, {})
-    return [(k, v) for k, v in st.items() if torch.is_tensor(v) and v.shape == p.shape]
+    found = [(k, v) for k, v in st.items() if torch.is_tensor(v) and v.shape == p.shape and k != "exponents"]
+    if "exponents" in st:      # of 8-bit moments (ops/optim.py): those of a row's blocks move with it
+        if st["exponents"].shape[0] != p.shape[0]:
+            raise ValueError("8-bit moments of a parameter whose rows move need exponents by row: set its dp_comm or skip_allreduce mark before the first step")
+        found.append(("exponents", st["exponents"]))
+    return found
 
 
 @torch.no_grad()

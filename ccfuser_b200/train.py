@@ -22,7 +22,7 @@ class TrainStep:
     def __init__(self, model: nn.Module, lr: float = 1e-3, optimizer: str = "sgd", dp_group=None,
                  use_ddp: bool = True, aux_loss: bool = False, expert_dp_group=None, mean_expert_grads: bool = False,
                  fuse_expert_sgd: bool = False):
-        """``dp_group``: ranks over which the replicated parameters are averaged (default: all). ``expert_dp_group``:
+        """``optimizer``: "sgd", "adamw" (torch's), "fused_adamw" or "fused_adamw8" (``ops.optim.FusedAdamW`` with moments in fp32 or in 8 bits). ``dp_group``: ranks over which the replicated parameters are averaged (default: all). ``expert_dp_group``:
         ranks that hold replicas of this rank's experts (second value of ``make_ep_dp_groups``) when the expert-parallel
         group is smaller than the job. ``mean_expert_grads``: scale expert gradients by 1 / world size so that they
         follow the same mean-over-ranks convention as the replicated parameters. ``fuse_expert_sgd`` (plain SGD, fused
@@ -45,6 +45,9 @@ class TrainStep:
                 self.opt = torch.optim.SGD(params, lr=lr, foreach=True)
         elif optimizer == "adamw":
             self.opt = torch.optim.AdamW(params, lr=lr, fused=params[0].is_cuda)
+        elif optimizer in ("fused_adamw", "fused_adamw8"):
+            from .ops.optim import FusedAdamW
+            self.opt = FusedAdamW(params, lr=lr, state_bits=8 if optimizer == "fused_adamw8" else 32)
         else:
             raise ValueError(optimizer)
         self.device = params[0].device

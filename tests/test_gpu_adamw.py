@@ -270,3 +270,45 @@ def test_tensors_that_the_kernels_do_not_take():
         b.step()
     for p, q in zip(ours, ref):
         assert torch.allclose(p.double(), q.double(), rtol=1e-5, atol=1e-6)      # both follow the formula in fp32, in another order
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_than_two_to_the_31_weights(bits):
+    """The weights around 2^31 and the last ones, against the same weights as a tensor of their own (whose codes differ, as their numbers do)."""
+    from ccfuser_b200.ops.optim import adamw_step, state8, state_values
+    n = 2 ** 31 + 5000
+    p, g = torch.empty(n, device="cuda", dtype=torch.bfloat16).normal_(0, 1, generator=_gen(14)), torch.empty(n, device="cuda", dtype=torch.bfloat16).normal_(0, 1, generator=_gen(15))
+    if bits == 8:
+        m, v, e = state8(p)
+    else:
+        m, v, e = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda"), None
+    parts = [(2 ** 31 - 5 * 256, 2 ** 31 + 5 * 256), (n - 4 * 256 - 5000 % 256, n)]
+    small = [(p[a:b].clone(), g[a:b].clone()) for a, b in parts]
+    adamw_step([p], [g], [m], [v], 1, exponents=None if e is None else [e], seed=3, **RATES)
+    for (a, b), (q, h) in zip(parts, small):
+        if bits == 8:
+            cm, cv, ce = state8(q)
+            adamw_step([q], [h], [cm], [cv], 1, exponents=[ce], seed=3, **RATES)
+            block = slice(a // 256, a // 256 + ce.shape[1])
+            assert a % 256 == 0 and torch.equal(e[0, block], ce[0])
+            got = state_values(m[a:b], e[:, block]).float()
+            exact = h.float() * (1 - RATES["betas"][0])
+            assert bool(((got - exact).abs() <= exact.abs() / 8 + 2.0 ** -16).all())
+        else:
+            cm, cv = torch.zeros(q.shape, device="cuda"), torch.zeros(q.shape, device="cuda")
+            adamw_step([q], [h], [cm], [cv], 1, **RATES)
+            assert torch.equal(m[a:b], cm) and torch.equal(v[a:b], cv)
+        assert torch.equal(p[a:b], q)
+
+
+def test_steps_in_inference_mode_and_on_another_stream():
+    from ccfuser_b200.ops.optim import adamw_step, state8
+    runs = []
+    for how in (torch.no_grad, torch.inference_mode):
+        with how():
+            p, g = torch.ones(5000, device="cuda").half(), torch.full((5000,), 0.5, device="cuda").half()
+            m, v, e = state8(p)
+            for step in range(1, 4):
+                adamw_step([p], [g], [m], [v], step, exponents=[e], seed=1, **RATES)
+            runs.append([t.clone() for t in (p, m, v, e)])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))

@@ -254,3 +254,92 @@ def test_transforms_take_torch_operations():
     f(xs, w).sum().backward()
     R.assert_close(gx, xs.grad.double(), 8 * R.U * xs.grad.double().abs())
     assert isinstance(order, ExpertOrder)
+
+
+@pytest.mark.parametrize("tokens,k,experts,capacity,align", [(700000, 2, 8, None, 16), (300000, 8, 100, 20000, 1), (1100000, 1, 300, None, 128)])
+def test_orders_of_many_tiles(tokens, k, experts, capacity, align):
+    """More slots than a wave of blocks holds at a time, against torch's operations on the host (which are tested against loops)."""
+    from ccfuser_b200.ops.expert_sort import expert_order
+    idx = _idx(_gen(k), tokens, k, experts, skew=1)
+    for got, want in zip(expert_order(idx, experts, capacity, align), expert_order(idx.cpu(), experts, capacity, align)):
+        assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("tokens,d", [(70001, 32768), (33000, 65537)])
+def test_more_than_two_to_the_31_elements(tokens, d):
+    """Rows of 16 bytes and odd ones; a third of the tokens is looked at."""
+    from ccfuser_b200.ops.expert_sort import return_rows, sort_by_expert
+    g = _gen(d)
+    idx = _idx(g, tokens, 1, 5)
+    x = torch.empty(tokens, d, device="cuda", dtype=torch.bfloat16).normal_(0, 1, generator=g).requires_grad_(True)
+    rows, order = sort_by_expert(x, idx, 5)
+    look = torch.arange(0, order.row_slot.numel(), 3, device="cuda")
+    look = look[order.row_slot[look] >= 0]
+    assert bool((rows.detach()[look] == x.detach()[order.row_slot[look].long()]).all())
+    w = torch.rand(tokens, 1, device="cuda", generator=g)
+    values = rows.detach().requires_grad_(True)
+    y = return_rows(values, order, w)
+    token = torch.arange(1, tokens, 3, device="cuda")
+    on = order.slot_row[token, 0] >= 0
+    want = torch.where(on[:, None], x.detach()[token].float() * w[token], 0.0).bfloat16()
+    assert torch.equal(y.detach()[token], want)
+    d_rows, = torch.autograd.grad(y, [values], y.detach())
+    want = torch.where((order.row_slot[look] >= 0)[:, None], (y.detach().float()[order.row_slot[look].long()] * w[order.row_slot[look].long()]), 0.0).bfloat16()
+    assert torch.equal(d_rows[look], want)
+    dx, = torch.autograd.grad(rows, [x], d_rows)
+    assert torch.equal(dx[token], torch.where(on[:, None], d_rows[order.slot_row[token, 0].clamp(min=0).long()], torch.zeros((), dtype=dx.dtype, device="cuda")))
+
+
+def test_inference_mode_saved_tensor_hooks_and_recomputation():
+    from torch.utils.checkpoint import checkpoint
+
+    from ccfuser_b200.ops.expert_sort import return_rows, sort_by_expert
+    g = _gen(21)
+    idx = _idx(g, 90, 2, 6)
+    x, w = torch.randn(90, 40, generator=g, device="cuda").half().requires_grad_(True), torch.rand(90, 2, generator=g, device="cuda").requires_grad_(True)
+
+    def f(x, w):
+        rows, order = sort_by_expert(x, idx, 6, align=4)
+        return return_rows(torch.tanh(rows), order, w)
+
+    want = torch.autograd.grad(f(x, w), [x, w], torch.ones(90, 40, device="cuda").half())
+    with torch.inference_mode():
+        y = f(x, w)
+    assert torch.equal(y.clone(), f(x, w).detach())
+    strided = lambda t: t if t.dim() == 0 else torch.stack([t, t], dim=-1)[..., 1]  # noqa: E731
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: strided(t.cuda())):
+        y = f(x, w)
+    got = torch.autograd.grad(y, [x, w], torch.ones_like(y))
+    again = checkpoint(f, x, w, use_reentrant=False)
+    third = torch.autograd.grad(again, [x, w], torch.ones_like(again))
+    for a, b, c in zip(want, got, third):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_calls_from_two_threads():
+    import threading
+
+    from ccfuser_b200.ops.expert_sort import return_rows, sort_by_expert
+    g = _gen(22)
+    sets = [(_idx(g, 2000, 2, 16), torch.randn(2000, 129, generator=g, device="cuda")) for _ in range(2)]
+    want, got = [], [[], []]
+
+    def call(i):
+        rows, order = sort_by_expert(sets[i][1], sets[i][0], 16)
+        return return_rows(rows, order)
+
+    want = [call(i) for i in range(2)]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(call(i))
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(len(r) == 20 and torch.equal(y, want[i]) for i, r in enumerate(got) for y in r)

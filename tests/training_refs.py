@@ -114,6 +114,9 @@ def stored(x, rows, bits, second):
             if top > 0:
                 mantissa, e = math.frexp(top)            # [1/2, 1)
                 e = max(e - 1 + (mantissa > 0.9375), -87)
+            if e > 127:      # no power of two of fp32
+                out += [math.nan] * len(block)
+                continue
             for i in block:
                 a = abs(flat[i]) * 2.0 ** -e
                 binade = max(math.frexp(a)[1] - 1 if a else lowest, lowest)
