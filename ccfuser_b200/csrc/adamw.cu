@@ -24,7 +24,12 @@ constexpr int kAdamPer = 8;                                   // weights of a th
 constexpr int kAdamChunk = kAdamThreads * kAdamPer;           // of a block
 constexpr int kAdamMost = 400;                                // tensors of a launch: kernel arguments end at 32 KB
 constexpr int kAdamFew = 32;
-constexpr int kAdam8Blocks = 5;                               // per SM: 200 M weights of bf16 424 us; 4: 470, 6 spill registers: 422 (fp32 477, 518, 489)
+// 8-bit moments. Blocks per SM: as many as leave the registers in place (16-bit weights: four 470, five 424, six 415 us for 200 M; fp32 518, 477, 489)
+template <int kType>
+constexpr int kAdam8Blocks = kType == kFp32 ? 5 : 6;
+// Blocks of weights that a warp takes one after another, while two waves of thread blocks are left: what a thread block does first (its tensor, its constants) is a tenth of
+// one turn. 285 M weights of 14 tensors with one, four, eight and sixteen turns 710, 599, 581 and 561 us. Not fp32 weights: the loop does not fit their registers (738 -> 845).
+constexpr int kAdam8Turns = 16;
 
 struct AdamScalars {
   float decay, rate, inv_root, pad0;   // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
@@ -50,7 +55,7 @@ struct AdamTable {
   AdamScalars now;
   float b1, one_b1, b2, one_b2, eps;
   float minus_zero;
-  int count;
+  int count, turns;                    // turns: blocks of weights of a warp, one after another
   AdamEntry entry[kCount];
 };
 static_assert(sizeof(AdamTable<kAdamMost>) <= 32764);
@@ -104,14 +109,21 @@ __device__ __forceinline__ unsigned block_exponent(unsigned largest) {
   return largest >= 0x7f800000u ? 255u : max((largest + 0xfffffu) >> 23, 40u);
 }
 // ---- the step --------------------------------------------------------------------------------------------------------
+// The entry of this thread block: the last one whose first block is not behind it.
 template <int kCount>
 __device__ __forceinline__ int find_entry(const AdamTable<kCount>& a) {
-  int lo = 0, hi = a.count;   // the last entry whose first block is not behind this one
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.entry[mid].first_block <= blockIdx.x) lo = mid; else hi = mid;
+  if (a.count == 1) return 0;
+  __shared__ int found;
+  if (threadIdx.x == 0) {
+    int lo = 0, hi = a.count;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.entry[mid].first_block <= blockIdx.x) lo = mid; else hi = mid;
+    }
+    found = lo;
   }
-  return lo;
+  __syncthreads();
+  return found;
 }
 
 struct AdamRates {
@@ -151,6 +163,7 @@ __device__ __forceinline__ void store_eight(void* base, long long at, const floa
   }
 }
 
+// Moments in fp32. Bound by memory: 22 bytes a weight of bf16, 28 of fp32; 285 M weights of 14 tensors 901 us (the copy rate says 960), 18.9 M fp32 weights of 96 tensors 79 us (81).
 template <int kType, int kCount>
 __global__ void __launch_bounds__(kAdamThreads) adamw32_kernel(const __grid_constant__ AdamTable<kCount> a) {
   const AdamEntry& e = a.entry[find_entry(a)];
@@ -187,7 +200,8 @@ __global__ void __launch_bounds__(kAdamThreads) adamw32_kernel(const __grid_cons
 }
 
 // A warp has a block of CCF_ADAMW_BLOCK weights, eight a lane, as pairs: one instruction for two operations, each rounded as alone. Bound by its
-// instructions next to 10 bytes a weight of bf16.
+// integer instructions (55 a weight of all kinds; ALU pipe 67 %, issue slots 76 %) next to 10 bytes a weight of bf16: 285 M weights of 14 tensors 565 us of bf16 (436 at the copy rate),
+// 750 of fp32 (697). Scalar arithmetic instead of pairs 464 us where pairs take 424, constants as pairs in the arguments 443, shifts as products 440 (200 M).
 struct Place {
   long long block, at;   // of the tensor's blocks, first weight of this lane
   int here;              // its number of weights, 0 to 8
@@ -274,117 +288,121 @@ __device__ __forceinline__ void update_pairs(float (&p)[8], const f32x2 (&m)[4],
 }
 
 template <int kType, int kCount>
-__global__ void __launch_bounds__(kAdamThreads, kAdam8Blocks) adamw8_kernel(const __grid_constant__ AdamTable<kCount> a) {
+__global__ void __launch_bounds__(kAdamThreads, kAdam8Blocks<kType>) adamw8_kernel(const __grid_constant__ AdamTable<kCount> a) {
   const AdamEntry& e = a.entry[find_entry(a)];
   const AdamScalars s = a.device != nullptr ? *a.device : a.now;
   const AdamRates r = {a.b1, a.one_b1, a.b2, a.one_b2, a.eps};
-  const Place place = place_of(static_cast<long long>(blockIdx.x - e.first_block) * (kAdamThreads / 32), e.n, e.width, e.row_blocks);
-  const long long at = place.at, block = place.block;
-  const int here = place.here;
-  if (__all_sync(0xffffffffu, here == 0)) return;      // a warp behind the last block
   unsigned char* const pm = static_cast<unsigned char*>(e.m);
   unsigned char* const pv = static_cast<unsigned char*>(e.v);
-  const bool whole = here == kAdamPer && e.vectors != 0;
-  float p[8] = {}, g[8] = {};
-  uint2 cm = {}, cv = {};
-  if (whole) {
-    cm = *reinterpret_cast<const uint2*>(pm + at);
-    cv = *reinterpret_cast<const uint2*>(pv + at);
-    load_eight<kType>(e.g, at, g);
-    load_eight<kType>(e.p, at, p);
-  } else {
-    unsigned bm[2] = {}, bv[2] = {};
+  long long first = static_cast<long long>(blockIdx.x - e.first_block) * (kType == kFp32 ? 1 : a.turns) * (kAdamThreads / 32);
+#pragma unroll 1
+  for (int turn = 0; turn < (kType == kFp32 ? 1 : a.turns); ++turn, first += kAdamThreads / 32) {
+    const Place place = place_of(first, e.n, e.width, e.row_blocks);
+    const long long at = place.at, block = place.block;
+    const int here = place.here;
+    if (__all_sync(0xffffffffu, here == 0)) return;      // a warp behind the last block
+    const bool whole = here == kAdamPer && e.vectors != 0;
+    float p[8] = {}, g[8] = {};
+    uint2 cm = {}, cv = {};
+    if (whole) {
+      cm = *reinterpret_cast<const uint2*>(pm + at);
+      cv = *reinterpret_cast<const uint2*>(pv + at);
+      load_eight<kType>(e.g, at, g);
+      load_eight<kType>(e.p, at, p);
+    } else {
+      unsigned bm[2] = {}, bv[2] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i >= here) break;
-      bm[i / 4] |= static_cast<unsigned>(pm[at + i]) << (8 * (i & 3));
-      bv[i / 4] |= static_cast<unsigned>(pv[at + i]) << (8 * (i & 3));
-      g[i] = load_elem<kType>(e.g, at + i);
-      p[i] = load_elem<kType>(e.p, at + i);
-    }
-    cm = make_uint2(bm[0], bm[1]);
-    cv = make_uint2(bv[0], bv[1]);
-  }
-  const Scale old(e.e[2 * block], e.e[2 * block + 1]);
-  const f32x2 nought = bc2(a.minus_zero);
-  f32x2 m[4], v[4];
-  float top_m = 0.f, top_v = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const f32x2 g2 = pk2(g[2 * i], g[2 * i + 1]);
-    m[i] = mul2(first_pair(i < 2 ? cm.x : cm.y, i & 1), bc2(old.m));
-    v[i] = mul2(mul2(second_pair(i < 2 ? cv.x : cv.y, i & 1), bc2(0x1p100f)), bc2(old.v));
-    m[i] = add2(product2(m[i], bc2(r.b1), nought), product2(g2, bc2(r.one_b1), nought));
-    v[i] = add2(product2(v[i], bc2(r.b2), nought), product2(mul2(g2, g2), bc2(r.one_b2), nought));
-    float x, y;
-    upk2(m[i], x, y);
-    top_m = largest(top_m, x, y);
-    upk2(v[i], x, y);
-    top_v = largest(top_v, x, y);
-  }
-  const unsigned all_m = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m)), all_v = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
-  // the weights first: their registers are free for the codes then
-  if (r.eps >= 1e-10f) update_pairs<true>(p, m, v, r, s);
-  else update_pairs<false>(p, m, v, r, s);
-  if (whole) {
-    store_eight<kType>(e.p, at, p);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < here) store_elem<kType>(e.p, at + i, p[i]);
-  }
-  const unsigned em = block_exponent(all_m), ev = block_exponent(all_v);
-  const bool near = em <= 127 + 14 && ev <= 127 + 30;      // else the factors of the way back leave the range of fp32 and are two
-  const f32x2 im = bc2(power_of_two(near ? 127 - 112 - static_cast<int>(em) : em == 255 ? 0 : 127 + 8 - static_cast<int>(em)));
-  const f32x2 iv = bc2(power_of_two(near ? 127 - 96 - static_cast<int>(ev) : ev == 255 ? 0 : 127 + 4 - static_cast<int>(ev)));
-  const unsigned key = s.key + e.key + static_cast<unsigned>(at);
-  unsigned nm[2], nv[2];
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    unsigned wm[4], wv[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      f32x2 dm = mul2(m[2 * q + i], im), dv = mul2(v[2 * q + i], iv);
-      if (!near) {
-        dm = mul2(dm, bc2(0x1p-120f));
-        dv = mul2(dv, bc2(0x1p-100f));
+      for (int i = 0; i < 8; ++i) {
+        if (i >= here) break;
+        bm[i / 4] |= static_cast<unsigned>(pm[at + i]) << (8 * (i & 3));
+        bv[i / 4] |= static_cast<unsigned>(pv[at + i]) << (8 * (i & 3));
+        g[i] = load_elem<kType>(e.g, at + i);
+        p[i] = load_elem<kType>(e.p, at + i);
       }
-      float xm[2], xv[2];
-      upk2(dm, xm[0], xm[1]);
-      upk2(dv, xv[0], xv[1]);
+      cm = make_uint2(bm[0], bm[1]);
+      cv = make_uint2(bv[0], bv[1]);
+    }
+    const Scale old(e.e[2 * block], e.e[2 * block + 1]);
+    const f32x2 nought = bc2(a.minus_zero);
+    f32x2 m[4], v[4];
+    float top_m = 0.f, top_v = 0.f;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const unsigned h = mix(key + 4 * q + 2 * i + k), u = __float_as_uint(xm[k]);
-        wm[2 * i + k] = u + (h << 12 >> 12);      // does not reach the sign
-        wv[2 * i + k] = __float_as_uint(xv[k]) + (h >> 12);
+    for (int i = 0; i < 4; ++i) {
+      const f32x2 g2 = pk2(g[2 * i], g[2 * i + 1]);
+      m[i] = mul2(first_pair(i < 2 ? cm.x : cm.y, i & 1), bc2(old.m));
+      v[i] = mul2(mul2(second_pair(i < 2 ? cv.x : cv.y, i & 1), bc2(0x1p100f)), bc2(old.v));
+      m[i] = add2(product2(m[i], bc2(r.b1), nought), product2(g2, bc2(r.one_b1), nought));
+      v[i] = add2(product2(v[i], bc2(r.b2), nought), product2(mul2(g2, g2), bc2(r.one_b2), nought));
+      float x, y;
+      upk2(m[i], x, y);
+      top_m = largest(top_m, x, y);
+      upk2(v[i], x, y);
+      top_v = largest(top_v, x, y);
+    }
+    const unsigned all_m = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m)), all_v = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
+    // the weights first: their registers are free for the codes then
+    if (r.eps >= 1e-10f) update_pairs<true>(p, m, v, r, s);
+    else update_pairs<false>(p, m, v, r, s);
+    if (whole) {
+      store_eight<kType>(e.p, at, p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < here) store_elem<kType>(e.p, at + i, p[i]);
+    }
+    const unsigned em = block_exponent(all_m), ev = block_exponent(all_v);
+    const bool near = em <= 127 + 14 && ev <= 127 + 30;      // else the factors of the way back leave the range of fp32 and are two
+    const f32x2 im = bc2(power_of_two(near ? 127 - 112 - static_cast<int>(em) : em == 255 ? 0 : 127 + 8 - static_cast<int>(em)));
+    const f32x2 iv = bc2(power_of_two(near ? 127 - 96 - static_cast<int>(ev) : ev == 255 ? 0 : 127 + 4 - static_cast<int>(ev)));
+    const unsigned key = s.key + e.key + static_cast<unsigned>(at);
+    unsigned nm[2], nv[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      unsigned wm[4], wv[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f32x2 dm = mul2(m[2 * q + i], im), dv = mul2(v[2 * q + i], iv);
+        if (!near) {
+          dm = mul2(dm, bc2(0x1p-120f));
+          dv = mul2(dv, bc2(0x1p-100f));
+        }
+        float xm[2], xv[2];
+        upk2(dm, xm[0], xm[1]);
+        upk2(dv, xv[0], xv[1]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const unsigned h = mix(key + 4 * q + 2 * i + k), u = __float_as_uint(xm[k]);
+          wm[2 * i + k] = u + (h << 12 >> 12);      // does not reach the sign
+          wv[2 * i + k] = __float_as_uint(xv[k]) + (h >> 12);
+        }
+      }
+      nm[q] = em == 255 ? 0u : four_codes<false>(wm);
+      nv[q] = four_codes<true>(wv);
+      if ((nv[q] - 0x01010101u) & ~nv[q] & 0x80808080u) {      // a code of 0: of 0 alone
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float o[2];
+          upk2(v[2 * q + i / 2], o[0], o[1]);
+          if ((nv[q] >> (8 * i) & 0xffu) == 0 && o[i & 1] > 0.f) nv[q] |= 1u << (8 * i);
+        }
+      }
+      if (ev == 255) nv[q] = 0;
+    }
+    if (whole) {
+      *reinterpret_cast<uint2*>(pm + at) = make_uint2(nm[0], nm[1]);
+      *reinterpret_cast<uint2*>(pv + at) = make_uint2(nv[0], nv[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i >= here) break;
+        pm[at + i] = static_cast<unsigned char>(nm[i / 4] >> (8 * (i & 3)));
+        pv[at + i] = static_cast<unsigned char>(nv[i / 4] >> (8 * (i & 3)));
       }
     }
-    nm[q] = em == 255 ? 0u : four_codes<false>(wm);
-    nv[q] = four_codes<true>(wv);
-    if ((nv[q] - 0x01010101u) & ~nv[q] & 0x80808080u) {      // a code of 0: of 0 alone
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float o[2];
-        upk2(v[2 * q + i / 2], o[0], o[1]);
-        if ((nv[q] >> (8 * i) & 0xffu) == 0 && o[i & 1] > 0.f) nv[q] |= 1u << (8 * i);
-      }
+    if ((threadIdx.x & 31) == 0) {
+      e.e[2 * block] = static_cast<unsigned char>(em);
+      e.e[2 * block + 1] = static_cast<unsigned char>(ev);
     }
-    if (ev == 255) nv[q] = 0;
-  }
-  if (whole) {
-    *reinterpret_cast<uint2*>(pm + at) = make_uint2(nm[0], nm[1]);
-    *reinterpret_cast<uint2*>(pv + at) = make_uint2(nv[0], nv[1]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i >= here) break;
-      pm[at + i] = static_cast<unsigned char>(nm[i / 4] >> (8 * (i & 3)));
-      pv[at + i] = static_cast<unsigned char>(nv[i / 4] >> (8 * (i & 3)));
-    }
-  }
-  if ((threadIdx.x & 31) == 0) {
-    e.e[2 * block] = static_cast<unsigned char>(em);
-    e.e[2 * block + 1] = static_cast<unsigned char>(ev);
   }
 }
 
@@ -461,11 +479,18 @@ static int launch_adamw(const CcfAdamw& a, int first, int count, cudaStream_t st
   t.minus_zero = -0.f;
   t.count = count;
   long long blocks = 0;
+  for (int i = 0; i < count; ++i) blocks += blocks_of(a.tensors[first + i]);
+  t.turns = 1;
+  if (a.tensors[first].e != nullptr && kType != kFp32) {
+    const long long wave = kAdam8Blocks<kType> * sm_count();
+    while (t.turns < kAdam8Turns && blocks / (2 * t.turns) >= 2 * wave) t.turns *= 2;
+  }
+  blocks = 0;
   for (int i = 0; i < count; ++i) {
     const CcfAdamwTensor& from = a.tensors[first + i];
     t.entry[i] = {from.p, from.g, from.m, from.v, from.e, from.n, from.n / from.rows, row_blocks_of(from.n, from.rows), static_cast<unsigned>(blocks),
                   static_cast<unsigned>(from.number) * 0x9E3779B9u, vectors_of(from.p, from.g, from.m, from.v, from.n, from.rows)};
-    blocks += blocks_of(from);
+    blocks += (blocks_of(from) + t.turns - 1) / t.turns;
   }
   const auto kern = a.tensors[first].e != nullptr ? adamw8_kernel<kType, kCount> : adamw32_kernel<kType, kCount>;
   kern<<<static_cast<unsigned>(blocks), kAdamThreads, 0, st>>>(t);

@@ -256,8 +256,8 @@ def _spread(values, slot_row, row_slot, weights):
 def expert_order(idx: torch.Tensor, num_experts: int, capacity: Optional[int] = None, align: int = 1) -> ExpertOrder:
     """The rows of a call's slots. ``idx [..., top_k]`` (int64 or int32): the expert of each slot; a number outside [0, num_experts) is no expert's, and that slot
     has no row. ``capacity``: rows that an expert takes at most, the first ones. ``align``: every expert's rows begin at a multiple of it."""
-    if idx.is_cuda and idx.numel() > 0 and not N.transformed(idx):
-        module = _module()
+    if idx.is_cuda and idx.numel() > 0 and not N.transformed(idx) and not torch.jit.is_tracing():      # a trace would miss the launches
+        module = N.torch_module()
         if module is not None:      # checks its arguments as below
             return ExpertOrder(*module.expert_order(idx, num_experts, capacity, align))
         _check_idx(idx, num_experts, capacity, align)

@@ -105,7 +105,7 @@ def state_values(codes: torch.Tensor, exponents: torch.Tensor, second: bool = Fa
     rows = exponents.shape[0] if exponents.dim() == 3 else 1
     if codes.device != exponents.device:
         raise ValueError(f"codes are on {codes.device}, their exponents on {exponents.device}")
-    if not codes.is_cuda or codes.numel() == 0 or N.transformed(codes):
+    if not codes.is_cuda or codes.numel() == 0 or N.transformed(codes) or torch.jit.is_tracing():
         return _decode(codes, exponents.reshape(rows, -1, 2), second).to(dtype)
     module = N.torch_module()
     if module is not None:

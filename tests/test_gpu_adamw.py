@@ -312,3 +312,19 @@ def test_steps_in_inference_mode_and_on_another_stream():
                 adamw_step([p], [g], [m], [v], step, exponents=[e], seed=1, **RATES)
             runs.append([t.clone() for t in (p, m, v, e)])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_turns_of_large_tensors():
+    """Blocks of weights that a warp takes one after another, ends of tensors and rows among them: the codes of torch's operations."""
+    from ccfuser_b200.ops.optim import adamw_step
+    shapes, rows = [(3, 1500001), (9,), (2, 2000003), (4096,), (4000007,), (5, 700, 1024)], [3, 1, 2, 1, 1, 5]
+    p, g, _, _ = _set(16, shapes, torch.bfloat16)
+    state = _state8(17, p, rows)
+    host = [[t.cpu() for t in ts] for ts in (p, g, *state)]
+    for (a, b, m, v, e) in ((p, g, *state), host):
+        adamw_step(a, b, m, v, 2, exponents=e, seed=11, **RATES)
+    for ts, hs in zip(state, host[2:]):
+        for a, b in zip(ts, hs):
+            assert torch.equal(a.cpu(), b)
+    for a, b in zip(p, host[0]):
+        R.assert_close(a, b.double(), R.half_step(a.dtype) * 2 * b.double().abs() + 64 * R.U * (b.double().abs() + 0.1))

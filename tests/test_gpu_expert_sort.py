@@ -343,3 +343,18 @@ def test_calls_from_two_threads():
     for t in threads:
         t.join()
     assert all(len(r) == 20 and torch.equal(y, want[i]) for i, r in enumerate(got) for y in r)
+
+
+def test_traced_calls():
+    """A trace holds the order as operations of torch and the rows as functions of their own: other inputs give other rows."""
+    from ccfuser_b200.ops.expert_sort import return_rows, sort_by_expert
+    g = _gen(23)
+
+    def f(x, idx, w):
+        rows, order = sort_by_expert(x, idx, 6, align=4)
+        return return_rows(rows * 2, order, w)
+
+    sets = [(torch.randn(50, 24, generator=g, device="cuda"), _idx(g, 50, 2, 6), torch.rand(50, 2, generator=g, device="cuda")) for _ in range(2)]
+    traced = torch.jit.trace(f, sets[0], check_trace=False)
+    for s in sets:
+        assert torch.equal(traced(*s), f(*s))
