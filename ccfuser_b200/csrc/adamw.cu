@@ -46,7 +46,7 @@ struct AdamEntry {
   long long n, width;                  // width: weights of a row
   unsigned row_blocks;                 // blocks of CCF_ADAMW_BLOCK of a row; 0: one row alone
   unsigned first_block, key;           // key: added to the step's
-  unsigned vectors;                    // eight weights, and their codes, can be read at once wherever a lane begins
+  unsigned vectors;                    // 1: eight weights and their moments are read at once wherever a lane begins, 2: their gradients too
 };
 
 template <int kCount>
@@ -152,6 +152,15 @@ __device__ __forceinline__ void load_eight(const void* base, long long at, float
   }
 }
 template <int kType>
+__device__ __forceinline__ void load_gradients(const AdamEntry& e, long long at, float (&g)[8]) {
+  if ((e.vectors & 2) != 0) {
+    load_eight<kType>(e.g, at, g);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = load_elem<kType>(e.g, at + i);
+  }
+}
+template <int kType>
 __device__ __forceinline__ void store_eight(void* base, long long at, const float (&f)[8]) {
   uint4* q = reinterpret_cast<uint4*>(static_cast<char*>(base) + at * kElemBytes<kType>);
 #pragma unroll
@@ -171,11 +180,10 @@ __global__ void __launch_bounds__(kAdamThreads) adamw32_kernel(const __grid_cons
   const AdamRates r = {a.b1, a.one_b1, a.b2, a.one_b2, a.eps};
   const long long n = e.n, at = static_cast<long long>(blockIdx.x - e.first_block) * kAdamChunk + threadIdx.x * kAdamPer;
   if (at >= n) return;
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(e.p) | reinterpret_cast<uintptr_t>(e.g) | reinterpret_cast<uintptr_t>(e.m) | reinterpret_cast<uintptr_t>(e.v);
-  if ((bits & 15) == 0 && at + kAdamPer <= n) {
+  if ((e.vectors & 1) != 0 && at + kAdamPer <= n) {
     float p[8], g[8], m[8], v[8];
     load_eight<kType>(e.p, at, p);
-    load_eight<kType>(e.g, at, g);
+    load_gradients<kType>(e, at, g);
     load_eight<kFp32>(e.m, at, m);
     load_eight<kFp32>(e.v, at, v);
 #pragma unroll
@@ -224,9 +232,12 @@ __device__ __forceinline__ Place place_of(long long first, long long n, long lon
   p.here = left >= kAdamPer ? kAdamPer : left > 0 ? static_cast<int>(left) : 0;
   return p;
 }
-inline unsigned vectors_of(const void* p, const void* g, const void* m, const void* v, long long n, long long rows) {
-  const uintptr_t wide = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g), codes = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v);
-  return wide % 16 == 0 && codes % 8 == 0 && (rows == 1 || n / rows % 8 == 0);
+// Gradients by themselves: those that lie in a bucket of many begin anywhere.
+inline unsigned vectors_of(const void* p, const void* g, const void* m, const void* v, long long n, long long rows, bool eight) {
+  const uintptr_t moments = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v);
+  const bool rows_too = rows == 1 || n / rows % 8 == 0;
+  return (reinterpret_cast<uintptr_t>(p) % 16 == 0 && moments % (eight ? 8 : 16) == 0 && rows_too ? 1u : 0u) |
+         (reinterpret_cast<uintptr_t>(g) % 16 == 0 && rows_too ? 2u : 0u);
 }
 
 // A product that is rounded before something is added to it. The compiler merges a packed product with the packed sum behind it (a code of one weight in some
@@ -301,13 +312,13 @@ __global__ void __launch_bounds__(kAdamThreads, kAdam8Blocks<kType>) adamw8_kern
     const long long at = place.at, block = place.block;
     const int here = place.here;
     if (__all_sync(0xffffffffu, here == 0)) return;      // a warp behind the last block
-    const bool whole = here == kAdamPer && e.vectors != 0;
+    const bool whole = here == kAdamPer && (e.vectors & 1) != 0;
     float p[8] = {}, g[8] = {};
     uint2 cm = {}, cv = {};
     if (whole) {
       cm = *reinterpret_cast<const uint2*>(pm + at);
       cv = *reinterpret_cast<const uint2*>(pv + at);
-      load_eight<kType>(e.g, at, g);
+      load_gradients<kType>(e, at, g);
       load_eight<kType>(e.p, at, p);
     } else {
       unsigned bm[2] = {}, bv[2] = {};
@@ -422,7 +433,7 @@ __global__ void __launch_bounds__(kAdamThreads)
     if (place[k].here == 0) continue;
     e[k][0] = ex[2 * place[k].block];
     e[k][1] = ex[2 * place[k].block + 1];
-    if (place[k].here == kAdamPer && vectors != 0) {
+    if (place[k].here == kAdamPer && (vectors & 1) != 0) {
       c[k] = __ldg(reinterpret_cast<const uint2*>(codes + place[k].at));
     } else {
       unsigned b[2] = {};
@@ -442,7 +453,7 @@ __global__ void __launch_bounds__(kAdamThreads)
       const unsigned word = i < 2 ? c[k].x : c[k].y;
       upk2(kSecond ? mul2(mul2(second_pair(word, i & 1), bc2(0x1p100f)), bc2(scale.v)) : mul2(first_pair(word, i & 1), bc2(scale.m)), f[2 * i], f[2 * i + 1]);
     }
-    if (place[k].here == kAdamPer && vectors != 0) {
+    if (place[k].here == kAdamPer && (vectors & 1) != 0) {
       store_eight<kType>(out, place[k].at, f);
     } else {
 #pragma unroll
@@ -489,7 +500,7 @@ static int launch_adamw(const CcfAdamw& a, int first, int count, cudaStream_t st
   for (int i = 0; i < count; ++i) {
     const CcfAdamwTensor& from = a.tensors[first + i];
     t.entry[i] = {from.p, from.g, from.m, from.v, from.e, from.n, from.n / from.rows, row_blocks_of(from.n, from.rows), static_cast<unsigned>(blocks),
-                  static_cast<unsigned>(from.number) * 0x9E3779B9u, vectors_of(from.p, from.g, from.m, from.v, from.n, from.rows)};
+                  static_cast<unsigned>(from.number) * 0x9E3779B9u, vectors_of(from.p, from.g, from.m, from.v, from.n, from.e != nullptr ? from.rows : 1, from.e != nullptr)};
     blocks += (blocks_of(from) + t.turns - 1) / t.turns;
   }
   const auto kern = a.tensors[first].e != nullptr ? adamw8_kernel<kType, kCount> : adamw32_kernel<kType, kCount>;
@@ -563,7 +574,7 @@ int ccf_state_values(const void* codes, const unsigned char* e, void* out, long 
   const auto kern = type == kBf16   ? (second ? state_values_kernel<kBf16, true> : state_values_kernel<kBf16, false>)
                     : type == kFp16 ? (second ? state_values_kernel<kFp16, true> : state_values_kernel<kFp16, false>)
                                     : (second ? state_values_kernel<kFp32, true> : state_values_kernel<kFp32, false>);
-  kern<<<static_cast<unsigned>(blocks), kAdamThreads, 0, st>>>(c, e, out, n, n / rows, row_blocks_of(n, rows), vectors_of(out, nullptr, c, nullptr, n, rows));
+  kern<<<static_cast<unsigned>(blocks), kAdamThreads, 0, st>>>(c, e, out, n, n / rows, row_blocks_of(n, rows), vectors_of(out, nullptr, c, nullptr, n, rows, true));
   return launch_result();
 }
 

@@ -3,7 +3,8 @@
 // traced or the tensors are not on a GPU.
 #include <c10/cuda/CUDAGuard.h>
 
-#include <cmath>
+#include <torch/csrc/autograd/python_variable.h>
+
 #include <unordered_set>
 
 #include "adamw.h"
@@ -50,15 +51,15 @@ Order new_order(CcfOrder& o, const at::Tensor& idx, int64_t experts, const std::
   o.wide = idx.scalar_type() == at::kLong;
   o.rows = ccf_order_rows(o.slots, o.experts, o.capacity, o.align);
   TORCH_CHECK_VALUE(o.rows >= 0, "at most 2^31 - 1 rows in one call");
-  const int64_t scratch = ccf_order_scratch(o.slots, o.experts) / 4, small = 2 * experts + 1;
-  const at::Tensor all = at::empty({o.slots + o.rows + small + scratch}, at::TensorOptions(idx.device()).dtype(at::kInt));
-  const Order r = {part_of(all, 0, idx.sizes()), part_of(all, o.slots, {o.rows}), part_of(all, o.slots + o.rows, {experts}),
-                   part_of(all, o.slots + o.rows + experts, {experts + 1})};
+  const auto up = [](int64_t n) { return (n + 3) / 4 * 4; };      // each on 16 bytes
+  const int64_t at_base = up(experts), at_slots = at_base + up(experts + 1), at_rows = at_slots + up(o.slots), at_scratch = at_rows + up(o.rows);
+  const at::Tensor all = at::empty({at_scratch + ccf_order_scratch(o.slots, o.experts) / 4}, at::TensorOptions(idx.device()).dtype(at::kInt));
+  const Order r = {part_of(all, at_slots, idx.sizes()), part_of(all, at_rows, {o.rows}), part_of(all, 0, {experts}), part_of(all, at_base, {experts + 1})};
   o.slot_row = r.slot_row.data_ptr<int>();
   o.row_slot = r.row_slot.data_ptr<int>();
   o.counts = r.counts.data_ptr<int>();
   o.base = r.base.data_ptr<int>();
-  o.scratch = all.data_ptr<int>() + o.slots + o.rows + small;
+  o.scratch = all.data_ptr<int>() + at_scratch;
   return r;
 }
 
@@ -146,7 +147,6 @@ struct SortNode : TokenNode {
 
 struct ReturnNode : TokenNode {
   int64_t rows;
-  at::ScalarType weight_type;
   std::vector<int64_t> weight_shape;
   ReturnNode() { twice = true; }
   std::string name() const override { return "CcfReturnRowsBackward"; }
@@ -289,6 +289,27 @@ struct AdamwCall {
   std::vector<CcfAdamwTensor> tensors;
 };
 
+// The tensors of a list or tuple, without a count of references for each (a step of 60 tensors took the host 34 us with
+// std::vector<at::Tensor>, 19 so).
+// The interpreter's lock is held as long as they are used.
+struct TensorList {
+  py::object fast;      // keeps the items
+  std::vector<const at::Tensor*> items;
+  TensorList(const py::object& list, const char* name) {
+    fast = py::reinterpret_steal<py::object>(PySequence_Fast(list.ptr(), name));
+    if (!fast) throw py::error_already_set();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast.ptr());
+    PyObject** const from = PySequence_Fast_ITEMS(fast.ptr());
+    items.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      TORCH_CHECK_TYPE(THPVariable_Check(from[i]), name, ": element ", i, " is no tensor");
+      items.push_back(&THPVariable_Unpack(from[i]));
+    }
+  }
+  size_t size() const { return items.size(); }
+  const at::Tensor& operator[](size_t i) const { return *items[i]; }
+};
+
 void check_state(const at::Tensor& p, const at::Tensor& g, const at::Tensor& m, const at::Tensor& v, const at::Tensor* e, size_t i) {
   TORCH_CHECK_TYPE(g.layout() == at::kStrided && g.scalar_type() == p.scalar_type(), "grads: tensor ", i, " is ", g.layout(), " of ", g.scalar_type(), ", its parameter ",
                    p.scalar_type());
@@ -306,16 +327,22 @@ void check_state(const at::Tensor& p, const at::Tensor& g, const at::Tensor& m, 
 }
 
 // One step; false, with nothing changed, where a tensor is not one for the kernels (another type or device, not contiguous).
-bool adamw_step(const std::vector<at::Tensor>& params, const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& first, const std::vector<at::Tensor>& second,
-                const std::optional<std::vector<at::Tensor>>& exponents, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t seed, int64_t step,
-                const OptTensor& counter, const OptTensor& device_lr, const std::optional<std::vector<int64_t>>& numbers) {
+bool adamw_step(const py::object& params_, const py::object& grads_, const py::object& first_, const py::object& second_, const py::object& exponents_, double lr, double beta1,
+                double beta2, double eps, double weight_decay, int64_t seed, int64_t step, const OptTensor& counter, const OptTensor& device_lr,
+                const std::optional<std::vector<int64_t>>& numbers) {
+  const TensorList params(params_, "params"), grads(grads_, "grads"), first(first_, "exp_avgs"), second(second_, "exp_avg_sqs");
+  const bool eight = !exponents_.is_none();
+  const TensorList exponents(eight ? exponents_ : py::object(py::list()), "exponents");
   const size_t n = params.size();
+  TORCH_CHECK_VALUE(grads.size() == n && first.size() == n && second.size() == n && (!eight || exponents.size() == n) && (!numbers.has_value() || numbers->size() == n), n,
+                    " params need as many gradients, moments, exponents and numbers");
   std::vector<at::Tensor> packed_grads;      // lives until the launches
   std::vector<AdamwCall> calls;
   std::unordered_set<const void*> seen;
+  seen.reserve(n);
   for (size_t i = 0; i < n; ++i) {
     const at::Tensor &p = params[i], &g = grads[i], &m = first[i], &v = second[i];
-    const at::Tensor* const e = exponents.has_value() ? &(*exponents)[i] : nullptr;
+    const at::Tensor* const e = eight ? &exponents[i] : nullptr;
     if (!p.is_cuda() || !kernel_type(p) || !p.is_contiguous() || !m.is_contiguous() || !v.is_contiguous() || (e != nullptr && !e->is_contiguous())) return false;
     check_state(p, g, m, v, e, i);
     if (p.numel() == 0) continue;
@@ -380,7 +407,7 @@ bool adamw_step(const std::vector<at::Tensor>& params, const std::vector<at::Ten
     changed(params[i]);
     changed(first[i]);
     changed(second[i]);
-    if (exponents.has_value()) changed((*exponents)[i]);
+    if (eight) changed(exponents[i]);
   }
   if (counter.has_value()) changed(*counter);
   return true;
@@ -405,6 +432,6 @@ void ccf_torch::add_training_ops(py::module_& m) {
   m.def("sort_by_expert", &sort_by_expert, free);
   m.def("sort_rows", &sort_rows, free);
   m.def("return_rows", &return_rows, free);
-  m.def("adamw_step", &adamw_step, free);
+  m.def("adamw_step", &adamw_step);
   m.def("state_values", &state_values, free);
 }

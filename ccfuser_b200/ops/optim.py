@@ -155,11 +155,6 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     the list. ``step`` is the number of this step, from 1. With ``counter``, an int64 tensor of one element on the tensors' device, that is raised by one instead and read on the device, so that a captured
     call counts its replays; then ``lr`` may be an fp32 tensor of one element there. Values that are not finite make a weight NaN as in torch, and with 8-bit moments from the
     next step on all weights of its block. Tensors on a CPU, of fp64 or not contiguous take torch's operations, to the same codes."""
-    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
-    exponents = None if exponents is None else list(exponents)
-    numbers = None if numbers is None else [int(n) for n in numbers]
-    if any(t is not None and len(t) != len(params) for t in (grads, exp_avgs, exp_avg_sqs, exponents, numbers)):
-        raise ValueError(f"{len(params)} params need as many gradients, moments, exponents and numbers")
     if (step is None) == (counter is None):
         raise ValueError("either step or counter")
     if counter is None and step < 1:
@@ -174,12 +169,17 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if not (0.0 <= lr and 0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0 and 0.0 <= eps and 0.0 <= weight_decay):
         raise ValueError(f"lr, eps and weight_decay are at least 0, betas in [0, 1), got {lr}, {eps}, {weight_decay}, {beta1, beta2}")
     seed = (int(seed) + (1 << 63)) % (1 << 64) - (1 << 63)      # as C's 64 bits
-    if not params:
-        return
+    params, grads, exp_avgs, exp_avg_sqs = (t if isinstance(t, (list, tuple)) else list(t) for t in (params, grads, exp_avgs, exp_avg_sqs))
+    exponents = exponents if exponents is None or isinstance(exponents, (list, tuple)) else list(exponents)
+    numbers = numbers if numbers is None or isinstance(numbers, (list, tuple)) else list(numbers)
     rates = (lr, beta1, beta2, float(eps), float(weight_decay), seed)
-    traced = N.transformed(params[0])      # no memory to look at
-    module = N.torch_module() if params[0].is_cuda and not traced else None
+    traced = bool(params) and N.transformed(params[0])      # no memory to look at
+    module = N.torch_module() if params and params[0].is_cuda and not traced else None
     if module is not None and module.adamw_step(params, grads, exp_avgs, exp_avg_sqs, exponents, *rates, 0 if step is None else int(step), counter, device_lr, numbers):
+        return
+    if any(t is not None and len(t) != len(params) for t in (grads, exp_avgs, exp_avg_sqs, exponents, numbers)):
+        raise ValueError(f"{len(params)} params need as many gradients, moments, exponents and numbers")
+    if not params:
         return
     tensors = list(zip(params, grads, exp_avgs, exp_avg_sqs, [None] * len(params) if exponents is None else exponents))
     seen = set()
