@@ -13,11 +13,12 @@ namespace ccf {
 
 // ---- order -----------------------------------------------------------------------------------------------------------
 // Bound by latency: a few bytes a slot. Up to a block's threads in slots one block does it all. Above, each block counts its slots' experts in a first kernel, and in
-// the second adds up the counts of the blocks in front of it. Both kernels, of a captured graph: 16384 slots of 64 experts 7.6 us with blocks of 512 threads and 8.4 with 1024
-// (of 128 experts 9.0 and 8.4); 131072 of 256 with at most 16, 32, 64 and 128 blocks 31.7, 20.8, 17.0 and 19.8; 524288 107, 58, 36 and 29.
+// the second adds up the counts of the blocks in front of it. Both kernels, of a captured graph, with blocks of 512 and of 1024 threads: 16384 slots of 64 experts 7.0 and 8.5 us, of
+// 128 6.7 and 8.7, 65536 of 128 8.6 and 9.0, of 256 11.0 and 9.9, 131072 of 256 12.5 and 11.5, 524288 25.2 and 22.3 (with at most 16, 32 and 64 blocks instead of 128, these two:
+// 31, 19, 13 and 108, 57, 33).
 constexpr int kOrderThreads = 1024;
-constexpr int kOrderBlocks = 64;                  // a block reads the counts of as many; twice that for more than kOrderMany slots
-constexpr long long kOrderMany = 1 << 18;
+constexpr int kOrderBlocks = 128;                 // a block reads the counts of as many
+constexpr long long kOrderMany = 1 << 24;         // slots x experts from which on blocks have kOrderThreads, else half of them
 constexpr int kOrderMost = 8;                     // slots of a thread at a time
 
 struct OrderShape {
@@ -28,14 +29,14 @@ inline OrderShape order_shape(long long slots, int experts) {
   OrderShape s;
   const int least = (experts + 31) / 32 * 32;      // one thread per expert
   const long long want = (slots + 31) / 32 * 32;
-  const int most = experts <= 64 ? kOrderThreads / 2 : kOrderThreads, blocks = slots > kOrderMany ? 2 * kOrderBlocks : kOrderBlocks;
+  const int most = slots * experts < kOrderMany ? kOrderThreads / 2 : kOrderThreads;
   s.threads = want > most ? most : static_cast<int>(want);
   if (s.threads < least) s.threads = least;
   s.per = 1;
-  while (s.per < kOrderMost && static_cast<long long>(s.threads) * s.per * blocks < slots) s.per *= 2;
+  while (s.per < kOrderMost && static_cast<long long>(s.threads) * s.per * kOrderBlocks < slots) s.per *= 2;
   const long long tile = static_cast<long long>(s.threads) * s.per;
   const long long all = (slots + tile - 1) / tile;
-  s.tiles = static_cast<int>((all + blocks - 1) / blocks);
+  s.tiles = static_cast<int>((all + kOrderBlocks - 1) / kOrderBlocks);
   s.blocks = static_cast<int>((all + s.tiles - 1) / s.tiles);
   return s;
 }
@@ -141,13 +142,19 @@ __global__ void __launch_bounds__(kOrderThreads) order_place_kernel(const __grid
   if (gridDim.x > 1) {
     wait_for_previous();
     const int* const counts = behind(static_cast<const int*>(o.scratch));
-    const int blocks = static_cast<int>(gridDim.x);
-    for (int i = tid; i < blocks * E; i += blockDim.x) {
-      const int v = counts[i];
-      if (v == 0) continue;
-      const int x = i % E;
-      atomicAdd(&total[x], v);
-      if (i < static_cast<int>(blockIdx.x) * E) atomicAdd(&before[x], v);
+    // a thread adds up every `groups`-th block's count of one expert
+    const int blocks = static_cast<int>(gridDim.x), mine = static_cast<int>(blockIdx.x), width = E < 32 ? E : (E + 31) / 32 * 32, groups = blockDim.x / width;
+    const int group = tid / width, x = tid - group * width;
+    if (x < E && group < groups) {
+      int all = 0, front = 0;
+#pragma unroll 8
+      for (int b = group; b < blocks; b += groups) {
+        const int v = counts[b * E + x];
+        all += v;
+        if (b < mine) front += v;
+      }
+      atomicAdd(&total[x], all);
+      atomicAdd(&before[x], front);
     }
   } else if (tid < E) {
     int run = 0;

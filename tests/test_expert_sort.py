@@ -67,7 +67,7 @@ def test_row_counts():
         assert want % align == 0
     assert lib.ccf_order_rows(2 ** 30, 1024, 2 ** 30, 65536) == S.order_rows(2 ** 30, 1024, None, 65536) == 2 ** 30 + 1023 * 65536
     assert lib.ccf_order_rows(-1, 4, 1, 1) == lib.ccf_order_rows(8, 0, 1, 1) == lib.ccf_order_rows(8, 4, 0, 1) == lib.ccf_order_rows(8, 4, 1, 0) == -1
-    assert lib.ccf_order_scratch(1024, 65) == 0 < lib.ccf_order_scratch(1025, 65) == 2 * 65 * 4
+    assert lib.ccf_order_scratch(512, 65) == 0 < lib.ccf_order_scratch(513, 65) == 2 * 65 * 4 and lib.ccf_order_scratch(1024, 1024) == 0
     assert lib.ccf_order_scratch(0, 4) == lib.ccf_order_scratch(8, 0) == lib.ccf_order_scratch(8, 1025) == -1
 
 
