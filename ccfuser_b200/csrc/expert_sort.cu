@@ -591,8 +591,8 @@ __global__ void __launch_bounds__(kRowThreads) return_odd_rows_bwd_kernel(const 
 
 // ---- a few tokens: order and rows in one launch ----------------------------------------------------------------------------
 // Every block orders all slots for itself and copies the rows of its tokens. Of a captured graph, with the two or three kernels above: 16 tokens of 2048, two of 64
-// experts, 2.8 us (6.6), 128 tokens 3.0 (5.9), 256 4.6 (6.3), 512 5.5 (7.5), in tiles of 128 rows 10.3 (14.2); 128 tokens with eight of 256 experts 7.9 (14.0).
-constexpr int kFewThreads = 256, kFewPer = 4, kFewSlots = kFewThreads * kFewPer, kFewExperts = kFewThreads;
+// experts, 2.7 us (6.5), 128 tokens 3.0 (5.9), 256 4.5 (6.2), 512 5.5 (8.8), 1024 8.7 (9.2); 512 in tiles of 128 rows 10.4 (15.0), 128 tokens with eight of 256 experts 7.9 (14.7).
+constexpr int kFewThreads = 256, kFewPer = 8, kFewSlots = kFewThreads * kFewPer, kFewExperts = kFewThreads;
 
 // kBytes: of an element where rows do not all begin on 16 bytes, else 0
 template <int kPer, int kBytes>
@@ -832,8 +832,10 @@ int ccf_sort_by_expert(const CcfOrder* o, const CcfRows* r, void* stream) {
   const long long want = r->tokens + (r->rows - o->slots > 0 ? (r->rows - o->slots) / 8 : 0);
   const unsigned blocks = static_cast<unsigned>(want < sm_count() ? want : sm_count());
   const int bytes = aligned ? 0 : elem_bytes(r->type);
-  const auto kern = o->slots <= kFewThreads ? (bytes == 0 ? sort_few_kernel<1, 0> : bytes == 2 ? sort_few_kernel<1, 2> : sort_few_kernel<1, 4>)
-                                            : (bytes == 0 ? sort_few_kernel<kFewPer, 0> : bytes == 2 ? sort_few_kernel<kFewPer, 2> : sort_few_kernel<kFewPer, 4>);
+  const auto pick = [bytes](auto aligned_rows, auto halves, auto floats) { return bytes == 0 ? aligned_rows : bytes == 2 ? halves : floats; };
+  const auto kern = o->slots <= kFewThreads       ? pick(sort_few_kernel<1, 0>, sort_few_kernel<1, 2>, sort_few_kernel<1, 4>)
+                    : o->slots <= 4 * kFewThreads ? pick(sort_few_kernel<4, 0>, sort_few_kernel<4, 2>, sort_few_kernel<4, 4>)
+                                                  : pick(sort_few_kernel<kFewPer, 0>, sort_few_kernel<kFewPer, 2>, sort_few_kernel<kFewPer, 4>);
   kern<<<blocks, kFewThreads, 0, st>>>(*o, *r);
   const int rc = launch_result();
   return rc < 0 ? rc : 1;
