@@ -255,9 +255,12 @@ __device__ __forceinline__ void zero_rows(const CcfRows& a, Unit* out, int units
   }
 }
 
-// 16-byte units that a lane has in flight
+// 16-byte units that a lane has in flight, and slots whose units: 16384 tokens of 4096 bf16, two slots, back: two units of two slots 65 us (floor 62), one of two 86, one or two of
+// four 85, four of two 76; its gradient: one unit 110, two 107, four 108 (eight slots of 1024 fp16 111, 101 and 135); sorted: two, four and eight 67, 66 and 64 (8192 of 2048
+// in tiles of 128 rows: 24.2, 23.7 and 24.5).
 constexpr int kSortUnits = 4, kReturnUnits = 2, kReturnSlots = 2, kReturnBwdUnits = 2;
-// warps per SM up to which tokens are shared by several
+// Warps per SM up to which tokens are shared by several. 8192 tokens of 2048 bf16, two slots, with 16 and 64: back 19.0 and 19.6 us, its gradient 36.9 and 36.7 (six slots of 4096
+// tokens 43 and 62), sorted 26.2 and 23.7.
 constexpr int kSortWarps = 64, kReturnWarps = 16;
 
 __global__ void __launch_bounds__(kRowThreads) sort_rows_kernel(const __grid_constant__ CcfRows a, const __grid_constant__ RowShape s, long long ld) {
@@ -435,7 +438,9 @@ __global__ void __launch_bounds__(kRowThreads) return_rows_bwd_kernel(const __gr
 
 // ---- rows that do not all begin on 16 bytes ---------------------------------------------------------------------------------
 // The same over the aligned 16-byte pieces of what is written: each is put together from the two aligned pieces of a source that it lies across. Single
-// elements took 266, 221 and 80 us where these take 94, 144 and 74 (16384 tokens of 3001 bf16, two slots; back, its gradient, sorted; floors 45, 75 and 45).
+// elements took 266, 221 and 80 us where these take 82, 134 and 74 (16384 tokens of 3001 bf16, two slots; back, its gradient, sorted; floors 45, 75 and 45). Two pieces of the
+// way back in flight 106, of its gradient 144.
+constexpr int kReturnPieces = 1;     // that a lane has in flight on the way back
 // pieces of a row of `bytes` at `row`
 __device__ __forceinline__ int piece_count(const char* row, int bytes) {
   const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
@@ -509,34 +514,41 @@ __global__ void __launch_bounds__(kRowThreads) sort_odd_rows_kernel(const __grid
 
 template <int kType>
 __global__ void __launch_bounds__(kRowThreads) return_odd_rows_kernel(const __grid_constant__ CcfRows a, const __grid_constant__ RowShape s) {
-  constexpr int kJ = kReturnSlots, kE = kElemsPer16<kType>, kBytes = kElemBytes<kType>;
+  constexpr int kU = kReturnPieces, kJ = kReturnSlots, kE = kElemsPer16<kType>, kBytes = kElemBytes<kType>;
   const RowPlace at(s);
   if (at.token >= a.tokens) return;
   const int bytes = a.d * kBytes;
   char* const y = static_cast<char*>(a.tokens_out) + at.token * bytes;
   const int pieces = piece_count(y, bytes);
-  for (int c = at.unit; c < pieces; c += at.step) {
-    const int rel = piece_begin(y, c);
-    Values<kType> sum = {};
+  for (int c = at.unit; c < pieces; c += kU * at.step) {
+    Values<kType> sum[kU] = {};
     for (int j0 = 0; j0 < a.top_k; j0 += kJ) {
-      uint4 v[kJ];
+      uint4 v[kU][kJ];
       float w[kJ];
       int row[kJ];
 #pragma unroll
       for (int j = 0; j < kJ; ++j) {
         row[j] = slot_of(a, at, true, j0 + j, w[j]);
-        if (row[j] >= 0) v[j] = load_across(static_cast<const char*>(a.rows_in) + static_cast<long long>(row[j]) * bytes, bytes, rel);
+        const char* const from = static_cast<const char*>(a.rows_in) + static_cast<long long>(row[j]) * bytes;
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+          if (row[j] >= 0 && c + u * at.step < pieces) v[u][j] = load_across(from, bytes, piece_begin(y, c + u * at.step));
       }
 #pragma unroll
       for (int j = 0; j < kJ; ++j) {
         if (row[j] < 0) continue;
-        Values<kType> f;
-        unpack16<kType>(v[j], f);
 #pragma unroll
-        for (int i = 0; i < kE; ++i) sum[i] = fmaf(w[j], f[i], sum[i]);
+        for (int u = 0; u < kU; ++u) {
+          Values<kType> f;
+          unpack16<kType>(v[u][j], f);
+#pragma unroll
+          for (int i = 0; i < kE; ++i) sum[u][i] = fmaf(w[j], f[i], sum[u][i]);
+        }
       }
     }
-    store_piece<kBytes>(y, bytes, rel, pack16<kType>(sum));
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+      if (c + u * at.step < pieces) store_piece<kBytes>(y, bytes, piece_begin(y, c + u * at.step), pack16<kType>(sum[u]));
   }
 }
 
@@ -560,7 +572,7 @@ __global__ void __launch_bounds__(kRowThreads) return_odd_rows_bwd_kernel(const 
       const char* const y = static_cast<const char*>(a.rows_in) + static_cast<long long>(row) * bytes;
       const char* const grid = a.rows_out != nullptr ? out : y;
       const int pieces = piece_count(grid, bytes);
-#pragma unroll 2
+#pragma unroll 1
       for (int c = at.unit; c < pieces; c += at.step) {
         const int rel = piece_begin(grid, c);
         Values<kType> dy;
@@ -715,7 +727,7 @@ static int launch_sort(const CcfRows& r, int early, cudaStream_t st) {
 template <int kType>
 static int launch_return(const CcfRows& r, cudaStream_t st) {
   const bool aligned = rows_aligned(r, r.d, r.rows_in, r.tokens_out, nullptr);
-  const RowShape s = row_shape(r.tokens, units_of(r, aligned), aligned ? kReturnUnits : 1, kReturnWarps * sm_count());
+  const RowShape s = row_shape(r.tokens, units_of(r, aligned), aligned ? kReturnUnits : 1, (aligned ? kReturnWarps : kSortWarps) * sm_count());
   if (aligned) return_rows_kernel<kType><<<row_blocks(s, r.tokens), kRowThreads, 0, st>>>(r, s);
   else return_odd_rows_kernel<kType><<<row_blocks(s, r.tokens), kRowThreads, 0, st>>>(r, s);
   return launch_result();
