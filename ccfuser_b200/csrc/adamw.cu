@@ -32,7 +32,7 @@ constexpr int kAdam8Blocks = kType == kFp32 ? 5 : 6;
 constexpr int kAdam8Turns = 16;
 
 struct AdamScalars {
-  float decay, rate, inv_root, pad0;   // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  float decay, rate, inv_root, pad0;   // lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
   unsigned key, pad1, pad2, pad3;
 };
 static_assert(sizeof(AdamScalars) == 32);
@@ -70,7 +70,7 @@ __host__ __device__ inline unsigned long long split_mix(unsigned long long x) {
 __host__ __device__ inline AdamScalars adam_scalars(double lr, double b1, double b2, double wd, unsigned long long seed, long long step) {
   AdamScalars s = {};
   const double t = static_cast<double>(step);
-  s.decay = static_cast<float>(1.0 - lr * wd);
+  s.decay = static_cast<float>(lr * wd);
   s.rate = static_cast<float>(lr / (1.0 - pow(b1, t)));
   s.inv_root = static_cast<float>(1.0 / sqrt(1.0 - pow(b2, t)));
   s.key = static_cast<unsigned>(split_mix(split_mix(seed) ^ static_cast<unsigned long long>(step)) >> 32);
@@ -108,6 +108,7 @@ struct Scale {
 __device__ __forceinline__ unsigned block_exponent(unsigned largest) {
   return largest >= 0x7f800000u ? 255u : max((largest + 0xfffffu) >> 23, 40u);
 }
+
 // ---- the step --------------------------------------------------------------------------------------------------------
 // The entry of this thread block: the last one whose first block is not behind it.
 template <int kCount>
@@ -135,9 +136,10 @@ __device__ __forceinline__ void moments(float g, float& m, float& v, const AdamR
   m = __fadd_rn(__fmul_rn(m, r.b1), __fmul_rn(g, r.one_b1));
   v = __fadd_rn(__fmul_rn(v, r.b2), __fmul_rn(__fmul_rn(g, g), r.one_b2));
 }
+// What is taken off is added up first: 1 - lr wd of 1 - 1e-6 would be a hundredth of lr wd off in fp32, the same way in every step.
 __device__ __forceinline__ float updated(float p, float m, float v, const AdamRates& r, const AdamScalars& s) {
   const float root = fmaf(sqrtf(v), s.inv_root, r.eps);
-  return fmaf(p, s.decay, -s.rate * (m / root));
+  return p - fmaf(p, s.decay, s.rate * (m / root));
 }
 
 template <int kType>
@@ -293,8 +295,8 @@ template <bool kFast>
 __device__ __forceinline__ void update_pairs(float (&p)[8], const f32x2 (&m)[4], const f32x2 (&v)[4], const AdamRates& r, const AdamScalars& s) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const f32x2 step = mul2(mul2(m[i], inverse_roots<kFast>(v[i], r, s)), bc2(-s.rate));
-    upk2(fma2(pk2(p[2 * i], p[2 * i + 1]), bc2(s.decay), step), p[2 * i], p[2 * i + 1]);
+    const f32x2 step = mul2(mul2(m[i], inverse_roots<kFast>(v[i], r, s)), bc2(-s.rate)), old = pk2(p[2 * i], p[2 * i + 1]);
+    upk2(add2(old, fma2(old, bc2(-s.decay), step)), p[2 * i], p[2 * i + 1]);
   }
 }
 

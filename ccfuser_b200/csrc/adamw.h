@@ -32,7 +32,7 @@ typedef struct CcfAdamw {
 
 int ccf_sizeof_adamw();
 int ccf_sizeof_adamw_tensor();
-// launches made, or a negative code (nothing was launched then). Either all tensors have 8-bit moments or none.
+// launches made, or a negative code (-2: arguments, nothing was launched). Either all tensors have 8-bit moments or none.
 int ccf_adamw(const CcfAdamw* a, void* stream);
 // What a step reads from the device: the counter there is raised by one and is the number of this step; lr comes from `device_lr` unless that is null
 int ccf_adamw_scalars(const CcfAdamw* a, long long* counter, const float* device_lr, void* scalars, void* stream);

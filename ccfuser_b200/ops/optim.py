@@ -242,7 +242,8 @@ def _adamw_torch(p, g, m, v, e, key, lr, beta1, beta2, eps, wd, step):
     first = first * beta1 + g * (1 - beta1)
     second = second * beta2 + g * g * (1 - beta2)
     update = first / (second.sqrt() / math.sqrt(1 - beta2 ** step) + eps)
-    p.copy_(p.to(wide) * (1 - lr * wd) - update * (lr / (1 - beta1 ** step)))
+    old = p.to(wide)
+    p.copy_(old - (old * (lr * wd) + update * (lr / (1 - beta1 ** step))))
     if e is None:
         m.copy_(first)
         v.copy_(second)

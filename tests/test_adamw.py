@@ -297,3 +297,14 @@ def test_fake_tensors():
                 p.grad = torch.empty_like(p)
             opt.step()
             assert opt.state[params[0]]["exp_avg"].shape == (100, 100)
+
+
+def test_a_small_decay_is_not_rounded_away():
+    """1000 steps of lr wd = 3e-7 without gradients: 1 - lr wd is 1 - 2.98e-7 or 1 - 3.58e-7 in fp32; what is taken off is a sum of its own and rounded to a step of the weights, which
+    spread over a binade are off by half a step up or down."""
+    p = torch.linspace(1.0, 2.0, 4096)
+    old, zeros = p.double(), [torch.zeros(4096) for _ in range(3)]
+    for step in range(1, 1001):
+        adamw_step([p], [zeros[0]], [zeros[1]], [zeros[2]], step, lr=3e-3, weight_decay=1e-4)
+    lost = float(((old - p.double()) / old).mean())
+    assert abs(lost - 3e-4) < 0.05 * 3e-4, lost

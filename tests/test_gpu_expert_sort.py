@@ -358,3 +358,20 @@ def test_traced_calls():
     traced = torch.jit.trace(f, sets[0], check_trace=False)
     for s in sets:
         assert torch.equal(traced(*s), f(*s))
+
+
+@pytest.mark.parametrize("shape,d", [((2,), 16), ((3,), 7), ((2, 3, 4, 2), 40), ((1, 1, 5), 33)])
+def test_tokens_of_any_shape(shape, d):
+    from ccfuser_b200.ops.expert_sort import return_rows, sort_by_expert
+    g = _gen(24)
+    idx = torch.randint(0, 4, shape, generator=g, device="cuda")
+    x, w = torch.randn(*shape[:-1], d, generator=g, device="cuda").requires_grad_(True), torch.rand(shape, generator=g, device="cuda").requires_grad_(True)
+    rows, order = sort_by_expert(x, idx, 4, align=2)
+    T.check_order(order, idx, 4, None, 2)
+    y = return_rows(rows, order, w)
+    assert y.shape == x.shape
+    ref, size = T.returned(rows, order.slot_row, w)
+    R.assert_close(y, ref, shape[-1] * R.U * size)
+    dx, dw = torch.autograd.grad(y, [x, w], torch.ones_like(y))
+    assert dx.shape == x.shape and dw.shape == w.shape
+    R.assert_close(dx, w.detach().double().sum(dim=-1, keepdim=True).expand(x.shape), shape[-1] * 2 * R.U * w.detach().double().sum(dim=-1, keepdim=True).expand(x.shape))
