@@ -266,15 +266,9 @@ __device__ __forceinline__ float largest(float a, float b, float c) {
 // codes from bits 20 to 27 of four words, the first moment's sign from bit 31
 template <bool kSecond>
 __device__ __forceinline__ unsigned four_codes(const unsigned* w) {
-  unsigned x = __byte_perm(w[0], w[1], 0x7632), y = __byte_perm(w[2], w[3], 0x7632);      // upper halves
-  if constexpr (kSecond) {
-    x >>= 4;
-    y >>= 4;
-  } else {
-    x = (x >> 4 & 0x007f007fu) | (x >> 8 & 0x00800080u);
-    y = (y >> 4 & 0x007f007fu) | (y >> 8 & 0x00800080u);
-  }
-  return __byte_perm(x, y, 0x6420);
+  const unsigned x = __byte_perm(w[0], w[1], 0x7632), y = __byte_perm(w[2], w[3], 0x7632);      // upper halves
+  const unsigned codes = __byte_perm(x >> 4, y >> 4, 0x6420);
+  return kSecond ? codes : codes | (__byte_perm(x, y, 0x7531) & 0x80808080u);
 }
 // The inverses of sqrt(v) / sqrt(1 - b2^t) + eps by the hardware's approximations (2^-22 off); subnormal v count as 0 there, which eps covers from 1e-10 on.
 template <bool kFast>
