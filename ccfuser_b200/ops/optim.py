@@ -187,7 +187,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         _check_state(*t, i)
         if counter is not None and t[0].device != counter.device:
             raise ValueError(f"counter: on {counter.device}, the tensors beside it on {t[0].device}")
-        place = id(t[0]) if traced else t[0].data_ptr()
+        place = id(t[0]) if traced or t[0].device.type == "meta" else t[0].data_ptr()
         if t[0].numel() and place in seen:
             raise ValueError(f"params: tensor {i} is there twice")
         seen.add(place)

@@ -308,3 +308,55 @@ def test_a_small_decay_is_not_rounded_away():
         adamw_step([p], [zeros[0]], [zeros[1]], [zeros[2]], step, lr=3e-3, weight_decay=1e-4)
     lost = float(((old - p.double()) / old).mean())
     assert abs(lost - 3e-4) < 0.05 * 3e-4, lost
+
+
+def _ranks(rank, world):
+    from ccfuser_b200 import MoEConfig, MoELayer
+    from ccfuser_b200.parallel.ddp import allreduce_replicated_grads
+    from ccfuser_b200.parallel.placement import rebalance_experts
+    torch.manual_seed(10)
+    layer = MoELayer(MoEConfig(d_model=70, d_ffn=90, num_experts=6, dtype=torch.float32, backend="cpu", ep_size=world, max_tokens=64))
+    opt = FusedAdamW(layer.parameters(), lr=1e-2, state_bits=8)
+
+    def step(seed):
+        opt.zero_grad()
+        layer(torch.randn(64, 70, generator=torch.Generator().manual_seed(seed + rank))).square().sum().backward()
+        allreduce_replicated_grads(layer)
+        opt.step()
+
+    def moments():
+        return {n: [state_values(s["exp_avg"], s["exponents"], False, torch.float32), state_values(s["exp_avg_sq"], s["exponents"], True, torch.float32), p.detach().clone()]
+                for n, p in layer.named_parameters() for s in [opt.state[p]] if "exponents" in s}
+
+    step(1)
+    step(3)
+    before = moments()
+    placement = [4, 1, 5, 0, 3, 2]
+    rebalance_experts(layer, placement, opt)
+    after = moments()
+    step(5)
+    return before, after, placement, layer.gate.gate.weight.detach().clone()
+
+
+def test_moments_move_between_ranks_and_replicas_stay_alike():
+    from mp_util import run_ranks
+    res = run_ranks(_ranks, 2)
+    before, after, placement = [r[0] for r in res], [r[1] for r in res], res[0][2]
+    assert set(before[0]) == {"experts.htoh4.weight", "experts.h4toh.weight"}
+    for rank in range(2):
+        for name in before[0]:
+            for k in range(3):
+                for slot in range(3):
+                    source = placement[rank * 3 + slot]
+                    assert torch.equal(after[rank][name][k][slot], before[source // 3][name][k][source % 3]), (name, k)
+    assert torch.equal(res[0][3], res[1][3])
+
+
+def test_meta_tensors():
+    for bits in (32, 8):
+        params = [torch.nn.Parameter(torch.empty(100, 100, device="meta")), torch.nn.Parameter(torch.empty(3, device="meta"))]
+        opt = FusedAdamW(params, state_bits=bits)
+        for p in params:
+            p.grad = torch.empty_like(p)
+        opt.step()
+        assert opt.state[params[0]]["exp_avg"].device.type == "meta"

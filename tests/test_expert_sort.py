@@ -146,6 +146,12 @@ def test_masked_places_do_not_count():
     assert y[:, 0].tolist() == [1, 0, 5]
 
 
+def test_meta_tensors():
+    x, idx = torch.empty(5, 8, device="meta", dtype=torch.bfloat16), torch.empty(5, 2, dtype=torch.int32, device="meta")
+    rows, order = S.sort_by_expert(x, idx, 4, capacity=3, align=8)
+    assert rows.shape == (S.order_rows(10, 4, 3, 8), 8) and S.return_rows(rows, order, torch.empty(5, 2, device="meta")).shape == (5, 8)
+
+
 def test_fake_tensors_and_compile():
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():
