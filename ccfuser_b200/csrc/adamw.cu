@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(kAdamThreads) adamw32_kernel(const __grid_cons
 }
 
 // A warp has a block of CCF_ADAMW_BLOCK weights, eight a lane, as pairs: one instruction for two operations, each rounded as alone. Bound by its
-// integer instructions (55 a weight of all kinds; ALU pipe 67 %, issue slots 76 %) next to 10 bytes a weight of bf16: 285 M weights of 14 tensors 565 us of bf16 (436 at the copy rate),
-// 750 of fp32 (697). Scalar arithmetic instead of pairs 464 us where pairs take 424, constants as pairs in the arguments 443, shifts as products 440 (200 M).
+// integer instructions (60 a weight of all kinds; ALU pipe 63 %, issue slots 73 %) next to 10 bytes a weight of bf16: 285 M weights of 14 tensors 560 to 583 us of bf16 (436 at the copy rate),
+// 722 of fp32 (697). Scalar arithmetic instead of pairs 464 us where pairs take 424, constants as pairs in the arguments 443, shifts as products 440 (200 M).
 struct Place {
   long long block, at;   // of the tensor's blocks, first weight of this lane
   int here;              // its number of weights, 0 to 8
