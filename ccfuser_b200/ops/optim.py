@@ -314,6 +314,13 @@ def _encode(x, rows, bits, second):
     return _unblocks(torch.where(finite, code, 0).to(torch.uint8), x.shape), e.squeeze(-1).to(torch.uint8)
 
 
+def _check_group(group):
+    """What torch's AdamW can do and this one cannot is refused rather than left out."""
+    for name in ("maximize", "amsgrad"):
+        if group.get(name):
+            raise ValueError(f"FusedAdamW has no {name}")
+
+
 class FusedAdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` on ``adamw_step``: all tensors of a step in one launch per type (400 of them at most), moments in fp32 whatever the weights' type
     or, with ``state_bits=8``, in 8 bits (2 bytes a weight instead of 8; tensors of fewer than 4096 weights and fp64 ones keep theirs in full). The mean of what
@@ -406,9 +413,15 @@ class FusedAdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """Moments keep the types that they were saved in: torch's own loading casts them to the weights'."""
+        """Moments keep the types that they were saved in: torch's own loading casts them to the weights'. Groups with ``maximize`` or ``amsgrad`` are refused."""
         seen = []
-        handle = self.register_load_state_dict_pre_hook(lambda _, d: seen.append(d))      # behind the hooks that change it
+
+        def look(_, saved):
+            for group in saved["param_groups"]:
+                _check_group(group)
+            seen.append(saved)
+
+        handle = self.register_load_state_dict_pre_hook(look)      # behind the hooks that change it, before anything is taken over
         try:
             super().load_state_dict(state_dict)
         finally:
