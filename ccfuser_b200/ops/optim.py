@@ -319,6 +319,8 @@ def _check_group(group):
     for name in ("maximize", "amsgrad"):
         if group.get(name):
             raise ValueError(f"FusedAdamW has no {name}")
+    if group.get("state_bits", 32) not in (8, 32):
+        raise ValueError(f"state_bits: 8 or 32, got {group['state_bits']}")
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -332,14 +334,18 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32, seed: int = 0,
                  capturable: bool = False):
-        if state_bits not in (8, 32):
-            raise ValueError(f"state_bits: 8 or 32, got {state_bits}")
+        _check_group({"state_bits": state_bits})
         if torch.is_tensor(lr) and not capturable:
             raise ValueError("lr: a tensor with capturable=True only")
         if not (torch.is_tensor(lr) or lr >= 0.0) or eps < 0.0 or weight_decay < 0.0 or not all(0.0 <= b < 1.0 for b in betas):
             raise ValueError(f"lr, eps and weight_decay are at least 0, betas in [0, 1), got {lr}, {eps}, {weight_decay}, {betas}")
         self._counters = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed, capturable=capturable))
+
+    def add_param_group(self, param_group):
+        if isinstance(param_group, dict):
+            _check_group(param_group)
+        super().add_param_group(param_group)
 
     def __setstate__(self, state):
         super().__setstate__(state)

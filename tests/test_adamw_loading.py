@@ -52,3 +52,16 @@ def test_what_it_cannot_do_is_refused_and_nothing_changes(flag):
     _train(plain, theirs, 1, 2)
     opt.load_state_dict(plain.state_dict())
     assert opt.param_groups[0]["lr"] == 0.5 and opt.state[params[0]]["step"] == 2
+
+
+@pytest.mark.parametrize("option", [dict(maximize=True), dict(amsgrad=True), dict(state_bits=4), dict(state_bits=16)])
+def test_options_of_a_group_are_refused_like_the_constructors(option):
+    a, b = _params()
+    with pytest.raises(ValueError):
+        FusedAdamW([{"params": [a], **option}])
+    opt = FusedAdamW([a])
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [b], **option})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": [b], "state_bits": 8, "maximize": False})
+    assert [g["state_bits"] for g in opt.param_groups] == [32, 8]
