@@ -230,9 +230,8 @@ def _adamw_each(tensors, numbers, rates, step, counter, device_lr, traced):
     if others:
         if counter is not None:      # the number of the step is needed on the host
             step, lr = int(counter), lr if device_lr is None else float(device_lr)
-        key = _split_mix(_split_mix(seed & _M64) ^ step) >> 32
         for i, p, g, m, v, e in others:
-            _adamw_torch(p, g, m, v, e, (key + i * 0x9E3779B9) & _M32, lr, beta1, beta2, eps, wd, step)
+            _adamw_torch(p, g, m, v, e, _rounding_key(seed, step, i), lr, beta1, beta2, eps, wd, step)
 
 
 def _adamw_torch(p, g, m, v, e, key, lr, beta1, beta2, eps, wd, step):
@@ -323,6 +322,38 @@ def _check_group(group):
         raise ValueError(f"state_bits: 8 or 32, got {group['state_bits']}")
 
 
+def _state8_rows(group, p):
+    """The rows of a parameter's exponents, 0 where its moments are not held in 8 bits."""
+    if group["state_bits"] != 8 or p.numel() < STATE8_LEAST or p.dtype not in N.DTYPE_CODE:
+        return 0
+    # rows that move between ranks (parallel/placement.py) take their blocks along
+    return p.shape[0] if p.dim() >= 2 and (getattr(p, "skip_allreduce", False) or hasattr(p, "dp_comm")) else 1
+
+
+def _rounding_key(seed, step, number):
+    return (_split_mix(_split_mix(seed & _M64) ^ step) >> 32) + number * 0x9E3779B9 & _M32
+
+
+_PIECE = 1 << 24           # moments that are encoded at a time, a multiple of STATE_BLOCK
+
+
+def _state8_of(p, first, second, rows, key):
+    """Given moments of ``p`` in 8 bits on its device, rounded as by a step with this key; in pieces, for the hash takes 64 bits a weight."""
+    m, v, e = state8(p, rows)
+    width = p.numel() // rows
+    tall = max(1, _PIECE // width)
+    for r in range(0, rows, tall):
+        for c in range(0, width, _PIECE):
+            cut = slice(r, r + tall), slice(c, c + _PIECE)
+            at = torch.arange(r, min(r + tall, rows), device=p.device)[:, None] * width + torch.arange(c, min(c + _PIECE, width), device=p.device)
+            h = _mix((at + key) & _M32)
+            for k, (codes, x, bits) in enumerate(((m, first, h & 0xFFFFF), (v, second, h >> 12))):
+                x = x.detach().reshape(rows, width)[cut].to(device=p.device, dtype=torch.float32)
+                codes.view(rows, width)[cut], part = _encode(x, x.shape[0], bits.int(), k == 1)
+                e[cut[0], c // STATE_BLOCK:c // STATE_BLOCK + part.shape[1], k] = part
+    return m, v, e
+
+
 class FusedAdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` on ``adamw_step``: all tensors of a step in one launch per type (400 of them at most), moments in fp32 whatever the weights' type
     or, with ``state_bits=8``, in 8 bits (2 bytes a weight instead of 8; tensors of fewer than 4096 weights and fp64 ones keep theirs in full). The mean of what
@@ -348,10 +379,13 @@ class FusedAdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
 
     def __setstate__(self, state):
+        own = self.__dict__.get("param_groups", [])      # while a checkpoint is loaded
         super().__setstate__(state)
-        for group in self.param_groups:
-            for k, v in (("state_bits", 32), ("seed", 0), ("capturable", False)):
-                group.setdefault(k, v)
+        for k, group in enumerate(self.param_groups):
+            if "state_bits" not in group and k < len(own):      # another optimizer's group: it says nothing of these
+                group.update((name, own[k][name]) for name in ("state_bits", "seed", "capturable"))
+            for name, v in (("state_bits", 32), ("seed", 0), ("capturable", False)):
+                group.setdefault(name, v)
         self._counters = {}
 
     def __getstate__(self):
@@ -371,10 +405,9 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _start(self, k, group, p):
         state = self.state[p]
-        if group["state_bits"] == 8 and p.numel() >= STATE8_LEAST and p.dtype in N.DTYPE_CODE:
-            # rows that move between ranks (parallel/placement.py) take their blocks along
-            moves = p.dim() >= 2 and (getattr(p, "skip_allreduce", False) or hasattr(p, "dp_comm"))
-            state["exp_avg"], state["exp_avg_sq"], state["exponents"] = state8(p, p.shape[0] if moves else 1)
+        rows = _state8_rows(group, p)
+        if rows:
+            state["exp_avg"], state["exp_avg_sq"], state["exponents"] = state8(p, rows)
         else:
             kind = torch.float64 if p.dtype == torch.float64 else torch.float32
             state["exp_avg"], state["exp_avg_sq"] = (torch.zeros(p.shape, dtype=kind, device=p.device) for _ in range(2))
@@ -418,8 +451,24 @@ class FusedAdamW(torch.optim.Optimizer):
                            exponents=e if eight else None, seed=group["seed"] + (k << 32), numbers=numbers, counter=counter)
         return loss
 
+    @staticmethod
+    def _loaded(k, group, number, p, saved):
+        """The state of a parameter from a saved one."""
+        step, rows = int(saved["step"]), _state8_rows(group, p)
+        if rows and "exponents" not in saved:
+            key = _rounding_key(group["seed"] + (k << 32), step, number)
+            m, v, e = _state8_of(p, saved["exp_avg"], saved["exp_avg_sq"], rows, key)
+            return {"step": step, "exp_avg": m, "exp_avg_sq": v, "exponents": e}
+        kind = torch.uint8 if "exponents" in saved else torch.float64 if p.dtype == torch.float64 else torch.float32
+        state = {name: saved[name].detach().to(device=p.device, dtype=torch.uint8 if name == "exponents" else kind, copy=True).contiguous()
+                 for name in ("exp_avg", "exp_avg_sq", "exponents") if name in saved}
+        state["step"] = step
+        return state
+
     def load_state_dict(self, state_dict):
-        """Moments keep the types that they were saved in: torch's own loading casts them to the weights'. Groups with ``maximize`` or ``amsgrad`` are refused."""
+        """Options come from the saved groups, as in torch; those of ``torch.optim.AdamW`` know no ``state_bits`` and ``seed``, so that these and ``capturable`` stay the
+        optimizer's own, and with ``state_bits=8`` their moments are brought into 8 bits. Else moments keep the types that they were saved in: torch's own loading casts them
+        to the weights'. Groups with ``maximize`` or ``amsgrad`` are refused."""
         seen = []
 
         def look(_, saved):
@@ -433,17 +482,11 @@ class FusedAdamW(torch.optim.Optimizer):
         finally:
             handle.remove()
         saved = seen[-1]
-        ids = [i for group in saved["param_groups"] for i in group["params"]]
-        params = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(ids, params):
-            state = saved["state"].get(i)
-            if not state:
-                continue
-            kind = torch.uint8 if "exponents" in state else torch.float64 if p.dtype == torch.float64 else torch.float32
-            for name in ("exp_avg", "exp_avg_sq", "exponents"):
-                if name in state:
-                    self.state[p][name] = state[name].detach().to(device=p.device, dtype=torch.uint8 if name == "exponents" else kind, copy=True).contiguous()
-            self.state[p]["step"] = int(state["step"])
+        for k, (group, old) in enumerate(zip(self.param_groups, saved["param_groups"])):
+            for number, (p, i) in enumerate(zip(group["params"], old["params"])):
+                state = saved["state"].get(i)
+                if state:
+                    self.state[p].update(self._loaded(k, group, number, p, state))
         for k, group in enumerate(self.param_groups):
             if group["capturable"]:
                 for p in group["params"]:

@@ -3,8 +3,10 @@ import copy
 
 import pytest
 import torch
+import training_refs as T
 
-from ccfuser_b200.ops.optim import FusedAdamW
+from ccfuser_b200.ops import optim as O
+from ccfuser_b200.ops.optim import FusedAdamW, adamw_step, state_values
 
 
 def _params(dtype=torch.float32):
@@ -65,3 +67,62 @@ def test_options_of_a_group_are_refused_like_the_constructors(option):
     assert len(opt.param_groups) == 1
     opt.add_param_group({"params": [b], "state_bits": 8, "maximize": False})
     assert [g["state_bits"] for g in opt.param_groups] == [32, 8]
+
+
+@pytest.mark.parametrize("piece", [256, 1024, 1 << 24])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_torchs_checkpoint_in_8_bits(dtype, capturable, piece, monkeypatch):
+    """Groups keep what torch's know nothing of; moments come into 8 bits as a step would round them, in pieces of any size, and train on."""
+    monkeypatch.setattr(O, "_PIECE", piece)
+    g = torch.Generator().manual_seed(4)
+    make = lambda: [torch.nn.Parameter(torch.ones(s, dtype=dtype)) for s in ((3, 1500), (70, 70), (9,), (4, 1100))]  # noqa: E731
+    theirs, params = make(), make()
+    params[0].skip_allreduce = True      # an expert's: exponents by row
+    ref = torch.optim.AdamW([{"params": theirs[:1], "lr": 0.1}, {"params": theirs[1:], "lr": 0.2}])
+    for _ in range(3):
+        for p in theirs[:3]:             # the last has no gradient yet
+            p.grad = torch.randn(p.shape, generator=g).to(dtype)
+        ref.step()
+    opt = FusedAdamW([{"params": params[:1]}, {"params": params[1:], "seed": 11}], state_bits=8, seed=7, capturable=capturable)
+    opt.load_state_dict(ref.state_dict())
+    assert [(q["lr"], q["state_bits"], q["seed"], q["capturable"]) for q in opt.param_groups] == [(0.1, 8, 7, capturable), (0.2, 8, 11, capturable)]
+    for p, q, rows, seed, number in ((params[0], theirs[0], 3, 7, 0), (params[1], theirs[1], 1, 11 + (1 << 32), 0)):
+        state = opt.state[p]
+        assert state["exponents"].shape[0] == rows and state["exp_avg"].dtype == torch.uint8 and int(state["step"]) == 3
+        bits = T.rounding_bits(seed, 3, number, p.numel())
+        for k, (name, these) in enumerate((("exp_avg", [b & 0xFFFFF for b in bits]), ("exp_avg_sq", [b >> 12 for b in bits]))):
+            got = state_values(state[name], state["exponents"], k == 1, torch.float32)
+            assert torch.equal(got.double(), T.stored(ref.state[q][name], rows, these, k == 1)), name
+    small = opt.state[params[2]]
+    assert "exponents" not in small and torch.equal(small["exp_avg"], ref.state[theirs[2]]["exp_avg"].float())
+    # the next step is one on these codes, and what starts later has 8 bits
+    want = {n: t.clone() for n, t in opt.state[params[1]].items() if n != "step"}
+    weight, grads = params[1].detach().clone(), [torch.randn(p.shape, generator=g).to(dtype) for p in params]
+    for p, grad in zip(params, grads):
+        p.grad = grad
+    opt.step()
+    adamw_step([weight], [grads[1]], [want["exp_avg"]], [want["exp_avg_sq"]], 4, lr=0.2, exponents=[want["exponents"]], seed=11 + (1 << 32))
+    assert torch.equal(weight, params[1]) and all(torch.equal(t, opt.state[params[1]][n]) for n, t in want.items())
+    assert opt.state[params[3]]["exp_avg"].dtype == torch.uint8 and int(opt.state[params[0]]["step"]) == 4
+
+
+def test_own_options_come_from_the_checkpoint():
+    params, others = _params(), _params()
+    a = FusedAdamW(params, state_bits=8, seed=3)
+    _train(a, params, 1, 2)
+    b = FusedAdamW(others, seed=5)
+    b.load_state_dict(a.state_dict())
+    assert (b.param_groups[0]["state_bits"], b.param_groups[0]["seed"]) == (8, 3) and torch.equal(a.state[params[0]]["exponents"], b.state[others[0]]["exponents"])
+
+
+def test_values_that_are_not_finite_come_into_8_bits_as_in_a_step():
+    p, q = torch.nn.Parameter(torch.ones(80, 64)), torch.nn.Parameter(torch.ones(80, 64))
+    ref = torch.optim.AdamW([p])
+    p.grad = torch.ones_like(p)
+    ref.step()
+    ref.state[p]["exp_avg"][0, 0] = torch.inf
+    opt = FusedAdamW([q], state_bits=8)
+    opt.load_state_dict(ref.state_dict())
+    first = state_values(opt.state[q]["exp_avg"], opt.state[q]["exponents"], dtype=torch.float32).reshape(-1)
+    assert first[:256].isnan().all() and first[256:].isfinite().all()
