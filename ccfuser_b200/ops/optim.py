@@ -370,7 +370,7 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError("lr: a tensor with capturable=True only")
         if not (torch.is_tensor(lr) or lr >= 0.0) or eps < 0.0 or weight_decay < 0.0 or not all(0.0 <= b < 1.0 for b in betas):
             raise ValueError(f"lr, eps and weight_decay are at least 0, betas in [0, 1), got {lr}, {eps}, {weight_decay}, {betas}")
-        self._counters = {}
+        self._counters, self._saved = {}, None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed, capturable=capturable))
 
     def add_param_group(self, param_group):
@@ -379,17 +379,26 @@ class FusedAdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
 
     def __setstate__(self, state):
-        own = self.__dict__.get("param_groups", [])      # while a checkpoint is loaded
-        super().__setstate__(state)
-        for k, group in enumerate(self.param_groups):
-            if "state_bits" not in group and k < len(own):      # another optimizer's group: it says nothing of these
-                group.update((name, own[k][name]) for name in ("state_bits", "seed", "capturable"))
+        saved = self.__dict__.get("_saved")      # a checkpoint that is being loaded
+        for k, group in enumerate(state["param_groups"]):
+            if "state_bits" not in group and saved is not None:      # another optimizer's group: it says nothing of these
+                group.update((name, self.param_groups[k][name]) for name in ("state_bits", "seed", "capturable"))
             for name, v in (("state_bits", 32), ("seed", 0), ("capturable", False)):
                 group.setdefault(name, v)
-        self._counters = {}
+            for number, (p, i) in enumerate(zip(group["params"], saved["param_groups"][k]["params"] if saved is not None else ())):
+                if saved["state"].get(i):
+                    state["state"][p] = self._loaded(k, group, number, p, saved["state"][i])
+        super().__setstate__(state)      # up to here nothing has changed
+        self._counters, self._saved = {}, None
+        if saved is not None:
+            for k, group in enumerate(self.param_groups):
+                if group["capturable"]:
+                    for p in group["params"]:
+                        if "step" in self.state.get(p, {}):
+                            self._counter(k, p)
 
     def __getstate__(self):
-        return {k: v for k, v in super().__getstate__().items() if k != "_counters"}
+        return {k: v for k, v in super().__getstate__().items() if k not in ("_counters", "_saved")}
 
     def _counter(self, k, p):
         """The number of the last step of group ``k`` on the parameter's device."""
@@ -454,41 +463,35 @@ class FusedAdamW(torch.optim.Optimizer):
     @staticmethod
     def _loaded(k, group, number, p, saved):
         """The state of a parameter from a saved one."""
-        step, rows = int(saved["step"]), _state8_rows(group, p)
+        step, first, second, rows = int(saved["step"]), saved["exp_avg"], saved["exp_avg_sq"], _state8_rows(group, p)
+        if first.shape != p.shape or second.shape != p.shape:
+            raise ValueError(f"moments of {tuple(first.shape)} and {tuple(second.shape)} for a parameter of {tuple(p.shape)}")
+        made = {"step": step}
         if rows and "exponents" not in saved:
-            key = _rounding_key(group["seed"] + (k << 32), step, number)
-            m, v, e = _state8_of(p, saved["exp_avg"], saved["exp_avg_sq"], rows, key)
-            return {"step": step, "exp_avg": m, "exp_avg_sq": v, "exponents": e}
+            made.update(zip(("exp_avg", "exp_avg_sq", "exponents"), _state8_of(p, first, second, rows, _rounding_key(group["seed"] + (k << 32), step, number))))
         kind = torch.uint8 if "exponents" in saved else torch.float64 if p.dtype == torch.float64 else torch.float32
-        state = {name: saved[name].detach().to(device=p.device, dtype=torch.uint8 if name == "exponents" else kind, copy=True).contiguous()
-                 for name in ("exp_avg", "exp_avg_sq", "exponents") if name in saved}
-        state["step"] = step
-        return state
+        for name, t in saved.items():
+            if name not in made:
+                made[name] = t.detach().to(device=p.device, dtype=kind if name in ("exp_avg", "exp_avg_sq") else None, copy=True).contiguous() if torch.is_tensor(t) else t
+        return made
 
     def load_state_dict(self, state_dict):
         """Options come from the saved groups, as in torch; those of ``torch.optim.AdamW`` know no ``state_bits`` and ``seed``, so that these and ``capturable`` stay the
-        optimizer's own, and with ``state_bits=8`` their moments are brought into 8 bits. Else moments keep the types that they were saved in: torch's own loading casts them
-        to the weights'. Groups with ``maximize`` or ``amsgrad`` are refused."""
-        seen = []
-
-        def look(_, saved):
+        optimizer's own, and with ``state_bits=8`` their moments are brought into 8 bits. Else moments keep the types that they were saved in: torch's own loading would cast all of
+        them, codes too, to the weights' type first, and is given none. Groups with ``maximize`` or ``amsgrad`` are refused, with nothing changed."""
+        def take(_, saved):
             for group in saved["param_groups"]:
                 _check_group(group)
-            seen.append(saved)
+                missing = [name for name in ("lr", "betas", "eps", "weight_decay") if name not in group]
+                if missing:
+                    raise ValueError(f"no checkpoint of AdamW: its groups have no {', '.join(missing)}")
+            self._saved = saved
+            mine = {i for group in saved["param_groups"] for i in group["params"]}
+            return {**saved, "state": {i: s for i, s in saved["state"].items() if i not in mine}}
 
-        handle = self.register_load_state_dict_pre_hook(look)      # behind the hooks that change it, before anything is taken over
+        handle = self.register_load_state_dict_pre_hook(take)      # behind the hooks that change it, before anything is taken over
         try:
-            super().load_state_dict(state_dict)
+            super().load_state_dict(state_dict)                    # ends in __setstate__, then hooks that look at what was loaded
         finally:
             handle.remove()
-        saved = seen[-1]
-        for k, (group, old) in enumerate(zip(self.param_groups, saved["param_groups"])):
-            for number, (p, i) in enumerate(zip(group["params"], old["params"])):
-                state = saved["state"].get(i)
-                if state:
-                    self.state[p].update(self._loaded(k, group, number, p, state))
-        for k, group in enumerate(self.param_groups):
-            if group["capturable"]:
-                for p in group["params"]:
-                    if "step" in self.state.get(p, {}):
-                        self._counter(k, p)
+            self._saved = None

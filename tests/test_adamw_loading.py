@@ -126,3 +126,59 @@ def test_values_that_are_not_finite_come_into_8_bits_as_in_a_step():
     opt.load_state_dict(ref.state_dict())
     first = state_values(opt.state[q]["exp_avg"], opt.state[q]["exponents"], dtype=torch.float32).reshape(-1)
     assert first[:256].isnan().all() and first[256:].isfinite().all()
+
+
+class _Made(torch.utils._python_dispatch.TorchDispatchMode):
+    """The bytes an element of the largest tensors that operations make."""
+
+    def __init__(self, numel):
+        super().__init__()
+        self.numel, self.widest = numel, 0
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        if torch.is_tensor(out) and out.numel() >= self.numel:
+            self.widest = max(self.widest, out.element_size())
+        return out
+
+
+@pytest.mark.parametrize("dtype,bits,widest", [(torch.bfloat16, 8, 1), (torch.float32, 8, 1), (torch.bfloat16, 32, 4)])
+def test_loading_makes_nothing_wider_than_what_it_keeps(dtype, bits, widest):
+    params, others = _params(dtype), _params(dtype)
+    a, b = FusedAdamW(params, state_bits=bits), FusedAdamW(others)
+    _train(a, params, 1, 2)
+    saved = a.state_dict()
+    with _Made(params[0].numel()) as made:
+        b.load_state_dict(saved)
+    assert made.widest == widest
+    _assert_same(_all_of(a), _all_of(b))
+
+
+def test_hooks_of_a_load_see_the_dictionary_and_what_came_of_it():
+    params, others = _params(torch.bfloat16), _params(torch.bfloat16)
+    a, b = FusedAdamW(params, state_bits=8), FusedAdamW(others)
+    _train(a, params, 1, 2)
+    seen = []
+    b.register_load_state_dict_pre_hook(lambda _, d: {**d, "param_groups": [{**g, "lr": 0.25} for g in d["param_groups"]]})
+    b.register_load_state_dict_post_hook(lambda opt: seen.append({n: t for n, t in opt.state[others[0]].items()}))
+    b.load_state_dict(a.state_dict())
+    assert b.param_groups[0]["lr"] == 0.25 and seen[0].keys() == a.state[params[0]].keys()
+    assert seen[0]["exp_avg"].dtype == torch.uint8 and torch.equal(seen[0]["exp_avg"], a.state[params[0]]["exp_avg"])
+
+
+def test_a_load_that_fails_changes_nothing():
+    params, theirs = _params(), _params()
+    opt, ref = FusedAdamW(params, state_bits=8, lr=1e-2), torch.optim.AdamW(theirs, lr=0.5)
+    _train(opt, params, 1, 2)
+    _train(ref, theirs, 1, 2)
+    before = _all_of(opt)
+    broken = copy.deepcopy(ref.state_dict())
+    del broken["state"][1]["exp_avg_sq"]
+    cut = copy.deepcopy(ref.state_dict())
+    cut["state"][0]["exp_avg"] = cut["state"][0]["exp_avg"][1:]
+    for bad in (broken, cut, torch.optim.SGD(theirs).state_dict(), torch.optim.AdamW(theirs[:1]).state_dict()):
+        with pytest.raises((KeyError, ValueError)):
+            opt.load_state_dict(bad)
+        _assert_same(_all_of(opt), before)
+    opt.load_state_dict(ref.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.5
