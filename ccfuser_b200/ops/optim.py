@@ -385,6 +385,10 @@ class FusedAdamW(torch.optim.Optimizer):
                 group.update((name, self.param_groups[k][name]) for name in ("state_bits", "seed", "capturable"))
             for name, v in (("state_bits", 32), ("seed", 0), ("capturable", False)):
                 group.setdefault(name, v)
+            if saved is not None:      # as a step reads them: numbers, or a rate beside the counter, wherever the checkpoint was read to
+                group["betas"] = tuple(float(b) for b in group["betas"])
+                if torch.is_tensor(group["lr"]):
+                    group["lr"] = group["lr"].detach().to(device=group["params"][0].device, dtype=torch.float32) if group["capturable"] else float(group["lr"])
             for number, (p, i) in enumerate(zip(group["params"], saved["param_groups"][k]["params"] if saved is not None else ())):
                 if saved["state"].get(i):
                     state["state"][p] = self._loaded(k, group, number, p, saved["state"][i])

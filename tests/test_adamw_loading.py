@@ -182,3 +182,17 @@ def test_a_load_that_fails_changes_nothing():
         _assert_same(_all_of(opt), before)
     opt.load_state_dict(ref.state_dict())
     assert opt.param_groups[0]["lr"] == 0.5
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_rates_that_torch_keeps_in_tensors(capturable):
+    params, theirs = _params(), _params()
+    ref = torch.optim.AdamW(theirs, lr=torch.tensor(0.1, dtype=torch.float64), betas=(torch.tensor(0.8), torch.tensor(0.99)))
+    opt = FusedAdamW(params, capturable=capturable)
+    opt.load_state_dict(ref.state_dict())
+    lr = opt.param_groups[0]["lr"]
+    assert torch.is_tensor(lr) == capturable and (not capturable or lr.dtype == torch.float32)
+    want, weights = copy.deepcopy(params), [p.detach().clone() for p in params]
+    _train(FusedAdamW(want, lr=float(lr), betas=tuple(float(torch.tensor(b)) for b in (0.8, 0.99))), want, 1, 2)
+    _train(opt, params, 1, 2)
+    assert all(torch.equal(p, q) and not torch.equal(p, w) for p, q, w in zip(params, want, weights))
