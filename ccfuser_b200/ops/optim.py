@@ -434,34 +434,54 @@ class FusedAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
-        for k, group in enumerate(self.param_groups):
-            batches = {}
-            # a parameter's number is its place in the group, whether or not those before it have gradients: replicas on several ranks round alike
-            for number, p in enumerate(group["params"]):
-                if p.grad is None:
-                    continue
-                state = self.state[p]
-                if capturing and not (group["capturable"] and "step" in state):
-                    raise RuntimeError("FusedAdamW: a step in a CUDA graph needs capturable=True and a step before the capture")
-                if "step" not in state:
-                    state = self._start(k, group, p)
-                if group["capturable"]:
-                    key = (p.device, "exponents" in state)
-                else:
-                    state["step"] += 1
-                    key = (state["step"], "exponents" in state)
-                batches.setdefault(key, []).append((p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("exponents"), number))
+        batches, started = {}, []      # by group, number of the step (or device) and width of the moments
+        try:
+            for k, group in enumerate(self.param_groups):
+                # a parameter's number is its place in the group, whether or not those before it have gradients: replicas on several ranks round alike
+                for number, p in enumerate(group["params"]):
+                    if p.grad is None:
+                        continue
+                    state = self.state[p]
+                    if capturing and not (group["capturable"] and "step" in state):
+                        raise RuntimeError("FusedAdamW: a step in a CUDA graph needs capturable=True and a step before the capture")
+                    if "step" not in state:
+                        started.append(p)
+                        state = self._start(k, group, p)
+                    key = (k, p.device if group["capturable"] else state["step"] + 1, "exponents" in state)
+                    batches.setdefault(key, []).append((p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("exponents"), number))
+            if len(batches) > 1:      # each call looks at its own tensors before it changes one
+                for batch in batches.values():
+                    for p, g, *_ in batch:
+                        if g.layout is not torch.strided or g.dtype is not p.dtype:
+                            raise TypeError(f"a gradient is {g.layout} of {g.dtype}, its parameter {p.dtype}")
             raised = set()
-            for (step, eight), batch in batches.items():
+            for (k, at, eight), batch in batches.items():
+                group = self.param_groups[k]
                 p, g, m, v, e, numbers = zip(*batch)
-                counter = None
+                step, counter = at, None
                 if group["capturable"]:
                     step, counter = None, self._counter(k, p[0])
-                    if counter.device in raised:      # raised by the batch before
+                    again = (k, at) in raised
+                    if again:      # by the batch before
                         counter -= 1
-                    raised.add(counter.device)
-                adamw_step(p, g, m, v, step, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                           exponents=e if eight else None, seed=group["seed"] + (k << 32), numbers=numbers, counter=counter)
+                try:
+                    adamw_step(p, g, m, v, step, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                               exponents=e if eight else None, seed=group["seed"] + (k << 32), numbers=numbers, counter=counter)
+                except BaseException:
+                    if counter is not None and again:
+                        counter += 1
+                    raise
+                raised.add((k, at))
+                if counter is None:
+                    for q in p:
+                        self.state[q]["step"] = at
+                if started:
+                    done = {id(q) for q in p}
+                    started = [q for q in started if id(q) not in done]
+        except BaseException:
+            for p in started:      # a step that was refused leaves no trace
+                self.state.pop(p, None)
+            raise
         return loss
 
     @staticmethod
