@@ -216,7 +216,7 @@ def rebalance_experts(layer, placement: Sequence[int], optimizer: Optional[torch
     Collective over the layer's expert-parallel group; every rank passes the same placement. Parameters are updated
     in place (their storage, and hence every pointer the kernels hold, stays valid). Per-parameter optimizer state
     with the parameter's shape (momentum, Adam moments) travels with it. Data-parallel replicas of the group must
-    apply the same placement.
+    apply the same placement. A call that raises has moved nothing (a gate's own ``permute_experts`` comes first).
     """
     cfg = layer.config
     e_loc, world, rank = cfg.experts_per_rank, cfg.ep_size, layer.ep_rank
@@ -227,29 +227,29 @@ def rebalance_experts(layer, placement: Sequence[int], optimizer: Optional[torch
     if placement == list(range(e)):
         return
     group = layer.ep_group if world > 1 else None
+    # everything is looked at before the first row moves: a refusal leaves the layer whole
+    gate, experts, router = layer.gate, [], []
     for p in layer.experts.parameters():
         if p.shape[0] != e_loc:
             raise ValueError("expert parameters must carry the local expert index first")
-        tensors = [("param", p.data)] + _state_tensors(optimizer, p)
-        for _, t in tensors:
-            t.copy_(_exchange_rows(t, placement, e_loc, rank, world, group))
-        if p.grad is not None:
-            p.grad = None                                           # gradients of the old layout are meaningless now
-    gate = layer.gate
+        experts.append((p, [p.data] + [t for _, t in _state_tensors(optimizer, p)]))
     if hasattr(gate, "permute_experts"):
-        gate.permute_experts(placement, optimizer)
+        gate.permute_experts(placement, optimizer)                  # may refuse as well
     else:
         lin = getattr(gate, "gate", None)
         if not isinstance(lin, nn.Linear) or lin.out_features != e:
             raise TypeError("the gate needs a `gate` nn.Linear over all experts or a permute_experts(placement, optimizer) "
                             "method for its rows to follow the experts")
-        perm = torch.tensor(placement, device=lin.weight.device, dtype=torch.long)
-        for p in (lin.weight, lin.bias):
-            if p is None:
-                continue
-            for _, t in [("param", p.data)] + _state_tensors(optimizer, p):
-                t.copy_(t[perm].clone())
-            p.grad = None
+        router = [(p, [p.data] + [t for _, t in _state_tensors(optimizer, p)]) for p in (lin.weight, lin.bias) if p is not None]
+    for p, tensors in experts:
+        for t in tensors:
+            t.copy_(_exchange_rows(t, placement, e_loc, rank, world, group))
+        p.grad = None                                               # gradients of the old layout are meaningless now
+    for p, tensors in router:
+        perm = torch.tensor(placement, device=p.device, dtype=torch.long)
+        for t in tensors:
+            t.copy_(t[perm].clone())
+        p.grad = None
     history = getattr(layer, "placement_history", None)
     layer.placement_history = compose(history, placement) if history is not None else list(placement)
 
