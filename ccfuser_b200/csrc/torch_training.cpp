@@ -120,11 +120,14 @@ at::Tensor run_return(const at::Tensor& rows_, const at::Tensor& slot_row, const
   return y;
 }
 
+// where a number is none of `count`: what the kernels leave out, and torch's operations must not see
+at::Tensor outside(const at::Tensor& numbers, int64_t count) { return numbers.lt(0).logical_or(numbers.ge(count)); }
+
 // by torch's operations, which record a graph: each slot's row, zeros where it has none: [tokens, top_k, d]
 at::Tensor torch_slots(const at::Tensor& rows, const at::Tensor& slot_row) {
   const int64_t k = slot_row.size(-1), tokens = slot_row.numel() / k;
-  const at::Tensor at = slot_row.reshape({tokens, k});
-  return rows.to(at::kFloat).index_select(0, at.clamp_min(0).reshape({-1}).to(at::kLong)).reshape({tokens, k, rows.size(1)}).masked_fill(at.lt(0).unsqueeze(2), 0);
+  const at::Tensor at = slot_row.reshape({tokens, k}), none = outside(at, rows.size(0));
+  return rows.to(at::kFloat).index_select(0, at.masked_fill(none, 0).reshape({-1}).to(at::kLong)).reshape({tokens, k, rows.size(1)}).masked_fill(none.unsqueeze(2), 0);
 }
 
 struct SortNode : TokenNode {
@@ -183,11 +186,11 @@ struct ReturnNode : TokenNode {
     if (!grads[0].defined()) return out;
     const at::Tensor slot_row = kept(0), row_slot = kept(1), weights = kept(2), values = kept(3);
     const int64_t k = slot_row.size(-1), tokens = slot_row.numel() / k, d = grads[0].size(-1);
-    const at::Tensor dy = grads[0].reshape({tokens, d}).to(at::kFloat), slot = row_slot.clamp_min(0).to(at::kLong);
+    const at::Tensor dy = grads[0].reshape({tokens, d}).to(at::kFloat), none = outside(row_slot, tokens * k), slot = row_slot.masked_fill(none, 0).to(at::kLong);
     if (task_should_compute_output(0)) {
       at::Tensor g = dy.index_select(0, at::floor_divide(slot, k));
       if (weights.defined()) g = g * weights.reshape({-1}).to(at::kFloat).index_select(0, slot).unsqueeze(1);
-      out[0] = g.masked_fill(row_slot.lt(0).unsqueeze(1), 0).to(grads[0].scalar_type());
+      out[0] = g.masked_fill(none.unsqueeze(1), 0).to(grads[0].scalar_type());
     }
     if (weights.defined() && values.defined() && task_should_compute_output(1))
       out[1] = (torch_slots(values, slot_row) * dy.unsqueeze(1)).sum(2).to(weights.scalar_type()).reshape(weight_shape);

@@ -232,12 +232,17 @@ def _order_torch(idx, num_experts, capacity, align):
     return ExpertOrder(slot_row.view(idx.shape), row_slot[:rows], counts.int(), base.int())
 
 
+def _outside(numbers, count):
+    """Where a number is none of ``count``: what the kernels leave out, and torch's operations must not see."""
+    return (numbers < 0) | (numbers >= count)
+
+
 def _slots(rows, slot_row):
     """Each slot's row in fp32 (fp64), zeros where it has none: [..., top_k, d]."""
-    at = slot_row.long()
     if rows.shape[0] == 0:
-        return _wide(rows).sum(dim=0).expand(*at.shape, rows.shape[1])      # zeros, with the graph of the rows
-    return _wide(rows)[at.clamp(min=0)].masked_fill((at < 0).unsqueeze(-1), 0.0)
+        return _wide(rows).sum(dim=0).expand(*slot_row.shape, rows.shape[1])      # zeros, with the graph of the rows
+    none = _outside(slot_row, rows.shape[0])
+    return _wide(rows)[slot_row.masked_fill(none, 0).long()].masked_fill(none.unsqueeze(-1), 0.0)
 
 
 def _spread(values, slot_row, row_slot, weights):
@@ -245,11 +250,12 @@ def _spread(values, slot_row, row_slot, weights):
     values = values.reshape(math.prod(values.shape[:-1]), values.shape[-1])
     if row_slot.shape[0] == 0:
         return values[:0]
-    slot = row_slot.clamp(min=0).long()
+    none = _outside(row_slot, values.shape[0] * slot_row.shape[-1])
+    slot = row_slot.masked_fill(none, 0).long()
     rows = _wide(values)[torch.div(slot, slot_row.shape[-1], rounding_mode="floor")]
     if weights is not None:
         rows = rows * _wide(weights.reshape(-1))[slot].unsqueeze(1)
-    return rows.masked_fill((row_slot < 0).unsqueeze(1), 0.0).to(values.dtype)
+    return rows.masked_fill(none.unsqueeze(1), 0.0).to(values.dtype)
 
 
 # ---- what users call ------------------------------------------------------------------------------------------------------
@@ -307,5 +313,5 @@ def return_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch.
     _check_return(rows, order, weights)
     slots = _slots(rows, order.slot_row)
     if weights is not None:
-        slots = slots * _wide(weights).masked_fill(order.slot_row < 0, 0.0).unsqueeze(-1)
+        slots = slots * _wide(weights).masked_fill(_outside(order.slot_row, rows.shape[0]), 0.0).unsqueeze(-1)
     return slots.sum(dim=-2).to(rows.dtype)
