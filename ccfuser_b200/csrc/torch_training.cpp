@@ -189,7 +189,7 @@ struct ReturnNode : TokenNode {
     const at::Tensor dy = grads[0].reshape({tokens, d}).to(at::kFloat), none = outside(row_slot, tokens * k), slot = row_slot.masked_fill(none, 0).to(at::kLong);
     if (task_should_compute_output(0)) {
       at::Tensor g = dy.index_select(0, at::floor_divide(slot, k));
-      if (weights.defined()) g = g * weights.reshape({-1}).to(at::kFloat).index_select(0, slot).unsqueeze(1);
+      if (weights.defined()) g = g * weights.reshape({-1}).to(at::kFloat).index_select(0, slot).masked_fill(none, 0).unsqueeze(1);
       out[0] = g.masked_fill(none.unsqueeze(1), 0).to(grads[0].scalar_type());
     }
     if (weights.defined() && values.defined() && task_should_compute_output(1))

@@ -254,7 +254,7 @@ def _spread(values, slot_row, row_slot, weights):
     slot = row_slot.masked_fill(none, 0).long()
     rows = _wide(values)[torch.div(slot, slot_row.shape[-1], rounding_mode="floor")]
     if weights is not None:
-        rows = rows * _wide(weights.reshape(-1))[slot].unsqueeze(1)
+        rows = rows * _wide(weights.reshape(-1))[slot].masked_fill(none, 0.0).unsqueeze(1)
     return rows.masked_fill(none.unsqueeze(1), 0.0).to(values.dtype)
 
 

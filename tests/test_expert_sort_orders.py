@@ -47,3 +47,34 @@ def test_slots_behind_the_last_are_none(device):
     order = ExpertOrder(*(torch.tensor(v, dtype=torch.int32, device=device) for v in ([[0], [2]], [0, 2, 1, 7], [4], [0, 4])))
     x = torch.arange(1.0, 7.0, dtype=torch.float64, device=device).view(2, 3)
     assert sort_rows(x, order).tolist() == [[1, 2, 3], [0, 0, 0], [4, 5, 6], [0, 0, 0]]
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("device", [pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_second_derivatives_do_not_see_the_weight_of_a_slot_without_a_row(device, bad):
+    """The first slot's, which rows without a slot would read."""
+    idx = torch.tensor([[-1, 0], [1, 0], [0, 1]], device=device)
+    order = expert_order(idx, 2, align=4)
+    assert int((order.row_slot < 0).sum()) > 0
+    g = torch.Generator().manual_seed(5)
+    rows, w, dy, c = (torch.randn(s, generator=g).to(device) for s in ((order.row_slot.numel(), 8), (3, 2), (3, 8), (order.row_slot.numel(), 8)))
+    got = []
+    for value in (1.0, bad):
+        w[0, 0] = value
+        args = [t.clone().requires_grad_(True) for t in (rows, w, dy)]
+        d_rows, d_w = torch.autograd.grad(return_rows(args[0], order, args[1]), args[:2], args[2], create_graph=True)
+        got.append([t.detach() for t in (d_rows, d_w) + torch.autograd.grad((d_rows * c).sum() + d_w.square().sum(), args)])
+    for a, b in zip(*got):
+        assert a.isfinite().all() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_spreading_does_not_see_it_either(bad):
+    """The same operations on the host, as the Python nodes take them."""
+    from ccfuser_b200.ops.expert_sort import _spread
+    idx = torch.tensor([[-1, 0], [1, 0], [0, 1]])
+    order = expert_order(idx, 2, align=4)
+    dy, w = torch.ones(3, 8, requires_grad=True), torch.tensor([[bad, 1.0], [2.0, 3.0], [4.0, 5.0]], requires_grad=True)
+    out = _spread(dy, order.slot_row, order.row_slot, w)
+    d, dw = torch.autograd.grad(out, [dy, w], torch.ones_like(out))
+    assert out.isfinite().all() and d[:, 0].tolist() == [1.0, 5.0, 9.0] and dw.tolist() == [[0.0, 8.0], [8.0, 8.0], [8.0, 8.0]]
