@@ -751,13 +751,14 @@ static int launch_return_bwd(const CcfRows& r, cudaStream_t st) {
   return launch_result();
 }
 
-static size_t order_shared(const OrderShape& s, int experts) { return (static_cast<size_t>(s.threads / 32) * experts + 4 * experts + 1) * sizeof(int); }
+constexpr size_t order_shared(int threads, int experts) { return (static_cast<size_t>(threads / 32) * experts + 4 * experts + 1) * sizeof(int); }
 
 template <int kPer>
 static cudaError_t launch_place(const CcfOrder& o, const OrderShape& s, int early, cudaStream_t st) {
-  const size_t shared = order_shared(s, o.experts);
-  if (shared > 48 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(order_place_kernel<kPer>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
+  const size_t shared = order_shared(s.threads, o.experts);
+  if (shared > 48 * 1024) {      // the most of any call: another thread's call may come between this and the launch
+    constexpr int most = static_cast<int>(order_shared(kOrderThreads, CCF_SORT_MAX_EXPERTS));
+    const cudaError_t err = cudaFuncSetAttribute(order_place_kernel<kPer>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (err != cudaSuccess) return err;
   }
   cudaLaunchConfig_t cfg = {};
