@@ -153,6 +153,13 @@ __device__ __forceinline__ void load_eight(const void* base, long long at, float
     for (int j = 0; j < kElemsPer16<kType>; ++j) f[i * kElemsPer16<kType> + j] = part[j];
   }
 }
+// One weight. A plain read: load_elem's is for data that nothing writes while the kernel runs, and weights are written.
+template <int kType>
+__device__ __forceinline__ float load_weight(const void* p, long long i) {
+  if constexpr (kType == kFp32) return static_cast<const float*>(p)[i];
+  else if constexpr (kType == kFp16) return __half2float(static_cast<const __half*>(p)[i]);
+  else return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
 template <int kType>
 __device__ __forceinline__ void load_gradients(const AdamEntry& e, long long at, float (&g)[8]) {
   if ((e.vectors & 2) != 0) {
@@ -205,7 +212,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw32_kernel(const __grid_cons
     moments(load_elem<kType>(e.g, i), m, v, r);
     pm[i] = m;
     pv[i] = v;
-    store_elem<kType>(e.p, i, updated(load_elem<kType>(e.p, i), m, v, r, s));
+    store_elem<kType>(e.p, i, updated(load_weight<kType>(e.p, i), m, v, r, s));
   }
 }
 
@@ -324,7 +331,7 @@ __global__ void __launch_bounds__(kAdamThreads, kAdam8Blocks<kType>) adamw8_kern
         bm[i / 4] |= static_cast<unsigned>(pm[at + i]) << (8 * (i & 3));
         bv[i / 4] |= static_cast<unsigned>(pv[at + i]) << (8 * (i & 3));
         g[i] = load_elem<kType>(e.g, at + i);
-        p[i] = load_elem<kType>(e.p, at + i);
+        p[i] = load_weight<kType>(e.p, at + i);
       }
       cm = make_uint2(bm[0], bm[1]);
       cv = make_uint2(bv[0], bv[1]);
