@@ -448,16 +448,15 @@ class FusedAdamW(torch.optim.Optimizer):
                         started.append(p)
                         state = self._start(k, group, p)
                     key = (k, p.device if group["capturable"] else state["step"] + 1, "exponents" in state)
-                    batches.setdefault(key, []).append((p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("exponents"), number))
+                    batches.setdefault(key, []).append((p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("exponents"), number, state))
             if len(batches) > 1:      # each call looks at its own tensors before it changes one
                 for batch in batches.values():
-                    for p, g, *_ in batch:
-                        if g.layout is not torch.strided or g.dtype is not p.dtype:
-                            raise TypeError(f"a gradient is {g.layout} of {g.dtype}, its parameter {p.dtype}")
+                    if [t[1].layout for t in batch].count(torch.strided) != len(batch):
+                        raise TypeError("FusedAdamW: gradients are strided")
             raised = set()
             for (k, at, eight), batch in batches.items():
                 group = self.param_groups[k]
-                p, g, m, v, e, numbers = zip(*batch)
+                p, g, m, v, e, numbers, states = zip(*batch)
                 step, counter = at, None
                 if group["capturable"]:
                     step, counter = None, self._counter(k, p[0])
@@ -473,8 +472,8 @@ class FusedAdamW(torch.optim.Optimizer):
                     raise
                 raised.add((k, at))
                 if counter is None:
-                    for q in p:
-                        self.state[q]["step"] = at
+                    for state in states:
+                        state["step"] = at
                 if started:
                     done = {id(q) for q in p}
                     started = [q for q in started if id(q) not in done]
