@@ -7,7 +7,8 @@
 // for m (17 binades down to the smallest), 5 and 3 for v (33 binades), with gradual underflow. A scale that is a power of two makes a code the upper
 // bits of a float, so that coding is an integer addition and a shift. What counts for training is the rounding: with b2 = 0.999 a step changes v by 0.1 %
 // where codes lie 6 to 12 % apart, and rounding to nearest would lose every such change. A value is rounded up or down by 20 bits of a hash, up as often as
-// it is near, so that the mean of what is stored is the value. A positive v never becomes 0: m / sqrt(v) would be without bound.
+// it is near, so that the mean of what is stored is the value, for m at every size and for v down to the smallest code, some 2^-33 of its block's largest value. A positive v
+// never becomes 0 (m / sqrt(v) would be without bound): below that it is held as the smallest code, which is more than it is, and its weights move less.
 // The hash: MurmurHash3's last step (Appleby, 2011) of the weight's number plus a key of (seed, step, tensor), which comes from SplitMix64
 // (Steele, Lea, Flood: "Fast splittable pseudorandom number generators", 2014).
 //
@@ -181,7 +182,8 @@ __device__ __forceinline__ void store_eight(void* base, long long at, const floa
   }
 }
 
-// Moments in fp32. Bound by memory: 22 bytes a weight of bf16, 28 of fp32; 285 M weights of 14 tensors 901 us (the copy rate says 960), 18.9 M fp32 weights of 96 tensors 79 us (81).
+// Moments in fp32. Bound by memory: 22 bytes a weight of bf16, 28 of fp32; 285 M weights of 14 tensors 901 us at full clocks and 960 to 1005
+// in a long run, where the card holds its clock down for power (the copy rate says 960), 18.9 M fp32 weights of 96 tensors 79 to 82 us (81).
 template <int kType, int kCount>
 __global__ void __launch_bounds__(kAdamThreads) adamw32_kernel(const __grid_constant__ AdamTable<kCount> a) {
   const AdamEntry& e = a.entry[find_entry(a)];
@@ -216,9 +218,10 @@ __global__ void __launch_bounds__(kAdamThreads) adamw32_kernel(const __grid_cons
   }
 }
 
-// A warp has a block of CCF_ADAMW_BLOCK weights, eight a lane, as pairs: one instruction for two operations, each rounded as alone. Bound by its
-// integer instructions (60 a weight of all kinds; ALU pipe 63 %, issue slots 73 %) next to 10 bytes a weight of bf16: 285 M weights of 14 tensors 560 to 583 us of bf16 (436 at the copy rate),
-// 722 of fp32 (697). Scalar arithmetic instead of pairs 464 us where pairs take 424, constants as pairs in the arguments 443, shifts as products 440 (200 M).
+// A warp has a block of CCF_ADAMW_BLOCK weights, eight a lane, as pairs: one instruction for two operations, each rounded as alone. Bound by what
+// an SM does in a clock, and by nothing of it alone: no pipe is full (ALU 63 %, issue slots 73 %, 60 instructions a weight), the first stall is for memory, as nothing of a turn is read
+// before the turn in front of it is stored, and the time goes with the clock: 285 M weights of 14 tensors of bf16 564 us at 1965 MHz, 602 to 618 at the 1750 that a long run is held to (436 at the
+// copy rate); 722 of fp32 (697). Scalar arithmetic instead of pairs 464 us where pairs take 424, constants as pairs in the arguments 443, shifts as products 440 (200 M).
 struct Place {
   long long block, at;   // of the tensor's blocks, first weight of this lane
   int here;              // its number of weights, 0 to 8
@@ -277,7 +280,8 @@ __device__ __forceinline__ unsigned four_codes(const unsigned* w) {
   const unsigned codes = __byte_perm(x >> 4, y >> 4, 0x6420);
   return kSecond ? codes : codes | (__byte_perm(x, y, 0x7531) & 0x80808080u);
 }
-// The inverses of sqrt(v) / sqrt(1 - b2^t) + eps by the hardware's approximations (2^-22 off); subnormal v count as 0 there, which eps covers from 1e-10 on.
+// The inverses of sqrt(v) / sqrt(1 - b2^t) + eps by the hardware's approximations; subnormal v count as 0 there, which eps covers from 1e-10 on. They are some 2^-22 of
+// the update off, where moments of 3 bits of mantissa are up to an eighth off themselves; the step with moments in fp32 rounds correctly. Below 1e-10 it is rounded correctly here too.
 template <bool kFast>
 __device__ __forceinline__ f32x2 inverse_roots(f32x2 v2, const AdamRates& r, const AdamScalars& s) {
   float v[2], root[2];

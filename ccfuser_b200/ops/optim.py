@@ -341,6 +341,7 @@ def _state8_of(p, first, second, rows, key):
     """Given moments of ``p`` in 8 bits on its device, rounded as by a step with this key; in pieces, for the hash takes 64 bits a weight."""
     m, v, e = state8(p, rows)
     width = p.numel() // rows
+    first, second = (t.detach().reshape(rows, width) for t in (first, second))
     tall = max(1, _PIECE // width)
     for r in range(0, rows, tall):
         for c in range(0, width, _PIECE):
@@ -348,7 +349,7 @@ def _state8_of(p, first, second, rows, key):
             at = torch.arange(r, min(r + tall, rows), device=p.device)[:, None] * width + torch.arange(c, min(c + _PIECE, width), device=p.device)
             h = _mix((at + key) & _M32)
             for k, (codes, x, bits) in enumerate(((m, first, h & 0xFFFFF), (v, second, h >> 12))):
-                x = x.detach().reshape(rows, width)[cut].to(device=p.device, dtype=torch.float32)
+                x = x[cut].to(device=p.device, dtype=torch.float32)
                 codes.view(rows, width)[cut], part = _encode(x, x.shape[0], bits.int(), k == 1)
                 e[cut[0], c // STATE_BLOCK:c // STATE_BLOCK + part.shape[1], k] = part
     return m, v, e
@@ -360,7 +361,7 @@ class FusedAdamW(torch.optim.Optimizer):
     8 bits hold is right, so that moments go on following changes of a fraction of their steps; ``seed`` chooses the hash that decides.
 
     ``capturable=True``: for steps captured in a CUDA graph. The number of the step then lies on the device, one for all parameters of a group and device, and ``lr`` may be an fp32 tensor of
-    one element there; the first step is taken before the capture. ``state_dict`` has the names of torch's (``step``, ``exp_avg``, ``exp_avg_sq``, and ``exponents`` for 8 bits), and
+    one element there; the first step is taken before the capture, and a graph holds the moments that it was captured with: after ``load_state_dict`` it is captured anew. ``state_dict`` has the names of torch's (``step``, ``exp_avg``, ``exp_avg_sq``, and ``exponents`` for 8 bits), and
     loads those of ``torch.optim.AdamW``. Expert weights (and the router's) share exponents inside an expert only, so that ``rebalance_experts`` moves their moments with them."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32, seed: int = 0,
