@@ -389,7 +389,8 @@ class FusedAdamW(torch.optim.Optimizer):
             if saved is not None:      # as a step reads them: numbers, or a rate beside the counter, wherever the checkpoint was read to
                 group["betas"] = tuple(float(b) for b in group["betas"])
                 if torch.is_tensor(group["lr"]):
-                    group["lr"] = group["lr"].detach().to(device=group["params"][0].device, dtype=torch.float32) if group["capturable"] else float(group["lr"])
+                    beside = group["params"][0].device if group["params"] else group["lr"].device
+                    group["lr"] = group["lr"].detach().to(device=beside, dtype=torch.float32) if group["capturable"] else float(group["lr"])
             for number, (p, i) in enumerate(zip(group["params"], saved["param_groups"][k]["params"] if saved is not None else ())):
                 if saved["state"].get(i):
                     state["state"][p] = self._loaded(k, group, number, p, saved["state"][i])

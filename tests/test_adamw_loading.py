@@ -196,3 +196,12 @@ def test_rates_that_torch_keeps_in_tensors(capturable):
     _train(FusedAdamW(want, lr=float(lr), betas=tuple(float(torch.tensor(b)) for b in (0.8, 0.99))), want, 1, 2)
     _train(opt, params, 1, 2)
     assert all(torch.equal(p, q) and not torch.equal(p, w) for p, q, w in zip(params, want, weights))
+
+
+def test_a_group_without_parameters():
+    params, theirs = _params(), _params()
+    make = lambda cls, p: cls([{"params": p}, {"params": []}], lr=torch.tensor(0.1), capturable=True)  # noqa: E731
+    a, b = make(FusedAdamW, params), make(FusedAdamW, theirs)
+    _train(a, params, 1, 1)
+    b.load_state_dict(a.state_dict())
+    _assert_same(_all_of(a), _all_of(b))
